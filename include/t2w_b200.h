@@ -607,6 +607,99 @@ T2W_API int t2w_test_attn_gathered(const void* qkv_bf16, int32_t rows, int32_t h
                                    const void* pool_bf16, int32_t pool_rows, int32_t pool_ld, const int32_t* kv_idx,
                                    int32_t n_idx, int32_t pair, void* out_bf16, int32_t* err, void* stream);
 
+/* ---- Paged K/V cache held in 8 bits (no reference counterpart: the reference keeps its caches in 16 bits, one slot a
+ * frame, and its tables on the host).  Replaces a stream's cached keys and values with pages of `page` tokens:
+ *   codes   e4m3 [pages][kv_heads][page][head_dim] for K and for V (a page may lie at any pitch: *_page_ld bytes);
+ *   scales  fp32 [pages][kv_heads] for K and for V (pitch *_scale_ld floats), powers of two from 2^-64 to 2^64;
+ *   table   int32 [requests][max_blocks] (pitch table_ld): the page of tokens b * page .. of a request.
+ * A value is code * scale.  page is 16, 32, 64 or 128, head_dim 64 or 128, q_heads a multiple of kv_heads with at most
+ * 128 query heads to a key head; one layer has its own codes and scales, all layers of a step share table and plan.
+ * Device pointers are on the current device; every call is asynchronous on `stream` and reads no host memory later, so
+ * all of them may be captured in a CUDA graph.  What goes wrong on the GPU (a pool that is used up, lengths that do not
+ * fit) makes a plan void: it then has no rows, and the calls that take it write nothing but zeros for their rows;
+ * t2w_paged_status tells. */
+#define T2W_DT_BF16 0
+#define T2W_DT_FP16 1
+
+/* int32 entries of a plan for these sizes (negative: a status); at (may be NULL) receives the places of q_start
+ * [requests + 1], kv_len [requests], slot [rows] and request [rows] in it.  max_fresh: the most new rows of one request. */
+T2W_API int64_t t2w_paged_plan_ints(int32_t requests, int32_t rows, int32_t max_fresh, int32_t page, int32_t q_heads,
+                                    int32_t kv_heads, int32_t head_dim, int64_t* at);
+
+/* A step's tables from its requests' lengths.  fresh[r]: new rows of request r in this step (0 .. max_fresh); their sum
+ * is at most `rows`, and rows past it are padding.  With free_pages / free_count the new rows are to be appended: kv_len
+ * = length + fresh, pages that this takes come off the end of the free list (request by request, block by block) into
+ * `table`, and slot[i] = page * page_size + place of row i.  Without them the rows only look at what is cached: kv_len =
+ * length, slot = -1.  kv_len and free_left (each may be NULL, or the very arrays that `length` and `free_count` are)
+ * receive the new lengths and the pages left; with arrays of their own the call may be made again with the same result. */
+typedef struct t2w_paged_plan_args {
+  int32_t requests, rows, max_fresh, page, q_heads, kv_heads, head_dim, causal;
+  int32_t table_ld, max_blocks, pages;
+  const int32_t* fresh;      /* device [requests] */
+  const int32_t* length;     /* device [requests] */
+  int32_t* table;            /* device [requests][table_ld] */
+  const int32_t* free_pages; /* device [pages] or NULL */
+  const int32_t* free_count; /* device [1] or NULL */
+  int32_t* kv_len;           /* device [requests] or NULL */
+  int32_t* free_left;        /* device [1] or NULL */
+  int32_t* plan;             /* device, t2w_paged_plan_ints entries, 16-byte aligned */
+} t2w_paged_plan_args;
+T2W_API int t2w_paged_plan(const t2w_paged_plan_args* a, void* stream);
+
+/* The status that a plan and the calls that took it recorded (T2W_OK, T2W_ERR_INVALID, T2W_ERR_EXHAUSTED,
+ * T2W_ERR_TIMEOUT), by a copy on `stream` that this call waits for. */
+T2W_API int t2w_paged_status(const int32_t* plan, void* stream);
+
+/* Pages of the requests with done[r] != 0 back onto the end of the free list (request by request, block by block); their
+ * table entries become -1 and their lengths 0.  *status (device) becomes T2W_ERR_INVALID, and nothing is given back,
+ * where that would make more free pages than there are. */
+T2W_API int t2w_paged_release(const int32_t* done, int32_t* length, int32_t* table, int32_t requests, int32_t page,
+                              int32_t table_ld, int32_t max_blocks, int32_t pages, int32_t* free_pages,
+                              int32_t* free_count, int32_t* status, void* stream);
+
+/* The step's new keys and values [rows][kv_heads][head_dim] (dtype T2W_DT_*, head_dim contiguous, pitches in elements,
+ * 16-byte aligned) into their pages.  A page and head's scale is the least power of two by which its largest magnitude
+ * fits e4m3; it never falls, and codes written earlier are rounded again where it grows.  A page and head that is given
+ * an infinity or a NaN reads as NaN from then on.  A page that is appended to belongs to one request. */
+typedef struct t2w_paged_append_args {
+  int32_t requests, rows, max_fresh, page, q_heads, kv_heads, head_dim, pages, dtype;
+  const void* k;
+  const void* v;
+  int64_t k_row_ld, k_head_ld, v_row_ld, v_head_ld;
+  void* k_codes;
+  void* v_codes;
+  float* k_scale;
+  float* v_scale;
+  int64_t k_page_ld, v_page_ld, k_scale_ld, v_scale_ld;
+  const int32_t* plan;
+} t2w_paged_append_args;
+T2W_API int t2w_paged_append(const t2w_paged_append_args* a, void* stream);
+
+/* Attention of the plan's rows over their requests' pages: q [rows][q_heads][head_dim] (dtype, head_dim contiguous,
+ * pitches in elements, 16-byte aligned), key head h / (q_heads / kv_heads) for query head h.  Row i of request r sees
+ * keys j < kv_len[r], or with `causal` (as in the plan) j < kv_len[r] - (queries of r behind row i).  out: dtype
+ * [rows][q_heads][head_dim] contiguous; lse: fp32 [rows][q_heads] or NULL, the natural log of the sum of exponentials.
+ * A row that sees no key, and padding, gives zeros and -inf.  workspace: t2w_paged_workspace_bytes, 16-byte aligned. */
+typedef struct t2w_paged_attn_args {
+  int32_t requests, rows, max_fresh, page, q_heads, kv_heads, head_dim, causal, pages, dtype, table_ld;
+  float scale;
+  const void* q;
+  int64_t q_row_ld, q_head_ld;
+  const void* k_codes;
+  const void* v_codes;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t k_page_ld, v_page_ld, k_scale_ld, v_scale_ld;
+  const int32_t* table;
+  int32_t* plan;
+  void* out;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+} t2w_paged_attn_args;
+T2W_API size_t t2w_paged_workspace_bytes(int32_t max_fresh, int32_t q_heads, int32_t kv_heads, int32_t head_dim);
+T2W_API int t2w_paged_attn(const t2w_paged_attn_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,7 +15,7 @@ from .build import INCLUDE, LIB_PATH
 T2W_OK = 0
 STATUS = {-1: "invalid argument or shape", -2: "CUDA error", -3: "out of device memory", -4: "kernel wait timed out",
           -5: "unsupported config or device", -6: "workspace too small",
-          -7: "Token2Wav cache pool exhausted (key slots, conv-cache row slots or cache handles)"}
+          -7: "Token2Wav cache pool exhausted (key slots, conv-cache row slots, cache handles or pages)"}
 PREC = {"bf16": 0, "fp8": 1}
 FLAG_GRAPH = 1
 EPI = {"f32": 0, "bf16": 1, "gelu": 2, "resid": 3, "qkv": 4, "silu": 5, "leaky": 6, "gelu_fp8": 8}
@@ -123,6 +123,34 @@ class TConvArgs(ctypes.Structure):
                 ("resid_in", ctypes.c_void_p)]
 
 
+class PagedPlanArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("requests", "rows", "max_fresh", "page", "q_heads", "kv_heads", "head_dim",
+                                              "causal", "table_ld", "max_blocks", "pages")] + \
+               [(n, ctypes.c_void_p) for n in ("fresh", "length", "table", "free_pages", "free_count", "kv_len",
+                                               "free_left", "plan")]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("requests", "rows", "max_fresh", "page", "q_heads", "kv_heads", "head_dim",
+                                              "pages", "dtype")] + \
+               [(n, ctypes.c_void_p) for n in ("k", "v")] + \
+               [(n, ctypes.c_int64) for n in ("k_row_ld", "k_head_ld", "v_row_ld", "v_head_ld")] + \
+               [(n, ctypes.c_void_p) for n in ("k_codes", "v_codes", "k_scale", "v_scale")] + \
+               [(n, ctypes.c_int64) for n in ("k_page_ld", "v_page_ld", "k_scale_ld", "v_scale_ld")] + \
+               [("plan", ctypes.c_void_p)]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("requests", "rows", "max_fresh", "page", "q_heads", "kv_heads", "head_dim",
+                                              "causal", "pages", "dtype", "table_ld")] + \
+               [("scale", ctypes.c_float), ("q", ctypes.c_void_p), ("q_row_ld", ctypes.c_int64),
+                ("q_head_ld", ctypes.c_int64)] + \
+               [(n, ctypes.c_void_p) for n in ("k_codes", "v_codes", "k_scale", "v_scale")] + \
+               [(n, ctypes.c_int64) for n in ("k_page_ld", "v_page_ld", "k_scale_ld", "v_scale_ld")] + \
+               [(n, ctypes.c_void_p) for n in ("table", "plan", "out", "lse", "workspace")] + \
+               [("workspace_bytes", ctypes.c_size_t)]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
 _F = ctypes.c_float
@@ -205,6 +233,13 @@ _SIGS = {
                                ctypes.c_int),
     "t2w_hift_counts": ([_P, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64),
                          ctypes.POINTER(ctypes.c_int64)], ctypes.c_int),
+    "t2w_paged_plan_ints": ([_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(ctypes.c_int64)], ctypes.c_int64),
+    "t2w_paged_plan": ([ctypes.POINTER(PagedPlanArgs), _P], ctypes.c_int),
+    "t2w_paged_status": ([_P, _P], ctypes.c_int),
+    "t2w_paged_release": ([_P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P], ctypes.c_int),
+    "t2w_paged_append": ([ctypes.POINTER(PagedAppendArgs), _P], ctypes.c_int),
+    "t2w_paged_workspace_bytes": ([_I, _I, _I, _I], ctypes.c_size_t),
+    "t2w_paged_attn": ([ctypes.POINTER(PagedAttnArgs), _P], ctypes.c_int),
     "t2w_gemm_e4m3": ([_P, _I, _I, _P, _I, ctypes.c_int64, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _I, _P,
                        ctypes.POINTER(_P), _F, _P], ctypes.c_int),
 }

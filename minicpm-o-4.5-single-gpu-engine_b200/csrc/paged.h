@@ -1,0 +1,117 @@
+// What the kernels of the paged 8-bit K/V cache share: the layout of a plan's buffer, the split of an attention call's
+// key tiles over its workers, and the cache's number format.
+//
+// A value is code * scale: code e4m3, scale 2^e with e in [kScaleMin, kScaleMax], one scale per page and head (K and V
+// each have their own).  A power of two because a page that is appended to may have to raise its scale: codes already
+// written are then divided by a power of two, which is exact but for codes that become subnormal, and a floating-point
+// code loses nothing by it against a scale of full precision.  A page and head that was given a value that is not finite
+// has the scale NaN from then on: all of it reads as NaN, and rows that its mask hides from a query still cannot reach it.
+#pragma once
+
+#include <stdint.h>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace t2w {
+
+constexpr int kScaleMin = -64, kScaleMax = 64;
+
+// ---------------------------------------------------------------- a plan's buffer (int32)
+// header, then q_start [B + 1], kv_len [B], slot [rows], request [rows], bases [B + 1] x 3 (new pages, runs, tiles), starts
+// int4 [workers], runs int4 [max_runs].  Every part begins on a 16-byte boundary.
+struct PlanHead {
+  int n_runs;   // runs of rows that go into one page
+  int tiles;    // key tiles of the attention over all its segments
+  int per;      // tiles of a worker
+  int workers;  // workers that have any
+  int status;   // T2W_OK, or what made the plan void
+  int used;     // rows that belong to a request (the rest is padding)
+  int free_left;
+  int pad;
+};
+struct PlanLayout {
+  int64_t q_start, kv_len, slot, request, new_base, run_base, tile_base, starts, runs, total;  // in int32
+  int max_runs, max_workers;
+};
+
+// How an attention call is cut.  A segment is what one softmax runs over: (request, key head, query tile); its keys come
+// in tiles of `kt`.  The tiles of all segments, in that order, are dealt to the workers in equal contiguous shares, so
+// that ragged lengths cost no balance; a segment that is cut by a share's end is finished by k_paged_merge.
+struct PagedCut {
+  int mma;    // 1: tcgen05 tiles of 128 query rows, a worker is a CTA; 0: at most 16 rows, a worker is a warp
+  int tq;     // query tokens of a tile (rows = tokens * group)
+  int kt;     // keys of a tile
+  int workers;  // workers at most
+  int min_per;  // tiles of a worker at least
+};
+
+inline int64_t round4(int64_t n) { return (n + 3) & ~int64_t(3); }
+
+PagedCut paged_cut(int max_fresh, int q_heads, int kv_heads, int head_dim);
+PlanLayout paged_layout(int64_t requests, int64_t rows, int page, const PagedCut& cut);
+
+// ---------------------------------------------------------------- tiles of a request (device)
+// sum over i < n of floor((a i + b) / m), a, b >= 0 (the lattice points under a line, by Euclid's algorithm on a and m)
+T2W_DEV long long floor_sum(long long n, long long m, long long a, long long b) {
+  long long s = 0;
+  while (n > 0) {
+    if (a >= m) {
+      s += n * (n - 1) / 2 * (a / m);
+      a %= m;
+    }
+    if (b >= m) {
+      s += n * (b / m);
+      b %= m;
+    }
+    const long long top = a * n + b;
+    if (top < m) break;
+    n = top / m;
+    b = top % m;
+    const long long t = m;
+    m = a;
+    a = t;
+  }
+  return s;
+}
+// Keys that the last query of query tile qt sees.
+T2W_DEV int tile_keys(int f, int kv, int causal, int tq, int qt) {
+  if (!causal) return kv;
+  const long long v = (long long)kv - f + (long long)(qt + 1) * tq;
+  return v < 0 ? 0 : v > kv ? kv : (int)v;
+}
+// Key tiles of a segment: one at least, so that rows that see nothing are written too.
+T2W_DEV int seg_tiles(int keys, int kt) { return keys > 0 ? (keys + kt - 1) / kt : 1; }
+// Key tiles of the first x query tiles of one key head.
+T2W_DEV long long tiles_before(int f, int kv, int causal, int tq, int kt, int x) {
+  if (x <= 0) return 0;
+  if (!causal) return (long long)x * seg_tiles(kv, kt);
+  if (x == 1) return seg_tiles(tile_keys(f, kv, causal, tq, 0), kt);
+  const long long c = (long long)kv - f + tq;  // keys of query tile 0, were the last tile whole
+  long long none = c > 0 ? 0 : -c / tq + 1;    // query tiles that see nothing
+  if (none > x) none = x;
+  long long s = none;
+  if (none < x) {
+    s += floor_sum(x - none, kt, tq, c + none * tq + kt - 1);
+    const long long last = c + (long long)(x - 1) * tq;
+    if (last > kv) s += seg_tiles(kv, kt) - (last + kt - 1) / kt;
+  }
+  return s;
+}
+
+// ---------------------------------------------------------------- numbers
+// The scale's exponent for a largest magnitude (finite): the least e with amax <= 448 2^e, kept in range.
+T2W_DEV int scale_exp(float amax) {
+  if (amax == 0.f) return kScaleMin;
+  const int e = (int)ue8m0_for_amax(amax) - 127;
+  return e < kScaleMin ? kScaleMin : e > kScaleMax ? kScaleMax : e;
+}
+T2W_DEV float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
+// Two e4m3 codes as two halves (exact).
+T2W_DEV uint32_t e4m3x2_to_f16x2(uint32_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)v));
+  return r;
+}
+
+}  // namespace t2w

@@ -1,0 +1,428 @@
+// The step's tables, built on the GPU from the requests' lengths: offsets, key counts, new pages, every row's slot and
+// request, the runs of rows that go into one page, and the split of the attention's key tiles over its workers.
+//
+// Mathematics: four exclusive prefix sums over the requests (rows, new pages, runs, tiles) and, for each row, page, run
+// and worker, the request that its index falls into (a binary search in the sums).  Nothing of it depends on the layer,
+// so one plan serves a step's every layer.
+//
+// Bound: latency.  A step of 64 single tokens moves 1.6 KB; what it costs is one launch and a chain of a few dependent
+// loads and a block-wide scan.  So one block does it all where the step is small: the sums stay in its shared memory
+// and no second launch waits for them.  A large step's rows are written by a second launch over many blocks, which reads
+// the sums from the plan.
+#include "paged.h"
+
+namespace t2w {
+
+PagedCut paged_cut(int max_fresh, int q_heads, int kv_heads, int head_dim) {
+  const int group = q_heads / kv_heads;
+  PagedCut c;
+  c.mma = 0;
+  (void)head_dim;
+  c.tq = max_fresh;
+  c.kt = 32;
+  c.workers = 16 * num_sms();
+  c.min_per = 2;
+  (void)group;
+  return c;
+}
+
+PlanLayout paged_layout(int64_t requests, int64_t rows, int page, const PagedCut& cut) {
+  PlanLayout l;
+  l.max_workers = cut.workers;
+  int64_t runs = rows / page + 2 * requests;  // a request's rows touch at most two pages more than they fill
+  l.max_runs = (int)(runs < rows ? runs : rows);
+  int64_t at = sizeof(PlanHead) / 4;
+  auto take = [&](int64_t n) {
+    const int64_t a = at;
+    at += round4(n);
+    return a;
+  };
+  l.q_start = take(requests + 1);
+  l.kv_len = take(requests);
+  l.slot = take(rows);
+  l.request = take(rows);
+  l.new_base = take(requests + 1);
+  l.run_base = take(requests + 1);
+  l.tile_base = take(requests + 1);
+  l.starts = take(4 * (int64_t)l.max_workers);
+  l.runs = take(4 * (int64_t)l.max_runs);
+  l.total = at;
+  return l;
+}
+
+namespace {
+
+struct PlanDev {
+  int requests, rows, max_fresh, page, shift /* page == 1 << shift */, table_ld, max_blocks, pages, causal, kv_heads;
+  PagedCut cut;
+  PlanLayout lay;
+  const int* fresh;
+  const int* length;
+  int* table;
+  const int* free_pages;  // nullptr: the caches do not grow
+  const int* free_count;
+  int* kv_len_out;        // where the key counts go besides the plan (may be `length`), or nullptr
+  int* free_left_out;     // the same for the free count (may be `free_count`)
+  int* buf;
+  int scattered;          // the rows are written by k_plan_rows
+};
+
+struct Sums {
+  long long rows, pages, runs, tiles;
+};
+T2W_DEV Sums add(const Sums& a, const Sums& b) {
+  return Sums{a.rows + b.rows, a.pages + b.pages, a.runs + b.runs, a.tiles + b.tiles};
+}
+T2W_DEV Sums shfl_up(const Sums& s, int d) {
+  return Sums{__shfl_up_sync(~0u, s.rows, d), __shfl_up_sync(~0u, s.pages, d), __shfl_up_sync(~0u, s.runs, d),
+              __shfl_up_sync(~0u, s.tiles, d)};
+}
+
+// Pages of n tokens.
+T2W_DEV int pages_of(int n, int shift) { return (int)(((long long)n + (1 << shift) - 1) >> shift); }
+
+// What request r adds to each sum; false where its lengths are not to be used.
+T2W_DEV bool of_request(const PlanDev& p, int f, int len, Sums& s) {
+  s = Sums{0, 0, 0, 0};
+  if (f < 0 || len < 0 || f > p.max_fresh || (p.free_pages && (long long)len + f > 0x7fffffffLL)) return false;
+  const int kv = p.free_pages ? len + f : len;
+  if (pages_of(kv, p.shift) > p.max_blocks) return false;
+  s.rows = f;
+  if (p.free_pages && f > 0) {
+    s.pages = pages_of(kv, p.shift) - pages_of(len, p.shift);
+    s.runs = pages_of(kv, p.shift) - (len >> p.shift);
+  }
+  if (f > 0) s.tiles = p.kv_heads * tiles_before(f, kv, p.causal, p.cut.tq, p.cut.kt, (f + p.cut.tq - 1) / p.cut.tq);
+  return true;
+}
+
+// The last i in [0, n) with base[i] <= x (base ascending, base[0] = 0 <= x): zero-wide entries are passed over.
+T2W_DEV int find(const int* base, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (base[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// The rows' slots and requests, the new pages' table entries and the runs, items i0, i0 + step, ... of each.
+T2W_DEV void scatter(const PlanDev& p, const int* q_start, const int* new_base, const int* run_base, const int* kv_len,
+                     int n_rows, int n_pages, int n_runs, int free_n, int i0, int step) {
+  int* const slot = p.buf + p.lay.slot;
+  int* const request = p.buf + p.lay.request;
+  PlanHead* const head = reinterpret_cast<PlanHead*>(p.buf);
+  // page of block b of request r: from the free list where it is new in this step (its table entry may not be written yet)
+  auto page_of = [&](int r, int b, int len) {
+    const int first = pages_of(len, p.shift);
+    const int g = b < first ? p.table[(size_t)r * p.table_ld + b] : p.free_pages[free_n - 1 - (new_base[r] + b - first)];
+    if ((unsigned)g < (unsigned)p.pages) return g;
+    atomicExch(&head->status, T2W_ERR_INVALID);  // a page that the cache does not have
+    return -1;
+  };
+  for (int i = i0; i < p.rows; i += step) {
+    if (i >= n_rows) {
+      slot[i] = -1;
+      request[i] = -1;
+      continue;
+    }
+    const int r = find(q_start, p.requests, i);
+    request[i] = r;
+    if (!p.free_pages) {
+      slot[i] = -1;
+      continue;
+    }
+    const int f = q_start[r + 1] - q_start[r], len = kv_len[r] - f, pos = len + i - q_start[r];
+    const int g = page_of(r, pos >> p.shift, len);
+    slot[i] = g < 0 ? -1 : g * p.page + (pos & (p.page - 1));
+  }
+  for (int i = i0; i < n_pages; i += step) {
+    const int r = find(new_base, p.requests, i);
+    const int f = q_start[r + 1] - q_start[r], first = pages_of(kv_len[r] - f, p.shift), b = first + i - new_base[r];
+    p.table[(size_t)r * p.table_ld + b] = page_of(r, b, kv_len[r] - f);
+  }
+  for (int i = i0; i < n_runs; i += step) {
+    const int r = find(run_base, p.requests, i);
+    const int f = q_start[r + 1] - q_start[r], len = kv_len[r] - f, b = (len >> p.shift) + i - run_base[r];
+    const int from = max(len, b * p.page), to = (int)min((long long)kv_len[r], (long long)(b + 1) * p.page);
+    reinterpret_cast<int4*>(p.buf + p.lay.runs)[i] =
+        make_int4(q_start[r] + from - len, to - from, page_of(r, b, len), from - b * p.page);
+  }
+}
+
+constexpr int kHeld = 2048;  // requests whose sums fit the block's shared memory
+
+__global__ void __launch_bounds__(1024) k_plan(const PlanDev p) {
+  __shared__ Sums warp_sum[32];
+  __shared__ Sums carry_s;
+  __shared__ int bad_s;
+  __shared__ int held[5][kHeld + 1];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5, n = p.requests;
+  pdl_wait();
+  pdl_launch();
+  PlanHead* const head = reinterpret_cast<PlanHead*>(p.buf);
+  int* const q_start = n <= kHeld ? held[0] : p.buf + p.lay.q_start;
+  int* const new_base = n <= kHeld ? held[1] : p.buf + p.lay.new_base;
+  int* const run_base = n <= kHeld ? held[2] : p.buf + p.lay.run_base;
+  int* const tile_base = n <= kHeld ? held[4] : p.buf + p.lay.tile_base;
+  int* const kv_len = n <= kHeld ? held[3] : p.buf + p.lay.kv_len;
+  const int free_n = p.free_pages ? *p.free_count : 0;
+  if (tid == 0) {
+    bad_s = 0;
+    carry_s = Sums{0, 0, 0, 0};
+  }
+  __syncthreads();
+  // the sums, and whether the step can be had at all: a plan is made whole or not at all
+  Sums total;
+  for (int r0 = 0; r0 < n; r0 += blockDim.x) {
+    const int r = r0 + tid;
+    Sums mine{0, 0, 0, 0};
+    int f = 0, len = 0;
+    if (r < n) {
+      f = p.fresh[r];
+      len = p.length[r];
+      if (!of_request(p, f, len, mine)) bad_s = 1;
+    }
+    Sums inc = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const Sums o = shfl_up(inc, d);
+      if (lane >= d) inc = add(inc, o);
+    }
+    if (lane == 31) warp_sum[warp] = inc;
+    __syncthreads();
+    if (warp == 0) {
+      Sums w = lane < warps ? warp_sum[lane] : Sums{0, 0, 0, 0};
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const Sums o = shfl_up(w, d);
+        if (lane >= d) w = add(w, o);
+      }
+      warp_sum[lane] = w;
+    }
+    __syncthreads();
+    Sums base = carry_s;
+    if (warp) base = add(base, warp_sum[warp - 1]);
+    if (r < n) {
+      q_start[r] = (int)min(base.rows + inc.rows - mine.rows, 0x7fffffffLL);
+      new_base[r] = (int)min(base.pages + inc.pages - mine.pages, 0x7fffffffLL);
+      run_base[r] = (int)min(base.runs + inc.runs - mine.runs, 0x7fffffffLL);
+      tile_base[r] = (int)min(base.tiles + inc.tiles - mine.tiles, 0x7fffffffLL);
+      kv_len[r] = p.free_pages ? len + f : len;
+    }
+    __syncthreads();
+    if (tid == 0) carry_s = add(carry_s, warp_sum[warps - 1]);
+    __syncthreads();
+  }
+  total = carry_s;
+  int status = T2W_OK;
+  if (bad_s || total.rows > p.rows || total.tiles > 0x7fffffffLL) status = T2W_ERR_INVALID;
+  else if (p.free_pages && (free_n < 0 || free_n > p.pages)) status = T2W_ERR_INVALID;
+  else if (p.free_pages && total.pages > free_n) status = T2W_ERR_EXHAUSTED;
+  __syncthreads();
+  if (status != T2W_OK) {  // void: no rows, no pages, the lengths as they were
+    total = Sums{0, 0, 0, 0};
+    for (int r = tid; r < n; r += blockDim.x) {
+      q_start[r] = new_base[r] = run_base[r] = tile_base[r] = 0;
+      kv_len[r] = p.length[r];
+    }
+  }
+  const int n_rows = (int)total.rows, n_pages = (int)total.pages, n_runs = (int)total.runs, tiles = (int)total.tiles;
+  const int per = max((int)(((long long)tiles + p.cut.workers - 1) / p.cut.workers), p.cut.min_per);
+  const int workers = tiles ? (int)(((long long)tiles + per - 1) / per) : 0;
+  if (tid == 0) {
+    q_start[n] = n_rows;
+    new_base[n] = n_pages;
+    run_base[n] = n_runs;
+    tile_base[n] = tiles;
+    *head = PlanHead{n_runs, tiles, per, workers, status, n_rows, free_n - n_pages, 0};
+  }
+  __syncthreads();
+  if (n <= kHeld) {
+    for (int r = tid; r <= n; r += blockDim.x) {
+      p.buf[p.lay.q_start + r] = q_start[r];
+      p.buf[p.lay.new_base + r] = new_base[r];
+      p.buf[p.lay.run_base + r] = run_base[r];
+      if (r < n) p.buf[p.lay.kv_len + r] = kv_len[r];
+    }
+  }
+  // the workers' starts: worker w begins at tile w * per of all
+  for (int w = tid; w < workers; w += blockDim.x) {
+    const int r = find(tile_base, n, w * per);
+    const int f = q_start[r + 1] - q_start[r], kv = kv_len[r], nq = (f + p.cut.tq - 1) / p.cut.tq;
+    const int one = (tile_base[r + 1] - tile_base[r]) / p.kv_heads;  // tiles of one key head
+    const int rem = w * per - tile_base[r], hk = rem / one, in = rem - hk * one;
+    int lo = 0, hi = nq;  // the query tile: the last x with tiles_before(x) <= in
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (tiles_before(f, kv, p.causal, p.cut.tq, p.cut.kt, mid) <= in) lo = mid; else hi = mid;
+    }
+    reinterpret_cast<int4*>(p.buf + p.lay.starts)[w] =
+        make_int4(r, hk, lo, in - (int)tiles_before(f, kv, p.causal, p.cut.tq, p.cut.kt, lo));
+  }
+  if (!p.scattered)
+    scatter(p, q_start, new_base, run_base, kv_len, n_rows, n_pages, n_runs, free_n, tid, blockDim.x);
+  // where the caller keeps its lengths: last, since they may be what was read above
+  if (p.kv_len_out)
+    for (int r = tid; r < n; r += blockDim.x) p.kv_len_out[r] = kv_len[r];
+  if (p.free_left_out && tid == 0) *p.free_left_out = free_n - n_pages;
+}
+
+// The second launch of a large step.
+__global__ void __launch_bounds__(256) k_plan_rows(const PlanDev p) {
+  pdl_wait();
+  pdl_launch();
+  const PlanHead h = *reinterpret_cast<const PlanHead*>(p.buf);
+  const int n_pages = p.buf[p.lay.new_base + p.requests];
+  scatter(p, p.buf + p.lay.q_start, p.buf + p.lay.new_base, p.buf + p.lay.run_base, p.buf + p.lay.kv_len, h.used,
+          n_pages, h.n_runs, h.free_left + n_pages, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
+}
+
+// Pages of finished requests back onto the end of the free list, in request and block order; their lengths become 0.
+__global__ void __launch_bounds__(1024) k_release(const int* done, int* length, int* table, int n, int shift, int table_ld,
+                                                  int max_blocks, int pages, int* free_pages, int* free_count,
+                                                  int* status) {
+  __shared__ int warp_sum[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  pdl_wait();
+  pdl_launch();
+  const int at0 = *free_count;
+  __syncthreads();
+  int at = at0, bad = at0 < 0 || at0 > pages;
+  for (int r0 = 0; r0 < n; r0 += blockDim.x) {
+    const int r = r0 + tid;
+    int mine = 0;
+    if (r < n && done[r]) {
+      const int len = length[r];
+      if (len < 0 || pages_of(len, shift) > max_blocks) bad = 1;
+      else mine = pages_of(len, shift);
+    }
+    bad = __syncthreads_or(bad);
+    int inc = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(~0u, inc, d);
+      if (lane >= d) inc += o;
+    }
+    if (lane == 31) warp_sum[warp] = inc;
+    __syncthreads();
+    int base = at + inc - mine, sum = 0;
+    for (int w = 0; w < warps; ++w) {
+      if (w < warp) base += warp_sum[w];
+      sum += warp_sum[w];
+    }
+    if (!bad && (long long)at + sum > pages) bad = 1;  // more pages than there are: one of them was given back before
+    if (!bad && r < n && done[r]) {
+      for (int b = 0; b < mine; ++b) {
+        int& e = table[(size_t)r * table_ld + b];
+        free_pages[base + b] = e;
+        e = -1;
+      }
+      length[r] = 0;
+    }
+    if (!bad) at += sum;
+    __syncthreads();
+  }
+  if (tid == 0) {
+    if (bad) atomicExch(status, T2W_ERR_INVALID);
+    *free_count = at;
+  }
+}
+
+bool page_ok(int page) { return page == 16 || page == 32 || page == 64 || page == 128; }
+int page_shift(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
+
+}  // namespace
+}  // namespace t2w
+
+using namespace t2w;
+
+extern "C" int64_t t2w_paged_plan_ints(int32_t requests, int32_t rows, int32_t max_fresh, int32_t page, int32_t q_heads,
+                                       int32_t kv_heads, int32_t head_dim, int64_t* at) {
+  if (requests <= 0 || rows < 0 || max_fresh <= 0 || !page_ok(page) || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads)
+    return T2W_ERR_INVALID;
+  if ((head_dim != 64 && head_dim != 128) || q_heads / kv_heads > 128) return T2W_ERR_UNSUPPORTED;
+  const PlanLayout l = paged_layout(requests, rows, page, paged_cut(max_fresh, q_heads, kv_heads, head_dim));
+  if (l.total > 0x7fffffffLL) return T2W_ERR_INVALID;
+  if (at) {
+    at[0] = l.q_start;
+    at[1] = l.kv_len;
+    at[2] = l.slot;
+    at[3] = l.request;
+  }
+  return l.total;
+}
+
+extern "C" int t2w_paged_plan(const t2w_paged_plan_args* a, void* stream) {
+  if (!a || !a->fresh || !a->length || !a->table || !a->plan || (reinterpret_cast<uintptr_t>(a->plan) & 15))
+    return T2W_ERR_INVALID;
+  if ((a->free_pages == nullptr) != (a->free_count == nullptr)) return T2W_ERR_INVALID;
+  if (a->max_blocks <= 0 || a->table_ld < a->max_blocks || a->pages <= 0 || (int64_t)a->pages * a->page > 0x7fffffffLL)
+    return T2W_ERR_INVALID;
+  const int64_t ints = t2w_paged_plan_ints(a->requests, a->rows, a->max_fresh, a->page, a->q_heads, a->kv_heads,
+                                           a->head_dim, nullptr);
+  if (ints < 0) return (int)ints;
+  PlanDev p;
+  p.requests = a->requests;
+  p.rows = a->rows;
+  p.max_fresh = a->max_fresh;
+  p.page = a->page;
+  p.shift = page_shift(a->page);
+  p.table_ld = a->table_ld;
+  p.max_blocks = a->max_blocks;
+  p.pages = a->pages;
+  p.causal = a->causal != 0;
+  p.kv_heads = a->kv_heads;
+  p.cut = paged_cut(a->max_fresh, a->q_heads, a->kv_heads, a->head_dim);
+  p.lay = paged_layout(a->requests, a->rows, a->page, p.cut);
+  p.fresh = a->fresh;
+  p.length = a->length;
+  p.table = a->table;
+  p.free_pages = a->free_pages;
+  p.free_count = a->free_count;
+  p.kv_len_out = a->kv_len;
+  p.free_left_out = a->free_left;
+  p.buf = a->plan;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  p.scattered = a->rows > 4096;
+  const bool small = a->rows <= 1024 && a->requests <= 256;
+  cudaError_t e = launch_k(k_plan, dim3(1), dim3(small ? 256 : 1024), 0, st, p);
+  if (e == cudaSuccess && p.scattered) {
+    const int grid = (a->rows + 255) / 256;
+    e = launch_k(k_plan_rows, dim3(grid < 4 * num_sms() ? grid : 4 * num_sms()), dim3(256), 0, st, p);
+  }
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    return T2W_ERR_CUDA;
+  }
+  return T2W_OK;
+}
+
+extern "C" int t2w_paged_status(const int32_t* plan, void* stream) {
+  if (!plan) return T2W_ERR_INVALID;
+  int32_t v = 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaMemcpyAsync(&v, &reinterpret_cast<const PlanHead*>(plan)->status, sizeof v, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    return T2W_ERR_CUDA;
+  }
+  return v;
+}
+
+extern "C" int t2w_paged_release(const int32_t* done, int32_t* length, int32_t* table, int32_t requests, int32_t page,
+                                 int32_t table_ld, int32_t max_blocks, int32_t pages, int32_t* free_pages,
+                                 int32_t* free_count, int32_t* status, void* stream) {
+  if (!done || !length || !table || !free_pages || !free_count || !status || requests <= 0 || !page_ok(page) ||
+      max_blocks <= 0 || table_ld < max_blocks || pages <= 0)
+    return T2W_ERR_INVALID;
+  const cudaError_t e = launch_k(k_release, dim3(1), dim3(requests <= 256 ? 256 : 1024), 0, static_cast<cudaStream_t>(stream),
+                                 done, length, table, requests, page_shift(page), table_ld, max_blocks, pages, free_pages, free_count,
+                                 status);
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    return T2W_ERR_CUDA;
+  }
+  return T2W_OK;
+}

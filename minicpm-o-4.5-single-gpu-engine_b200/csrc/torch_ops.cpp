@@ -8,6 +8,7 @@
 // every op is argument conversion around one t2w_* call (include/t2w_b200.h).  Solver and slot-pool objects cross the
 // boundary as int handles (their addresses), as the ctypes binding passes them.
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
@@ -287,6 +288,229 @@ void encode(int64_t encoder, c10::IntArrayRef handles, c10::IntArrayRef n_tokens
                                  graph ? T2W_FLAG_GRAPH : 0u, stream_of(mu)));
 }
 
+// ---- paged 8-bit K/V cache ------------------------------------------------------------------------------------------
+
+const int32_t* i32_of(const char* op, const char* name, const at::Tensor& t, const at::Tensor& like, int64_t n = -1) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.device() == like.device() && (n < 0 || t.numel() == n),
+              op, ": ", name, " is contiguous int32", n < 0 ? std::string() : " of " + std::to_string(n) + " entries",
+              " on ", like.device().str());
+  return t.data_ptr<int32_t>();
+}
+
+int32_t to_i32(const char* op, const char* name, int64_t v) {
+  TORCH_CHECK(v >= 0 && v <= 0x7fffffff, op, ": ", name, " ", v, " does not fit 32 bits");
+  return (int32_t)v;
+}
+
+// [requests, blocks] int32 whose rows may be strided (a view of a larger table)
+void table_of(const char* op, const at::Tensor& t, const at::Tensor& like, int32_t& ld, int32_t& blocks) {
+  TORCH_CHECK(t.dim() == 2 && t.scalar_type() == at::kInt && t.device() == like.device() && (t.size(1) <= 1 || t.stride(1) == 1),
+              op, ": table is int32 [requests, blocks] with contiguous rows on ", like.device().str());
+  blocks = to_i32(op, "blocks", t.size(1));
+  ld = t.size(0) > 1 ? to_i32(op, "the table's row stride", t.stride(0)) : blocks;
+}
+
+struct Pages {
+  int32_t pages, heads, page, hd;
+  void* codes[2];
+  float* scale[2];
+  int64_t page_ld[2], scale_ld[2];
+};
+
+Pages pages_of(const char* op, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs) {
+  Pages p{};
+  const at::Tensor* c[2] = {&kc, &vc};
+  const at::Tensor* s[2] = {&ks, &vs};
+  for (int w = 0; w < 2; ++w) {
+    TORCH_CHECK(c[w]->is_cuda() && c[w]->dim() == 4 && c[w]->scalar_type() == at::kFloat8_e4m3fn && c[w]->sizes() == kc.sizes() &&
+                    c[w]->device() == kc.device(),
+                op, ": codes are float8_e4m3fn [pages, kv_heads, page, head_dim], K and V alike, on one GPU");
+    const int64_t hd = c[w]->size(3), page = c[w]->size(2);
+    TORCH_CHECK(c[w]->stride(3) == 1 && c[w]->stride(2) == hd && (c[w]->size(1) == 1 || c[w]->stride(1) == page * hd),
+                op, ": a page's codes are contiguous [kv_heads, page, head_dim] (pages may lie at any pitch)");
+    TORCH_CHECK(s[w]->dim() == 2 && s[w]->scalar_type() == at::kFloat && s[w]->size(0) == kc.size(0) && s[w]->size(1) == kc.size(1) &&
+                    (s[w]->size(1) == 1 || s[w]->stride(1) == 1) && s[w]->device() == kc.device(),
+                op, ": scales are fp32 [pages, kv_heads] with contiguous rows");
+    p.codes[w] = c[w]->data_ptr();
+    p.scale[w] = s[w]->data_ptr<float>();
+    p.page_ld[w] = c[w]->size(0) > 1 ? c[w]->stride(0) : c[w]->size(1) * page * hd;
+    p.scale_ld[w] = s[w]->size(0) > 1 ? s[w]->stride(0) : s[w]->size(1);
+  }
+  p.pages = to_i32(op, "pages", kc.size(0));
+  p.heads = to_i32(op, "kv_heads", kc.size(1));
+  p.page = to_i32(op, "page", kc.size(2));
+  p.hd = to_i32(op, "head_dim", kc.size(3));
+  return p;
+}
+
+int32_t dtype_of(const char* op, const at::Tensor& t) {
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, op, ": rows are bf16 or fp16");
+  return t.scalar_type() == at::kHalf ? T2W_DT_FP16 : T2W_DT_BF16;
+}
+
+// [rows, heads, hd] with a contiguous last dimension
+void rows_of(const char* op, const char* name, const at::Tensor& t, const at::Tensor& like, int64_t rows, int64_t heads,
+             int64_t hd, int64_t& row_ld, int64_t& head_ld) {
+  TORCH_CHECK(t.dim() == 3 && t.size(0) == rows && t.size(1) == heads && t.size(2) == hd && t.stride(2) == 1 &&
+                  t.device() == like.device(),
+              op, ": ", name, " is [", rows, ", ", heads, ", ", hd, "] with contiguous head_dim on ", like.device().str());
+  row_ld = rows > 1 ? t.stride(0) : heads * hd;
+  head_ld = heads > 1 ? t.stride(1) : hd;
+  TORCH_CHECK(row_ld >= 0 && head_ld >= 0 && row_ld % 8 == 0 && head_ld % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+              op, ": ", name, " lies on 16-byte boundaries (strides a multiple of 8 elements)");
+}
+
+void plan_of(const char* op, const at::Tensor& plan, const at::Tensor& like, int32_t requests, int32_t rows, int32_t max_fresh,
+             int32_t page, int32_t q_heads, int32_t kv_heads, int32_t hd) {
+  const int64_t n = t2w_paged_plan_ints(requests, rows, max_fresh, page, q_heads, kv_heads, hd, nullptr);
+  if (n < 0) check("t2w_paged_plan_ints", (int)n);
+  i32_of(op, "a plan made for these sizes", plan, like, n);
+}
+
+at::Tensor paged_plan(const at::Tensor& fresh, const at::Tensor& length, at::Tensor& table, int64_t page, int64_t rows,
+                      int64_t max_fresh, int64_t q_heads, int64_t kv_heads, int64_t head_dim, bool causal,
+                      const std::optional<at::Tensor>& free_pages, const std::optional<at::Tensor>& free_count,
+                      const std::optional<at::Tensor>& kv_len, const std::optional<at::Tensor>& free_left) {
+  const char* op = "paged_plan";
+  TORCH_CHECK(fresh.is_cuda(), "b200t2w ops take CUDA tensors");
+  const c10::DeviceGuard guard(fresh.device());
+  t2w_paged_plan_args a{};
+  a.requests = to_i32(op, "requests", fresh.numel());
+  a.rows = to_i32(op, "rows", rows);
+  a.max_fresh = to_i32(op, "max_fresh", max_fresh);
+  a.page = to_i32(op, "page", page);
+  a.q_heads = to_i32(op, "q_heads", q_heads);
+  a.kv_heads = to_i32(op, "kv_heads", kv_heads);
+  a.head_dim = to_i32(op, "head_dim", head_dim);
+  a.causal = causal;
+  a.fresh = i32_of(op, "fresh", fresh, fresh);
+  a.length = i32_of(op, "length", length, fresh, a.requests);
+  table_of(op, table, fresh, a.table_ld, a.max_blocks);
+  TORCH_CHECK(table.size(0) == a.requests, op, ": the table has a row for each request");
+  a.table = table.data_ptr<int32_t>();
+  TORCH_CHECK(free_pages.has_value() == free_count.has_value(), op, ": free_pages and free_count come together");
+  a.pages = 1;
+  if (free_pages) {
+    a.free_pages = i32_of(op, "free_pages", *free_pages, fresh);
+    a.free_count = i32_of(op, "free_count", *free_count, fresh, 1);
+    a.pages = to_i32(op, "pages", free_pages->numel());
+  }
+  if (kv_len) a.kv_len = const_cast<int32_t*>(i32_of(op, "kv_len", *kv_len, fresh, a.requests));
+  if (free_left) a.free_left = const_cast<int32_t*>(i32_of(op, "free_left", *free_left, fresh, 1));
+  const int64_t n = t2w_paged_plan_ints(a.requests, a.rows, a.max_fresh, a.page, a.q_heads, a.kv_heads, a.head_dim, nullptr);
+  if (n < 0) check("t2w_paged_plan", (int)n);
+  at::Tensor plan = at::empty({n}, fresh.options());
+  a.plan = plan.data_ptr<int32_t>();
+  check("t2w_paged_plan", t2w_paged_plan(&a, stream_of(fresh)));
+  return plan;
+}
+
+void paged_append(const at::Tensor& k, const at::Tensor& v, at::Tensor& k_codes, at::Tensor& v_codes, at::Tensor& k_scale,
+                  at::Tensor& v_scale, const at::Tensor& plan, int64_t requests, int64_t max_fresh, int64_t q_heads) {
+  const char* op = "paged_append";
+  const Pages p = pages_of(op, k_codes, v_codes, k_scale, v_scale);
+  const c10::DeviceGuard guard(k_codes.device());
+  t2w_paged_append_args a{};
+  a.requests = to_i32(op, "requests", requests);
+  a.rows = to_i32(op, "rows", k.size(0));
+  a.max_fresh = to_i32(op, "max_fresh", max_fresh);
+  a.page = p.page;
+  a.q_heads = to_i32(op, "q_heads", q_heads);
+  a.kv_heads = p.heads;
+  a.head_dim = p.hd;
+  a.pages = p.pages;
+  a.dtype = dtype_of(op, k);
+  TORCH_CHECK(v.scalar_type() == k.scalar_type(), op, ": k and v have one type");
+  rows_of(op, "k", k, k_codes, a.rows, p.heads, p.hd, a.k_row_ld, a.k_head_ld);
+  rows_of(op, "v", v, k_codes, a.rows, p.heads, p.hd, a.v_row_ld, a.v_head_ld);
+  plan_of(op, plan, k_codes, a.requests, a.rows, a.max_fresh, a.page, a.q_heads, a.kv_heads, a.head_dim);
+  if (a.rows == 0) return;
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.k_codes = p.codes[0];
+  a.v_codes = p.codes[1];
+  a.k_scale = p.scale[0];
+  a.v_scale = p.scale[1];
+  a.k_page_ld = p.page_ld[0];
+  a.v_page_ld = p.page_ld[1];
+  a.k_scale_ld = p.scale_ld[0];
+  a.v_scale_ld = p.scale_ld[1];
+  a.plan = plan.data_ptr<int32_t>();
+  check("t2w_paged_append", t2w_paged_append(&a, stream_of(k_codes)));
+}
+
+std::vector<at::Tensor> paged_attn(const at::Tensor& q, const at::Tensor& k_codes, const at::Tensor& v_codes,
+                                   const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& table,
+                                   at::Tensor& plan, int64_t requests, int64_t max_fresh, bool causal, double scale, bool lse) {
+  const char* op = "paged_attn";
+  const Pages p = pages_of(op, k_codes, v_codes, k_scale, v_scale);
+  const c10::DeviceGuard guard(k_codes.device());
+  TORCH_CHECK(q.dim() == 3, op, ": q is [rows, q_heads, head_dim]");
+  t2w_paged_attn_args a{};
+  a.requests = to_i32(op, "requests", requests);
+  a.rows = to_i32(op, "rows", q.size(0));
+  a.max_fresh = to_i32(op, "max_fresh", max_fresh);
+  a.page = p.page;
+  a.q_heads = to_i32(op, "q_heads", q.size(1));
+  a.kv_heads = p.heads;
+  a.head_dim = p.hd;
+  a.causal = causal;
+  a.pages = p.pages;
+  a.dtype = dtype_of(op, q);
+  a.scale = (float)scale;
+  rows_of(op, "q", q, k_codes, a.rows, a.q_heads, p.hd, a.q_row_ld, a.q_head_ld);
+  plan_of(op, plan, k_codes, a.requests, a.rows, a.max_fresh, a.page, a.q_heads, a.kv_heads, a.head_dim);
+  int32_t blocks = 0;
+  table_of(op, table, k_codes, a.table_ld, blocks);
+  TORCH_CHECK(table.size(0) == a.requests, op, ": the table has a row for each request");
+  at::Tensor out = at::empty({a.rows, a.q_heads, a.head_dim}, q.options());
+  std::vector<at::Tensor> r{out};
+  if (lse) r.push_back(at::empty({a.rows, a.q_heads}, q.options().dtype(at::kFloat)));
+  if (a.rows == 0) return r;
+  const size_t ws = t2w_paged_workspace_bytes(a.max_fresh, a.q_heads, a.kv_heads, a.head_dim);
+  at::Tensor workspace = at::empty({(int64_t)ws}, q.options().dtype(at::kByte));
+  a.q = q.data_ptr();
+  a.k_codes = p.codes[0];
+  a.v_codes = p.codes[1];
+  a.k_scale = p.scale[0];
+  a.v_scale = p.scale[1];
+  a.k_page_ld = p.page_ld[0];
+  a.v_page_ld = p.page_ld[1];
+  a.k_scale_ld = p.scale_ld[0];
+  a.v_scale_ld = p.scale_ld[1];
+  a.table = table.data_ptr<int32_t>();
+  a.plan = plan.data_ptr<int32_t>();
+  a.out = out.data_ptr();
+  a.lse = lse ? r[1].data_ptr<float>() : nullptr;
+  a.workspace = workspace.data_ptr();
+  a.workspace_bytes = ws;
+  check("t2w_paged_attn", t2w_paged_attn(&a, stream_of(k_codes)));
+  return r;
+}
+
+void paged_release(const at::Tensor& done, at::Tensor& length, at::Tensor& table, int64_t page, at::Tensor& free_pages,
+                   at::Tensor& free_count, at::Tensor& status) {
+  const char* op = "paged_release";
+  TORCH_CHECK(done.is_cuda(), "b200t2w ops take CUDA tensors");
+  const c10::DeviceGuard guard(done.device());
+  const int32_t n = to_i32(op, "requests", done.numel());
+  int32_t ld = 0, blocks = 0;
+  table_of(op, table, done, ld, blocks);
+  TORCH_CHECK(table.size(0) == n, op, ": the table has a row for each request");
+  check("t2w_paged_release",
+        t2w_paged_release(i32_of(op, "done", done, done), const_cast<int32_t*>(i32_of(op, "length", length, done, n)),
+                          table.data_ptr<int32_t>(), n, to_i32(op, "page", page), ld, blocks,
+                          to_i32(op, "pages", free_pages.numel()), const_cast<int32_t*>(i32_of(op, "free_pages", free_pages, done)),
+                          const_cast<int32_t*>(i32_of(op, "free_count", free_count, done, 1)),
+                          const_cast<int32_t*>(i32_of(op, "status", status, done, 1)), stream_of(done)));
+}
+
+int64_t paged_status(const at::Tensor& plan) {
+  const c10::DeviceGuard guard(plan.device());
+  TORCH_CHECK(plan.numel() >= 8, "paged_status: a plan");
+  return t2w_paged_status(i32_of("paged_status", "plan", plan, plan), stream_of(plan));
+}
+
 }  // namespace
 
 TORCH_LIBRARY(b200t2w, m) {
@@ -324,4 +548,18 @@ TORCH_LIBRARY(b200t2w, m) {
   m.def("encode(int encoder, int[] handles, int[] n_tokens, int[] final, int[] tokens, Tensor(a!) mu, "
         "Tensor(b!) workspace, bool graph) -> ()",
         &encode);
+  m.def("paged_plan(Tensor fresh, Tensor length, Tensor(a!) table, int page, int rows, int max_fresh, int q_heads, "
+        "int kv_heads, int head_dim, bool causal, Tensor? free_pages, Tensor? free_count, Tensor? kv_len, "
+        "Tensor? free_left) -> Tensor",
+        &paged_plan);
+  m.def("paged_append(Tensor k, Tensor v, Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) k_scale, "
+        "Tensor(d!) v_scale, Tensor plan, int requests, int max_fresh, int q_heads) -> ()",
+        &paged_append);
+  m.def("paged_attn(Tensor q, Tensor k_codes, Tensor v_codes, Tensor k_scale, Tensor v_scale, Tensor table, "
+        "Tensor(a!) plan, int requests, int max_fresh, bool causal, float scale, bool lse) -> Tensor[]",
+        &paged_attn);
+  m.def("paged_release(Tensor done, Tensor(a!) length, Tensor(b!) table, int page, Tensor(c!) free_pages, "
+        "Tensor(d!) free_count, Tensor(e!) status) -> ()",
+        &paged_release);
+  m.def("paged_status(Tensor plan) -> int", &paged_status);
 }

@@ -1,0 +1,572 @@
+"""GPU: the paged 8-bit K/V cache (``b200t2w.paged``) against a plain statement in 64 bits.
+
+Tables, slots and codes are whole numbers and have to be equal.  Attention: with A = sum_j p_j |v_j| and B = scale *
+max_j sum_d |q_d k_jd| of a row, an output o may be off by
+
+    u |o| + (2^-10 + 2^-15 B) A,    u = 2^-8 (bf16) or 2^-10 (fp16)
+
+u: the output's rounding (half an ulp is 2^-9, 2^-11; doubled).  2^-10: weights rounded to 11 bits (2^-11), the same
+again for their sum being of unrounded weights, weights under 2^-25 of the largest flushed.  2^-15 B: a score is a sum of
+up to 128 products in fp32, each addition off by at most 2^-23 of B, and a weight's relative error is its score's error
+(twice, for the weight and the sum).  The log-sum may be off by 2^-16 B + 2^-19 max(1, |lse|)."""
+
+import math
+
+import pytest
+import torch
+
+from b200t2w import lib as L
+from b200t2w import ops as O
+from b200t2w import paged
+
+pytestmark = pytest.mark.gpu
+
+E_MIN, E_MAX = -64, 64
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _dev():
+    assert torch.cuda.is_available()
+    assert L.load().t2w_device_ok(torch.cuda.current_device()) == 1
+
+
+# ---- the statement in 64 bits ---------------------------------------------------------------------------------------
+
+
+def round_e4m3(x):
+    """float64 -> the nearest e4m3 value, ties to even (|x| <= 448)."""
+    _, e = torch.frexp(x)
+    step = torch.exp2((e - 1).clamp(min=-6).double() - 3)
+    return torch.round(x / step) * step
+
+
+def exponent(amax):
+    """The least e with amax <= 448 2^e, in [E_MIN, E_MAX]."""
+    if amax == 0:
+        return E_MIN
+    e = math.ceil(math.log2(amax / 448))
+    while 448.0 * 2.0 ** e < amax:
+        e += 1
+    while 448.0 * 2.0 ** (e - 1) >= amax:
+        e -= 1
+    return min(max(e, E_MIN), E_MAX)
+
+
+class Model:
+    """The cache as a list of tokens for each request, and pages for their codes, all in 64 bits on the CPU."""
+
+    def __init__(self, pages, heads, page, hd, requests, blocks):
+        self.page, self.pages = page, pages
+        self.codes = [torch.zeros(pages, heads, page, hd, dtype=torch.float64) for _ in range(2)]
+        self.scale = [torch.ones(pages, heads, dtype=torch.float64) for _ in range(2)]
+        self.table = [[-1] * blocks for _ in range(requests)]
+        self.length = [0] * requests
+        self.free = list(range(pages - 1, -1, -1))
+
+    def plan(self, fresh):
+        slots, owner, starts = [], [], [0]
+        for r, f in enumerate(fresh):
+            for b in range(-(-self.length[r] // self.page), -(-(self.length[r] + f) // self.page)):
+                self.table[r][b] = self.free.pop()
+            for i in range(f):
+                b, o = divmod(self.length[r] + i, self.page)
+                slots.append(self.table[r][b] * self.page + o)
+                owner.append(r)
+            self.length[r] += f
+            starts.append(starts[-1] + f)
+        return slots, owner, starts
+
+    def append(self, w, x, slots, owner):
+        """x [rows, heads, hd] float64 into codes and scales w (0: K, 1: V), run by run."""
+        codes, scale = self.codes[w], self.scale[w]
+        i = 0
+        while i < len(slots):
+            g, o = divmod(slots[i], self.page)
+            n = 1
+            while i + n < len(slots) and owner[i + n] == owner[i] and slots[i + n] == slots[i] + n and (o + n) < self.page:
+                n += 1
+            for h in range(x.shape[1]):
+                part = x[i:i + n, h]
+                old = float(scale[g, h]) if o else 2.0 ** E_MIN
+                if not bool(torch.isfinite(part).all()) or old != old:
+                    scale[g, h] = math.nan
+                    codes[g, h, :o + n] = 0
+                    continue
+                s = max(old, 2.0 ** exponent(float(part.abs().max())))
+                if o and s > old:
+                    codes[g, h, :o] = round_e4m3(codes[g, h, :o] * (old / s))
+                codes[g, h, o:o + n] = round_e4m3((part / s).clamp(-448, 448))
+                scale[g, h] = s
+            i += n
+
+    def values(self, w, r, h):
+        """[length, hd] float64."""
+        at = [self.table[r][b] for b in range(-(-self.length[r] // self.page))]
+        if not at:
+            return torch.zeros(0, self.codes[w].shape[3], dtype=torch.float64)
+        x = self.codes[w][at, h] * self.scale[w][at, h][:, None, None]
+        return x.reshape(-1, x.shape[-1])[:self.length[r]]
+
+
+def attention(q, k, v, causal, scale):
+    """q [f, hd], k, v [n, hd] float64 -> out, lse, A, B (see the module's text); each row over the keys it sees alone."""
+    f, n = q.shape[0], k.shape[0]
+    out, lse = torch.zeros(f, k.shape[1], dtype=torch.float64), torch.full((f,), -math.inf, dtype=torch.float64)
+    A, B = torch.zeros_like(out), torch.zeros(f, dtype=torch.float64)
+    for i in range(f):
+        end = max(0, min(n, n - f + i + 1)) if causal else n
+        if end == 0:
+            continue
+        s = (k[:end] @ q[i]) * scale
+        p = torch.softmax(s, 0)
+        out[i], lse[i], A[i] = p @ v[:end], torch.logsumexp(s, 0), p @ v[:end].abs()
+        B[i] = (k[:end].abs() @ q[i].abs()).max() * scale
+    return out, lse, A, B
+
+
+def held(out, lse, ref):
+    """Whether out [f, hd] and lse [f] are within what the module's text allows of attention()'s ref."""
+    o, l, A, B = ref
+    u = 2.0 ** -8 if out.dtype == torch.bfloat16 else 2.0 ** -10
+    d = (out.double().cpu() - o).abs()
+    lim = u * o.abs() + (2.0 ** -10 + 2.0 ** -15 * B[:, None]) * A + 1e-30
+    nan = torch.isnan(o)
+    assert torch.equal(torch.isnan(out.cpu()), nan)
+    assert bool((d <= lim)[~nan].all()), float((d / lim)[~nan].max())
+    got = lse.double().cpu()
+    none, lnan = l == -math.inf, torch.isnan(l)
+    assert torch.equal(got == -math.inf, none) and torch.equal(torch.isnan(got), lnan)
+    ok = ~none & ~lnan
+    lim = 2.0 ** -16 * B + 2.0 ** -19 * l.abs().clamp(min=1)
+    assert bool(((got - l).abs() <= lim)[ok].all()), float(((got - l).abs() / lim)[ok].max())
+
+
+def check_attention(m, q, out, lse, starts, heads, causal, scale, fresh):
+    group = q.shape[1] // heads
+    qd = q.double().cpu()
+    for r, f in enumerate(fresh):
+        for h in range(q.shape[1]):
+            a, b = starts[r], starts[r] + f
+            ref = attention(qd[a:b, h], m.values(0, r, h // group), m.values(1, r, h // group), causal, scale)
+            held(out[a:b, h], lse[a:b, h], ref)
+
+
+def i32(xs):
+    return torch.tensor(xs, device="cuda", dtype=torch.int32)
+
+
+def normal(gen, *shape, dtype=torch.bfloat16):
+    """Normal values whose size differs from row to row and head to head."""
+    x = torch.randn(*shape, device="cuda", generator=gen)
+    return (x * torch.exp(0.7 * torch.randn(*shape[:-1], 1, device="cuda", generator=gen))).to(dtype)
+
+
+def same_cache(c, m, layer=0):
+    """The device's codes and scales against the model's, where a request holds tokens."""
+    for w, (codes, scale) in enumerate(((c.k, c.k_scale), (c.v, c.v_scale))):
+        codes, scale = codes[layer].double().cpu(), scale[layer].double().cpu()
+        for r, n in enumerate(m.length):
+            for b in range(-(-n // m.page)):
+                g, here = m.table[r][b], min(m.page, n - b * m.page)
+                assert torch.equal(scale[g].nan_to_num(-1), m.scale[w][g].nan_to_num(-1)), (w, r, b)
+                assert torch.equal(codes[g, :, :here], m.codes[w][g, :, :here]), (w, r, b)
+
+
+def step(c, m, gen, fresh, q_heads, dtype, causal, pad=0, max_fresh=None, check=True):
+    """One step of a cache and its model: plan, append, attend, everything compared."""
+    heads, hd = c.kv_heads, c.head_dim
+    rows = sum(fresh) + pad
+    p = c.plan(i32(fresh), rows, max(fresh) if max_fresh is None else max_fresh, causal)
+    slots, owner, starts = m.plan(fresh)
+    assert p.q_start.tolist() == starts and p.kv_len.tolist() == m.length and c.length.tolist() == m.length
+    assert p.slot.tolist() == slots + [-1] * pad and p.request.tolist() == owner + [-1] * pad
+    assert c.free_count.tolist() == [len(m.free)] and c.free[:len(m.free)].tolist() == m.free
+    for r, n in enumerate(m.length):
+        b = -(-n // c.page)
+        assert c.table[r, :b].tolist() == m.table[r][:b]
+    qkv = normal(gen, rows, q_heads + 2 * heads, hd, dtype=dtype)
+    q, k, v = qkv[:, :q_heads], qkv[:, q_heads:q_heads + heads], qkv[:, q_heads + heads:]
+    c.append(0, k, v, p)
+    for w, x in ((0, k), (1, v)):
+        m.append(w, x[:sum(fresh)].double().cpu(), slots, owner)
+    same_cache(c, m)
+    out, lse = c.attend(0, q, p, lse=True)
+    p.check()
+    check_attention(m, q, out, lse, starts, heads, causal, hd ** -0.5, fresh)
+    assert not out[sum(fresh):].any() and bool((lse[sum(fresh):] == -math.inf).all())
+    return p, q, out
+
+
+# ---- steps of a cache -----------------------------------------------------------------------------------------------
+
+STEPS = [
+    # page, head_dim, kv_heads, group, dtype, causal, steps of new rows for each request
+    (16, 64, 2, 1, torch.bfloat16, True, [[1, 17, 0, 33], [1, 1, 1, 1], [0, 0, 1, 0], [1, 15, 16, 1]]),
+    (16, 128, 1, 4, torch.float16, True, [[5, 16, 100], [1, 1, 1], [2, 0, 3], [1, 1, 1]]),
+    (32, 64, 3, 2, torch.bfloat16, False, [[50, 31, 1, 64], [50, 50, 2, 7], [1, 1, 1, 1]]),
+    (64, 128, 2, 8, torch.bfloat16, True, [[130, 1], [1, 1], [65, 200], [1, 0]]),
+    (128, 64, 1, 3, torch.float16, False, [[129, 127, 128], [1, 1, 1], [40, 41, 1]]),
+    (64, 64, 8, 1, torch.bfloat16, False, [[75, 60], [50, 50], [50, 49], [50, 50], [3, 2]]),
+    (16, 64, 1, 16, torch.bfloat16, True, [[300], [1], [1], [9]]),
+    (32, 128, 1, 5, torch.float16, True, [[97, 3], [1, 1], [3, 3]]),
+    (16, 128, 1, 128, torch.bfloat16, True, [[40, 2], [1, 1]]),
+]
+
+
+@pytest.mark.parametrize("page,hd,heads,group,dtype,causal,steps", STEPS)
+def test_steps_of_a_cache(page, hd, heads, group, dtype, causal, steps):
+    n = len(steps[0])
+    blocks = max(-(-sum(s[r] for s in steps) // page) for r in range(n)) + 1
+    pages = n * blocks + 2
+    c = paged.B200PagedCache(1, pages, page, heads, hd, n, blocks * page, q_heads=heads * group)
+    # what pages hold before they are written must not matter: codes that are NaN, scales that are NaN or infinite
+    for t in (c.k, c.v):
+        t.view(torch.uint8).fill_(0x7f)
+    c.k_scale.fill_(math.nan)
+    c.v_scale.fill_(math.inf)
+    m = Model(pages, heads, page, hd, n, blocks)
+    gen = torch.Generator(device="cuda").manual_seed(page + hd + group)
+    for i, fresh in enumerate(steps):
+        step(c, m, gen, fresh, heads * group, dtype, causal, pad=i % 3)
+
+
+@pytest.mark.parametrize("lens", [[0, 0, 0], [0, 1, 2], [1, 1, 1], [15, 16, 17], [31, 32, 33], [63, 64, 65], [700, 0, 129]])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("fresh", [[1, 1, 1], [3, 0, 5], [70, 33, 130]])
+def test_rows_that_only_look(lens, causal, fresh):
+    """Without a free list the rows see what is cached: a causal row before the first key, and any row of an empty
+    request, sees nothing."""
+    page, heads, hd, group = 16, 2, 64, 2
+    c = paged.B200PagedCache(1, 160, page, heads, hd, 3, 720, q_heads=heads * group)
+    m = Model(160, heads, page, hd, 3, 45)
+    gen = torch.Generator(device="cuda").manual_seed(sum(lens))
+    if sum(lens):
+        step(c, m, gen, lens, heads * group, torch.bfloat16, False)
+    rows = sum(fresh)
+    p = paged.plan(i32(fresh), c.length, c.table, page, rows=rows, q_heads=heads * group, kv_heads=heads, head_dim=hd,
+                   causal=causal, max_fresh=max(fresh))
+    starts = [0, fresh[0], fresh[0] + fresh[1], rows]
+    assert p.kv_len.tolist() == lens and p.q_start.tolist() == starts and p.slot.tolist() == [-1] * rows
+    q = normal(gen, rows, heads * group, hd)
+    out, lse = c.attend(0, q, p, lse=True)
+    p.check()
+    check_attention(m, q, out, lse, starts, heads, causal, hd ** -0.5, fresh)
+
+
+@pytest.mark.parametrize("hd,group,fresh", [(64, 1, 1), (128, 4, 1), (128, 2, 8), (64, 2, 20), (128, 4, 64)])
+def test_a_long_history_is_split_and_joined(hd, group, fresh):
+    """One request alone over the whole GPU: its keys are split over many workers, whose parts are joined."""
+    page, heads, n = 32, 2, 6011
+    c = paged.B200PagedCache(1, 200, page, heads, hd, 1, 6400, q_heads=heads * group)
+    m = Model(200, heads, page, hd, 1, 200)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    for part in (n - fresh, fresh):
+        p = c.plan(i32([part]), part, part)
+        slots, owner, starts = m.plan([part])
+        k, v = normal(gen, part, heads, hd, dtype=torch.float16), normal(gen, part, heads, hd, dtype=torch.float16)
+        c.append(0, k, v, p)
+        m.append(0, k.double().cpu(), slots, owner)
+        m.append(1, v.double().cpu(), slots, owner)
+    same_cache(c, m)
+    q = normal(gen, fresh, heads * group, hd, dtype=torch.float16)
+    out, lse = c.attend(0, q, p, scale=0.3, lse=True)
+    p.check()
+    check_attention(m, q, out, lse, starts, heads, True, 0.3, [fresh])
+    again = c.attend(0, q, p, scale=0.3)
+    assert torch.equal(out, again)
+
+
+def test_scales_that_differ_by_page():
+    """Pages whose values differ by many powers of two, up and down: K's and V's scales follow each page."""
+    page, heads, hd, n = 16, 1, 64, 200
+    for fresh in (1, 40):
+        c = paged.B200PagedCache(1, 16, page, heads, hd, 1, 256)
+        m = Model(16, heads, page, hd, 1, 16)
+        gen = torch.Generator(device="cuda").manual_seed(fresh)
+        for part in (n, fresh):
+            p = c.plan(i32([part]), part, part)
+            slots, owner, starts = m.plan([part])
+            size = 2.0 ** ((torch.arange(part, device="cuda") // 16 * 7) % 23 - 11.0)
+            k = (torch.randn(part, heads, hd, device="cuda", generator=gen) * size[:, None, None].clamp(max=4)).to(torch.bfloat16)
+            v = (torch.randn(part, heads, hd, device="cuda", generator=gen) * size[:, None, None]).to(torch.bfloat16)
+            c.append(0, k, v, p)
+            m.append(0, k.double().cpu(), slots, owner)
+            m.append(1, v.double().cpu(), slots, owner)
+        same_cache(c, m)
+        q = normal(gen, fresh, heads, hd)
+        out, lse = c.attend(0, q, p, lse=True)
+        check_attention(m, q, out, lse, starts, heads, True, hd ** -0.5, [fresh])
+
+
+@pytest.mark.parametrize("value", [0.0, 2.0 ** -80, 448.0 * 2.0 ** -70, 1e-3, 448.0, 449.0, 3.0e38])
+def test_scale_range(value):
+    """Nothing but zeros, values under the smallest scale's range, the edge of a power of two, and over the largest."""
+    page, heads, hd = 16, 1, 64
+    c = paged.B200PagedCache(1, 4, page, heads, hd, 1, 64)
+    m = Model(4, heads, page, hd, 1, 4)
+    for n, f in ((3, value), (2, value * 0.37), (4, value)):
+        p = c.plan(i32([n]), n, n)
+        slots, owner, _ = m.plan([n])
+        x = torch.full((n, heads, hd), f, device="cuda").to(torch.bfloat16)
+        x[:, :, 1::2] *= -0.3
+        c.append(0, x, x, p)
+        for w in (0, 1):
+            m.append(w, x.double().cpu(), slots, owner)
+        same_cache(c, m)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("fresh", [1, 40])
+def test_not_finite(bad, fresh):
+    """A page and head given a value that is not finite reads as NaN: in rows that see one of its keys and in no others."""
+    page, heads, hd, group = 16, 2, 64, 2
+    for w in (0, 1):
+        c = paged.B200PagedCache(1, 16, page, heads, hd, 2, 128, q_heads=heads * group)
+        m = Model(16, heads, page, hd, 2, 8)
+        gen = torch.Generator(device="cuda").manual_seed(w)
+        for fresh_n, put in (([30, 20], None), ([fresh, fresh], (fresh - 1, 1)), ([1, 1], None)):
+            rows = sum(fresh_n)
+            p = c.plan(i32(fresh_n), rows, max(fresh_n))
+            slots, owner, starts = m.plan(fresh_n)
+            kv = [normal(gen, rows, heads, hd), normal(gen, rows, heads, hd)]
+            if put:
+                kv[w][put[0], put[1], 5] = bad  # request 0's last new row, head 1
+            c.append(0, kv[0], kv[1], p)
+            for i in (0, 1):
+                m.append(i, kv[i].double().cpu(), slots, owner)
+            same_cache(c, m)
+            q = normal(gen, rows, heads * group, hd)
+            out, lse = c.attend(0, q, p, lse=True)
+            check_attention(m, q, out, lse, starts, heads, True, hd ** -0.5, fresh_n)
+            if put:
+                assert out.isnan().any() and not out[:, :group].isnan().any() and not out[starts[1]:].isnan().any()
+
+
+def test_queries_of_any_size():
+    """bf16 queries from 2^-30 to 2^30 within a row, and scores far from zero."""
+    page, heads, hd = 32, 1, 64
+    for fresh in (1, 33):
+        c = paged.B200PagedCache(1, 8, page, heads, hd, 1, 256)
+        m = Model(8, heads, page, hd, 1, 8)
+        gen = torch.Generator(device="cuda").manual_seed(fresh)
+        for n in (100, fresh):
+            p = c.plan(i32([n]), n, n)
+            slots, owner, starts = m.plan([n])
+            k, v = normal(gen, n, heads, hd), normal(gen, n, heads, hd)
+            c.append(0, k, v, p)
+            m.append(0, k.double().cpu(), slots, owner)
+            m.append(1, v.double().cpu(), slots, owner)
+        for size in (2.0 ** -30, 2.0 ** 30):
+            q = normal(gen, fresh, heads, hd) * size
+            q[:, :, ::3] *= 2.0 ** -12
+            out, lse = c.attend(0, q, p, scale=2.0 / size, lse=True)
+            check_attention(m, q, out, lse, starts, heads, True, 2.0 / size, [fresh])
+
+
+# ---- layouts, streams, graphs ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("fresh", [1, 50])
+def test_pitches_and_far_pages(fresh):
+    """K and V pages interleaved in one pool of more than 2^31 bytes, pages at its end, a table that is a view."""
+    page, heads, hd, n = 64, 8, 128, 2
+    per = heads * page * hd
+    pages = (1 << 31) // (2 * per) + 40
+    pool = torch.zeros(pages, 2, heads, page, hd, device="cuda", dtype=torch.uint8)
+    codes = pool.view(torch.float8_e4m3fn)
+    scales = torch.ones(pages, 2, heads, device="cuda")
+    m = Model(40, heads, page, hd, n, 4)
+    big = torch.full((n, 9), -1, device="cuda", dtype=torch.int32)
+    table = big[:, 2:6]
+    free = torch.arange(pages, device="cuda", dtype=torch.int32)
+    free[:40] = torch.arange(pages - 1, pages - 41, -1, device="cuda", dtype=torch.int32)
+    count, length = i32([40]), i32([0, 0])
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for f in ([70, 64], [fresh, fresh]):
+        rows = sum(f)
+        p = paged.plan(i32(f), length, table, page, rows=rows, q_heads=heads, kv_heads=heads, head_dim=hd,
+                       max_fresh=max(f), free=free, free_count=count, kv_len=length, free_left=count)
+        slots, owner, starts = m.plan(f)
+        # the model's page g is the pool's page g + pages - 40
+        assert p.slot.tolist() == [s + (pages - 40) * page for s in slots]
+        k, v = normal(gen, rows, heads, hd), normal(gen, rows, heads, hd)
+        paged.append(k, v, codes[:, 0], codes[:, 1], scales[:, 0], scales[:, 1], p)
+        m.append(0, k.double().cpu(), slots, owner)
+        m.append(1, v.double().cpu(), slots, owner)
+        q = normal(gen, rows, heads, hd)
+        out, lse = paged.attend(q, codes[:, 0], codes[:, 1], scales[:, 0], scales[:, 1], p, lse=True)
+        p.check()
+        check_attention(m, q, out, lse, starts, heads, True, hd ** -0.5, f)
+    assert not pool[:pages - 40].any()
+    assert bool((big[:, :2] == -1).all()) and bool((big[:, 6:] == -1).all())
+
+
+@pytest.mark.parametrize("fresh", [1, 30])
+def test_graph_and_streams(fresh):
+    """A step captured on a side stream and replayed equals the same steps called one by one, bit for bit."""
+    page, heads, hd, n = 16, 2, 64, 3
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    first = [normal(gen, 60, heads, hd) for _ in range(2)]
+    feed = [[normal(gen, n * fresh, heads, hd) for _ in range(3)] for _ in range(3)]
+    start = i32([20, 17, 23])
+    counts = i32([fresh] * n)
+
+    def fill(c):
+        c.append(0, first[0], first[1], c.plan(start, 60, 23))
+
+    a = paged.B200PagedCache(1, 64, page, heads, hd, n, 256)
+    fill(a)
+    want = []
+    for q, k, v in feed:
+        p = a.plan(counts, n * fresh, fresh)
+        a.append(0, k, v, p)
+        want.append(a.attend(0, q, p, lse=True))
+    b = paged.B200PagedCache(1, 64, page, heads, hd, n, 256)
+    fill(b)
+    held_in = [torch.zeros_like(t) for t in feed[0]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        p = b.plan(counts, n * fresh, fresh)
+        b.append(0, held_in[1], held_in[2], p)
+        got = b.attend(0, held_in[0], p, lse=True)
+    for x, ref in zip(feed, want):
+        for d, s in zip(held_in, x):
+            d.copy_(s)
+        graph.replay()
+        for g, r in zip(got, ref):
+            assert torch.equal(g, r)
+    torch.cuda.synchronize()
+    assert torch.equal(a.length, b.length) and torch.equal(a.table, b.table)
+
+
+# ---- many requests, pages given back, plans that are void -------------------------------------------------------------
+
+
+@pytest.mark.parametrize("requests,page,most", [(1, 16, 9000), (300, 32, 1), (3000, 16, 7), (50, 128, 700)])
+def test_tables_of_many_requests(requests, page, most):
+    gen = torch.Generator().manual_seed(requests)
+    length = torch.randint(0, 400, (requests,), generator=gen).tolist()
+    fresh = torch.randint(0, most + 1, (requests,), generator=gen).tolist()
+    fresh[-1] = most
+    blocks = max(-(-(a + b) // page) for a, b in zip(length, fresh))
+    pages = sum(-(-(a + b) // page) for a, b in zip(length, fresh))
+    m = Model(pages, 1, page, 1, requests, blocks)
+    m.plan(length)
+    free, table, count = i32(m.free + [0] * (pages - len(m.free))), i32(m.table), i32([len(m.free)])
+    rows = sum(fresh) + 5
+    p = paged.plan(i32(fresh), i32(length), table, page, rows=rows, q_heads=2, kv_heads=1, head_dim=64, max_fresh=most,
+                   free=free, free_count=count)
+    slots, owner, starts = m.plan(fresh)
+    p.check()
+    assert p.slot.tolist() == slots + [-1] * 5 and p.request.tolist() == owner + [-1] * 5
+    assert p.q_start.tolist() == starts and p.kv_len.tolist() == m.length and p.free_left.tolist() == [len(m.free)]
+    assert table.tolist() == m.table and count.tolist() == [pages - sum(-(-a // page) for a in length)]
+
+
+def test_release_gives_pages_back_in_order():
+    c = paged.B200PagedCache(1, 12, 16, 1, 64, 4, 64)
+    p = c.plan(i32([20, 1, 33, 16]), 70, 33)
+    p.check()
+    assert c.table[:, :3].tolist() == [[0, 1, -1], [2, -1, -1], [3, 4, 5], [6, -1, -1]]
+    c.release(i32([0, 1, 1, 0]))
+    c.check()
+    assert c.free_count.tolist() == [9] and c.free[5:9].tolist() == [2, 3, 4, 5]
+    assert c.length.tolist() == [20, 0, 0, 16] and c.table[2].tolist() == [-1] * 4
+    c.plan(i32([0, 17, 0, 1]), 18, 17).check()
+    assert c.table[1, :2].tolist() == [5, 4] and c.table[3, :2].tolist() == [6, 3]
+    full = paged.B200PagedCache(1, 2, 16, 1, 64, 1, 32)
+    full.length.fill_(32)  # a table row that names pages which the free list still has
+    full.release(i32([1]))
+    with pytest.raises(L.T2WError) as e:
+        full.check()
+    assert e.value.status == -1 and full.free_count.tolist() == [2] and full.length.tolist() == [32]
+
+
+def test_void_plans():
+    """Pages used up, a table row too short, more rows than were said, lengths below zero: nothing changes, the status
+    tells, and the calls that take the plan write zeros."""
+    for fresh, rows, most, status in (([40, 33], 73, 40, -7), ([65, 0], 65, 65, -1), ([3, 2], 4, 3, -1), ([3, 2], 5, 2, -1),
+                                      ([-1, 2], 5, 3, -1)):
+        c = paged.B200PagedCache(1, 5, 16, 2, 64, 2, 64)
+        c.plan(i32([10, 1]), 11, 10).check()
+        before = [t.clone() for t in (c.table, c.length, c.free, c.free_count, c.k_scale, c.k.view(torch.uint8))]
+        p = c.plan(i32(fresh), rows, most)
+        with pytest.raises(L.T2WError) as e:
+            p.check()
+        assert e.value.status == status, fresh
+        x = torch.ones(rows, 2, 64, device="cuda", dtype=torch.bfloat16)
+        c.append(0, x, x, p)
+        out, lse = c.attend(0, x, p, lse=True)
+        assert not out.any() and bool((lse == -math.inf).all())
+        assert p.request.tolist() == [-1] * rows and p.slot.tolist() == [-1] * rows
+        for a, b in zip(before, (c.table, c.length, c.free, c.free_count, c.k_scale, c.k.view(torch.uint8))):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("fresh", [1, 40])
+def test_a_table_entry_that_is_no_page(fresh):
+    """An entry outside the pool is not followed: the status tells."""
+    c = paged.B200PagedCache(1, 16, 16, 1, 64, 1, 128)
+    x = torch.ones(40, 1, 64, device="cuda", dtype=torch.bfloat16)
+    c.append(0, x, x, c.plan(i32([40]), 40, 40))
+    p = c.plan(i32([fresh]), fresh, fresh)
+    p.check()
+    for entry in (-1, 16, 2 ** 31 - 1):
+        c.table[0, 1] = entry
+        c.attend(0, x[:fresh], p)
+        with pytest.raises(L.T2WError) as e:
+            p.check()
+        assert e.value.status == -1
+        c.table[0, 1] = 1
+        p.buffer[4] = 0
+
+
+def test_refusals():
+    def cache(**kw):
+        return paged.B200PagedCache(**{**dict(layers=1, pages=4, page=16, kv_heads=2, head_dim=64, requests=1, max_tokens=64,
+                                              q_heads=4), **kw})
+
+    for kw, status in ((dict(page=8), -1), (dict(page=48), -1), (dict(head_dim=96), -5), (dict(q_heads=3), -1),
+                       (dict(kv_heads=1, q_heads=129), -5)):
+        with pytest.raises(L.T2WError) as e:
+            cache(**kw)
+        assert e.value.status == status, kw
+    with pytest.raises(ValueError):
+        cache(pages=0)
+    c = cache()
+    with pytest.raises(RuntimeError):
+        c.plan(torch.ones(1, device="cuda", dtype=torch.int64), 1, 1)
+    with pytest.raises(RuntimeError):
+        c.plan(i32([1, 1]), 2, 1)  # two requests, and tables for one
+    with pytest.raises(RuntimeError):
+        c.plan(torch.ones(1, dtype=torch.int32), 1, 1)  # on the CPU
+    p = c.plan(i32([3]), 3, 3)
+    k = torch.ones(3, 2, 64, device="cuda", dtype=torch.bfloat16)
+    q = torch.ones(3, 4, 64, device="cuda", dtype=torch.bfloat16)
+    c.append(0, k, k, p)
+    for bad in (k[:2], k[:, :1], k.float(), k[:, :, ::2], torch.ones(3, 2, 65, device="cuda", dtype=k.dtype)[:, :, 1:],
+                torch.ones(3, 2, 68, device="cuda", dtype=k.dtype)[:, :, :64], k.cpu()):
+        with pytest.raises((RuntimeError, ValueError)):
+            c.append(0, bad, k, p)
+        with pytest.raises((RuntimeError, ValueError)):
+            c.append(0, k, bad, p)
+    for bad in (q[:2], q[:, :2], q.float(), q[:, :, :32], torch.ones(3, 4, 65, device="cuda", dtype=q.dtype)[:, :, 1:]):
+        with pytest.raises((RuntimeError, ValueError)):
+            c.attend(0, bad, p)
+    with pytest.raises((RuntimeError, ValueError)):
+        paged.attend(q, c.k[0].view(torch.uint8), c.v[0], c.k_scale[0], c.v_scale[0], p)
+    with pytest.raises((RuntimeError, ValueError)):
+        paged.attend(q, c.k[0], c.v[0], c.k_scale[0].double(), c.v_scale[0], p)
+    with pytest.raises(ValueError):
+        paged.attend(q, c.k[0].reshape(2, 2, 32, 64), c.v[0].reshape(2, 2, 32, 64), c.k_scale[0], c.v_scale[0], p)
+    with pytest.raises(L.T2WError):
+        c.attend(0, q, p, scale=math.nan)
+    # a plan made for other sizes is not taken for this one
+    with pytest.raises(RuntimeError):
+        O.call("paged_attn", q, c.k[0], c.v[0], c.k_scale[0], c.v_scale[0], c.table, p.buffer[:-4], 1, 3, True, 0.125, False)
+    none = c.plan(i32([0]), 0, 1)
+    assert c.attend(0, q[:0], none).shape == (0, 4, 64)
+    c.append(0, k[:0], k[:0], none)
+    none.check()
