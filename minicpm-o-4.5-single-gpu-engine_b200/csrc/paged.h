@@ -18,33 +18,40 @@ namespace t2w {
 constexpr int kScaleMin = -64, kScaleMax = 64;
 
 // ---------------------------------------------------------------- a plan's buffer (int32)
-// header, then q_start [B + 1], kv_len [B], slot [rows], request [rows], bases [B + 1] x 3 (new pages, runs, tiles), starts
-// int4 [workers], runs int4 [max_runs].  Every part begins on a 16-byte boundary.
+// header, then q_start [B + 1], kv_len [B], slot [rows], request [rows], bases [B + 1] x 4 (new pages, runs, places, segments), starts
+// 2 x int4 [workers], runs int4 [max_runs].  Every part begins on a 16-byte boundary.
 struct PlanHead {
   int n_runs;   // runs of rows that go into one page
-  int tiles;    // key tiles of the attention over all its segments
-  int per;      // tiles of a worker
+  int tiles;    // places of the attention's key tiles (see PagedCut)
+  int per;      // places of a worker
   int workers;  // workers that have any
   int status;   // T2W_OK, or what made the plan void
   int used;     // rows that belong to a request (the rest is padding)
   int free_left;
-  int pad;
+  int extra;    // places before each segment's first tile
 };
 struct PlanLayout {
-  int64_t q_start, kv_len, slot, request, new_base, run_base, tile_base, starts, runs, total;  // in int32
+  int64_t q_start, kv_len, slot, request, new_base, run_base, tile_base, seg_base, starts, runs, total;  // in int32
   int max_runs, max_workers;
 };
 
 // How an attention call is cut.  A segment is what one softmax runs over: (request, key head, query tile); its keys come
-// in tiles of `kt`.  The tiles of all segments, in that order, are dealt to the workers in equal contiguous shares, so
-// that ragged lengths cost no balance; a segment that is cut by a share's end is finished by k_paged_merge.
+// in tiles of `kt`.  The tiles of all segments, in that order, are numbered, and the places are dealt to the workers in
+// equal contiguous shares, so that ragged lengths cost no balance; a segment that is cut by a share's end is finished by
+// k_paged_merge.  In large calls each segment's first tile has `extra` empty places before it: what it costs a worker to
+// begin a segment, in tiles, so that a share of many short segments is not the one that the others wait for.
 struct PagedCut {
   int mma;    // 1: tcgen05 tiles of 128 query rows, a worker is a CTA; 0: at most 16 rows, a worker is a warp
   int tq;     // query tokens of a tile (rows = tokens * group)
   int kt;     // keys of a tile
   int workers;  // workers at most
-  int min_per;  // tiles of a worker at least
+  int min_per;  // places of a worker at least
+  int extra;
 };
+
+// Blocks of 4 warps that an SM holds of the kernel for few query rows.
+constexpr int few_blocks(int hd, int nq) { return hd == 128 ? 2 : (nq == 2 ? 3 : 4); }
+constexpr int few_stages = 3;  // tiles of a warp's ring (8 KB each, 4 KB where head_dim is 64): the SM's rings hold 196 KB
 
 inline int64_t round4(int64_t n) { return (n + 3) & ~int64_t(3); }
 
@@ -111,6 +118,15 @@ T2W_DEV float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); 
 T2W_DEV uint32_t e4m3x2_to_f16x2(uint32_t v) {
   uint32_t r;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)v));
+  return r;
+}
+
+// Four codes as two pairs of halves: lo of the lower two.
+T2W_DEV uint2 e4m3x4_to_f16x4(uint32_t v) {
+  uint2 r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(r.x), "=r"(r.y)
+      : "r"(v));
   return r;
 }
 

@@ -20,10 +20,641 @@ struct AttnDev {
   float scale;
   const PlanHead* head;
   const int *q_start, *kv_len, *request;
+  const int4* starts;  // two entries for each worker
+  int tq, kt, part_rows, block_workers;
+  float* ws;  // the parts of cut segments, two for each worker
   void* out;
   float* lse;
   int* status;
 };
+
+// Four columns of a finished row: O / l, and with the first columns its log-sum.
+template <bool HALF>
+T2W_DEV void store_row(const AttnDev& p, int row, int head, int hd, int d, float4 o, float M, float l) {
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  uint2 u;
+  if constexpr (HALF) {
+    const __half2 a = __floats2half2_rn(o.x * inv, o.y * inv), b = __floats2half2_rn(o.z * inv, o.w * inv);
+    u = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  } else {
+    u = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  }
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + ((size_t)row * p.q_heads + head) * hd + d) = u;
+  if (d == 0 && p.lse)
+    p.lse[(size_t)row * p.q_heads + head] = l != 0.f ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
+}
+
+// x * 2^e for |e| up to 254 without leaving the range on the way.
+T2W_DEV float scaled(float x, int e) {
+  const int a = e / 2;
+  return x * exp2i(a) * exp2i(e - a);
+}
+T2W_DEV void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+T2W_DEV uint32_t pack_f16x2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// One query row's factor for halves: the exponent shift that brings its largest magnitude into [2^14, 2^15), so that
+// bf16 rows keep all their bits over 2^28 of range as halves.  Half rows and rows that are not finite stay as they are.
+template <bool HALF>
+T2W_DEV int row_shift(uint32_t max_bits16) {
+  if (HALF || max_bits16 == 0 || max_bits16 >= 0x7f80u) return 0;
+  return 14 - ((int)(max_bits16 >> 7) - 127);
+}
+template <bool HALF>
+T2W_DEV uint32_t row_half2(uint32_t u, int shift, bool negate) {
+  if constexpr (HALF) return negate ? u ^ 0x80008000u : u;
+  const float a = scaled(__uint_as_float(u << 16), shift), b = scaled(__uint_as_float(u & 0xffff0000u), shift);
+  return negate ? pack_f16x2(-a, -b) : pack_f16x2(a, b);
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRaise = 8.f;  // the reference exponent is raised when a row's largest one passes it by more than this
+
+// A worker's unfinished rows of a segment: O [rows][HD], then the reference exponents [rows] and the sums [rows].
+T2W_DEV float* part_of(float* ws, int slot, int rows, int hd) { return ws + (size_t)slot * rows * (hd + 2); }
+
+// ---------------------------------------------------------------- at most 16 query rows to a key head
+//
+// What bounds it: the cache is read once, 2 HD bytes for each key against 4 HD flops a query row, so HBM does.  A
+// worker is one warp with a contiguous share of the key tiles (32 keys), so that nothing waits for another warp; only
+// where one segment fills the shares of a whole block do its 4 warps join what they have, so that a long history comes
+// to a quarter of the parts.
+//
+// A tile's bytes come to the warp's own ring in shared memory by asynchronous copies, one tile or two ahead across the
+// ends of segments, and from there in the tensor core's fragments.  Scores: Q is the A operand (16 rows x 16 dims; a
+// thread's four dims of a step are any four that K's fragment has in the same place, so a thread takes 16 consecutive
+// bytes of a key's row with one load), K the B operand (16 dims x 8 keys).  Output: O^T = V^T P^T, the scores'
+// accumulator layout being that of P^T as B operand; V^T as A operand wants two keys' bytes of one dim in a register,
+// which one byte permute of two rows' words gives.  So each byte is widened once (e4m3 to half, exact) and in a register.
+// The 16-byte pieces of a 128-byte line are permuted (swizzle()) so that neither K's reads (8 rows' pieces t) nor V's (4
+// rows two apart, piece g) meet in a bank.
+//
+// Exponents: key j with scales s_k, s_v of its page weighs 2^(x_j + log2 s_v - M) on its V codes, M the running maximum
+// of x_j + log2 s_v: the weights of the largest contributions have all the bits that a half has whatever the scales, and
+// what is 2^-24 of the largest contribution is lost.  The sum of exponentials is kept in units of 2^M too.
+template <int HD>
+struct FewStage {
+  uint8_t k[32 * HD], v[32 * HD];
+  float ks[2], vs[2];  // of the tile's two halves
+};
+template <int HD>
+T2W_DEV uint32_t swizzle(int row, int piece) {  // byte offset of 16-byte piece `piece` of row `row`
+  if constexpr (HD == 128) return row * 128 + ((piece ^ (((row >> 1) & 3) << 1) ^ ((row & 1) << 2)) << 4);
+  const int line = row >> 1;
+  return line * 128 + ((((row & 1) * 4 + piece) ^ ((line & 3) << 1)) << 4);
+}
+// The cache streams through L2 (evicted first), so that the plan, the tables and the parts stay there.
+T2W_DEV uint64_t l2_policy_evict_first() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+T2W_DEV void copy16(uint32_t dst, const void* src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
+}
+T2W_DEV void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+template <int HD, bool HALF, int NQ, bool P16>
+__global__ void __launch_bounds__(128, few_blocks(HD, NQ)) k_paged_few(const AttnDev p) {
+  extern __shared__ __align__(16) uint8_t ring[];
+  constexpr int kC = HD / 64, kM = HD / 16, kS = few_stages;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int w = 4 * blockIdx.x + warp, group = p.q_heads / p.kv_heads;
+  const FewStage<HD>* const stage = reinterpret_cast<const FewStage<HD>*>(ring) + warp * kS;
+  const uint32_t ring0 = smem_u32(stage);
+  const uint64_t policy = l2_policy_evict_first();
+  // this lane's places in a stage: of what it copies (even and odd 512 bytes), of K's row g piece t (the pieces of the
+  // second 64 dims are 64 bytes on or back: xor), of V's rows 2t and 2t + 1 piece g (8 bytes of it where HD is 64)
+  uint32_t put[2], get_k, get_v[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    put[i] = swizzle<HD>(i * (512 / HD) + lane / (HD / 16), lane % (HD / 16)) - i * 512;
+    get_v[i] = 32 * HD + (HD == 128 ? swizzle<HD>(2 * t + i, g) : swizzle<HD>(2 * t + i, g >> 1) + 8 * (g & 1));
+  }
+  get_k = swizzle<HD>(g, t);
+  pdl_wait();
+  pdl_launch();
+  const int4 head4 = *reinterpret_cast<const int4*>(p.head);  // n_runs, tiles, per, workers
+  int4 seg = p.starts[2 * w], of = p.starts[2 * w + 1];  // request, key head, query tile (always 0), key tile; rows, lengths
+  const int extra = p.head->extra;
+  const int4 seg0 = p.starts[8 * blockIdx.x], of0 = p.starts[8 * blockIdx.x + 1];  // the block's first worker's
+  if (w >= head4.w) return;
+  // one segment over all of the block's places (its key count is that of the few rows' only query tile)
+  const bool filled = seg0.w >= 0 && 4 * blockIdx.x + 3 < head4.w && seg_tiles(of0.z, 32) - seg0.w >= 4 * head4.z;
+  const int stop = min((w + 1) * head4.z, head4.y);
+  int zero = w * head4.z - seg.w;  // the place of the segment's tile 0
+
+  // ---- the copies, which run ahead: tiles lkt .. lkt1 - 1 of the segment with tile 0 at lzero, then the next segments'
+  int lr = seg.x, lhk = seg.y, lkt = max(seg.w, 0), lkt1 = 0, lnt = 0, lkv = 0, lzero = zero, base = -64;
+  int pgA = 0, pgB = 0;  // lane i: the pages of tile base + i
+  bool live = true;
+  auto open = [&](int kv) {
+    lkv = kv;
+    lnt = seg_tiles(lkv, 32);
+    lkt1 = min(lnt, stop - lzero);
+    base = -64;
+    live = lkt < lkt1;
+  };
+  auto send = [&](int at) {
+    if (live) {
+      if (lkt - base >= 32) {
+        base = lkt;
+        const int mine = lkt + lane;
+        if (mine < lkt1) {
+          const int b = (mine * 32) >> p.shift;
+          const int* const table = p.table + (size_t)lr * p.table_ld;
+          pgA = mine * 32 < lkv ? table[b] : 0;
+          pgB = P16 && mine * 32 + 16 < lkv ? table[b + 1] : pgA;
+          if ((unsigned)pgA >= (unsigned)p.pages || (unsigned)pgB >= (unsigned)p.pages) {
+            atomicExch(p.status, T2W_ERR_INVALID);
+            pgA = pgB = 0;
+          }
+        }
+      }
+      const uint32_t to = ring0 + at * (uint32_t)sizeof(FewStage<HD>);
+      const long long a = __shfl_sync(~0u, pgA, lkt - base), b = P16 ? (long long)__shfl_sync(~0u, pgB, lkt - base) : a;
+      const long long in = ((long long)lhk * p.page + (P16 ? 0 : (lkt * 32) & (p.page - 1))) * HD + 16 * lane;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {  // a half tile's rows lie one after the other: the warp copies 512 bytes at a time
+        const uint8_t* const lo = p.codes[x] + a * p.page_ld[x] + in;
+        const uint8_t* const hi = P16 ? p.codes[x] + b * p.page_ld[x] + in : lo + 16 * HD;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i)
+          copy16(to + x * 32 * HD + i * 512 + put[i & 1], i < HD / 32 ? lo + i * 512 : hi + (i - HD / 32) * 512, policy);
+      }
+      if (lane < 4)
+        copy4(to + 64 * HD + 4 * lane,  // ks, vs
+              p.scales[lane >> 1] + (lane & 1 ? b : a) * p.scale_ld[lane >> 1] + lhk);
+      if (++lkt == lkt1) {
+        lzero += lnt + extra;
+        if (lkt1 < lnt || lzero >= stop) {
+          live = false;
+        } else {
+          lkt = 0;
+          if (++lhk == p.kv_heads) {
+            lhk = 0;
+            do lr++;
+            while (p.q_start[lr + 1] == p.q_start[lr]);  // (tiles are left, so there is a request with rows)
+            open(p.kv_len[lr]);
+          } else {  // the same pages
+            lkt1 = min(lnt, stop - lzero);
+            if (base != 0) base = -64;
+          }
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  open(of.z);
+#pragma unroll
+  for (int i = 0; i < kS - 1; ++i) send(i);
+
+  // ---- the segments
+  int at = 0;  // the stage of the next tile
+  bool first = true;
+  while (zero < stop) {
+    const int hk = seg.y, row0 = of.x, f = of.y, kv = of.z;
+    const int rows = f * group, nt = seg_tiles(kv, 32);
+    const int kt0 = max(seg.w, 0), kt1 = min(nt, stop - zero);
+    if (kt1 <= kt0) break;
+    // queries, as halves
+    uint32_t qa[NQ][kC][4][2];
+    float c_row[NQ];
+    int end[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int row = g + 8 * n;
+      uint4 v[kC][2];
+      uint32_t m = 0;
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          v[c][i] = make_uint4(0, 0, 0, 0);
+          if (row < rows) {
+            const uint16_t* q = static_cast<const uint16_t*>(p.q) + (row0 + row / group) * p.q_row_ld +
+                                (hk * group + row % group) * p.q_head_ld;
+            v[c][i] = __ldg(reinterpret_cast<const uint4*>(q + 64 * c + 16 * t + 8 * i));
+          }
+          const uint4 u = v[c][i];
+          m = __vmaxu2(__vmaxu2(m, u.x & 0x7fff7fffu), u.y & 0x7fff7fffu);
+          m = __vmaxu2(__vmaxu2(m, u.z & 0x7fff7fffu), u.w & 0x7fff7fffu);
+        }
+      m = max(m & 0xffffu, m >> 16);
+      m = max(m, __shfl_xor_sync(~0u, m, 1));
+      m = max(m, __shfl_xor_sync(~0u, m, 2));
+      const int sh = row_shift<HALF>(m);
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        const uint32_t u[8] = {v[c][0].x, v[c][0].y, v[c][0].z, v[c][0].w, v[c][1].x, v[c][1].y, v[c][1].z, v[c][1].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) qa[n][c][j][i] = row_half2<HALF>(u[2 * j + i], sh, p.scale < 0.f);
+      }
+      c_row[n] = scaled(fabsf(p.scale) * kLog2e, -sh);
+      end[n] = p.causal ? kv - f + row / group + 1 : kv;
+    }
+    const int all_see = p.causal ? kv - f + 1 : kv;  // keys that every row sees
+    float M[NQ], l[NQ], o[NQ][kM][4];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      M[n] = -INFINITY;
+      l[n] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kM; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    }
+    for (int kt = kt0; kt < kt1; ++kt) {
+      __syncwarp();  // every lane is done with the stage that is filled again
+      send(at ? at - 1 : kS - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kS - 1) : "memory");
+      __syncwarp();
+      const FewStage<HD>& st = stage[at];
+      const uint8_t* const bytes = st.k;
+      at = at + 1 == kS ? 0 : at + 1;
+      float d[4][4] = {};
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        uint4 kr[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kr[j] = *reinterpret_cast<const uint4*>(bytes + 8 * HD * j + (get_k ^ (64 * c)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint2 u = e4m3x4_to_f16x4(i == 0 ? kr[j].x : i == 1 ? kr[j].y : i == 2 ? kr[j].z : kr[j].w);
+            mma_f16(d[j], qa[0][c][i][0], NQ == 2 ? qa[NQ - 1][c][i][0] : 0u, qa[0][c][i][1], NQ == 2 ? qa[NQ - 1][c][i][1] : 0u,
+                    u.x, u.y);
+          }
+      }
+      const int kb = kt * 32;
+      constexpr int kH = P16 ? 2 : 1;  // pages of the tile
+      float lv[kH], unit[kH];
+      bool vbad = false;
+#pragma unroll
+      for (int i = 0; i < kH; ++i) {
+        const int e = (int)(__float_as_uint(st.vs[i]) >> 23) - 127;
+        const bool bad = !(st.vs[i] < INFINITY);
+        vbad |= bad;
+        lv[i] = bad ? 0.f : (float)e;
+        unit[i] = exp2i(bad ? 0 : -e);
+      }
+      const bool part = kb + 32 > all_see;  // some row does not see all of the tile
+      uint32_t pw[NQ][4];
+      bool raise[NQ];
+      float fac[NQ];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        float x[4][2], ck[kH];
+#pragma unroll
+        for (int i = 0; i < kH; ++i) ck[i] = c_row[n] * st.ks[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) x[j][i] = fmaf(d[j][2 * n + i], ck[P16 ? j >> 1 : 0], lv[P16 ? j >> 1 : 0]);
+        if (part) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (kb + 8 * j + 2 * t + i >= end[n]) x[j][i] = -INFINITY;
+        }
+        float mx = fmax3(fmax3(x[0][0], x[0][1], x[1][0]), fmax3(x[1][1], x[2][0], x[2][1]), fmaxf(x[3][0], x[3][1]));
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+        raise[n] = mx > M[n] + kRaise;
+        const float m_new = raise[n] ? mx : M[n];
+        fac[n] = raise[n] ? exp2_approx(M[n] - m_new) : 1.f;  // 2^-inf = 0 the first time
+        M[n] = m_new;
+        const float ref = m_new == -INFINITY ? 0.f : m_new;
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float e0 = exp2_approx(x[j][0] - ref), e1 = exp2_approx(x[j][1] - ref);
+          sum[j >> 1] += e0 + e1;
+          pw[n][j] = pack_f16x2(e0, e1);
+        }
+        // the exponentials without their values' scale: 2^(x - M) = w 2^-lv
+        l[n] *= fac[n];
+        if constexpr (P16) l[n] = fmaf(sum[0], unit[0], fmaf(sum[1], unit[kH - 1], l[n]));
+        else l[n] = fmaf(sum[0] + sum[1], unit[0], l[n]);
+        if (vbad) {  // values that are NaN, where the row sees them
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (!(st.vs[P16 ? j >> 1 : 0] < INFINITY)) {
+              if (x[j][0] > -INFINITY) pw[n][j] |= 0x7fffu;
+              if (x[j][1] > -INFINITY) pw[n][j] |= 0x7fff0000u;
+            }
+        }
+      }
+      if (__any_sync(~0u, raise[0] || (NQ == 2 && raise[NQ - 1]))) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {  // the factors lie with the rows, the output has them as columns 2t, 2t + 1
+          const float f0 = __shfl_sync(~0u, fac[n], 8 * t), f1 = __shfl_sync(~0u, fac[n], 8 * t + 4);
+#pragma unroll
+          for (int i = 0; i < kM; ++i) {
+            o[n][i][0] *= f0;
+            o[n][i][1] *= f1;
+            o[n][i][2] *= f0;
+            o[n][i][3] *= f1;
+          }
+        }
+      }
+      const bool tail = kb + 32 > kv;  // places of the page past the last key may hold anything, NaN codes too
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t vw[4][HD / 32];  // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the half
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint8_t* const q = bytes + (16 * i + 8 * (j >> 1)) * HD + get_v[j & 1];
+          if constexpr (HD == 128) {
+            const uint4 u = *reinterpret_cast<const uint4*>(q);
+            vw[j][0] = u.x;
+            vw[j][1] = u.y;
+            vw[j][HD / 32 - 2] = u.z;
+            vw[j][HD / 32 - 1] = u.w;
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(q);
+            vw[j][0] = u.x;
+            vw[j][1] = u.y;
+          }
+        }
+        if (tail) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (kb + 16 * i + 2 * t + (j & 1) + 8 * (j >> 1) >= kv)
+#pragma unroll
+              for (int x = 0; x < HD / 32; ++x) vw[j][x] = 0;
+        }
+#pragma unroll
+        for (int x = 0; x < HD / 32; ++x)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint2 lo = e4m3x4_to_f16x4(__byte_perm(vw[0][x], vw[1][x], y ? 0x7362 : 0x5140));
+            const uint2 hi = e4m3x4_to_f16x4(__byte_perm(vw[2][x], vw[3][x], y ? 0x7362 : 0x5140));
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) mma_f16(o[n][2 * x + y], lo.x, lo.y, hi.x, hi.y, pw[n][2 * i], pw[n][2 * i + 1]);
+          }
+      }
+    }
+    // this thread's columns of queries 2t and 2t + 1: HD / 8 in a row
+    const bool whole = kt0 == 0 && kt1 == nt;
+    float* const part = filled ? reinterpret_cast<float*>(ring + warp * kS * sizeof(FewStage<HD>))
+                               : part_of(p.ws, 2 * w + (first ? 0 : 1), 16, HD);
+    if (filled) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();  // the warp's ring is read to the end
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      float sum = l[n];
+      sum += __shfl_xor_sync(~0u, sum, 1);
+      sum += __shfl_xor_sync(~0u, sum, 2);
+      const float top = sum != sum ? fmaxf(M[n], -1e30f) : M[n];  // a NaN counts, even where M saw nothing else
+      if (!whole && t == 0 && 8 * n + g < rows) {
+        part[16 * HD + 8 * n + g] = top;
+        part[16 * HD + 16 + 8 * n + g] = sum;
+      }
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int row = 8 * n + 2 * t + y;
+        const float ls = __shfl_sync(~0u, sum, 8 * t + 4 * y), Ms = __shfl_sync(~0u, top, 8 * t + 4 * y);
+        if (row >= rows) continue;
+#pragma unroll
+        for (int i = 0; i < kM; i += 2) {
+          const int d = g * (HD / 8) + 2 * i;
+          const float4 v = make_float4(o[n][i][y], o[n][i][2 + y], o[n][i + 1][y], o[n][i + 1][2 + y]);
+          if (whole) store_row<HALF>(p, row0 + row / group, hk * group + row % group, HD, d, v, Ms, ls);
+          else *reinterpret_cast<float4*>(part + row * HD + d) = v;
+        }
+      }
+    }
+    if (filled) {  // all four warps come here, each with its one segment
+      __syncthreads();
+      float* const out = part_of(p.ws, 2 * (4 * blockIdx.x), 16, HD);
+      const float* const in = reinterpret_cast<const float*>(ring);
+      constexpr int kLd = kS * (int)sizeof(FewStage<HD>) / 4;
+      for (int i = threadIdx.x; i < rows * (HD / 4); i += 128) {
+        const int row = i / (HD / 4), d = i % (HD / 4) * 4;
+        float m[4], top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          m[x] = in[x * kLd + 16 * HD + row];
+          top = fmaxf(top, m[x]);
+        }
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (top > -INFINITY) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float e = exp2_approx(m[x] - top);
+            const float4 v = *reinterpret_cast<const float4*>(in + x * kLd + row * HD + d);
+            acc.x = fmaf(e, v.x, acc.x);
+            acc.y = fmaf(e, v.y, acc.y);
+            acc.z = fmaf(e, v.z, acc.z);
+            acc.w = fmaf(e, v.w, acc.w);
+            sum = fmaf(e, in[x * kLd + 16 * HD + 16 + row], sum);
+          }
+        }
+        *reinterpret_cast<float4*>(out + row * HD + d) = acc;
+        if (d == 0) {
+          out[16 * HD + row] = top;
+          out[16 * HD + 16 + row] = sum;
+        }
+      }
+      return;
+    }
+    first = false;
+    zero += nt + extra;
+    seg.w = 0;
+    if (++seg.y == p.kv_heads && zero < stop) {
+      seg.y = 0;
+      do {
+        seg.x++;
+        of.x = p.q_start[seg.x];
+        of.y = p.q_start[seg.x + 1] - of.x;
+      } while (of.y == 0);
+      of.z = p.kv_len[seg.x];
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// ---------------------------------------------------------------- segments that were cut
+// Where worker w's start is the first cut of a segment, one warp for each row joins the parts of that segment; where
+// there are many of them, the whole block, its warps taking every 4th part.  The order is fixed, so the bits are too.
+// A block looks after 8 workers' starts, and rows blockIdx.y, + gridDim.y, ...  What it costs is a chain of loads after
+// the kernel in front of it has ended: so all that the plan tells is read before that, and the parts' rows are sent for
+// together with their exponents.
+struct Parts {
+  const float* ws;
+  int rows_ld, hd;
+  int w0, second;     // the first part's worker, and whether it is that worker's second
+  int lead, mid, b0;  // parts of single workers, of blocks (from block b0, block_workers each), and of single workers again
+  int block_workers, tail0, n;
+  T2W_DEV const float* at(int i) const {
+    const int slot = i == 0 && lead ? 2 * w0 + second
+                     : i < lead     ? 2 * (w0 + i)
+                     : i < lead + mid ? 2 * block_workers * (b0 + i - lead)
+                                      : 2 * (tail0 + i - lead - mid);
+    return ws + (size_t)slot * rows_ld * (hd + 2);
+  }
+};
+template <int HD>
+struct Joined {
+  static constexpr int N = HD / 32;
+  float acc[N], sum, top;
+};
+template <int N>
+T2W_DEV void load_cols(float (&u)[N], const float* v) {
+  if constexpr (N == 4) *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(v);
+  else *reinterpret_cast<float2*>(u) = *reinterpret_cast<const float2*>(v);
+}
+// Parts from, from + step, ... of a row: a lane holds one part's exponent and sum of 32, and N columns of all of them.
+template <int HD>
+T2W_DEV void join_parts(Joined<HD>& j, const Parts& parts, int from, int step, int row, int lane) {
+  constexpr int N = HD / 32, K = 4;
+  j.top = -INFINITY;
+  j.sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) j.acc[i] = 0.f;
+  for (int x0 = from; x0 < parts.n; x0 += 32 * step) {
+    const int n = min(32, (parts.n - x0 + step - 1) / step);
+    float top = -INFINITY, sum = 0.f;
+    if (lane < n) {
+      const float* q = parts.at(x0 + lane * step) + parts.rows_ld * HD + row;
+      top = __ldcg(q);
+      sum = __ldcg(q + parts.rows_ld);
+    }
+    float m = 0.f, e = 0.f;
+    for (int i0 = 0; i0 < n; i0 += K) {
+      float u[K][N];
+#pragma unroll
+      for (int i = 0; i < K; ++i) {
+#pragma unroll
+        for (int y = 0; y < N; ++y) u[i][y] = 0.f;
+        if (i0 + i < n) load_cols<N>(u[i], parts.at(x0 + (i0 + i) * step) + row * HD + lane * N);
+      }
+      if (i0 == 0) {
+        m = fmaxf(j.top, top);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+        const float ref = m == -INFINITY ? 0.f : m, old = exp2_approx(j.top - ref);
+        e = exp2_approx(top - ref);
+        j.top = m;
+        j.sum = fmaf(j.sum, old, warp_sum(lane < n ? e * sum : 0.f));
+#pragma unroll
+        for (int i = 0; i < N; ++i) j.acc[i] *= old;
+      }
+#pragma unroll
+      for (int i = 0; i < K; ++i) {
+        const float ei = __shfl_sync(~0u, e, i0 + i);
+#pragma unroll
+        for (int y = 0; y < N; ++y) j.acc[y] = fmaf(ei, u[i][y], j.acc[y]);
+      }
+    }
+  }
+}
+template <int HD, bool HALF>
+T2W_DEV void store_joined(const AttnDev& p, const Joined<HD>& j, int row, int head, int lane) {
+  if constexpr (HD == 128) {
+    store_row<HALF>(p, row, head, HD, lane * 4, make_float4(j.acc[0], j.acc[1], j.acc[2], j.acc[3]), j.top, j.sum);
+  } else {
+    const float c = __shfl_down_sync(~0u, j.acc[0], 1), d = __shfl_down_sync(~0u, j.acc[1], 1);
+    if ((lane & 1) == 0) store_row<HALF>(p, row, head, HD, lane * 2, make_float4(j.acc[0], j.acc[1], c, d), j.top, j.sum);
+  }
+}
+
+constexpr int kMany = 24;  // parts from which the whole block joins a row
+
+template <int HD, bool HALF>
+__global__ void __launch_bounds__(128, 8) k_paged_merge(const AttnDev p) {
+  __shared__ Joined<HD> js[4][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = p.q_heads / p.kv_heads;
+  // The plan was complete before the kernel in front of this one began (it waited for it), so it is read ahead of the
+  // wait, past this SM's L1.
+  const int4 h0 = __ldcg(reinterpret_cast<const int4*>(p.head)), h1 = __ldcg(reinterpret_cast<const int4*>(p.head) + 1);
+  const int per = h0.z, workers = h0.w, used = h1.y, extra = h1.w;
+  const int w = blockIdx.x * 8 + lane;
+  int4 seg = make_int4(0, 0, 0, 0);
+  int a = 0, nt = 0, row0 = 0, rows = 0;
+  bool mine = false;
+  if (lane < 8 && w > 0 && w < workers) {
+    seg = __ldcg(p.starts + 2 * w);
+    const int4 of = __ldcg(p.starts + 2 * w + 1);  // first row, rows, keys
+    a = w * per - seg.w;  // the place of the segment's tile 0
+    mine = seg.w > 0 && a >= (w - 1) * per;
+    nt = seg_tiles(tile_keys(of.y, of.z, p.causal, p.tq, seg.z), p.kt);
+    row0 = of.x + seg.z * p.tq;
+    rows = min(p.tq, of.y - seg.z * p.tq) * group;
+  }
+  unsigned todo = __ballot_sync(~0u, mine);
+  int turn = 0;
+  pdl_wait();
+  pdl_launch();
+  // padding
+  for (int row = used + blockIdx.y * gridDim.x + blockIdx.x; row < p.rows; row += gridDim.x * gridDim.y)
+    for (int i = threadIdx.x; i < p.q_heads * (HD / 4); i += blockDim.x)
+      store_row<HALF>(p, row, i / (HD / 4), HD, i % (HD / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
+  while (todo) {
+    const int i = __ffs(todo) - 1;
+    todo &= todo - 1;
+    const int r0 = __shfl_sync(~0u, row0, i), rn = __shfl_sync(~0u, rows, i), hk = __shfl_sync(~0u, seg.y, i);
+    const int at = __shfl_sync(~0u, a, i), end = at + __shfl_sync(~0u, nt, i);
+    Parts parts;
+    parts.ws = p.ws;
+    parts.rows_ld = p.part_rows;
+    parts.hd = HD;
+    parts.w0 = blockIdx.x * 8 + i - 1;
+    parts.second = at - extra > parts.w0 * per;
+    const int last = (end - 1) / per, bw = p.block_workers;
+    const int b0 = (at + bw * per - 1) / (bw * per), b1 = end / (bw * per);  // blocks that the segment fills
+    parts.block_workers = bw;
+    parts.b0 = b0;
+    parts.mid = bw > 1 && b1 > b0 ? b1 - b0 : 0;
+    parts.lead = parts.mid ? b0 * bw - parts.w0 : last - parts.w0 + 1;
+    parts.tail0 = b1 * bw;
+    parts.n = parts.mid ? parts.lead + parts.mid + last - b1 * bw + 1 : parts.lead;
+    for (int row = blockIdx.y; row < rn; row += gridDim.y) {
+      const int out_row = r0 + row / group, head = hk * group + row % group;
+      Joined<HD> j;
+      if (parts.n < kMany) {
+        if ((turn++ & 3) != warp) continue;
+        join_parts<HD>(j, parts, 0, 1, row, lane);
+        store_joined<HD, HALF>(p, j, out_row, head, lane);
+      } else {
+        join_parts<HD>(j, parts, warp, 4, row, lane);
+        js[warp][lane] = j;
+        __syncthreads();
+        if (warp == 0) {
+          float top = j.top;
+#pragma unroll
+          for (int x = 1; x < 4; ++x) top = fmaxf(top, js[x][0].top);
+          Joined<HD> s = {};
+          s.top = top;
+          if (top > -INFINITY)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const Joined<HD>& u = js[x][lane];
+              const float e = exp2_approx(u.top - top);
+              s.sum = fmaf(e, u.sum, s.sum);
+#pragma unroll
+              for (int y = 0; y < HD / 32; ++y) s.acc[y] = fmaf(e, u.acc[y], s.acc[y]);
+            }
+          store_joined<HD, HALF>(p, s, out_row, head, lane);
+        }
+        __syncthreads();
+      }
+    }
+  }
+}
 
 template <bool HALF>
 T2W_DEV float load16(const uint16_t* p) {
@@ -108,12 +739,32 @@ __global__ void __launch_bounds__(128) k_paged_rows(const AttnDev p) {
 
 using namespace t2w;
 
+namespace {
+
+template <int HD, bool HALF>
+cudaError_t launch_paged(const AttnDev& p, const PagedCut& cut, int max_rows, cudaStream_t st) {
+  if (cut.mma)
+    return launch_k(k_paged_rows<HD, HALF>, dim3((unsigned)(((long long)p.rows * p.q_heads + 3) / 4)), dim3(128), 0, st, p);
+  const int nq = max_rows > 8 ? 2 : 1;
+  constexpr int smem = 4 * few_stages * (int)sizeof(FewStage<HD>);
+  static std::atomic<uint64_t> done[4];
+  auto few = [&](auto* k, std::atomic<uint64_t>& d) {
+    const cudaError_t r = smem_attr_once(k, smem, d);
+    return r != cudaSuccess ? r : launch_k(k, dim3(cut.workers / 4), dim3(128), smem, st, p);
+  };
+  cudaError_t e;
+  if (p.page == 16) e = nq == 1 ? few(k_paged_few<HD, HALF, 1, true>, done[0]) : few(k_paged_few<HD, HALF, 2, true>, done[1]);
+  else e = nq == 1 ? few(k_paged_few<HD, HALF, 1, false>, done[2]) : few(k_paged_few<HD, HALF, 2, false>, done[3]);
+  if (e != cudaSuccess) return e;
+  return launch_k(k_paged_merge<HD, HALF>, dim3((cut.workers + 7) / 8, max_rows), dim3(128), 0, st, p);
+}
+
+}  // namespace
+
 extern "C" size_t t2w_paged_workspace_bytes(int32_t max_fresh, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
-  (void)max_fresh;
-  (void)q_heads;
-  (void)kv_heads;
-  (void)head_dim;
-  return 16;
+  if (max_fresh <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
+  const PagedCut c = paged_cut(max_fresh, q_heads, kv_heads, head_dim);
+  return 2 * (size_t)c.workers * 16 * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int t2w_paged_attn(const t2w_paged_attn_args* a, void* stream) {
@@ -143,8 +794,11 @@ extern "C" int t2w_paged_attn(const t2w_paged_attn_args* a, void* stream) {
   if ((reinterpret_cast<uintptr_t>(a->q) & 15) || a->q_row_ld % 8 || a->q_head_ld % 8 ||
       (reinterpret_cast<uintptr_t>(a->out) & 15))
     return T2W_ERR_INVALID;
-  const PlanLayout l = paged_layout(a->requests, a->rows, a->page,
-                                    paged_cut(a->max_fresh, a->q_heads, a->kv_heads, a->head_dim));
+  if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 15)) return T2W_ERR_INVALID;
+  if (a->workspace_bytes < t2w_paged_workspace_bytes(a->max_fresh, a->q_heads, a->kv_heads, a->head_dim))
+    return T2W_ERR_WORKSPACE;
+  const PagedCut cut = paged_cut(a->max_fresh, a->q_heads, a->kv_heads, a->head_dim);
+  const PlanLayout l = paged_layout(a->requests, a->rows, a->page, cut);
   p.table = a->table;
   p.table_ld = a->table_ld;
   p.page = a->page;
@@ -159,16 +813,22 @@ extern "C" int t2w_paged_attn(const t2w_paged_attn_args* a, void* stream) {
   p.q_start = a->plan + l.q_start;
   p.kv_len = a->plan + l.kv_len;
   p.request = a->plan + l.request;
+  p.starts = reinterpret_cast<const int4*>(a->plan + l.starts);
+  p.tq = cut.tq;
+  p.kt = cut.kt;
+  p.part_rows = 16;
+  p.block_workers = 4;
+  p.ws = static_cast<float*>(a->workspace);
   p.out = a->out;
   p.lse = a->lse;
   p.status = const_cast<int*>(&p.head->status);
   if (a->rows == 0) return T2W_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)(((long long)a->rows * a->q_heads + 3) / 4));
   const bool half = a->dtype == T2W_DT_FP16;
+  const int max_rows = a->max_fresh * (a->q_heads / a->kv_heads);
   cudaError_t e;
-  if (a->head_dim == 64) e = half ? launch_k(k_paged_rows<64, true>, grid, dim3(128), 0, st, p) : launch_k(k_paged_rows<64, false>, grid, dim3(128), 0, st, p);
-  else e = half ? launch_k(k_paged_rows<128, true>, grid, dim3(128), 0, st, p) : launch_k(k_paged_rows<128, false>, grid, dim3(128), 0, st, p);
+  if (a->head_dim == 64) e = half ? launch_paged<64, true>(p, cut, max_rows, st) : launch_paged<64, false>(p, cut, max_rows, st);
+  else e = half ? launch_paged<128, true>(p, cut, max_rows, st) : launch_paged<128, false>(p, cut, max_rows, st);
   if (e != cudaSuccess) {
     set_cuda_error(e);
     return T2W_ERR_CUDA;

@@ -14,15 +14,14 @@
 namespace t2w {
 
 PagedCut paged_cut(int max_fresh, int q_heads, int kv_heads, int head_dim) {
-  const int group = q_heads / kv_heads;
+  const int rows = max_fresh * (q_heads / kv_heads);
   PagedCut c;
-  c.mma = 0;
-  (void)head_dim;
+  c.mma = max_fresh > 16 || rows > 16;
   c.tq = max_fresh;
   c.kt = 32;
-  c.workers = 16 * num_sms();
+  c.workers = 4 * few_blocks(head_dim, rows > 8 ? 2 : 1) * num_sms();
   c.min_per = 2;
-  (void)group;
+  c.extra = 4;
   return c;
 }
 
@@ -44,7 +43,8 @@ PlanLayout paged_layout(int64_t requests, int64_t rows, int page, const PagedCut
   l.new_base = take(requests + 1);
   l.run_base = take(requests + 1);
   l.tile_base = take(requests + 1);
-  l.starts = take(4 * (int64_t)l.max_workers);
+  l.seg_base = take(requests + 1);
+  l.starts = take(8 * (int64_t)l.max_workers);
   l.runs = take(4 * (int64_t)l.max_runs);
   l.total = at;
   return l;
@@ -68,14 +68,14 @@ struct PlanDev {
 };
 
 struct Sums {
-  long long rows, pages, runs, tiles;
+  long long rows, pages, runs, tiles, segs;
 };
 T2W_DEV Sums add(const Sums& a, const Sums& b) {
-  return Sums{a.rows + b.rows, a.pages + b.pages, a.runs + b.runs, a.tiles + b.tiles};
+  return Sums{a.rows + b.rows, a.pages + b.pages, a.runs + b.runs, a.tiles + b.tiles, a.segs + b.segs};
 }
 T2W_DEV Sums shfl_up(const Sums& s, int d) {
   return Sums{__shfl_up_sync(~0u, s.rows, d), __shfl_up_sync(~0u, s.pages, d), __shfl_up_sync(~0u, s.runs, d),
-              __shfl_up_sync(~0u, s.tiles, d)};
+              __shfl_up_sync(~0u, s.tiles, d), __shfl_up_sync(~0u, s.segs, d)};
 }
 
 // Pages of n tokens.
@@ -83,7 +83,7 @@ T2W_DEV int pages_of(int n, int shift) { return (int)(((long long)n + (1 << shif
 
 // What request r adds to each sum; false where its lengths are not to be used.
 T2W_DEV bool of_request(const PlanDev& p, int f, int len, Sums& s) {
-  s = Sums{0, 0, 0, 0};
+  s = Sums{0, 0, 0, 0, 0};
   if (f < 0 || len < 0 || f > p.max_fresh || (p.free_pages && (long long)len + f > 0x7fffffffLL)) return false;
   const int kv = p.free_pages ? len + f : len;
   if (pages_of(kv, p.shift) > p.max_blocks) return false;
@@ -92,7 +92,11 @@ T2W_DEV bool of_request(const PlanDev& p, int f, int len, Sums& s) {
     s.pages = pages_of(kv, p.shift) - pages_of(len, p.shift);
     s.runs = pages_of(kv, p.shift) - (len >> p.shift);
   }
-  if (f > 0) s.tiles = p.kv_heads * tiles_before(f, kv, p.causal, p.cut.tq, p.cut.kt, (f + p.cut.tq - 1) / p.cut.tq);
+  if (f > 0) {
+    const int nq = (f + p.cut.tq - 1) / p.cut.tq;
+    s.tiles = p.kv_heads * tiles_before(f, kv, p.causal, p.cut.tq, p.cut.kt, nq);
+    s.segs = (long long)p.kv_heads * nq;
+  }
   return true;
 }
 
@@ -150,13 +154,13 @@ T2W_DEV void scatter(const PlanDev& p, const int* q_start, const int* new_base, 
   }
 }
 
-constexpr int kHeld = 2048;  // requests whose sums fit the block's shared memory
+constexpr int kHeld = 1536;  // requests whose sums fit the block's shared memory
 
 __global__ void __launch_bounds__(1024) k_plan(const PlanDev p) {
   __shared__ Sums warp_sum[32];
   __shared__ Sums carry_s;
   __shared__ int bad_s;
-  __shared__ int held[5][kHeld + 1];
+  __shared__ int held[6][kHeld + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5, n = p.requests;
   pdl_wait();
   pdl_launch();
@@ -165,11 +169,12 @@ __global__ void __launch_bounds__(1024) k_plan(const PlanDev p) {
   int* const new_base = n <= kHeld ? held[1] : p.buf + p.lay.new_base;
   int* const run_base = n <= kHeld ? held[2] : p.buf + p.lay.run_base;
   int* const tile_base = n <= kHeld ? held[4] : p.buf + p.lay.tile_base;
+  int* const seg_base = n <= kHeld ? held[5] : p.buf + p.lay.seg_base;
   int* const kv_len = n <= kHeld ? held[3] : p.buf + p.lay.kv_len;
   const int free_n = p.free_pages ? *p.free_count : 0;
   if (tid == 0) {
     bad_s = 0;
-    carry_s = Sums{0, 0, 0, 0};
+    carry_s = Sums{0, 0, 0, 0, 0};
   }
   __syncthreads();
   // the sums, and whether the step can be had at all: a plan is made whole or not at all
@@ -192,7 +197,7 @@ __global__ void __launch_bounds__(1024) k_plan(const PlanDev p) {
     if (lane == 31) warp_sum[warp] = inc;
     __syncthreads();
     if (warp == 0) {
-      Sums w = lane < warps ? warp_sum[lane] : Sums{0, 0, 0, 0};
+      Sums w = lane < warps ? warp_sum[lane] : Sums{0, 0, 0, 0, 0};
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const Sums o = shfl_up(w, d);
@@ -208,6 +213,7 @@ __global__ void __launch_bounds__(1024) k_plan(const PlanDev p) {
       new_base[r] = (int)min(base.pages + inc.pages - mine.pages, 0x7fffffffLL);
       run_base[r] = (int)min(base.runs + inc.runs - mine.runs, 0x7fffffffLL);
       tile_base[r] = (int)min(base.tiles + inc.tiles - mine.tiles, 0x7fffffffLL);
+      seg_base[r] = (int)min(base.segs + inc.segs - mine.segs, 0x7fffffffLL);
       kv_len[r] = p.free_pages ? len + f : len;
     }
     __syncthreads();
@@ -216,17 +222,22 @@ __global__ void __launch_bounds__(1024) k_plan(const PlanDev p) {
   }
   total = carry_s;
   int status = T2W_OK;
+  // a call with little for a worker to do has no empty places: its shares are short, and every start counts the same
+  const int extra = total.tiles >= 8LL * p.cut.workers ? p.cut.extra : 0;
+  total.tiles += extra * total.segs;
   if (bad_s || total.rows > p.rows || total.tiles > 0x7fffffffLL) status = T2W_ERR_INVALID;
   else if (p.free_pages && (free_n < 0 || free_n > p.pages)) status = T2W_ERR_INVALID;
   else if (p.free_pages && total.pages > free_n) status = T2W_ERR_EXHAUSTED;
   __syncthreads();
   if (status != T2W_OK) {  // void: no rows, no pages, the lengths as they were
-    total = Sums{0, 0, 0, 0};
+    total = Sums{0, 0, 0, 0, 0};
     for (int r = tid; r < n; r += blockDim.x) {
-      q_start[r] = new_base[r] = run_base[r] = tile_base[r] = 0;
+      q_start[r] = new_base[r] = run_base[r] = tile_base[r] = seg_base[r] = 0;
       kv_len[r] = p.length[r];
     }
   }
+  if (extra)
+    for (int r = tid; r < n; r += blockDim.x) tile_base[r] += extra * seg_base[r];
   const int n_rows = (int)total.rows, n_pages = (int)total.pages, n_runs = (int)total.runs, tiles = (int)total.tiles;
   const int per = max((int)(((long long)tiles + p.cut.workers - 1) / p.cut.workers), p.cut.min_per);
   const int workers = tiles ? (int)(((long long)tiles + per - 1) / per) : 0;
@@ -235,7 +246,7 @@ __global__ void __launch_bounds__(1024) k_plan(const PlanDev p) {
     new_base[n] = n_pages;
     run_base[n] = n_runs;
     tile_base[n] = tiles;
-    *head = PlanHead{n_runs, tiles, per, workers, status, n_rows, free_n - n_pages, 0};
+    *head = PlanHead{n_runs, tiles, per, workers, status, n_rows, free_n - n_pages, extra};
   }
   __syncthreads();
   if (n <= kHeld) {
@@ -250,15 +261,19 @@ __global__ void __launch_bounds__(1024) k_plan(const PlanDev p) {
   for (int w = tid; w < workers; w += blockDim.x) {
     const int r = find(tile_base, n, w * per);
     const int f = q_start[r + 1] - q_start[r], kv = kv_len[r], nq = (f + p.cut.tq - 1) / p.cut.tq;
-    const int one = (tile_base[r + 1] - tile_base[r]) / p.kv_heads;  // tiles of one key head
+    const int one = (tile_base[r + 1] - tile_base[r]) / p.kv_heads;  // places of one key head
     const int rem = w * per - tile_base[r], hk = rem / one, in = rem - hk * one;
-    int lo = 0, hi = nq;  // the query tile: the last x with tiles_before(x) <= in
+    auto before = [&](int x) { return (int)tiles_before(f, kv, p.causal, p.cut.tq, p.cut.kt, x) + x * extra; };
+    int lo = 0, hi = nq;  // the query tile: the last x with before(x) <= in
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (tiles_before(f, kv, p.causal, p.cut.tq, p.cut.kt, mid) <= in) lo = mid; else hi = mid;
+      if (before(mid) <= in) lo = mid; else hi = mid;
     }
-    reinterpret_cast<int4*>(p.buf + p.lay.starts)[w] =
-        make_int4(r, hk, lo, in - (int)tiles_before(f, kv, p.causal, p.cut.tq, p.cut.kt, lo));
+    // request, key head, query tile and key tile (below 0 where the share begins with empty places); then what a worker
+    // would look up for that request
+    int4* const start = reinterpret_cast<int4*>(p.buf + p.lay.starts) + 2 * w;
+    start[0] = make_int4(r, hk, lo, in - before(lo) - extra);
+    start[1] = make_int4(q_start[r], f, kv, 0);
   }
   if (!p.scattered)
     scatter(p, q_start, new_base, run_base, kv_len, n_rows, n_pages, n_runs, free_n, tid, blockDim.x);
