@@ -4,81 +4,16 @@
 // request's key count, or where the call is causal the count less the queries behind i; x_j = scale q . k_j, and
 // o = sum_j 2^(c x_j - m) v_j / sum_j 2^(c x_j - m), c = log2 e, with the running maximum m of one pass over the keys.
 // A row that sees no key gives zeros and the log-sum -inf.
-#include "paged.h"
+#include "paged_attn.cuh"
 
 namespace t2w {
 namespace {
 
-struct AttnDev {
-  const void* q;
-  long long q_row_ld, q_head_ld;
-  const uint8_t* codes[2];
-  const float* scales[2];
-  long long page_ld[2], scale_ld[2];
-  const int* table;
-  int table_ld, page, shift, pages, rows, q_heads, kv_heads, causal;
-  float scale;
-  const PlanHead* head;
-  const int *q_start, *kv_len, *request;
-  const int4* starts;  // two entries for each worker
-  int tq, kt, part_rows, block_workers;
-  float* ws;  // the parts of cut segments, two for each worker
-  void* out;
-  float* lse;
-  int* status;
-};
-
-// Four columns of a finished row: O / l, and with the first columns its log-sum.
-template <bool HALF>
-T2W_DEV void store_row(const AttnDev& p, int row, int head, int hd, int d, float4 o, float M, float l) {
-  const float inv = l != 0.f ? 1.f / l : 0.f;
-  uint2 u;
-  if constexpr (HALF) {
-    const __half2 a = __floats2half2_rn(o.x * inv, o.y * inv), b = __floats2half2_rn(o.z * inv, o.w * inv);
-    u = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-  } else {
-    u = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-  }
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + ((size_t)row * p.q_heads + head) * hd + d) = u;
-  if (d == 0 && p.lse)
-    p.lse[(size_t)row * p.q_heads + head] = l != 0.f ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
-}
-
-// x * 2^e for |e| up to 254 without leaving the range on the way.
-T2W_DEV float scaled(float x, int e) {
-  const int a = e / 2;
-  return x * exp2i(a) * exp2i(e - a);
-}
 T2W_DEV void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-T2W_DEV uint32_t pack_f16x2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// One query row's factor for halves: the exponent shift that brings its largest magnitude into [2^14, 2^15), so that
-// bf16 rows keep all their bits over 2^28 of range as halves.  Half rows and rows that are not finite stay as they are.
-template <bool HALF>
-T2W_DEV int row_shift(uint32_t max_bits16) {
-  if (HALF || max_bits16 == 0 || max_bits16 >= 0x7f80u) return 0;
-  return 14 - ((int)(max_bits16 >> 7) - 127);
-}
-template <bool HALF>
-T2W_DEV uint32_t row_half2(uint32_t u, int shift, bool negate) {
-  if constexpr (HALF) return negate ? u ^ 0x80008000u : u;
-  const float a = scaled(__uint_as_float(u << 16), shift), b = scaled(__uint_as_float(u & 0xffff0000u), shift);
-  return negate ? pack_f16x2(-a, -b) : pack_f16x2(a, b);
-}
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRaise = 8.f;  // the reference exponent is raised when a row's largest one passes it by more than this
-
-// A worker's unfinished rows of a segment: O [rows][HD], then the reference exponents [rows] and the sums [rows].
-T2W_DEV float* part_of(float* ws, int slot, int rows, int hd) { return ws + (size_t)slot * rows * (hd + 2); }
-
 // ---------------------------------------------------------------- at most 16 query rows to a key head
 //
 // What bounds it: the cache is read once, 2 HD bytes for each key against 4 HD flops a query row, so HBM does.  A
@@ -95,9 +30,9 @@ T2W_DEV float* part_of(float* ws, int slot, int rows, int hd) { return ws + (siz
 // The 16-byte pieces of a 128-byte line are permuted (swizzle()) so that neither K's reads (8 rows' pieces t) nor V's (4
 // rows two apart, piece g) meet in a bank.
 //
-// Exponents: key j with scales s_k, s_v of its page weighs 2^(x_j + log2 s_v - M) on its V codes, M the running maximum
-// of x_j + log2 s_v: the weights of the largest contributions have all the bits that a half has whatever the scales, and
-// what is 2^-24 of the largest contribution is lost.  The sum of exponentials is kept in units of 2^M too.
+// Exponents: key j with scales s_k, s_v of its page weighs 2^(x_j + log2 s_v - M) on its V codes, M a little
+// below the running maximum of x_j + log2 s_v (kBelow): the weights of the largest contributions have all the bits that a
+// half has whatever the scales.  The sum of exponentials is kept in units of 2^M too.
 template <int HD>
 struct FewStage {
   uint8_t k[32 * HD], v[32 * HD];
@@ -108,12 +43,6 @@ T2W_DEV uint32_t swizzle(int row, int piece) {  // byte offset of 16-byte piece 
   if constexpr (HD == 128) return row * 128 + ((piece ^ (((row >> 1) & 3) << 1) ^ ((row & 1) << 2)) << 4);
   const int line = row >> 1;
   return line * 128 + ((((row & 1) * 4 + piece) ^ ((line & 3) << 1)) << 4);
-}
-// The cache streams through L2 (evicted first), so that the plan, the tables and the parts stay there.
-T2W_DEV uint64_t l2_policy_evict_first() {
-  uint64_t p;
-  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
-  return p;
 }
 T2W_DEV void copy16(uint32_t dst, const void* src, uint64_t policy) {
   asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
@@ -331,7 +260,7 @@ __global__ void __launch_bounds__(128, few_blocks(HD, NQ)) k_paged_few(const Att
         mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
         raise[n] = mx > M[n] + kRaise;
-        const float m_new = raise[n] ? mx : M[n];
+        const float m_new = raise[n] ? mx - kBelow : M[n];
         fac[n] = raise[n] ? exp2_approx(M[n] - m_new) : 1.f;  // 2^-inf = 0 the first time
         M[n] = m_new;
         const float ref = m_new == -INFINITY ? 0.f : m_new;
@@ -656,84 +585,6 @@ __global__ void __launch_bounds__(128, 8) k_paged_merge(const AttnDev p) {
   }
 }
 
-template <bool HALF>
-T2W_DEV float load16(const uint16_t* p) {
-  const uint32_t u = *p;
-  if constexpr (HALF) return __half2float(*reinterpret_cast<const __half*>(&u));
-  return __uint_as_float(u << 16);
-}
-
-// One warp: one row and query head; a lane scores one key of 32 and then holds HD / 32 columns of the output.
-template <int HD, bool HALF>
-__global__ void __launch_bounds__(128) k_paged_rows(const AttnDev p) {
-  __shared__ float qs[4][HD];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long unit = (long long)blockIdx.x * 4 + warp;
-  pdl_wait();
-  pdl_launch();
-  if (unit >= (long long)p.rows * p.q_heads) return;
-  const int row = (int)(unit / p.q_heads), h = (int)(unit % p.q_heads), hk = h / (p.q_heads / p.kv_heads);
-  constexpr int N = HD / 32;
-  float o[N] = {};
-  float m = -INFINITY, l = 0.f;
-  const bool used = row < p.head->used;
-  if (used) {
-    const uint16_t* q = static_cast<const uint16_t*>(p.q) + row * p.q_row_ld + h * p.q_head_ld;
-    for (int i = lane; i < HD; i += 32) qs[warp][i] = load16<HALF>(q + i) * p.scale * 1.4426950408889634f;
-    __syncwarp();
-    const int r = p.request[row];
-    const int end = p.causal ? p.kv_len[r] - (p.q_start[r + 1] - row) + 1 : p.kv_len[r];
-    for (int j0 = 0; j0 < end; j0 += 32) {
-      const int j = j0 + lane;
-      float x = -INFINITY, sv = 0.f;
-      int g = 0;
-      if (j < end) {
-        g = p.table[(size_t)r * p.table_ld + (j >> p.shift)];
-        if ((unsigned)g >= (unsigned)p.pages) {
-          atomicExch(p.status, T2W_ERR_INVALID);
-          g = 0;
-        }
-        const uint8_t* k = p.codes[0] + g * p.page_ld[0] + ((size_t)hk * p.page + (j & (p.page - 1))) * HD;
-        float s = 0.f;
-        for (int i = 0; i < HD; i += 2) {
-          const uint32_t f = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(k + i));
-          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&f));
-          s += v.x * qs[warp][i] + v.y * qs[warp][i + 1];
-        }
-        x = s * p.scales[0][g * p.scale_ld[0] + hk];
-        sv = p.scales[1][g * p.scale_ld[1] + hk];
-      }
-      float top = x;
-#pragma unroll
-      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-      const float m_new = fmaxf(m, top), f = m == -INFINITY ? 0.f : exp2f(m - m_new);
-      const float e = j < end ? exp2f(x - (m_new == -INFINITY ? 0.f : m_new)) : 0.f;
-      l = l * f + warp_sum(e);
-      m = m_new;
-#pragma unroll
-      for (int i = 0; i < N; ++i) o[i] *= f;
-      for (int t = 0; t < 32 && j0 + t < end; ++t) {
-        const int gt = __shfl_sync(~0u, g, t);
-        const float w = __shfl_sync(~0u, e * sv, t);
-        const uint8_t* v = p.codes[1] + gt * p.page_ld[1] + ((size_t)hk * p.page + ((j0 + t) & (p.page - 1))) * HD;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint32_t f2 = e4m3x2_to_f16x2(v[lane + 32 * i]);
-          o[i] += w * __low2float(*reinterpret_cast<const __half2*>(&f2));
-        }
-      }
-    }
-  }
-  const float inv = l != 0.f ? 1.f / l : 0.f;
-  uint16_t* out = static_cast<uint16_t*>(p.out) + ((size_t)row * p.q_heads + h) * HD;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if constexpr (HALF) reinterpret_cast<__half*>(out)[lane + 32 * i] = __float2half_rn(o[i] * inv);
-    else reinterpret_cast<__nv_bfloat16*>(out)[lane + 32 * i] = __float2bfloat16_rn(o[i] * inv);
-  }
-  if (p.lse && lane == 0) p.lse[(size_t)row * p.q_heads + h] = l != 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
-}
-
 }  // namespace
 }  // namespace t2w
 
@@ -743,8 +594,10 @@ namespace {
 
 template <int HD, bool HALF>
 cudaError_t launch_paged(const AttnDev& p, const PagedCut& cut, int max_rows, cudaStream_t st) {
-  if (cut.mma)
-    return launch_k(k_paged_rows<HD, HALF>, dim3((unsigned)(((long long)p.rows * p.q_heads + 3) / 4)), dim3(128), 0, st, p);
+  if (cut.mma) {
+    const cudaError_t e = launch_paged_many(p, cut, HD, HALF, st);
+    return e != cudaSuccess ? e : launch_k(k_paged_merge<HD, HALF>, dim3((cut.workers + 7) / 8, 16), dim3(128), 0, st, p);
+  }
   const int nq = max_rows > 8 ? 2 : 1;
   constexpr int smem = 4 * few_stages * (int)sizeof(FewStage<HD>);
   static std::atomic<uint64_t> done[4];
@@ -764,7 +617,7 @@ cudaError_t launch_paged(const AttnDev& p, const PagedCut& cut, int max_rows, cu
 extern "C" size_t t2w_paged_workspace_bytes(int32_t max_fresh, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
   if (max_fresh <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
   const PagedCut c = paged_cut(max_fresh, q_heads, kv_heads, head_dim);
-  return 2 * (size_t)c.workers * 16 * (head_dim + 2) * sizeof(float);
+  return 2 * (size_t)c.workers * (c.mma ? 128 : 16) * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int t2w_paged_attn(const t2w_paged_attn_args* a, void* stream) {
@@ -812,12 +665,11 @@ extern "C" int t2w_paged_attn(const t2w_paged_attn_args* a, void* stream) {
   p.head = reinterpret_cast<const PlanHead*>(a->plan);
   p.q_start = a->plan + l.q_start;
   p.kv_len = a->plan + l.kv_len;
-  p.request = a->plan + l.request;
   p.starts = reinterpret_cast<const int4*>(a->plan + l.starts);
   p.tq = cut.tq;
   p.kt = cut.kt;
-  p.part_rows = 16;
-  p.block_workers = 4;
+  p.part_rows = cut.mma ? 128 : 16;
+  p.block_workers = cut.mma ? 1 : 4;
   p.ws = static_cast<float*>(a->workspace);
   p.out = a->out;
   p.lse = a->lse;

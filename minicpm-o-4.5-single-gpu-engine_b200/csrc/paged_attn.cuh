@@ -1,0 +1,107 @@
+// What the two forms of the paged attention share: the arguments, a finished row's store, the queries as halves, and the
+// parts of segments that were cut.
+#pragma once
+
+#include "paged.h"
+
+namespace t2w {
+
+struct AttnDev {
+  const void* q;
+  long long q_row_ld, q_head_ld;
+  const uint8_t* codes[2];
+  const float* scales[2];
+  long long page_ld[2], scale_ld[2];
+  const int* table;
+  int table_ld, page, shift, pages, rows, q_heads, kv_heads, causal;
+  float scale;
+  const PlanHead* head;
+  const int *q_start, *kv_len;
+  const int4* starts;  // two entries for each worker
+  int tq, kt, part_rows, block_workers;
+  float* ws;  // the parts of cut segments, two for each worker
+  void* out;
+  float* lse;
+  int* status;
+};
+
+// Four columns of a finished row: O / l, and with the first columns its log-sum.
+template <bool HALF>
+T2W_DEV void store_row(const AttnDev& p, int row, int head, int hd, int d, float4 o, float M, float l) {
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  uint2 u;
+  if constexpr (HALF) {
+    const __half2 a = __floats2half2_rn(o.x * inv, o.y * inv), b = __floats2half2_rn(o.z * inv, o.w * inv);
+    u = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  } else {
+    u = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  }
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + ((size_t)row * p.q_heads + head) * hd + d) = u;
+  if (d == 0 && p.lse)
+    p.lse[(size_t)row * p.q_heads + head] = l != 0.f ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
+}
+
+// Eight columns, in one 16-byte store.
+template <bool HALF>
+T2W_DEV void store_row8(const AttnDev& p, int row, int head, int hd, int d, const float* o, float M, float l) {
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = o[2 * i] * inv, b = o[2 * i + 1] * inv;
+    if constexpr (HALF) {
+      const __half2 v = __floats2half2_rn(a, b);
+      u[i] = *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+      u[i] = pack_bf16x2(a, b);
+    }
+  }
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + ((size_t)row * p.q_heads + head) * hd + d) =
+      make_uint4(u[0], u[1], u[2], u[3]);
+  if (d == 0 && p.lse)
+    p.lse[(size_t)row * p.q_heads + head] = l != 0.f ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
+}
+
+// The cache streams through L2 (evicted first), so that the plan, the tables and the parts stay there.
+T2W_DEV uint64_t l2_policy_evict_first() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+// x * 2^e for |e| up to 254 without leaving the range on the way.
+T2W_DEV float scaled(float x, int e) {
+  const int a = e / 2;
+  return x * exp2i(a) * exp2i(e - a);
+}
+T2W_DEV uint32_t pack_f16x2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// One query row's factor for halves: the exponent shift that brings its largest magnitude into [2^14, 2^15), so that
+// bf16 rows keep all their bits over 2^28 of range as halves.  Half rows and rows that are not finite stay as they are.
+template <bool HALF>
+T2W_DEV int row_shift(uint32_t max_bits16) {
+  if (HALF || max_bits16 == 0 || max_bits16 >= 0x7f80u) return 0;
+  return 14 - ((int)(max_bits16 >> 7) - 127);
+}
+template <bool HALF>
+T2W_DEV uint32_t row_half2(uint32_t u, int shift, bool negate) {
+  if constexpr (HALF) return negate ? u ^ 0x80008000u : u;
+  const float a = scaled(__uint_as_float(u << 16), shift), b = scaled(__uint_as_float(u & 0xffff0000u), shift);
+  return negate ? pack_f16x2(-a, -b) : pack_f16x2(a, b);
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+// A weight is 2^(x + log2 s_v - M) in a half: M is set 9 below a row's largest exponent and again when that would pass M
+// by more than 15 (65504 is the largest half), so that the largest weight is 2^9 or more and what falls under the halves'
+// smallest, 2^-25, is 2^-34 of the largest contribution.
+constexpr float kRaise = 15.f, kBelow = 9.f;
+
+// A worker's unfinished rows of a segment: O [rows][HD], then the reference exponents [rows] and the sums [rows].
+T2W_DEV float* part_of(float* ws, int slot, int rows, int hd) { return ws + (size_t)slot * rows * (hd + 2); }
+
+// Segments of up to 128 query rows on tcgen05 tiles (paged_attn_tc.cu): the parts of cut segments into p.ws.
+cudaError_t launch_paged_many(const AttnDev& p, const PagedCut& cut, int head_dim, bool half, cudaStream_t st);
+
+}  // namespace t2w

@@ -14,14 +14,22 @@
 namespace t2w {
 
 PagedCut paged_cut(int max_fresh, int q_heads, int kv_heads, int head_dim) {
-  const int rows = max_fresh * (q_heads / kv_heads);
+  const int group = q_heads / kv_heads;
   PagedCut c;
-  c.mma = max_fresh > 16 || rows > 16;
-  c.tq = max_fresh;
-  c.kt = 32;
-  c.workers = 4 * few_blocks(head_dim, rows > 8 ? 2 : 1) * num_sms();
-  c.min_per = 2;
-  c.extra = 4;
+  c.mma = (int64_t)max_fresh * group > 16;
+  if (c.mma) {
+    c.tq = 128 / group;
+    c.kt = 64;
+    c.workers = 2 * num_sms();
+    c.min_per = 4;
+    c.extra = 2;
+  } else {
+    c.tq = max_fresh;
+    c.kt = 32;
+    c.workers = 4 * few_blocks(head_dim, max_fresh * group > 8 ? 2 : 1) * num_sms();
+    c.min_per = 2;
+    c.extra = 4;
+  }
   return c;
 }
 
