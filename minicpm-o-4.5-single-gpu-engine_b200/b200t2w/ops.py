@@ -19,6 +19,7 @@ from . import lib as L
 from .build import OPS_PATH
 
 _loaded = False
+_ops: dict = {}
 
 
 def load(path: str | None = None):
@@ -36,7 +37,9 @@ def load(path: str | None = None):
 
 def call(name: str, *args):
     """``torch.ops.b200t2w.<name>(*args)``, with a failed status raised as ``T2WError``."""
-    op = getattr(load(), name)
+    op = _ops.get(name)
+    if op is None:
+        op = _ops[name] = getattr(load(), name).default  # the one overload: its call skips the search for it
     try:
         return op(*args)
     except RuntimeError as e:

@@ -17,8 +17,6 @@ device or alignment.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import lib as L
@@ -26,38 +24,16 @@ from . import ops as O
 
 
 class PagedPlan:
-    """One step's tables (see ``plan``).  ``buffer`` is what the kernels read; the properties are views of it."""
+    """One step's tables (see ``plan``): what the kernels read (``buffer``), and views of it,
 
-    __slots__ = ("buffer", "table", "free_left", "requests", "rows", "max_fresh", "page", "q_heads", "kv_heads",
-                 "head_dim", "causal", "_at")
+    ``q_start`` int32 [requests + 1]: the first row of each request, and the rows in use;
+    ``kv_len`` int32 [requests]: tokens of each request, this step's among them where they are appended;
+    ``slot`` int32 [rows]: page * page_size + place in the page of each row; -1 for padding and for rows not appended;
+    ``request`` int32 [rows]: the request of each row; -1 for padding;
+    ``free_left`` int32 [1]: the free pages left (where the rows are appended)."""
 
-    def _part(self, i: int, n: int) -> torch.Tensor:
-        if self._at is None:
-            at = (ctypes.c_int64 * 4)()
-            L.load().t2w_paged_plan_ints(self.requests, self.rows, self.max_fresh, self.page, self.q_heads, self.kv_heads,
-                                         self.head_dim, at)
-            self._at = tuple(at)
-        return self.buffer.narrow(0, self._at[i], n)
-
-    @property
-    def q_start(self) -> torch.Tensor:
-        """int32 [requests + 1]: the first row of each request, and the rows in use."""
-        return self._part(0, self.requests + 1)
-
-    @property
-    def kv_len(self) -> torch.Tensor:
-        """int32 [requests]: tokens of each request, this step's among them where they are appended."""
-        return self._part(1, self.requests)
-
-    @property
-    def slot(self) -> torch.Tensor:
-        """int32 [rows]: page * page_size + place in the page of each row; -1 for padding and for rows not appended."""
-        return self._part(2, self.rows)
-
-    @property
-    def request(self) -> torch.Tensor:
-        """int32 [rows]: the request of each row; -1 for padding."""
-        return self._part(3, self.rows)
+    __slots__ = ("buffer", "q_start", "kv_len", "slot", "request", "free_left", "table", "requests", "rows", "max_fresh",
+                 "page", "q_heads", "kv_heads", "head_dim", "causal")
 
     def check(self) -> None:
         """Wait for the GPU and raise ``T2WError`` if the plan is void or a call that took it met a fault."""
@@ -82,21 +58,20 @@ def plan(fresh: torch.Tensor, length: torch.Tensor, table: torch.Tensor, page: i
     splits over the GPU.  A tight ``max_fresh`` matters: at 16 rows to a key head and request or fewer (max_fresh * q_heads /
     kv_heads) the attention runs its form for single tokens."""
     most = rows if max_fresh is None else max_fresh
-    if free is not None and free_left is None:
-        free_left = torch.empty_like(free_count)
     p = PagedPlan()
-    p.buffer = O.call("paged_plan", fresh, length, table, page, rows, max(1, most), q_heads, kv_heads, head_dim, causal,
-                      free, free_count, kv_len, free_left)
-    p.table, p.free_left, p.requests, p.rows, p.max_fresh = table, free_left, fresh.numel(), rows, max(1, most)
-    p.page, p.q_heads, p.kv_heads, p.head_dim, p.causal, p._at = page, q_heads, kv_heads, head_dim, causal, None
+    p.buffer, p.q_start, p.kv_len, p.slot, p.request, p.free_left = O.call(
+        "paged_plan", fresh, length, table, page, rows, max(1, most), q_heads, kv_heads, head_dim, causal, free,
+        free_count, kv_len, free_left)
+    p.table, p.requests, p.rows, p.max_fresh = table, fresh.numel(), rows, max(1, most)
+    p.page, p.q_heads, p.kv_heads, p.head_dim, p.causal = page, q_heads, kv_heads, head_dim, causal
     return p
 
 
-def _fits(p: PagedPlan, codes: torch.Tensor, rows: torch.Tensor) -> None:
-    if codes.dim() != 4 or (codes.shape[1], codes.shape[2], codes.shape[3]) != (p.kv_heads, p.page, p.head_dim):
+def _fits(p: PagedPlan, codes: torch.Tensor, rows: torch.Tensor, heads: int) -> None:
+    if codes.shape[1:] != (p.kv_heads, p.page, p.head_dim):
         raise ValueError(f"the plan is for pages [{p.kv_heads}, {p.page}, {p.head_dim}], the codes are {tuple(codes.shape)}")
-    if rows.dim() != 3 or rows.shape[0] != p.rows:
-        raise ValueError(f"the plan is for {p.rows} rows [rows, heads, head_dim], got {tuple(rows.shape)}")
+    if rows.shape != (p.rows, heads, p.head_dim):
+        raise ValueError(f"the plan is for rows [{p.rows}, {heads}, {p.head_dim}], got {tuple(rows.shape)}")
 
 
 def append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
@@ -107,7 +82,7 @@ def append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: tor
     The scale of a page and head is the least power of two with which the largest magnitude ever given to it fits e4m3
     (at most 448 * 2^64, at least 2^-64).  Where a step's rows raise it, the codes already there are rounded again.  A
     page and head that is given an infinity or a NaN reads as NaN from then on."""
-    _fits(plan, k_codes, k)
+    _fits(plan, k_codes, k, plan.kv_heads)
     O.call("paged_append", k, v, k_codes, v_codes, k_scale, v_scale, plan.buffer, plan.requests, plan.max_fresh, plan.q_heads)
 
 
@@ -116,9 +91,7 @@ def attend(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scal
     """softmax(scale q k^T) v of the plan's rows ``q [rows, q_heads, head_dim]`` (bf16 or fp16) over their requests' pages;
     ``scale`` is 1 / sqrt(head_dim) unless given.  Returns the output (q's type) and, with ``lse``, the natural log of each
     row's sum of exponentials (fp32 ``[rows, q_heads]``).  A row that sees no key, and padding, gives zeros and -inf."""
-    _fits(plan, k_codes, q)
-    if q.shape[1] != plan.q_heads:
-        raise ValueError(f"the plan is for {plan.q_heads} query heads, got {q.shape[1]}")
+    _fits(plan, k_codes, q, plan.q_heads)
     r = O.call("paged_attn", q, k_codes, v_codes, k_scale, v_scale, plan.table, plan.buffer, plan.requests, plan.max_fresh,
                plan.causal, plan.head_dim ** -0.5 if scale is None else scale, lse)
     return tuple(r) if lse else r[0]

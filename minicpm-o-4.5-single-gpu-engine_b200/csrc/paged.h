@@ -38,19 +38,50 @@ struct PlanLayout {
 // How an attention call is cut.  A segment is what one softmax runs over: (request, key head, query tile); its keys come
 // in tiles of `kt`.  The tiles of all segments, in that order, are numbered, and the places are dealt to the workers in
 // equal contiguous shares, so that ragged lengths cost no balance; a segment that is cut by a share's end is finished by
-// k_paged_merge.  In large calls each segment's first tile has `extra` empty places before it: what it costs a worker to
+// k_paged_merge.  Where the worker is a block and a segment is a good deal shorter than a share, the shares end at the
+// nearest segment's end instead (whole segments).  In large calls each segment's first tile has `extra` empty places before it: what it costs a worker to
 // begin a segment, in tiles, so that a share of many short segments is not the one that the others wait for.
+enum class PagedForm {
+  kFew,   // at most 16 query rows to a key head: a worker is a warp
+  kMid,   // a worker is a block, with tiles of 64 rows
+  kMany,  // a worker is a block, with tcgen05 tiles of 128 rows
+};
 struct PagedCut {
-  int mma;    // 1: tcgen05 tiles of 128 query rows, a worker is a CTA; 0: at most 16 rows, a worker is a warp
+  PagedForm form;
+  int part_rows;  // rows of a segment's part in the workspace
   int tq;     // query tokens of a tile (rows = tokens * group)
   int kt;     // keys of a tile
   int workers;  // workers at most
   int min_per;  // places of a worker at least
   int extra;
+  bool whole;   // whether short segments are left whole
 };
 
-// Blocks of 4 warps that an SM holds of the kernel for few query rows.
-constexpr int few_blocks(int hd, int nq) { return hd == 128 ? 2 : (nq == 2 ? 3 : 4); }
+// Blocks of 8 warps that an SM holds of the kernel for few query rows.
+constexpr int few_warps = 8;
+constexpr int few_blocks(int hd, int nq) { return hd == 128 || nq == 2 ? 1 : 2; }
+#ifndef MB64
+#define MB64 4
+#endif
+#ifndef MB128
+#define MB128 3
+#endif
+#ifndef MS
+#define MS 3
+#endif
+#ifndef MW
+#define MW 4
+#endif
+#ifndef MQS
+#define MQS 1
+#endif
+#ifndef MIDRULE
+#define MIDRULE 1
+#endif
+constexpr int mid_blocks(int hd) { return hd == 128 ? MB128 : MB64; }
+constexpr int mid_warps = MW;
+constexpr int mid_stages = MS;
+// 
 constexpr int few_stages = 3;  // tiles of a warp's ring (8 KB each, 4 KB where head_dim is 64): the SM's rings hold 196 KB
 
 inline int64_t round4(int64_t n) { return (n + 3) & ~int64_t(3); }
@@ -60,22 +91,23 @@ PlanLayout paged_layout(int64_t requests, int64_t rows, int page, const PagedCut
 
 // ---------------------------------------------------------------- tiles of a request (device)
 // sum over i < n of floor((a i + b) / m), a, b >= 0 (the lattice points under a line, by Euclid's algorithm on a and m)
-T2W_DEV long long floor_sum(long long n, long long m, long long a, long long b) {
+// (a n + b < 2^32: the arguments are numbers of keys; division by 32 bits is several times faster)
+T2W_DEV long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
   long long s = 0;
   while (n > 0) {
     if (a >= m) {
-      s += n * (n - 1) / 2 * (a / m);
+      s += (long long)n * (n - 1) / 2 * (a / m);
       a %= m;
     }
     if (b >= m) {
-      s += n * (b / m);
+      s += (long long)n * (b / m);
       b %= m;
     }
-    const long long top = a * n + b;
+    const unsigned top = a * n + b;
     if (top < m) break;
     n = top / m;
     b = top % m;
-    const long long t = m;
+    const unsigned t = m;
     m = a;
     a = t;
   }
@@ -83,9 +115,8 @@ T2W_DEV long long floor_sum(long long n, long long m, long long a, long long b) 
 }
 // Keys that the last query of query tile qt sees.
 T2W_DEV int tile_keys(int f, int kv, int causal, int tq, int qt) {
-  if (!causal) return kv;
-  const long long v = (long long)kv - f + (long long)(qt + 1) * tq;
-  return v < 0 ? 0 : v > kv ? kv : (int)v;
+  const int behind = f - (qt + 1) * tq;  // queries behind the tile (it may be the last, and not whole)
+  return causal && behind > 0 ? max(kv - behind, 0) : kv;
 }
 // Key tiles of a segment: one at least, so that rows that see nothing are written too.
 T2W_DEV int seg_tiles(int keys, int kt) { return keys > 0 ? (keys + kt - 1) / kt : 1; }
@@ -94,14 +125,14 @@ T2W_DEV long long tiles_before(int f, int kv, int causal, int tq, int kt, int x)
   if (x <= 0) return 0;
   if (!causal) return (long long)x * seg_tiles(kv, kt);
   if (x == 1) return seg_tiles(tile_keys(f, kv, causal, tq, 0), kt);
-  const long long c = (long long)kv - f + tq;  // keys of query tile 0, were the last tile whole
-  long long none = c > 0 ? 0 : -c / tq + 1;    // query tiles that see nothing
+  const int c = kv - f + tq;           // keys of query tile 0, were the last tile whole
+  int none = c > 0 ? 0 : -c / tq + 1;  // query tiles that see nothing
   if (none > x) none = x;
   long long s = none;
   if (none < x) {
     s += floor_sum(x - none, kt, tq, c + none * tq + kt - 1);
-    const long long last = c + (long long)(x - 1) * tq;
-    if (last > kv) s += seg_tiles(kv, kt) - (last + kt - 1) / kt;
+    const long long last = (long long)c + (long long)(x - 1) * tq;
+    if (last > kv) s += seg_tiles(kv, kt) - (int)((last + kt - 1) / kt);
   }
   return s;
 }

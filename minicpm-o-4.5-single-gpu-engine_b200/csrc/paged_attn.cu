@@ -18,8 +18,8 @@ T2W_DEV void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint3
 //
 // What bounds it: the cache is read once, 2 HD bytes for each key against 4 HD flops a query row, so HBM does.  A
 // worker is one warp with a contiguous share of the key tiles (32 keys), so that nothing waits for another warp; only
-// where one segment fills the shares of a whole block do its 4 warps join what they have, so that a long history comes
-// to a quarter of the parts.
+// where one segment fills the shares of a whole block do its 8 warps join what they have, so that a long history comes
+// to an eighth of the parts.
 //
 // A tile's bytes come to the warp's own ring in shared memory by asynchronous copies, one tile or two ahead across the
 // ends of segments, and from there in the tensor core's fragments.  Scores: Q is the A operand (16 rows x 16 dims; a
@@ -51,33 +51,337 @@ T2W_DEV void copy4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 
-template <int HD, bool HALF, int NQ, bool P16>
-__global__ void __launch_bounds__(128, few_blocks(HD, NQ)) k_paged_few(const AttnDev p) {
-  extern __shared__ __align__(16) uint8_t ring[];
-  constexpr int kC = HD / 64, kM = HD / 16, kS = few_stages;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int w = 4 * blockIdx.x + warp, group = p.q_heads / p.kv_heads;
-  const FewStage<HD>* const stage = reinterpret_cast<const FewStage<HD>*>(ring) + warp * kS;
-  const uint32_t ring0 = smem_u32(stage);
-  const uint64_t policy = l2_policy_evict_first();
-  // this lane's places in a stage: of what it copies (even and odd 512 bytes), of K's row g piece t (the pieces of the
-  // second 64 dims are 64 bytes on or back: xor), of V's rows 2t and 2t + 1 piece g (8 bytes of it where HD is 64)
-  uint32_t put[2], get_k, get_v[2];
+// A lane's places in a stage: of what it copies of 1024 bytes of K or of V rows (of the first and the second 512, which
+// repeat), of K's row g piece t (the pieces of the second 64 dims are 64 bytes on or back: xor), and of V's rows 2t and
+// 2t + 1 piece g (8 bytes of it where HD is 64).
+template <int HD>
+T2W_DEV void stage_places(uint32_t (&put)[2], uint32_t& get_k, uint32_t (&get_v)[2]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     put[i] = swizzle<HD>(i * (512 / HD) + lane / (HD / 16), lane % (HD / 16)) - i * 512;
     get_v[i] = 32 * HD + (HD == 128 ? swizzle<HD>(2 * t + i, g) : swizzle<HD>(2 * t + i, g >> 1) + 8 * (g & 1));
   }
   get_k = swizzle<HD>(g, t);
+}
+
+// A warp's 8 NQ query rows of a segment: thread (g, t) = (lane / 4, lane % 4) has of rows g, g + 8, ... what the scores'
+// tiles give it, and columns 2t, 2t + 1 (+ 8 ...) of the transposed output.  Where the output alone takes half the
+// registers (QS), the queries' fragments lie in shared memory: 16 bytes of a lane for each 16 rows and step of 16 dims.
+template <int HD, int NQ, bool QS>
+struct Rows {
+  static constexpr int A = (NQ + 1) / 2;  // tiles of 16 rows
+  uint32_t qa[QS ? 1 : A][QS ? 1 : HD / 16][4];  // queries as halves, as A operands
+  float c[NQ];                     // scale * log2 e / the power of two that the row's queries were multiplied by
+  int end[NQ];                     // keys that the row sees
+  float M[NQ], l[NQ], o[NQ][HD / 16][4];
+};
+// Rows first .. of the segment that begins at row row0 and has `rows`; the segment's first row's query sees `before` + 1
+// keys where the call is causal.  qs: the warp's place in shared memory (QS).
+template <int HD, bool HALF, int NQ, bool QS>
+T2W_DEV void load_rows(const AttnDev& p, Rows<HD, NQ, QS>& q, uint4* qs, int row0, int first, int rows, int hk, int before, int kv) {
+  constexpr int kC = HD / 64, kM = HD / 16;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, group = p.group;
+#pragma unroll
+  for (int a = 0; a < (NQ + 1) / 2; ++a) {
+    uint32_t qa[kM][4];
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int n = 2 * a + y;
+      if (n >= NQ) {
+#pragma unroll
+        for (int i = 0; i < kM; ++i) qa[i][y] = qa[i][2 + y] = 0;
+        continue;
+      }
+      const int row = first + g + 8 * n;
+      uint4 v[kC][2];
+      uint32_t m = 0;
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          v[c][i] = make_uint4(0, 0, 0, 0);
+          if (row < rows) {
+            const uint16_t* x = static_cast<const uint16_t*>(p.q) + (row0 + over_group(p, row)) * p.q_row_ld +
+                                (hk * group + row - group * over_group(p, row)) * p.q_head_ld;
+            v[c][i] = __ldg(reinterpret_cast<const uint4*>(x + 64 * c + 16 * t + 8 * i));
+          }
+          const uint4 u = v[c][i];
+          m = __vmaxu2(__vmaxu2(m, u.x & 0x7fff7fffu), u.y & 0x7fff7fffu);
+          m = __vmaxu2(__vmaxu2(m, u.z & 0x7fff7fffu), u.w & 0x7fff7fffu);
+        }
+      m = max(m & 0xffffu, m >> 16);
+      m = max(m, __shfl_xor_sync(~0u, m, 1));
+      m = max(m, __shfl_xor_sync(~0u, m, 2));
+      const int sh = row_shift<HALF>(m);
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        const uint32_t u[8] = {v[c][0].x, v[c][0].y, v[c][0].z, v[c][0].w, v[c][1].x, v[c][1].y, v[c][1].z, v[c][1].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) qa[4 * c + j][2 * i + y] = row_half2<HALF>(u[2 * j + i], sh, p.scale < 0.f);
+      }
+      q.c[n] = scaled(fabsf(p.scale) * kLog2e, -sh);
+      q.end[n] = p.causal ? before + over_group(p, row) + 1 : kv;
+      q.M[n] = -INFINITY;
+      q.l[n] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kM; ++i) q.o[n][i][0] = q.o[n][i][1] = q.o[n][i][2] = q.o[n][i][3] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kM; ++i) {
+      if constexpr (QS) {
+        qs[(a * kM + i) * 32 + lane] = make_uint4(qa[i][0], qa[i][1], qa[i][2], qa[i][3]);
+      } else {
+#pragma unroll
+        for (int y = 0; y < 4; ++y) q.qa[a][i][y] = qa[i][y];
+      }
+    }
+  }
+  if constexpr (QS) __syncwarp();
+}
+// 32 keys from kb on: their scores, weights and products.  get_k, get_v: the lane's places in a stage (stage_places()).
+template <int HD, int NQ, bool QS, bool P16>
+T2W_DEV void tile_step(Rows<HD, NQ, QS>& q, const uint4* qs, const FewStage<HD>& st, uint32_t get_k, const uint32_t (&get_v)[2],
+                       int kb, int kv, int all_see) {
+  constexpr int kC = HD / 64, kM = HD / 16, kA = (NQ + 1) / 2, kH = P16 ? 2 : 1;  // kH: pages of the tile
+  const int lane = threadIdx.x & 31, t = lane & 3;
+  const uint8_t* const bytes = st.k;
+  float d[kA][4][4] = {};
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    uint4 kr[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) kr[j] = *reinterpret_cast<const uint4*>(bytes + 8 * HD * j + (get_k ^ (64 * c)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t qa[kA][4];
+#pragma unroll
+      for (int a = 0; a < kA; ++a) {
+        if constexpr (QS) {
+          const uint4 u = qs[(a * kM + 4 * c + i) * 32 + lane];
+          qa[a][0] = u.x;
+          qa[a][1] = u.y;
+          qa[a][2] = u.z;
+          qa[a][3] = u.w;
+        } else {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) qa[a][y] = q.qa[a][4 * c + i][y];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint2 u = e4m3x4_to_f16x4(i == 0 ? kr[j].x : i == 1 ? kr[j].y : i == 2 ? kr[j].z : kr[j].w);
+#pragma unroll
+        for (int a = 0; a < kA; ++a) mma_f16(d[a][j], qa[a][0], qa[a][1], qa[a][2], qa[a][3], u.x, u.y);
+      }
+    }
+  }
+  float ks[kH], lv[kH], unit[kH];
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < kH; ++i) {
+    const float vs = st.vs[i];
+    ks[i] = st.ks[i];
+    odd |= !(vs < INFINITY) || !(ks[i] < INFINITY);
+    const int e = vs < INFINITY ? (int)(__float_as_uint(vs) >> 23) - 127 : 0;
+    lv[i] = (float)e;
+    unit[i] = exp2i(-e);
+  }
+  const bool part = kb + 32 > all_see;  // some row does not see all of the tile
+  uint32_t pw[NQ][4];
+  float fac[NQ];
+  bool raised = false;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    float s[4][2], ck[kH], add[kH];
+#pragma unroll
+    for (int i = 0; i < kH; ++i) {
+      ck[i] = q.c[n] * ks[i];
+      if (ck[i] == 0.f) ck[i] = 1.1754944e-38f;  // (-inf times 0)
+      add[i] = lv[i];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) s[j][i] = d[n >> 1][j][2 * (n & 1) + i];
+    if (part) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (kb + 8 * j + 2 * t + i >= q.end[n]) s[j][i] = -INFINITY;
+    }
+    if (odd) {  // a scale that is not finite may only meet what the row sees
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (kb + 8 * j + 2 * t + i < q.end[n]) s[j][i] = fmaf(s[j][i], ck[P16 ? j >> 1 : 0], add[P16 ? j >> 1 : 0]);
+#pragma unroll
+      for (int i = 0; i < kH; ++i) {
+        ck[i] = 1.f;
+        add[i] = 0.f;
+      }
+    }
+    float mx;
+    if constexpr (P16) {
+      mx = fmaxf(fmaf(fmaxf(fmax3(s[0][0], s[0][1], s[1][0]), s[1][1]), ck[0], add[0]),
+                 fmaf(fmaxf(fmax3(s[2][0], s[2][1], s[3][0]), s[3][1]), ck[kH - 1], add[kH - 1]));
+    } else {
+      mx = fmaf(fmax3(fmax3(s[0][0], s[0][1], s[1][0]), fmax3(s[1][1], s[2][0], s[2][1]), fmaxf(s[3][0], s[3][1])), ck[0], add[0]);
+    }
+    mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+    const bool raise = mx > q.M[n] + kRaise;
+    raised |= raise;
+    const float m_new = raise ? mx - kBelow : q.M[n];
+    fac[n] = raise ? exp2_approx(q.M[n] - m_new) : 1.f;  // 2^-inf = 0 the first time
+    q.M[n] = m_new;
+    const float ref = m_new == -INFINITY ? 0.f : m_new;
+    float2 sum[2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float c = ck[P16 ? j >> 1 : 0], b = add[P16 ? j >> 1 : 0] - ref;
+      const float2 a = __ffma2_rn(make_float2(s[j][0], s[j][1]), make_float2(c, c), make_float2(b, b));
+      const float2 e = make_float2(exp2_approx(a.x), exp2_approx(a.y));
+      sum[j >> 1] = j & 1 ? __fadd2_rn(sum[j >> 1], e) : e;
+      pw[n][j] = pack_f16x2(e.x, e.y);
+    }
+    // the exponentials without their values' scale: 2^(x - M) = w 2^-lv
+    if constexpr (P16) {
+      q.l[n] = fmaf(q.l[n], fac[n], fmaf(sum[0].x + sum[0].y, unit[0], (sum[1].x + sum[1].y) * unit[kH - 1]));
+    } else {
+      const float2 u = __fadd2_rn(sum[0], sum[1]);
+      q.l[n] = fmaf(q.l[n], fac[n], (u.x + u.y) * unit[0]);
+    }
+    if (odd) {  // values that are NaN, where the row sees them
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (!(st.vs[P16 ? j >> 1 : 0] < INFINITY)) {
+          if (kb + 8 * j + 2 * t < q.end[n]) pw[n][j] |= 0x7fffu;
+          if (kb + 8 * j + 2 * t + 1 < q.end[n]) pw[n][j] |= 0x7fff0000u;
+        }
+    }
+  }
+  if (__any_sync(~0u, raised)) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {  // the factors lie with the rows, the output has them as columns 2t, 2t + 1
+      const float f0 = __shfl_sync(~0u, fac[n], 8 * t), f1 = __shfl_sync(~0u, fac[n], 8 * t + 4);
+#pragma unroll
+      for (int i = 0; i < kM; ++i) {
+        q.o[n][i][0] *= f0;
+        q.o[n][i][1] *= f1;
+        q.o[n][i][2] *= f0;
+        q.o[n][i][3] *= f1;
+      }
+    }
+  }
+  const bool tail = kb + 32 > kv;  // places of the page past the last key may hold anything, NaN codes too
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t vw[4][HD / 32];  // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the half
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint8_t* const v = bytes + (16 * i + 8 * (j >> 1)) * HD + get_v[j & 1];
+      if constexpr (HD == 128) {
+        const uint4 u = *reinterpret_cast<const uint4*>(v);
+        vw[j][0] = u.x;
+        vw[j][1] = u.y;
+        vw[j][HD / 32 - 2] = u.z;
+        vw[j][HD / 32 - 1] = u.w;
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(v);
+        vw[j][0] = u.x;
+        vw[j][1] = u.y;
+      }
+    }
+    if (tail) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (kb + 16 * i + 2 * t + (j & 1) + 8 * (j >> 1) >= kv)
+#pragma unroll
+          for (int x = 0; x < HD / 32; ++x) vw[j][x] = 0;
+    }
+#pragma unroll
+    for (int x = 0; x < HD / 32; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const uint2 lo = e4m3x4_to_f16x4(__byte_perm(vw[0][x], vw[1][x], y ? 0x7362 : 0x5140));
+        const uint2 hi = e4m3x4_to_f16x4(__byte_perm(vw[2][x], vw[3][x], y ? 0x7362 : 0x5140));
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) mma_f16(q.o[n][2 * x + y], lo.x, lo.y, hi.x, hi.y, pw[n][2 * i], pw[n][2 * i + 1]);
+      }
+  }
+}
+// This thread's columns of queries 2t and 2t + 1, HD / 8 in a row: finished rows (part nullptr) or a part's.
+template <int HD, bool HALF, int NQ, bool QS>
+T2W_DEV void store_rows(const AttnDev& p, const Rows<HD, NQ, QS>& q, int row0, int from, int rows, int hk, float* part, int part_rows) {
+  constexpr int kM = HD / 16;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, group = p.group;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    float sum = q.l[n];
+    sum += __shfl_xor_sync(~0u, sum, 1);
+    sum += __shfl_xor_sync(~0u, sum, 2);
+    const float top = sum != sum ? fmaxf(q.M[n], -1e30f) : q.M[n];  // a NaN counts, even where M saw nothing else
+    if (part && t == 0 && from + 8 * n + g < rows) {
+      part[part_rows * HD + from + 8 * n + g] = top;
+      part[part_rows * HD + part_rows + from + 8 * n + g] = sum;
+    }
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int row = from + 8 * n + 2 * t + y;
+      const float ls = __shfl_sync(~0u, sum, 8 * t + 4 * y), Ms = __shfl_sync(~0u, top, 8 * t + 4 * y);
+      if (row < rows && part) {
+#pragma unroll
+        for (int i = 0; i < kM; i += 2)
+          *reinterpret_cast<float4*>(part + row * HD + g * (HD / 8) + 2 * i) =
+              make_float4(q.o[n][i][y], q.o[n][i][2 + y], q.o[n][i + 1][y], q.o[n][i + 1][2 + y]);
+      } else if (row < rows) {
+        const float inv = ls != 0.f ? 1.f / ls : 0.f;
+        const int tok = over_group(p, row);
+        const size_t at = (size_t)(row0 + tok) * p.q_heads + hk * group + row - group * tok;
+        uint4* const out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at * HD + g * (HD / 8));
+#pragma unroll
+        for (int i = 0; i < kM; i += 4) {
+          uint32_t u[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float a = q.o[n][i + x][y] * inv, b = q.o[n][i + x][2 + y] * inv;
+            u[x] = HALF ? pack_f16x2(a, b) : pack_bf16x2(a, b);
+          }
+          out[i / 4] = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+        if (g == 0 && p.lse) p.lse[at] = ls != 0.f ? (Ms + log2f(ls)) * 0.6931471805599453f : -INFINITY;
+      }
+      __syncwarp();
+    }
+  }
+}
+
+template <int HD, bool HALF, int NQ, bool P16>
+__global__ void __launch_bounds__(32 * few_warps, few_blocks(HD, NQ)) k_paged_few(const AttnDev p) {
+  extern __shared__ __align__(16) uint8_t ring[];
+  constexpr int kC = HD / 64, kM = HD / 16, kS = few_stages;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int w = few_warps * blockIdx.x + warp, group = p.group;
+  const FewStage<HD>* const stage = reinterpret_cast<const FewStage<HD>*>(ring) + warp * kS;
+  const uint32_t ring0 = smem_u32(stage);
+  const uint64_t policy = l2_policy_evict_first();
+  uint32_t put[2], get_k, get_v[2];
+  stage_places<HD>(put, get_k, get_v);
   pdl_wait();
   pdl_launch();
   const int4 head4 = *reinterpret_cast<const int4*>(p.head);  // n_runs, tiles, per, workers
   int4 seg = p.starts[2 * w], of = p.starts[2 * w + 1];  // request, key head, query tile (always 0), key tile; rows, lengths
   const int extra = p.head->extra;
-  const int4 seg0 = p.starts[8 * blockIdx.x], of0 = p.starts[8 * blockIdx.x + 1];  // the block's first worker's
+  const int4 seg0 = p.starts[2 * few_warps * blockIdx.x], of0 = p.starts[2 * few_warps * blockIdx.x + 1];  // the block's first worker's
   if (w >= head4.w) return;
   // one segment over all of the block's places (its key count is that of the few rows' only query tile)
-  const bool filled = seg0.w >= 0 && 4 * blockIdx.x + 3 < head4.w && seg_tiles(of0.z, 32) - seg0.w >= 4 * head4.z;
+  const bool filled = seg0.w >= 0 && few_warps * blockIdx.x + few_warps - 1 < head4.w &&
+                      seg_tiles(of0.z, 32) - seg0.w >= few_warps * head4.z;
   const int stop = min((w + 1) * head4.z, head4.y);
   int zero = w * head4.z - seg.w;  // the place of the segment's tile 0
 
@@ -154,53 +458,9 @@ __global__ void __launch_bounds__(128, few_blocks(HD, NQ)) k_paged_few(const Att
     const int rows = f * group, nt = seg_tiles(kv, 32);
     const int kt0 = max(seg.w, 0), kt1 = min(nt, stop - zero);
     if (kt1 <= kt0) break;
-    // queries, as halves
-    uint32_t qa[NQ][kC][4][2];
-    float c_row[NQ];
-    int end[NQ];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      const int row = g + 8 * n;
-      uint4 v[kC][2];
-      uint32_t m = 0;
-#pragma unroll
-      for (int c = 0; c < kC; ++c)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          v[c][i] = make_uint4(0, 0, 0, 0);
-          if (row < rows) {
-            const uint16_t* q = static_cast<const uint16_t*>(p.q) + (row0 + row / group) * p.q_row_ld +
-                                (hk * group + row % group) * p.q_head_ld;
-            v[c][i] = __ldg(reinterpret_cast<const uint4*>(q + 64 * c + 16 * t + 8 * i));
-          }
-          const uint4 u = v[c][i];
-          m = __vmaxu2(__vmaxu2(m, u.x & 0x7fff7fffu), u.y & 0x7fff7fffu);
-          m = __vmaxu2(__vmaxu2(m, u.z & 0x7fff7fffu), u.w & 0x7fff7fffu);
-        }
-      m = max(m & 0xffffu, m >> 16);
-      m = max(m, __shfl_xor_sync(~0u, m, 1));
-      m = max(m, __shfl_xor_sync(~0u, m, 2));
-      const int sh = row_shift<HALF>(m);
-#pragma unroll
-      for (int c = 0; c < kC; ++c) {
-        const uint32_t u[8] = {v[c][0].x, v[c][0].y, v[c][0].z, v[c][0].w, v[c][1].x, v[c][1].y, v[c][1].z, v[c][1].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) qa[n][c][j][i] = row_half2<HALF>(u[2 * j + i], sh, p.scale < 0.f);
-      }
-      c_row[n] = scaled(fabsf(p.scale) * kLog2e, -sh);
-      end[n] = p.causal ? kv - f + row / group + 1 : kv;
-    }
+    Rows<HD, NQ, false> q;
+    load_rows<HD, HALF, NQ, false>(p, q, nullptr, row0, 0, rows, hk, kv - f, kv);
     const int all_see = p.causal ? kv - f + 1 : kv;  // keys that every row sees
-    float M[NQ], l[NQ], o[NQ][kM][4];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      M[n] = -INFINITY;
-      l[n] = 0.f;
-#pragma unroll
-      for (int i = 0; i < kM; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
-    }
     for (int kt = kt0; kt < kt1; ++kt) {
       __syncwarp();  // every lane is done with the stage that is filled again
       send(at ? at - 1 : kS - 1);
@@ -209,180 +469,34 @@ __global__ void __launch_bounds__(128, few_blocks(HD, NQ)) k_paged_few(const Att
       const FewStage<HD>& st = stage[at];
       const uint8_t* const bytes = st.k;
       at = at + 1 == kS ? 0 : at + 1;
-      float d[4][4] = {};
-#pragma unroll
-      for (int c = 0; c < kC; ++c) {
-        uint4 kr[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) kr[j] = *reinterpret_cast<const uint4*>(bytes + 8 * HD * j + (get_k ^ (64 * c)));
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint2 u = e4m3x4_to_f16x4(i == 0 ? kr[j].x : i == 1 ? kr[j].y : i == 2 ? kr[j].z : kr[j].w);
-            mma_f16(d[j], qa[0][c][i][0], NQ == 2 ? qa[NQ - 1][c][i][0] : 0u, qa[0][c][i][1], NQ == 2 ? qa[NQ - 1][c][i][1] : 0u,
-                    u.x, u.y);
-          }
-      }
-      const int kb = kt * 32;
-      constexpr int kH = P16 ? 2 : 1;  // pages of the tile
-      float lv[kH], unit[kH];
-      bool vbad = false;
-#pragma unroll
-      for (int i = 0; i < kH; ++i) {
-        const int e = (int)(__float_as_uint(st.vs[i]) >> 23) - 127;
-        const bool bad = !(st.vs[i] < INFINITY);
-        vbad |= bad;
-        lv[i] = bad ? 0.f : (float)e;
-        unit[i] = exp2i(bad ? 0 : -e);
-      }
-      const bool part = kb + 32 > all_see;  // some row does not see all of the tile
-      uint32_t pw[NQ][4];
-      bool raise[NQ];
-      float fac[NQ];
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        float x[4][2], ck[kH];
-#pragma unroll
-        for (int i = 0; i < kH; ++i) ck[i] = c_row[n] * st.ks[i];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) x[j][i] = fmaf(d[j][2 * n + i], ck[P16 ? j >> 1 : 0], lv[P16 ? j >> 1 : 0]);
-        if (part) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (kb + 8 * j + 2 * t + i >= end[n]) x[j][i] = -INFINITY;
-        }
-        float mx = fmax3(fmax3(x[0][0], x[0][1], x[1][0]), fmax3(x[1][1], x[2][0], x[2][1]), fmaxf(x[3][0], x[3][1]));
-        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-        raise[n] = mx > M[n] + kRaise;
-        const float m_new = raise[n] ? mx - kBelow : M[n];
-        fac[n] = raise[n] ? exp2_approx(M[n] - m_new) : 1.f;  // 2^-inf = 0 the first time
-        M[n] = m_new;
-        const float ref = m_new == -INFINITY ? 0.f : m_new;
-        float sum[2] = {0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float e0 = exp2_approx(x[j][0] - ref), e1 = exp2_approx(x[j][1] - ref);
-          sum[j >> 1] += e0 + e1;
-          pw[n][j] = pack_f16x2(e0, e1);
-        }
-        // the exponentials without their values' scale: 2^(x - M) = w 2^-lv
-        l[n] *= fac[n];
-        if constexpr (P16) l[n] = fmaf(sum[0], unit[0], fmaf(sum[1], unit[kH - 1], l[n]));
-        else l[n] = fmaf(sum[0] + sum[1], unit[0], l[n]);
-        if (vbad) {  // values that are NaN, where the row sees them
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (!(st.vs[P16 ? j >> 1 : 0] < INFINITY)) {
-              if (x[j][0] > -INFINITY) pw[n][j] |= 0x7fffu;
-              if (x[j][1] > -INFINITY) pw[n][j] |= 0x7fff0000u;
-            }
-        }
-      }
-      if (__any_sync(~0u, raise[0] || (NQ == 2 && raise[NQ - 1]))) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {  // the factors lie with the rows, the output has them as columns 2t, 2t + 1
-          const float f0 = __shfl_sync(~0u, fac[n], 8 * t), f1 = __shfl_sync(~0u, fac[n], 8 * t + 4);
-#pragma unroll
-          for (int i = 0; i < kM; ++i) {
-            o[n][i][0] *= f0;
-            o[n][i][1] *= f1;
-            o[n][i][2] *= f0;
-            o[n][i][3] *= f1;
-          }
-        }
-      }
-      const bool tail = kb + 32 > kv;  // places of the page past the last key may hold anything, NaN codes too
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t vw[4][HD / 32];  // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the half
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint8_t* const q = bytes + (16 * i + 8 * (j >> 1)) * HD + get_v[j & 1];
-          if constexpr (HD == 128) {
-            const uint4 u = *reinterpret_cast<const uint4*>(q);
-            vw[j][0] = u.x;
-            vw[j][1] = u.y;
-            vw[j][HD / 32 - 2] = u.z;
-            vw[j][HD / 32 - 1] = u.w;
-          } else {
-            const uint2 u = *reinterpret_cast<const uint2*>(q);
-            vw[j][0] = u.x;
-            vw[j][1] = u.y;
-          }
-        }
-        if (tail) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (kb + 16 * i + 2 * t + (j & 1) + 8 * (j >> 1) >= kv)
-#pragma unroll
-              for (int x = 0; x < HD / 32; ++x) vw[j][x] = 0;
-        }
-#pragma unroll
-        for (int x = 0; x < HD / 32; ++x)
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const uint2 lo = e4m3x4_to_f16x4(__byte_perm(vw[0][x], vw[1][x], y ? 0x7362 : 0x5140));
-            const uint2 hi = e4m3x4_to_f16x4(__byte_perm(vw[2][x], vw[3][x], y ? 0x7362 : 0x5140));
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) mma_f16(o[n][2 * x + y], lo.x, lo.y, hi.x, hi.y, pw[n][2 * i], pw[n][2 * i + 1]);
-          }
-      }
+      tile_step<HD, NQ, false, P16>(q, nullptr, st, get_k, get_v, kt * 32, kv, all_see);
     }
-    // this thread's columns of queries 2t and 2t + 1: HD / 8 in a row
     const bool whole = kt0 == 0 && kt1 == nt;
-    float* const part = filled ? reinterpret_cast<float*>(ring + warp * kS * sizeof(FewStage<HD>))
-                               : part_of(p.ws, 2 * w + (first ? 0 : 1), 16, HD);
+    float* const part = whole    ? nullptr
+                        : filled ? reinterpret_cast<float*>(ring + warp * kS * sizeof(FewStage<HD>))
+                                 : part_of(p.ws, 2 * w + (first ? 0 : 1), 16, HD);
     if (filled) {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       __syncwarp();  // the warp's ring is read to the end
     }
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float sum = l[n];
-      sum += __shfl_xor_sync(~0u, sum, 1);
-      sum += __shfl_xor_sync(~0u, sum, 2);
-      const float top = sum != sum ? fmaxf(M[n], -1e30f) : M[n];  // a NaN counts, even where M saw nothing else
-      if (!whole && t == 0 && 8 * n + g < rows) {
-        part[16 * HD + 8 * n + g] = top;
-        part[16 * HD + 16 + 8 * n + g] = sum;
-      }
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const int row = 8 * n + 2 * t + y;
-        const float ls = __shfl_sync(~0u, sum, 8 * t + 4 * y), Ms = __shfl_sync(~0u, top, 8 * t + 4 * y);
-        if (row >= rows) continue;
-#pragma unroll
-        for (int i = 0; i < kM; i += 2) {
-          const int d = g * (HD / 8) + 2 * i;
-          const float4 v = make_float4(o[n][i][y], o[n][i][2 + y], o[n][i + 1][y], o[n][i + 1][2 + y]);
-          if (whole) store_row<HALF>(p, row0 + row / group, hk * group + row % group, HD, d, v, Ms, ls);
-          else *reinterpret_cast<float4*>(part + row * HD + d) = v;
-        }
-      }
-    }
-    if (filled) {  // all four warps come here, each with its one segment
+    store_rows<HD, HALF, NQ, false>(p, q, row0, 0, rows, hk, part, 16);
+    if (filled) {  // all the block's warps come here, each with its one segment
       __syncthreads();
-      float* const out = part_of(p.ws, 2 * (4 * blockIdx.x), 16, HD);
+      float* const out = part_of(p.ws, 2 * few_warps * blockIdx.x, 16, HD);
       const float* const in = reinterpret_cast<const float*>(ring);
       constexpr int kLd = kS * (int)sizeof(FewStage<HD>) / 4;
-      for (int i = threadIdx.x; i < rows * (HD / 4); i += 128) {
+      for (int i = threadIdx.x; i < rows * (HD / 4); i += 32 * few_warps) {
         const int row = i / (HD / 4), d = i % (HD / 4) * 4;
-        float m[4], top = -INFINITY, sum = 0.f;
+        float m[few_warps], top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < few_warps; ++x) {
           m[x] = in[x * kLd + 16 * HD + row];
           top = fmaxf(top, m[x]);
         }
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         if (top > -INFINITY) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
+          for (int x = 0; x < few_warps; ++x) {
             const float e = exp2_approx(m[x] - top);
             const float4 v = *reinterpret_cast<const float4*>(in + x * kLd + row * HD + d);
             acc.x = fmaf(e, v.x, acc.x);
@@ -416,12 +530,108 @@ __global__ void __launch_bounds__(128, few_blocks(HD, NQ)) k_paged_few(const Att
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
+// ---------------------------------------------------------------- 17 to 64 query rows to a key head
+//
+// Windows: what bounds them is still HBM, or close to it the mma pipe (4 HD flops for each key and row), and a segment is
+// a few tiles long, so what counts is that a block begins and ends one cheaply and that other blocks run meanwhile.  A
+// worker is a block of 4 warps with 16 rows each; it takes 64 keys at a time, of which each warp copies a quarter (32
+// keys' K or V) into the block's ring and all four read all.  Tiles of 128 rows on tcgen05 (paged_attn_tc.cu) have the
+// faster products, but their hand-overs from copies to widening to products to softmax and back cost a 50-row window more
+// than its work.
+template <int HD, bool HALF, bool P16>
+__global__ void __launch_bounds__(32 * mid_warps, mid_blocks(HD)) k_paged_mid(const AttnDev p) {
+  extern __shared__ __align__(16) uint8_t ring[];
+  constexpr int kS = mid_stages;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int w = blockIdx.x, group = p.group;
+  const FewStage<HD>* const stage = reinterpret_cast<const FewStage<HD>*>(ring);
+  const uint64_t policy = l2_policy_evict_first();
+  uint32_t put[2], get_k, get_v[2];
+  stage_places<HD>(put, get_k, get_v);
+  pdl_wait();
+  pdl_launch();
+  Walk at;
+  if (!at.begin(p, w)) return;
+
+  // ---- copies: a tile's quarters are K and V codes of its keys 0-31 and 32-63; a warp has every mid_warps-th
+  constexpr int kOwn = 4 / mid_warps;
+  Walk ahead = at;
+  int kt_a = at.kt0, pgA[kOwn], pgB[kOwn];
+  bool live = true;
+  auto look_up = [&]() {
+    if (!live) return;
+#pragma unroll
+    for (int u = 0; u < kOwn; ++u) {
+      const int key = kt_a * 64 + 32 * ((warp + u * mid_warps) >> 1);
+      const int* const table = p.table + (size_t)ahead.r * p.table_ld + (key >> p.shift);
+      pgA[u] = key < ahead.kv ? __ldg(table) : -2;  // -2: no keys
+      pgB[u] = P16 && key + 16 < ahead.kv ? __ldg(table + 1) : pgA[u];
+    }
+  };
+  auto send = [&](int to_stage) {
+    if (live) {
+#pragma unroll
+      for (int u = 0; u < kOwn; ++u) {
+        const int half = (warp + u * mid_warps) >> 1, x = (warp + u * mid_warps) & 1;
+        if (pgA[u] == -2) continue;
+        if ((unsigned)pgA[u] >= (unsigned)p.pages || (unsigned)pgB[u] >= (unsigned)p.pages) {
+          atomicExch(p.status, T2W_ERR_INVALID);
+          pgA[u] = pgB[u] = 0;
+        }
+        const uint32_t to = smem_u32(ring) + (2 * to_stage + half) * (uint32_t)sizeof(FewStage<HD>);
+        const long long in =
+            ((long long)ahead.hk * p.page + (P16 ? 0 : (kt_a * 64 + 32 * half) & (p.page - 1))) * HD + 16 * lane;
+        const uint8_t* const lo = p.codes[x] + pgA[u] * p.page_ld[x] + in;
+        const uint8_t* const hi = P16 ? p.codes[x] + pgB[u] * p.page_ld[x] + in : lo + 16 * HD;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i)
+          copy16(to + x * 32 * HD + i * 512 + put[i & 1], i < HD / 32 ? lo + i * 512 : hi + (i - HD / 32) * 512, policy);
+        if (lane < 2)  // ks or vs
+          copy4(to + 64 * HD + 8 * x + 4 * lane, p.scales[x] + (lane ? pgB[u] : pgA[u]) * p.scale_ld[x] + ahead.hk);
+      }
+      if (++kt_a == ahead.kt1) {
+        live = ahead.next(p);
+        kt_a = 0;
+      }
+      look_up();
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  look_up();
+#pragma unroll
+  for (int i = 0; i < kS - 1; ++i) send(i);
+
+  // ---- segments
+  int st = 0;  // the stage of the next tile
+  do {
+    const int rows = at.rows(p, group), from = 16 * warp, row0 = at.row0 + at.qt * p.tq, before = at.kv - at.f + at.qt * p.tq;
+    const bool mine = from < rows;
+    // keys that all of the warp's rows see, and that one of them sees
+    const int all_see = p.causal ? before + over_group(p, from) + 1 : at.kv;
+    const int some_see = p.causal ? before + over_group(p, min(from + 16, rows) - 1) + 1 : at.kv;
+    Rows<HD, 2, false> q;
+    load_rows<HD, HALF, 2, false>(p, q, nullptr, row0, from, rows, at.hk, before, at.kv);
+    for (int kt = at.kt0; kt < at.kt1; ++kt) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kS - 2) : "memory");
+      __syncthreads();  // every warp's copies of this tile are there, and nobody reads the stage before it any more
+      send(st ? st - 1 : kS - 1);
+      if (mine)
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i)
+          if (kt * 64 + 32 * i < some_see)
+            tile_step<HD, 2, false, P16>(q, nullptr, stage[2 * st + i], get_k, get_v, kt * 64 + 32 * i, at.kv, all_see);
+      st = st + 1 == kS ? 0 : st + 1;
+    }
+    float* const part = at.kt0 == 0 && at.kt1 == at.nt ? nullptr : part_of(p.ws, 2 * w + (at.first ? 0 : 1), 16 * mid_warps, HD);
+    if (mine) store_rows<HD, HALF, 2, false>(p, q, row0, from, rows, at.hk, part, 16 * mid_warps);
+  } while (at.next(p));
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
 // ---------------------------------------------------------------- segments that were cut
-// Where worker w's start is the first cut of a segment, one warp for each row joins the parts of that segment; where
-// there are many of them, the whole block, its warps taking every 4th part.  The order is fixed, so the bits are too.
-// A block looks after 8 workers' starts, and rows blockIdx.y, + gridDim.y, ...  What it costs is a chain of loads after
-// the kernel in front of it has ended: so all that the plan tells is read before that, and the parts' rows are sent for
-// together with their exponents.
+// Where worker w's start is the first cut of a segment, a warp (or a few, for the rows' shares) joins the parts of that
+// segment: up to 4 parts a thread four columns of a row, more of them row by row.  The order is fixed, so the bits are too.  What it costs is a chain of loads after the kernel in front of it has ended:
+// so all that the plan tells is read before that, and the parts' rows are sent for together with their exponents.
 struct Parts {
   const float* ws;
   int rows_ld, hd;
@@ -446,19 +656,19 @@ T2W_DEV void load_cols(float (&u)[N], const float* v) {
   if constexpr (N == 4) *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(v);
   else *reinterpret_cast<float2*>(u) = *reinterpret_cast<const float2*>(v);
 }
-// Parts from, from + step, ... of a row: a lane holds one part's exponent and sum of 32, and N columns of all of them.
+// A row's parts: a lane holds one part's exponent and sum of 32, and N columns of all of them.
 template <int HD>
-T2W_DEV void join_parts(Joined<HD>& j, const Parts& parts, int from, int step, int row, int lane) {
-  constexpr int N = HD / 32, K = 4;
+T2W_DEV void join_parts(Joined<HD>& j, const Parts& parts, int row, int lane) {
+  constexpr int N = HD / 32, K = 8;
   j.top = -INFINITY;
   j.sum = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) j.acc[i] = 0.f;
-  for (int x0 = from; x0 < parts.n; x0 += 32 * step) {
-    const int n = min(32, (parts.n - x0 + step - 1) / step);
+  for (int x0 = 0; x0 < parts.n; x0 += 32) {
+    const int n = min(32, parts.n - x0);
     float top = -INFINITY, sum = 0.f;
     if (lane < n) {
-      const float* q = parts.at(x0 + lane * step) + parts.rows_ld * HD + row;
+      const float* q = parts.at(x0 + lane) + parts.rows_ld * HD + row;
       top = __ldcg(q);
       sum = __ldcg(q + parts.rows_ld);
     }
@@ -469,7 +679,7 @@ T2W_DEV void join_parts(Joined<HD>& j, const Parts& parts, int from, int step, i
       for (int i = 0; i < K; ++i) {
 #pragma unroll
         for (int y = 0; y < N; ++y) u[i][y] = 0.f;
-        if (i0 + i < n) load_cols<N>(u[i], parts.at(x0 + (i0 + i) * step) + row * HD + lane * N);
+        if (i0 + i < n) load_cols<N>(u[i], parts.at(x0 + i0 + i) + row * HD + lane * N);
       }
       if (i0 == 0) {
         m = fmaxf(j.top, top);
@@ -501,48 +711,31 @@ T2W_DEV void store_joined(const AttnDev& p, const Joined<HD>& j, int row, int he
   }
 }
 
-constexpr int kMany = 24;  // parts from which the whole block joins a row
-
 template <int HD, bool HALF>
-__global__ void __launch_bounds__(128, 8) k_paged_merge(const AttnDev p) {
-  __shared__ Joined<HD> js[4][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = p.q_heads / p.kv_heads;
+__global__ void __launch_bounds__(256) k_paged_merge(const AttnDev p) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = p.group;
   // The plan was complete before the kernel in front of this one began (it waited for it), so it is read ahead of the
   // wait, past this SM's L1.
   const int4 h0 = __ldcg(reinterpret_cast<const int4*>(p.head)), h1 = __ldcg(reinterpret_cast<const int4*>(p.head) + 1);
   const int per = h0.z, workers = h0.w, used = h1.y, extra = h1.w;
-  const int w = blockIdx.x * 8 + lane;
-  int4 seg = make_int4(0, 0, 0, 0);
-  int a = 0, nt = 0, row0 = 0, rows = 0;
+  // a warp has a start, and of its rows the share blockIdx.y of gridDim.y
+  const int w = blockIdx.x * 8 + warp, share = blockIdx.y, shares = gridDim.y;
   bool mine = false;
-  if (lane < 8 && w > 0 && w < workers) {
-    seg = __ldcg(p.starts + 2 * w);
-    const int4 of = __ldcg(p.starts + 2 * w + 1);  // first row, rows, keys
-    a = w * per - seg.w;  // the place of the segment's tile 0
-    mine = seg.w > 0 && a >= (w - 1) * per;
-    nt = seg_tiles(tile_keys(of.y, of.z, p.causal, p.tq, seg.z), p.kt);
-    row0 = of.x + seg.z * p.tq;
-    rows = min(p.tq, of.y - seg.z * p.tq) * group;
-  }
-  unsigned todo = __ballot_sync(~0u, mine);
-  int turn = 0;
-  pdl_wait();
-  pdl_launch();
-  // padding
-  for (int row = used + blockIdx.y * gridDim.x + blockIdx.x; row < p.rows; row += gridDim.x * gridDim.y)
-    for (int i = threadIdx.x; i < p.q_heads * (HD / 4); i += blockDim.x)
-      store_row<HALF>(p, row, i / (HD / 4), HD, i % (HD / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
-  while (todo) {
-    const int i = __ffs(todo) - 1;
-    todo &= todo - 1;
-    const int r0 = __shfl_sync(~0u, row0, i), rn = __shfl_sync(~0u, rows, i), hk = __shfl_sync(~0u, seg.y, i);
-    const int at = __shfl_sync(~0u, a, i), end = at + __shfl_sync(~0u, nt, i);
-    Parts parts;
+  int r0 = 0, rn = 0, head0 = 0;
+  Parts parts;
+  if (w > 0 && w < workers) {
+    const int4 seg = __ldcg(p.starts + 2 * w), of = __ldcg(p.starts + 2 * w + 1);  // of: first row, rows, keys
+    const int at = of.w - seg.w, before = __ldcg(p.starts + 2 * w - 1).w;  // the place of the segment's tile 0; where w - 1 begins
+    mine = seg.w > 0 && at >= before;
+    const int end = at + seg_tiles(tile_keys(of.y, of.z, p.causal, p.tq, seg.z), p.kt);
+    r0 = of.x + seg.z * p.tq;
+    rn = min(p.tq, of.y - seg.z * p.tq) * group;
+    head0 = seg.y * group;
     parts.ws = p.ws;
     parts.rows_ld = p.part_rows;
     parts.hd = HD;
-    parts.w0 = blockIdx.x * 8 + i - 1;
-    parts.second = at - extra > parts.w0 * per;
+    parts.w0 = w - 1;
+    parts.second = at - extra > before;
     const int last = (end - 1) / per, bw = p.block_workers;
     const int b0 = (at + bw * per - 1) / (bw * per), b1 = end / (bw * per);  // blocks that the segment fills
     parts.block_workers = bw;
@@ -551,37 +744,51 @@ __global__ void __launch_bounds__(128, 8) k_paged_merge(const AttnDev p) {
     parts.lead = parts.mid ? b0 * bw - parts.w0 : last - parts.w0 + 1;
     parts.tail0 = b1 * bw;
     parts.n = parts.mid ? parts.lead + parts.mid + last - b1 * bw + 1 : parts.lead;
-    for (int row = blockIdx.y; row < rn; row += gridDim.y) {
-      const int out_row = r0 + row / group, head = hk * group + row % group;
-      Joined<HD> j;
-      if (parts.n < kMany) {
-        if ((turn++ & 3) != warp) continue;
-        join_parts<HD>(j, parts, 0, 1, row, lane);
-        store_joined<HD, HALF>(p, j, out_row, head, lane);
-      } else {
-        join_parts<HD>(j, parts, warp, 4, row, lane);
-        js[warp][lane] = j;
-        __syncthreads();
-        if (warp == 0) {
-          float top = j.top;
+  }
+  pdl_wait();
+  pdl_launch();
+  // padding
+  for (int row = used + blockIdx.y * gridDim.x + blockIdx.x; row < p.rows; row += gridDim.x * gridDim.y)
+    for (int i = threadIdx.x; i < p.q_heads * (HD / 4); i += blockDim.x)
+      store_row<HALF>(p, row, i / (HD / 4), HD, i % (HD / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
+  if (!mine) return;
+  if (parts.n <= 4) {  // a thread four columns of a row
+    const float* part[4];
 #pragma unroll
-          for (int x = 1; x < 4; ++x) top = fmaxf(top, js[x][0].top);
-          Joined<HD> s = {};
-          s.top = top;
-          if (top > -INFINITY)
+    for (int i = 0; i < 4; ++i) part[i] = parts.at(min(i, parts.n - 1));
+#pragma unroll 2
+    for (int i = share * 32 + lane; i < rn * (HD / 4); i += 32 * shares) {
+      const int row = i / (HD / 4), d = i % (HD / 4) * 4;
+      float m[4], l[4], top = -INFINITY;
+      float4 v[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const Joined<HD>& u = js[x][lane];
-              const float e = exp2_approx(u.top - top);
-              s.sum = fmaf(e, u.sum, s.sum);
-#pragma unroll
-              for (int y = 0; y < HD / 32; ++y) s.acc[y] = fmaf(e, u.acc[y], s.acc[y]);
-            }
-          store_joined<HD, HALF>(p, s, out_row, head, lane);
-        }
-        __syncthreads();
+      for (int x = 0; x < 4; ++x) {
+        v[x] = __ldcg(reinterpret_cast<const float4*>(part[x] + row * HD + d));
+        m[x] = x < parts.n ? __ldcg(part[x] + p.part_rows * HD + row) : -INFINITY;
+        l[x] = __ldcg(part[x] + p.part_rows * HD + p.part_rows + row);
+        top = fmaxf(top, m[x]);
       }
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float sum = 0.f;
+      if (top > -INFINITY) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float e = exp2_approx(m[x] - top);
+          acc.x = fmaf(e, v[x].x, acc.x);
+          acc.y = fmaf(e, v[x].y, acc.y);
+          acc.z = fmaf(e, v[x].z, acc.z);
+          acc.w = fmaf(e, v[x].w, acc.w);
+          sum = fmaf(e, l[x], sum);
+        }
+      }
+      store_row<HALF>(p, r0 + over_group(p, row), head0 + row - group * over_group(p, row), HD, d, acc, top, sum);
     }
+    return;
+  }
+  for (int row = share; row < rn; row += shares) {
+    Joined<HD> j;
+    join_parts<HD>(j, parts, row, lane);
+    store_joined<HD, HALF>(p, j, r0 + over_group(p, row), head0 + row - group * over_group(p, row), lane);
   }
 }
 
@@ -594,22 +801,35 @@ namespace {
 
 template <int HD, bool HALF>
 cudaError_t launch_paged(const AttnDev& p, const PagedCut& cut, int max_rows, cudaStream_t st) {
-  if (cut.mma) {
+  auto merge = [&](int shares) {
+    return launch_k(k_paged_merge<HD, HALF>, dim3((cut.workers + 7) / 8, shares), dim3(256), 0, st, p);
+  };
+  if (cut.form == PagedForm::kMid) {
+    constexpr int smem = 2 * mid_stages * (int)sizeof(FewStage<HD>);
+    static std::atomic<uint64_t> done[2];
+    auto mid = [&](auto* k, std::atomic<uint64_t>& d) {
+      const cudaError_t r = smem_attr_once(k, smem, d);
+      return r != cudaSuccess ? r : launch_k(k, dim3(cut.workers), dim3(32 * mid_warps), smem, st, p);
+    };
+    const cudaError_t e = p.page == 16 ? mid(k_paged_mid<HD, HALF, true>, done[0]) : mid(k_paged_mid<HD, HALF, false>, done[1]);
+    return e != cudaSuccess ? e : merge(cut.form == PagedForm::kMany ? 32 : 16);
+  }
+  if (cut.form == PagedForm::kMany) {
     const cudaError_t e = launch_paged_many(p, cut, HD, HALF, st);
-    return e != cudaSuccess ? e : launch_k(k_paged_merge<HD, HALF>, dim3((cut.workers + 7) / 8, 16), dim3(128), 0, st, p);
+    return e != cudaSuccess ? e : merge(cut.form == PagedForm::kMany ? 32 : 16);
   }
   const int nq = max_rows > 8 ? 2 : 1;
-  constexpr int smem = 4 * few_stages * (int)sizeof(FewStage<HD>);
+  constexpr int smem = few_warps * few_stages * (int)sizeof(FewStage<HD>);
   static std::atomic<uint64_t> done[4];
   auto few = [&](auto* k, std::atomic<uint64_t>& d) {
     const cudaError_t r = smem_attr_once(k, smem, d);
-    return r != cudaSuccess ? r : launch_k(k, dim3(cut.workers / 4), dim3(128), smem, st, p);
+    return r != cudaSuccess ? r : launch_k(k, dim3(cut.workers / few_warps), dim3(32 * few_warps), smem, st, p);
   };
   cudaError_t e;
   if (p.page == 16) e = nq == 1 ? few(k_paged_few<HD, HALF, 1, true>, done[0]) : few(k_paged_few<HD, HALF, 2, true>, done[1]);
   else e = nq == 1 ? few(k_paged_few<HD, HALF, 1, false>, done[2]) : few(k_paged_few<HD, HALF, 2, false>, done[3]);
   if (e != cudaSuccess) return e;
-  return launch_k(k_paged_merge<HD, HALF>, dim3((cut.workers + 7) / 8, max_rows), dim3(128), 0, st, p);
+  return merge(max_rows < 8 ? max_rows : 8);
 }
 
 }  // namespace
@@ -617,7 +837,7 @@ cudaError_t launch_paged(const AttnDev& p, const PagedCut& cut, int max_rows, cu
 extern "C" size_t t2w_paged_workspace_bytes(int32_t max_fresh, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
   if (max_fresh <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
   const PagedCut c = paged_cut(max_fresh, q_heads, kv_heads, head_dim);
-  return 2 * (size_t)c.workers * (c.mma ? 128 : 16) * (head_dim + 2) * sizeof(float);
+  return 2 * (size_t)c.workers * c.part_rows * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int t2w_paged_attn(const t2w_paged_attn_args* a, void* stream) {
@@ -661,6 +881,8 @@ extern "C" int t2w_paged_attn(const t2w_paged_attn_args* a, void* stream) {
   p.q_heads = a->q_heads;
   p.kv_heads = a->kv_heads;
   p.causal = a->causal != 0;
+  p.group = a->q_heads / a->kv_heads;
+  p.group_mul = (65536 + p.group - 1) / p.group;
   p.scale = a->scale;
   p.head = reinterpret_cast<const PlanHead*>(a->plan);
   p.q_start = a->plan + l.q_start;
@@ -668,8 +890,8 @@ extern "C" int t2w_paged_attn(const t2w_paged_attn_args* a, void* stream) {
   p.starts = reinterpret_cast<const int4*>(a->plan + l.starts);
   p.tq = cut.tq;
   p.kt = cut.kt;
-  p.part_rows = cut.mma ? 128 : 16;
-  p.block_workers = cut.mma ? 1 : 4;
+  p.part_rows = cut.part_rows;
+  p.block_workers = cut.form == PagedForm::kFew ? few_warps : 1;
   p.ws = static_cast<float*>(a->workspace);
   p.out = a->out;
   p.lse = a->lse;

@@ -14,6 +14,7 @@ struct AttnDev {
   long long page_ld[2], scale_ld[2];
   const int* table;
   int table_ld, page, shift, pages, rows, q_heads, kv_heads, causal;
+  int group, group_mul;  // query heads to a key head, and ceil(2^16 / group)
   float scale;
   const PlanHead* head;
   const int *q_start, *kv_len;
@@ -24,6 +25,9 @@ struct AttnDev {
   float* lse;
   int* status;
 };
+
+// row / group for a row of a tile: exact below 128 rows, where row (group_mul group - 2^16) < 2^14.
+T2W_DEV int over_group(const AttnDev& p, int row) { return row * p.group_mul >> 16; }
 
 // Four columns of a finished row: O / l, and with the first columns its log-sum.
 template <bool HALF>
@@ -83,12 +87,13 @@ T2W_DEV uint32_t pack_f16x2(float a, float b) {
 template <bool HALF>
 T2W_DEV int row_shift(uint32_t max_bits16) {
   if (HALF || max_bits16 == 0 || max_bits16 >= 0x7f80u) return 0;
-  return 14 - ((int)(max_bits16 >> 7) - 127);
+  return min(14 - ((int)(max_bits16 >> 7) - 127), 127);
 }
 template <bool HALF>
 T2W_DEV uint32_t row_half2(uint32_t u, int shift, bool negate) {
   if constexpr (HALF) return negate ? u ^ 0x80008000u : u;
-  const float a = scaled(__uint_as_float(u << 16), shift), b = scaled(__uint_as_float(u & 0xffff0000u), shift);
+  const float f = exp2i(shift);
+  const float a = __uint_as_float(u << 16) * f, b = __uint_as_float(u & 0xffff0000u) * f;
   return negate ? pack_f16x2(-a, -b) : pack_f16x2(a, b);
 }
 
@@ -100,6 +105,61 @@ constexpr float kRaise = 15.f, kBelow = 9.f;
 
 // A worker's unfinished rows of a segment: O [rows][HD], then the reference exponents [rows] and the sums [rows].
 T2W_DEV float* part_of(float* ws, int slot, int rows, int hd) { return ws + (size_t)slot * rows * (hd + 2); }
+
+// A worker's walk over its segments: every role makes it for itself.
+struct Walk {
+  int r, hk, qt;       // the segment
+  int row0, f, kv;     // its request's first row, rows and keys
+  int kt0, kt1, nt;    // the tiles of it that are this worker's, and all of them
+  int zero, stop;      // the place of its tile 0; the end of the worker's places
+  int extra;
+  bool first;
+
+  T2W_DEV void cut(const AttnDev& p, int from) {
+    nt = seg_tiles(tile_keys(f, kv, p.causal, p.tq, qt), p.kt);
+    kt0 = from;
+    kt1 = min(nt, stop - zero);
+  }
+  T2W_DEV bool begin(const AttnDev& p, int w) {
+    const int4 h = *reinterpret_cast<const int4*>(p.head);  // n_runs, places, per, workers
+    const int4 s = p.starts[2 * w], of = p.starts[2 * w + 1];
+    extra = p.head->extra;
+    if (w >= h.w) return false;
+    r = s.x;
+    hk = s.y;
+    qt = s.z;
+    row0 = of.x;
+    f = of.y;
+    kv = of.z;
+    stop = p.starts[2 * w + 3].w;
+    zero = of.w - s.w;
+    if (zero >= stop) return false;
+    first = true;
+    cut(p, max(s.w, 0));
+    return kt0 < kt1;
+  }
+  T2W_DEV bool next(const AttnDev& p) {
+    if (kt1 < nt) return false;
+    zero += nt + extra;
+    if (zero >= stop) return false;
+    first = false;
+    if (++qt * p.tq >= f) {
+      qt = 0;
+      if (++hk == p.kv_heads) {
+        hk = 0;
+        do {
+          r++;
+          row0 = p.q_start[r];
+          f = p.q_start[r + 1] - row0;
+        } while (f == 0);  // places are left, so there is a request with rows
+        kv = p.kv_len[r];
+      }
+    }
+    cut(p, 0);
+    return true;
+  }
+  T2W_DEV int rows(const AttnDev& p, int group) const { return min(p.tq, f - qt * p.tq) * group; }
+};
 
 // Segments of up to 128 query rows on tcgen05 tiles (paged_attn_tc.cu): the parts of cut segments into p.ws.
 cudaError_t launch_paged_many(const AttnDev& p, const PagedCut& cut, int head_dim, bool half, cudaStream_t st);

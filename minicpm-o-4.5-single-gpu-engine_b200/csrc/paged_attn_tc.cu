@@ -12,11 +12,17 @@
 // chunks (a page holds 16 keys at least), and bf16 queries are brought into their range by a power of two for each row.
 // fp8 operands would spare the widening, but not the rounding of queries and weights to 4 bits.
 //
-// Two blocks an SM, each 3 warpgroups: warps 0-3 softmax (a thread a row), 4-7 widen, 8 the MMA issuer (9-11 only give up
-// their registers: 128 a softmax thread, 72 and 40 the others, of the 80 each that the block is launched with).  Warps
-// 4-7 copy the codes of the tiles ahead into a ring of their own with asynchronous copies, a thread its own pieces, and write them as halves in the
-// 128-byte swizzle that the tensor core reads.  K and V tiles have rings of their own, since a K tile is free as soon as
-// its scores are there.  A segment's output is finished during the next segment's first tile.
+// Two blocks an SM, each three warpgroups.  Warps 0-3 softmax, a thread a row; a segment's output is finished during the
+// next segment's first tile.  Warps 4-7 widen: they write a tile's codes as halves in the 128-byte swizzle that the tensor
+// core reads, K a tile ahead of V.  Warp 8 issues the products, warp 10 walks the segments and sends for the tiles ahead (a
+// bulk copy for each page), warp 11 brings the next segment's queries.  Of the 80 registers that a thread of the block is launched with, the three warpgroups take 128, 64
+// and 48.
+//
+// The roles' code is kept short (loops where the trip count is known, one walk over the segments for all): with the first
+// version's 62 KB the softmax warps waited for instructions most of the time.
+//
+// Segments of at most 64 rows (windows) lie in the upper rows of every other block's tiles: a warp's exponentials run on
+// the SM quarter that its TMEM lanes belong to, and so the two blocks of an SM use all four.
 //
 // What bounds it: for windows of some ten rows HBM (the codes are read once; 8 KB a tile at 64 columns), for longer
 // chunks the exponentials: 16 a clock and SM, 512 clocks a tile, against 256 (head_dim 64) or 512 (128) of the tensor
@@ -27,48 +33,43 @@ namespace t2w {
 namespace {
 
 constexpr int kRows = 128, kKeys = 64;
-constexpr int kThreads = 384, kWiden = 128;  // threads; of them widening
-constexpr int kTmem = 256;                   // S / W buffers at 0 and 64, O at 128
+constexpr int kThreads = 384;
+constexpr int kTmem = 256;  // S / W buffers at 0 and 64, O at 128
 
-// Rings by head_dim: query buffers, K and V tiles of halves, tiles of codes on their way.
+// Rings by head_dim: query buffers, K and V tiles of halves, and tiles of codes on their way (Ahead; a tile's K codes are
+// kept until they are widened, its V codes one step longer).
 template <int HD>
 struct Rings {
-  static constexpr int Q = HD == 64 ? 2 : 1, K = HD == 64 ? 2 : 1, V = HD == 64 ? 2 : 1, Raw = HD == 64 ? 4 : 2;
-  static constexpr int q_bytes = kRows * HD * 2, tile_bytes = kKeys * HD * 2, raw_bytes = 2 * kKeys * HD;
-  static constexpr int k_at = Q * q_bytes, v_at = k_at + K * tile_bytes, raw_at = v_at + V * tile_bytes;
-  static constexpr int aux_at = raw_at + Raw * raw_bytes;
+  static constexpr int Q = HD == 64 ? 2 : 1, K = HD == 64 ? 2 : 1, V = HD == 64 ? 2 : 1, Ahead = HD == 64 ? 3 : 1;
+  static constexpr int RawK = Ahead + 1, RawV = Ahead + 2;
+  static constexpr int q_bytes = kRows * HD * 2, tile_bytes = kKeys * HD * 2, raw_bytes = kKeys * HD;
+  static constexpr int k_at = Q * q_bytes, v_at = k_at + K * tile_bytes, raw_k_at = v_at + V * tile_bytes;
+  static constexpr int raw_v_at = raw_k_at + RawK * raw_bytes, aux_at = raw_v_at + RawV * raw_bytes;
+};
+// A segment, as the copies' warp tells the others; rows == 0: there are no more.
+struct Seg {
+  int row0, rows, head0;   // first token row, rows, first query head
+  int before, kv;          // keys ahead of the first token's own (causal), keys
+  int kt0, kt1, slot;      // key tiles; the part's slot, or -1 for a whole segment
 };
 struct Aux {
   uint64_t q_full[2], q_free[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], o_free;
-  uint64_t meta_full[4];  // by tile: ks, vs, and for a segment's first tile c_row
+  uint64_t meta_full[8], shift_full[4];  // by tile: ks, vs; by segment: shift
+  uint64_t raw_full[4], raw_k_empty[4], raw_v_empty[5], seg_full[8];
   uint32_t tmem;
   int pad;
-  float c_row[4][kRows];  // by segment: scale * log2 e / the power of two that the row's queries were multiplied by
-  float ks[4][4], vs[4][4];  // by tile: the scales of its 16-key chunks
-  float scale_raw[4][8];     // the same on their way
+  // By tile: the scales of its 16-key chunks.  The copies' warp is ahead of the softmax by six tiles at most: tile t is
+  // sent for once V of t - RawV (at most 5) has been widened, that is once the product of t - RawV - 2 is done.
+  float ks[8][4], vs[8][4];
+  Seg seg[8];                // by segment, as far ahead as the tiles
+  int16_t shift[4][kRows];   // by segment: the power of two that a row's queries were multiplied by
 };
 
-T2W_DEV void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+T2W_DEV void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
-T2W_DEV void tmem_ld32_nowait(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 T2W_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -85,78 +86,52 @@ T2W_DEV void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint3
 __host__ __device__ constexpr uint32_t idesc_half(int M, int N, bool b_mn_major = false) {
   return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-T2W_DEV void cp16(uint32_t dst, const void* src, uint64_t policy) {
-  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
-}
-T2W_DEV void cp4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-
-// A worker's walk over its segments: every role makes it for itself.
-struct Walk {
-  int r, hk, qt;       // the segment
-  int row0, f, kv;     // its request's first row, rows and keys
-  int kt0, kt1, nt;    // the tiles of it that are this worker's, and all of them
-  int zero, stop;      // the place of its tile 0; the end of the worker's places
-  int extra;
-  bool first;
-
-  T2W_DEV void cut(const AttnDev& p, int from) {
-    nt = seg_tiles(tile_keys(f, kv, p.causal, p.tq, qt), kKeys);
-    kt0 = from;
-    kt1 = min(nt, stop - zero);
-  }
-  T2W_DEV bool begin(const AttnDev& p, int w) {
-    const int4 h = *reinterpret_cast<const int4*>(p.head);  // n_runs, places, per, workers
-    const int4 s = p.starts[2 * w], of = p.starts[2 * w + 1];
-    extra = p.head->extra;
-    if (w >= h.w) return false;
-    r = s.x;
-    hk = s.y;
-    qt = s.z;
-    row0 = of.x;
-    f = of.y;
-    kv = of.z;
-    stop = min((w + 1) * h.z, h.y);
-    zero = w * h.z - s.w;
-    first = true;
-    cut(p, max(s.w, 0));
-    return kt0 < kt1;
-  }
-  T2W_DEV bool next(const AttnDev& p) {
-    if (kt1 < nt) return false;
-    zero += nt + extra;
-    if (zero >= stop) return false;
-    first = false;
-    if (++qt * p.tq >= f) {
-      qt = 0;
-      if (++hk == p.kv_heads) {
-        hk = 0;
-        do {
-          r++;
-          row0 = p.q_start[r];
-          f = p.q_start[r + 1] - row0;
-        } while (f == 0);  // places are left, so there is a request with rows
-        kv = p.kv_len[r];
-      }
+// mbar_wait() in as few instructions as it takes: each of the roles goes round its loop once a tile, and what of it is not
+// in the instruction cache costs more than the wait's looser look at the time.
+T2W_DEV bool bar_wait(uint64_t* bar, uint32_t parity, int* err) {
+  const uint32_t a = smem_u32(bar);
+  unsigned long long t0 = 0;
+  for (uint32_t i = 1; !mbar_try_wait(a, parity); ++i) {
+#ifdef NS
+    __nanosleep(NS);
+#endif
+    if (i & 1023u) continue;
+    const unsigned long long now = globaltimer();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) {
+      atomicExch(err, T2W_ERR_TIMEOUT);
+      return false;
     }
-    cut(p, 0);
-    return true;
   }
-  // rows of the segment
-  T2W_DEV int tokens(const AttnDev& p) const { return min(p.tq, f - qt * p.tq); }
-};
+  return true;
+}
+T2W_DEV void copy16_plain(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+T2W_DEV void bulk_load_hint(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
+}
+
+// log2 of a value scale; 0 for one that is not finite.
+T2W_DEV float exponent(float s) { return s < INFINITY ? (float)((int)(__float_as_uint(s) >> 23) - 127) : 0.f; }
+
+// The tile row that a segment's first row has.
+T2W_DEV int base_of(int rows) { return rows <= 64 && 2 * blockIdx.x >= gridDim.x ? 64 : 0; }
 
 template <int HD, bool HALF>
 __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   using R = Rings<HD>;
   Aux* const x = reinterpret_cast<Aux*>(smem + R::aux_at);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = blockIdx.x, group = p.q_heads / p.kv_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = blockIdx.x, group = p.group;
   constexpr int kPanels = HD / 64;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&x->q_full[i], 4);
+      mbar_init(&x->q_full[i], 1);
       mbar_init(&x->q_free[i], 1);
       mbar_init(&x->k_full[i], 4);
       mbar_init(&x->k_empty[i], 1);
@@ -166,7 +141,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
       mbar_init(&x->p_full[i], 4);
       mbar_init(&x->o_done[i], 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&x->meta_full[i], 4);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&x->shift_full[i], 1);
+      mbar_init(&x->raw_full[i], 1);
+      mbar_init(&x->raw_k_empty[i], 4);
+    }
+    for (int i = 0; i < 5; ++i) mbar_init(&x->raw_v_empty[i], 4);
+    for (int i = 0; i < 8; ++i) {
+      mbar_init(&x->meta_full[i], 1);
+      mbar_init(&x->seg_full[i], 1);
+    }
     mbar_init(&x->o_free, 4);
     fence_mbar_init();
   }
@@ -180,348 +164,427 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
   tc_fence_after();
   pdl_launch();
   const uint32_t tmem = x->tmem;
-  Walk at;
-  bool ok = at.begin(p, w);
+  bool ok = true;
+  auto next_seg = [&](int s) -> const Seg* {  // nullptr: none, or the wait gave up
+    if (!bar_wait(&x->seg_full[s & 7], (s >> 3) & 1, p.status)) {
+      ok = false;
+      return nullptr;
+    }
+    const Seg* const g = &x->seg[s & 7];
+    return g->rows ? g : nullptr;
+  };
 
-  if (warp >= 4 && warp < 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    // ---------------- widening: 128 threads, thread i has the 16-byte pieces i, i + 128, ... of a tile's codes
-    const int i = threadIdx.x - 128;
-    constexpr int kPieces = HD / 16, kN = kKeys * kPieces / kWiden, kStep = kWiden / kPieces;  // pieces a row, a thread; rows between
-    const int row_i = i / kPieces, piece = i % kPieces;
-    const uint64_t policy = l2_policy_evict_first();
-    const uint32_t raw0 = smem_u32(smem + R::raw_at) + 16 * i;
-    Walk ahead = at;  // the tile that is sent for next
-    int kt_a = at.kt0, sent = 0;
-    bool live = ok;
-    auto send = [&]() {
-      if (live) {
-        const int slot = sent % R::Raw;
-        const int* const table = p.table + (size_t)ahead.r * p.table_ld;
-        const int kb = kt_a * kKeys;
-        auto page_of = [&](int key) {
-          const int g = __ldg(table + (key >> p.shift));
-          if ((unsigned)g < (unsigned)p.pages) return (long long)g;
-          atomicExch(p.status, T2W_ERR_INVALID);
-          return 0ll;
-        };
-#pragma unroll
-        for (int j = 0; j < kN; ++j) {
-          const int key = kb + row_i + j * kStep;
-          if (key < ahead.kv) {
-            const long long g = page_of(key);
-            const long long in = ((long long)ahead.hk * p.page + (key & (p.page - 1))) * HD + 16 * piece;
-            const uint32_t dst = raw0 + slot * R::raw_bytes + j * (16 * kWiden);
-            cp16(dst, p.codes[0] + g * p.page_ld[0] + in, policy);
-            cp16(dst + kKeys * HD, p.codes[1] + g * p.page_ld[1] + in, policy);
-          }
-        }
-        if (i < 8) {  // chunk i & 3's scale of K or V; a chunk past the last key takes the first one's
-          const int key = kb + 16 * (i & 3), y = i >> 2;
-          if (kb < ahead.kv) {
-            const long long g = page_of(key < ahead.kv ? key : kb);
-            cp4(smem_u32(&x->scale_raw[slot][i]), p.scales[y] + g * p.scale_ld[y] + ahead.hk);
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp == 8) {
+      // ---------------- S_n, then W V of tile n - 1 (the products of one thread are in order: S_n writes over W_{n-2})
+      if (lane == 0) {
+        constexpr uint32_t idesc_s = idesc_half(kRows, kKeys), idesc_o = idesc_half(kRows, 64, true);
+        int s = -1, left = 0;              // the segment of S_n, and its tiles from n on
+        int sp = 0;                        // the segment of tile n - 1, and whether that tile is its first
+        bool first_p = false;
+        const Seg* g = nullptr;
+        for (int n = 0; ok; ++n) {
+          const bool had = n > 0;
+          if (left <= 1) {
+            g = next_seg(++s);
+            left = g ? g->kt1 - g->kt0 : 0;
+            if (!ok || (g && !bar_wait(&x->q_full[s % R::Q], (s / R::Q) & 1, p.status))) break;
           } else {
-            x->scale_raw[slot][i] = 1.f;
+            --left;
           }
-        }
-        ++sent;
-        if (++kt_a == ahead.kt1) {
-          live = ahead.next(p);
-          kt_a = 0;
+          const bool first_n = g && left == g->kt1 - g->kt0;
+          if (g) {
+            if (!bar_wait(&x->k_full[n % R::K], (n / R::K) & 1, p.status)) break;
+            tc_fence_after();
+            const uint32_t q0 = smem_u32(smem + (s % R::Q) * R::q_bytes), k0 = smem_u32(smem + R::k_at + (n % R::K) * R::tile_bytes);
+#pragma unroll 4
+            for (int kk = 0; kk < HD / 16; ++kk)
+              umma_f16(tmem + 64 * (n & 1), sdesc_sw128(q0 + (kk >> 2) * (kRows * 128) + 32 * (kk & 3), 1024, 16),
+                       sdesc_sw128(k0 + (kk >> 2) * (kKeys * 128) + 32 * (kk & 3), 1024, 16), idesc_s, kk ? 1u : 0u);
+            umma_commit(&x->s_full[n & 1]);
+            umma_commit(&x->k_empty[n % R::K]);
+            if (left == 1) umma_commit(&x->q_free[s % R::Q]);
+          }
+          if (had) {
+            const int t = n - 1;
+            if (!bar_wait(&x->v_full[t % R::V], (t / R::V) & 1, p.status) || !bar_wait(&x->p_full[t & 1], (t >> 1) & 1, p.status)) break;
+            // a segment's first product overwrites O: the softmax has read the previous segment's
+            if (first_p && sp > 0 && !bar_wait(&x->o_free, (sp - 1) & 1, p.status)) break;
+            tc_fence_after();
+            const uint32_t v0 = smem_u32(smem + R::v_at + (t % R::V) * R::tile_bytes);
+#pragma unroll
+            for (int c = 0; c < kPanels; ++c)
+#pragma unroll
+              for (int kk = 0; kk < kKeys / 16; ++kk)
+                umma_f16_ts(tmem + 128 + 64 * c, tmem + 64 * (t & 1) + 8 * kk,
+                            sdesc_sw128(v0 + c * (kKeys * 128) + kk * 16 * 128, 1024, 8192), idesc_o, !first_p || kk ? 1u : 0u);
+            umma_commit(&x->o_done[t & 1]);
+            umma_commit(&x->v_empty[t % R::V]);
+          }
+          if (!g) break;
+          first_p = first_n;
+          sp = s;
         }
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll
-    for (int j = 0; j < R::Raw - 1; ++j) send();
-    int t = 0;  // tiles so far
-    for (int s = 0; ok; ++s) {
-      // queries: thread i has row i
-      {
-        const int qb = s % R::Q, tokens = at.tokens(p), tok = i / group;
-        const bool has = tok < tokens;
-        const uint16_t* const q = static_cast<const uint16_t*>(p.q) + (long long)(at.row0 + at.qt * p.tq + tok) * p.q_row_ld +
-                                  (at.hk * group + i % group) * p.q_head_ld;
-        uint4 v[HD / 8];
-        uint32_t m = 0;
-#pragma unroll
-        for (int c = 0; c < HD / 8; ++c) {
-          v[c] = has ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0, 0, 0, 0);
-          m = __vmaxu2(__vmaxu2(m, v[c].x & 0x7fff7fffu), v[c].y & 0x7fff7fffu);
-          m = __vmaxu2(__vmaxu2(m, v[c].z & 0x7fff7fffu), v[c].w & 0x7fff7fffu);
-        }
-        const int sh = row_shift<HALF>(max(m & 0xffffu, m >> 16));
-        if (!(ok = __all_sync(~0u, mbar_wait(&x->q_free[qb], ((s / R::Q) & 1) ^ 1u, p.status)))) break;
-        uint8_t* const dst = smem + qb * R::q_bytes + i * 128;
-#pragma unroll
-        for (int c = 0; c < HD / 8; ++c) {
-          const bool neg = p.scale < 0.f;
-          const uint4 u = make_uint4(row_half2<HALF>(v[c].x, sh, neg), row_half2<HALF>(v[c].y, sh, neg),
-                                     row_half2<HALF>(v[c].z, sh, neg), row_half2<HALF>(v[c].w, sh, neg));
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * (kRows * 128) + (((c & 7) ^ (i & 7)) << 4)) = u;
-        }
-        x->c_row[s & 3][i] = scaled(fabsf(p.scale) * kLog2e, -sh);
-        fence_proxy_async_smem();
+    } else if (warp == 10) {
+      // ---------------- segments, codes and scales: lane x * 4 + c has the c-th page of a tile's K (x 0) or V, and chunk
+      // c's scale
+      const int unit = min(p.page, kKeys), c = lane & 3, y = (lane >> 2) & 1;  // keys of a copy
+      int t = 0, pg = 0, pg_scale = 0;
+      auto page = [&](int g) -> long long {
+        if ((unsigned)g < (unsigned)p.pages) return g;
+        atomicExch(p.status, T2W_ERR_INVALID);
+        return 0;
+      };
+      float scale = 0.f;  // of the tile before, which is on its way while that tile's codes are
+      auto publish = [&](int n) {
+        if (lane < 8) (y ? x->vs : x->ks)[n & 7][c] = scale;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&x->q_full[qb]);
-      }
-      for (int kt = at.kt0; kt < at.kt1; ++kt, ++t) {
-        send();  // into the slot of the tile before this one
-        asm volatile("cp.async.wait_group %0;" ::"n"(R::Raw - 1) : "memory");
-        const uint8_t* const raw = smem + R::raw_at + (t % R::Raw) * R::raw_bytes + 16 * i;
-        if (i < 8) (i < 4 ? x->ks : x->vs)[t & 3][i & 3] = x->scale_raw[t % R::Raw][i];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&x->meta_full[t & 3]);
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int n = y ? R::V : R::K, slot = t % n;
-          if (!(ok = __all_sync(~0u, mbar_wait(y ? &x->v_empty[slot] : &x->k_empty[slot], ((t / n) & 1) ^ 1u, p.status)))) break;
-          uint8_t* const dst = smem + (y ? R::v_at : R::k_at) + slot * R::tile_bytes;
-#pragma unroll
-          for (int j = 0; j < kN; ++j) {
-            const int row = row_i + j * kStep;
-            uint4 c = *reinterpret_cast<const uint4*>(raw + y * (kKeys * HD) + j * (16 * kWiden));
-            // places past the last key may hold anything; a weight of 0 does not hide a NaN value
-            if (y && kt * kKeys + row >= at.kv) c = make_uint4(0, 0, 0, 0);
-            const uint2 a = e4m3x4_to_f16x4(c.x), b = e4m3x4_to_f16x4(c.y), d = e4m3x4_to_f16x4(c.z), e = e4m3x4_to_f16x4(c.w);
-            uint8_t* const to = dst + (piece >> 2) * (kKeys * 128) + row * 128;
-            const int c0 = (piece & 3) * 2;
-            *reinterpret_cast<uint4*>(to + ((c0 ^ (row & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
-            *reinterpret_cast<uint4*>(to + (((c0 + 1) ^ (row & 7)) << 4)) = make_uint4(d.x, d.y, e.x, e.y);
+        if (lane == 0) mbar_arrive(&x->meta_full[n & 7]);
+      };
+      const uint64_t policy = l2_policy_evict_first();
+      Walk at;
+      bool more = at.begin(p, w);
+#pragma unroll 1
+      for (int s = 0;; ++s) {
+        if (lane == 0) {
+          Seg* const g = &x->seg[s & 7];
+          g->rows = more ? at.rows(p, group) : 0;
+          g->row0 = at.row0 + at.qt * p.tq;
+          g->head0 = at.hk * group;
+          g->before = at.kv - at.f + at.qt * p.tq;
+          g->kv = at.kv;
+          g->kt0 = at.kt0;
+          g->kt1 = at.kt1;
+          g->slot = at.kt0 == 0 && at.kt1 == at.nt ? -1 : 2 * w + (at.first ? 0 : 1);
+          mbar_arrive(&x->seg_full[s & 7]);
+        }
+        if (!more) break;
+#pragma unroll 1
+        for (int kt = at.kt0 - 1; kt < at.kt1; ++kt) {
+          // (a pass before the first tile only looks up its pages)
+          if (kt >= at.kt0) {
+            const int kb = kt * kKeys, sk = t % R::RawK, sv = t % R::RawV;
+            ok = bar_wait(&x->raw_k_empty[sk], ((t / R::RawK) & 1) ^ 1u, p.status) &&
+                 bar_wait(&x->raw_v_empty[sv], ((t / R::RawV) & 1) ^ 1u, p.status);
+            if (!(ok = __all_sync(~0u, ok))) break;
+            const int units = max(0, min((at.kv - kb + unit - 1) / unit, kKeys / unit));
+            if (lane == 0) mbar_expect_tx(&x->raw_full[sk], 2 * units * unit * HD);
+            __syncwarp();
+            if (lane < 8 && c < units) {
+              const int key = kb + c * unit;
+              bulk_load_hint(smem + (y ? R::raw_v_at + sv * R::raw_bytes : R::raw_k_at + sk * R::raw_bytes) + c * unit * HD,
+                             p.codes[y] + page(pg) * p.page_ld[y] + ((long long)at.hk * p.page + (key & (p.page - 1))) * HD,
+                             unit * HD, &x->raw_full[sk], policy);
+            }
+            if (t) publish(t - 1);
+            scale = lane < 8 && kb < at.kv ? __ldg(p.scales[y] + page(pg_scale) * p.scale_ld[y] + at.hk) : 1.f;
+            ++t;
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(y ? &x->v_full[slot] : &x->k_full[slot]);
+          if (kt + 1 < at.kt1) {
+            const int* const table = p.table + (size_t)at.r * p.table_ld;
+            const int kb = (kt + 1) * kKeys, key = kb + c * unit, key_s = kb + 16 * c;
+            pg = lane < 8 && c * unit < kKeys && key < at.kv ? __ldg(table + (key >> p.shift)) : 0;
+            pg_scale = lane < 8 && kb < at.kv ? __ldg(table + ((key_s < at.kv ? key_s : kb) >> p.shift)) : 0;
+          }
         }
         if (!ok) break;
+        more = at.next(p);
       }
-      if (!ok || !at.next(p)) break;
+      if (ok && t) publish(t - 1);
+    } else if (warp == 11) {
+      // ---------------- queries: copied as they are to where their halves go, all on their way at once, then a lane four rows
+      constexpr int kPieces = HD / 8;  // 16-byte pieces of a row
+      const bool neg = p.scale < 0.f;
+#pragma unroll 1
+      for (int s = 0;; ++s) {
+        const Seg* const g = next_seg(s);
+        if (!g) break;
+        const int qb = s % R::Q, rows = g->rows, base = base_of(rows);
+        const uint32_t dst = smem_u32(smem + qb * R::q_bytes);
+        auto place = [&](int row, int piece) { return (piece >> 3) * (kRows * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4); };
+        if (!(ok = __all_sync(~0u, bar_wait(&x->q_free[qb], ((s / R::Q) & 1) ^ 1u, p.status)))) break;
+#pragma unroll 1
+        for (int i = 0; i < kRows; i += 32) {
+          const int r = i + lane - base;
+          const long long from =
+              r >= 0 && r < rows ? (g->row0 + over_group(p, r)) * p.q_row_ld + (g->head0 + r - group * over_group(p, r)) * p.q_head_ld : -1;
+#pragma unroll 2
+          for (int j = lane; j < 32 * kPieces; j += 32) {
+            const int row = j / kPieces, piece = j % kPieces;
+            const long long q = __shfl_sync(~0u, from, row);
+            if (q >= 0) copy16_plain(dst + place(i + row, piece), static_cast<const uint16_t*>(p.q) + q + 8 * piece);
+          }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+#pragma unroll 1
+        for (int i = lane; i < kRows; i += 32) {
+          const bool has = i >= base && i < base + rows;
+          uint8_t* const at_row = smem + qb * R::q_bytes;
+          uint32_t m = 0;
+#pragma unroll 2
+          for (int c = 0; c < kPieces; ++c) {
+            const uint4 v = has ? *reinterpret_cast<const uint4*>(at_row + place(i, c)) : make_uint4(0, 0, 0, 0);
+            m = __vmaxu2(__vmaxu2(m, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
+            m = __vmaxu2(__vmaxu2(m, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
+          }
+          const int sh = row_shift<HALF>(max(m & 0xffffu, m >> 16));
+#pragma unroll 2
+          for (int c = 0; c < kPieces; ++c) {
+            uint4* const to = reinterpret_cast<uint4*>(at_row + place(i, c));
+            const uint4 v = has ? *to : make_uint4(0, 0, 0, 0);
+            *to = make_uint4(row_half2<HALF>(v.x, sh, neg), row_half2<HALF>(v.y, sh, neg), row_half2<HALF>(v.z, sh, neg),
+                             row_half2<HALF>(v.w, sh, neg));
+          }
+          x->shift[s & 3][i] = (int16_t)sh;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&x->q_full[qb]);
+          mbar_arrive(&x->shift_full[s & 3]);
+        }
+      }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-  } else if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    // ---------------- MMA issuer: S_0, S_1, then W_t V_t followed by S_{t + 2}
-    if (warp == 8 && lane == 0 && ok) {
-      constexpr uint32_t idesc_qk = idesc_half(kRows, kKeys), idesc_pv = idesc_half(kRows, 64, true);
-      Walk pv = at;  // the segment of the next W V; `at` is that of the next S
-      int js = at.kt0, ts = 0, seg = 0, jp = pv.kt0, tp = 0, segp = 0;
-      bool more_s = true, more_p = true;
-      auto issue_s = [&]() -> bool {
-        if (js == at.kt0 && !mbar_wait(&x->q_full[seg % R::Q], (seg / R::Q) & 1, p.status)) return false;
-        if (!mbar_wait(&x->k_full[ts % R::K], (ts / R::K) & 1, p.status)) return false;
-        tc_fence_after();
-        const uint32_t q0 = smem_u32(smem + (seg % R::Q) * R::q_bytes);
-        const uint32_t k0 = smem_u32(smem + R::k_at + (ts % R::K) * R::tile_bytes);
+  } else if (warp >= 4) {
+    // ---------------- widening: thread i has the 16-byte pieces i, i + 128, ... of a tile's K and of its V codes
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    const int i = threadIdx.x - 128;
+    constexpr int kPieces = HD / 16, kN = kKeys * kPieces / 128, kStep = 128 / kPieces;  // pieces a row, a thread; rows between
+    const int row_i = i / kPieces, piece = i % kPieces, c0 = (piece & 3) * 2;
+    // K of tile t, then V of tile t - 1
+    int s = 0, kt = 0, left = 0;  // the keys from the tile before's first one on
+    const Seg* g = next_seg(0);
+    if (g) kt = g->kt0;
+#pragma unroll 1
+    for (int t = 0; ok; ++t) {
+      if (g && !(ok = bar_wait(&x->raw_full[t % R::RawK], (t / R::RawK) & 1, p.status))) break;
+#pragma unroll 1
+      for (int y = g ? 0 : 1; y < (t ? 2 : 1); ++y) {
+        const int n = t - y, ring = y ? R::V : R::K, slot = n % ring;
+        if (!(ok = bar_wait(y ? &x->v_empty[slot] : &x->k_empty[slot], ((n / ring) & 1) ^ 1u, p.status))) break;
+        const uint8_t* const raw =
+            smem + (y ? R::raw_v_at + (n % R::RawV) * R::raw_bytes : R::raw_k_at + (n % R::RawK) * R::raw_bytes) + 16 * i;
+        uint8_t* const dst = smem + (y ? R::v_at : R::k_at) + slot * R::tile_bytes + (piece >> 2) * (kKeys * 128) + row_i * 128;
+        const int x0 = (c0 ^ (row_i & 7)) << 4;  // (rows kStep apart are the same in the swizzle's 8)
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          umma_f16(tmem + 64 * (ts & 1), sdesc_sw128(q0 + (kk >> 2) * (kRows * 128) + 32 * (kk & 3), 1024, 16),
-                   sdesc_sw128(k0 + (kk >> 2) * (kKeys * 128) + 32 * (kk & 3), 1024, 16), idesc_qk, kk ? 1u : 0u);
-        umma_commit(&x->s_full[ts & 1]);
-        umma_commit(&x->k_empty[ts % R::K]);
-        ++ts;
-        if (++js == at.kt1) {
-          umma_commit(&x->q_free[seg % R::Q]);
-          more_s = at.next(p);
-          js = 0;
-          ++seg;
+        for (int j = 0; j < kN; ++j) {
+          uint4 c = *reinterpret_cast<const uint4*>(raw + j * 2048);
+          // places past the last key may hold anything; a weight of 0 does not hide a NaN value
+          if (y && row_i + j * kStep >= left) c = make_uint4(0, 0, 0, 0);
+          const uint2 a = e4m3x4_to_f16x4(c.x), b = e4m3x4_to_f16x4(c.y), d = e4m3x4_to_f16x4(c.z), e = e4m3x4_to_f16x4(c.w);
+          *reinterpret_cast<uint4*>(dst + j * (kStep * 128) + x0) = make_uint4(a.x, a.y, b.x, b.y);
+          *reinterpret_cast<uint4*>(dst + j * (kStep * 128) + (x0 ^ 16)) = make_uint4(d.x, d.y, e.x, e.y);
         }
-        return true;
-      };
-      for (int i = 0; i < 2 && more_s && ok; ++i) ok = issue_s();
-      while (more_p && ok) {
-        if (!(ok = mbar_wait(&x->p_full[tp & 1], (tp >> 1) & 1, p.status))) break;
-        if (!(ok = mbar_wait(&x->v_full[tp % R::V], (tp / R::V) & 1, p.status))) break;
-        // a segment's first W V overwrites O: the softmax has read the previous segment's
-        if (jp == pv.kt0 && segp > 0 && !(ok = mbar_wait(&x->o_free, (segp - 1) & 1, p.status))) break;
-        tc_fence_after();
-        const uint32_t v0 = smem_u32(smem + R::v_at + (tp % R::V) * R::tile_bytes);
-#pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk)
-#pragma unroll
-          for (int c = 0; c < kPanels; ++c)
-            umma_f16_ts(tmem + 128 + 64 * c, tmem + 64 * (tp & 1) + 8 * kk,
-                        sdesc_sw128(v0 + c * (kKeys * 128) + kk * 16 * 128, 1024, 8192), idesc_pv,
-                        (jp > pv.kt0 || kk > 0) ? 1u : 0u);
-        umma_commit(&x->o_done[tp & 1]);
-        umma_commit(&x->v_empty[tp % R::V]);
-        ++tp;
-        if (++jp == pv.kt1) {
-          more_p = pv.next(p);
-          jp = 0;
-          ++segp;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(y ? &x->v_full[slot] : &x->k_full[slot]);
+          mbar_arrive(y ? &x->raw_v_empty[n % R::RawV] : &x->raw_k_empty[n % R::RawK]);
         }
-        if (more_s) ok = issue_s();
+      }
+      if (!ok || !g) break;
+      left = g->kv - kt * kKeys;
+      if (++kt == g->kt1) {
+        g = next_seg(++s);
+        if (g) kt = g->kt0;
       }
     }
   } else {
-    // ---------------- softmax: thread r has row r
+    // ---------------- softmax: thread r has the tile's row r
     asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     const int r = threadIdx.x;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    const uint32_t oreg = tmem + lanes + 128;
-    int t = 0;
-    struct Pending {
-      int row, head, t_last, slot;  // output row (-1: none), query head; the part's slot, or -1 for a whole segment
-      float l, M;
-    } pend{-1, 0, 0, -1, 0.f, 0.f};
-    bool have = false;
-    auto finish = [&]() -> bool {
-      if (!__all_sync(~0u, mbar_wait(&x->o_done[pend.t_last & 1], (pend.t_last >> 1) & 1, p.status))) return false;
-      tc_fence_after();
-      const float l = pend.l, M = l != l ? fmaxf(pend.M, -1e30f) : pend.M;  // a NaN counts, even where M saw nothing else
-      float* const part = part_of(p.ws, pend.slot, kRows, HD);
-#pragma unroll
-      for (int c = 0; c < HD / 32; ++c) {
-        float o[32];
-        tmem_ld32(oreg + 32 * c, o);
-        if (c == HD / 32 - 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&x->o_free);
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16, oreg = tmem + lanes + 128;
+    // the segment (kt: its next tile), the row's keys, factor, exponent and sum
+    int s = -1, kt = 0, kt1 = 0, row = 0, lim = 0;
+    bool mine = false, idle = true, have = false;
+    float c_row = 0.f, M = -INFINITY, l = 0.f;
+    // the segment before: output row (-1: none), query head; the part's slot (-1: a whole segment) and row
+    int o_row = -1, o_head = 0, o_slot = -1, o_part = 0;
+    float o_M = 0.f, o_l = 0.f;
+    const Seg* g = nullptr;
+#pragma unroll 1
+    for (int t = 0; ok; ++t) {
+      const bool first = kt == kt1;
+      if (first) {
+        if (s >= 0) {
+          o_row = mine ? g->row0 + over_group(p, row) : -1;
+          o_head = g->head0 + row - group * over_group(p, row);
+          o_slot = g->slot;
+          o_part = row;
+          o_M = l != l ? fmaxf(M, -1e30f) : M;  // a NaN counts, even where M saw nothing else
+          o_l = l;
+          have = true;
         }
-        if (pend.row >= 0 && pend.slot < 0) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) store_row8<HALF>(p, pend.row, pend.head, HD, 32 * c + i, o + i, M, l);
-        } else if (pend.row >= 0) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(part + r * HD + 32 * c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        g = next_seg(++s);
+        if (!ok) break;
+        if (g) {
+          kt = g->kt0;
+          kt1 = g->kt1;
+          row = r - base_of(g->rows);
+          mine = row >= 0 && row < g->rows;
+          // keys that it sees (a row that nobody reads sees all, so that a warp's others need no mask for it)
+          lim = mine && p.causal ? g->before + over_group(p, row) + 1 : g->kv;
+          idle = !__any_sync(~0u, mine);  // nobody reads such a warp's weights and outputs
+          if (!(ok = bar_wait(&x->shift_full[s & 3], (s >> 2) & 1, p.status))) break;
+          c_row = scaled(fabsf(p.scale) * kLog2e, -x->shift[s & 3][r]);
+          M = -INFINITY;
+          l = 0.f;
         }
-        __syncwarp();
       }
-      if (pend.row >= 0 && pend.slot >= 0) {
-        part[kRows * HD + r] = M;
-        part[kRows * HD + kRows + r] = l;
-      }
-      return true;
-    };
-    for (int s = 0; ok; ++s) {
-      const int tok = r / group, keys = at.tokens(p) > tok ? 1 : 0;
-      const int pos = at.qt * p.tq + tok;  // the row's query in its request
-      // keys that the row sees
-      const int lim = !keys ? 0 : p.causal ? at.kv - at.f + pos + 1 : at.kv;
-      const bool idle = __all_sync(~0u, !keys);  // its rows' weights and outputs are never read
-      float c_row = 0.f;
-      float M = -INFINITY, l = 0.f;
-      for (int kt = at.kt0; kt < at.kt1; ++kt, ++t) {
-        if (!(ok = __all_sync(~0u, mbar_wait(&x->meta_full[t & 3], (t >> 2) & 1, p.status) &&
-                                       mbar_wait(&x->s_full[t & 1], (t >> 1) & 1, p.status))))
-          break;
+      if (g) {
+        ok = bar_wait(&x->meta_full[t & 7], (t >> 3) & 1, p.status) && bar_wait(&x->s_full[t & 1], (t >> 1) & 1, p.status);
+        if (!(ok = __all_sync(~0u, ok))) break;
         tc_fence_after();
-        if (kt == at.kt0) c_row = x->c_row[s & 3][r];
+      }
+      if (g && !idle) {
         const uint32_t sbuf = tmem + lanes + 64 * (t & 1);
-        if (!idle) {
-          uint32_t sr[64];
-          tmem_ld32_nowait(sbuf, sr);
-          tmem_ld32_nowait(sbuf + 32, sr + 32);
-          float ck[4], lv[4], unit[4];
-          bool odd = false;
-#pragma unroll
+        const int kb = kt * kKeys;
+        const float* const ks = x->ks[t & 7];
+        const float* const vs = x->vs[t & 7];
+        const bool odd = !__all_sync(~0u, ks[lane & 3] < INFINITY && vs[lane & 3] < INFINITY);
+        // scores that their rows do not see, and all of them where a scale is not finite: it may only meet what a row sees
+        if (!__all_sync(~0u, kb + kKeys <= lim) || odd) {
+#pragma unroll 1
           for (int c = 0; c < 4; ++c) {
-            const float ks = x->ks[t & 3][c], vs = x->vs[t & 3][c];
-            odd |= !(ks < INFINITY) || !(vs < INFINITY);
-            const bool bad = !(vs < INFINITY);
-            const int e = bad ? 0 : (int)(__float_as_uint(vs) >> 23) - 127;
-            ck[c] = c_row * ks;
-            if (ck[c] == 0.f) ck[c] = 1.1754944e-38f;  // (-inf times 0)
-            lv[c] = (float)e;
-            unit[c] = exp2i(-e);
-          }
-          tmem_ld_wait();
-          const int kb = kt * kKeys;
-          if (!__all_sync(~0u, kb + kKeys <= lim)) {
+            float v[16];
+            tmem_ld16(sbuf + 16 * c, v);
+            uint32_t u[16];
 #pragma unroll
-            for (int i = 0; i < kKeys; ++i)
-              if (kb + i >= lim) sr[i] = __float_as_uint(-INFINITY);
-          }
-          if (odd) {  // a scale that is not finite: it may only meet what the row sees
-#pragma unroll
-            for (int i = 0; i < kKeys; ++i)
-              if (kb + i < lim) sr[i] = __float_as_uint(fmaf(__uint_as_float(sr[i]), ck[i >> 4], lv[i >> 4]));
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              ck[c] = 1.f;
-              lv[c] = 0.f;
+            for (int i = 0; i < 16; ++i) {
+              const float f = odd ? fmaf(v[i], c_row * ks[c], exponent(vs[c])) : v[i];
+              u[i] = __float_as_uint(kb + 16 * c + i < lim ? f : -INFINITY);
             }
+            tmem_st16(sbuf + 16 * c, u);
           }
-          float mx = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float m = fmax3(__uint_as_float(sr[16 * c]), __uint_as_float(sr[16 * c + 1]), __uint_as_float(sr[16 * c + 2]));
-#pragma unroll
-            for (int i = 3; i < 15; i += 2)
-              m = fmax3(m, __uint_as_float(sr[16 * c + i]), __uint_as_float(sr[16 * c + i + 1]));
-            m = fmaxf(m, __uint_as_float(sr[16 * c + 15]));
-            mx = fmaxf(mx, fmaf(m, ck[c], lv[c]));
-          }
-          const bool raise = mx > M + kRaise;
-          const float m_old = M;
-          M = raise ? mx - kBelow : M;
-          const float ref = M == -INFINITY ? 0.f : M;
-          uint32_t u[32];
-          float add = 0.f;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float2 c2 = make_float2(ck[c], ck[c]), d2 = make_float2(lv[c] - ref, lv[c] - ref);
-            float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float2 a = fma2(make_float2(__uint_as_float(sr[16 * c + 2 * i]), __uint_as_float(sr[16 * c + 2 * i + 1])), c2, d2);
-              const float2 e = make_float2(exp2_approx(a.x), exp2_approx(a.y));
-              sum = add2(sum, e);
-              u[8 * c + i] = pack_f16x2(e.x, e.y);
-            }
-            add = fmaf(sum.x + sum.y, unit[c], add);
-          }
-          if (odd) {  // values that are NaN, where the row sees them
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(x->vs[t & 3][i >> 3] < INFINITY)) {
-                if (kb + 2 * i < lim) u[i] |= 0x7fffu;
-                if (kb + 2 * i + 1 < lim) u[i] |= 0x7fff0000u;
-              }
-          }
-          tmem_st32(sbuf, u);
-          if (kt > at.kt0 && __any_sync(~0u, raise)) {
-            // O holds the tiles before relative to the old exponent; S_t's completion implies that of every product
-            // issued before it, so the waits skipped here never fall two phases behind
-            if (!(ok = __all_sync(~0u, mbar_wait(&x->o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, p.status)))) break;
-            tc_fence_after();
-            const float f = raise ? exp2_approx(m_old - M) : 1.f;
-            l *= f;
-#pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-              float o[32];
-              tmem_ld32(oreg + 32 * c, o);
-              uint32_t ou[32];
-#pragma unroll
-              for (int i = 0; i < 32; ++i) ou[i] = __float_as_uint(o[i] * f);
-              tmem_st32(oreg + 32 * c, ou);
-            }
-          }
-          l += add;
           tmem_st_wait();
         }
-        if (kt == at.kt0 && have) {
-          if (!(ok = finish())) break;
-          have = false;
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          float v[32];
+          tmem_ld32(sbuf + 32 * h, v);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float m = fmax3(v[16 * c], v[16 * c + 1], v[16 * c + 2]);
+#pragma unroll
+            for (int i = 3; i < 15; i += 2) m = fmax3(m, v[16 * c + i], v[16 * c + i + 1]);
+            m = fmaxf(m, v[16 * c + 15]);
+            // (-inf times a scale of 0 is no number, and fmaxf passes over it)
+            mx = fmaxf(mx, odd ? m : fmaf(m, c_row * ks[2 * h + c], exponent(vs[2 * h + c])));
+          }
+        }
+        const bool raise = mx > M + kRaise;
+        const float m_old = M;
+        M = raise ? mx - kBelow : M;
+        const float ref = M == -INFINITY ? 0.f : M;
+        float add = 0.f;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          float v[32];
+          tmem_ld32(sbuf + 32 * h, v);
+          uint32_t u[16];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float e2 = exponent(vs[2 * h + c]), d = (odd ? 0.f : e2) - ref;
+            float ck = odd ? 1.f : c_row * ks[2 * h + c];
+            ck = ck == 0.f ? 1.1754944e-38f : ck;  // (-inf times 0)
+            float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+#pragma unroll
+            for (int i = 16 * c; i < 16 * c + 16; i += 4) {
+              const float2 a = __ffma2_rn(make_float2(v[i], v[i + 1]), make_float2(ck, ck), make_float2(d, d));
+              const float2 b = __ffma2_rn(make_float2(v[i + 2], v[i + 3]), make_float2(ck, ck), make_float2(d, d));
+              const float2 ea = make_float2(exp2_approx(a.x), exp2_approx(a.y)), eb = make_float2(exp2_approx(b.x), exp2_approx(b.y));
+              s0 = __fadd2_rn(s0, ea);
+              s1 = __fadd2_rn(s1, eb);
+              u[i / 2] = pack_f16x2(ea.x, ea.y);
+              u[i / 2 + 1] = pack_f16x2(eb.x, eb.y);
+            }
+            add = fmaf((s0.x + s1.x) + (s0.y + s1.y), exp2i(-(int)e2), add);
+          }
+          // over the scores of the half that is done with: columns 0-15, then 16-31
+          tmem_st16(sbuf + 16 * h, u);
+        }
+        if (odd) {  // values that are NaN, where the row sees them
+          tmem_st_wait();
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            float v[16];
+            tmem_ld16(sbuf + 16 * h, v);
+            uint32_t u[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int key = kb + 32 * h + 2 * i;
+              u[i] = __float_as_uint(v[i]);
+              if (!(vs[2 * h + (i >> 3)] < INFINITY)) u[i] |= (key < lim ? 0x7fffu : 0u) | (key + 1 < lim ? 0x7fff0000u : 0u);
+            }
+            tmem_st16(sbuf + 16 * h, u);
+          }
+        }
+        if (!first && __any_sync(~0u, raise)) {
+          // O holds the tiles before relative to the old exponent
+          if (!(ok = __all_sync(~0u, bar_wait(&x->o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, p.status)))) break;
+          tc_fence_after();
+          const float f = raise ? exp2_approx(m_old - M) : 1.f;
+          l *= f;
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 16) {
+            float o[16];
+            tmem_ld16(oreg + c, o);
+            uint32_t ou[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ou[i] = __float_as_uint(o[i] * f);
+            tmem_st16(oreg + c, ou);
+          }
+        }
+        l += add;
+        tmem_st_wait();
+      }
+      if (first && have) {  // the segment before is finished
+        if (!(ok = __all_sync(~0u, bar_wait(&x->o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, p.status)))) break;
+        tc_fence_after();
+        float* const part = part_of(p.ws, o_slot, kRows, HD);
+        const float inv = o_l != 0.f ? 1.f / o_l : 0.f;
+        uint16_t* const out = static_cast<uint16_t*>(p.out) + ((size_t)o_row * p.q_heads + o_head) * HD;
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 16) {
+          float o[16];
+          tmem_ld16(oreg + c, o);
+          if (o_row >= 0 && o_slot < 0) {
+            uint32_t u[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float a = o[2 * i] * inv, b = o[2 * i + 1] * inv;
+              u[i] = HALF ? pack_f16x2(a, b) : pack_bf16x2(a, b);
+            }
+            reinterpret_cast<uint4*>(out + c)[0] = make_uint4(u[0], u[1], u[2], u[3]);
+            reinterpret_cast<uint4*>(out + c)[1] = make_uint4(u[4], u[5], u[6], u[7]);
+          } else if (o_row >= 0) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<float4*>(part + o_part * HD + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+          __syncwarp();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&x->p_full[t & 1]);
+        if (lane == 0) mbar_arrive(&x->o_free);
+        if (o_row >= 0 && o_slot >= 0) {
+          part[kRows * HD + o_part] = o_M;
+          part[kRows * HD + kRows + o_part] = o_l;
+        } else if (o_row >= 0 && p.lse) {
+          p.lse[(size_t)o_row * p.q_heads + o_head] = o_l != 0.f ? (o_M + log2f(o_l)) * 0.6931471805599453f : -INFINITY;
+        }
+        have = false;
       }
-      if (!ok) break;
-      pend.row = keys ? at.row0 + pos : -1;
-      pend.head = at.hk * group + r % group;
-      pend.t_last = t - 1;
-      pend.slot = at.kt0 == 0 && at.kt1 == at.nt ? -1 : 2 * w + (at.first ? 0 : 1);
-      pend.l = l;
-      pend.M = M;
-      have = true;
-      if (!at.next(p)) break;
+      if (!g) break;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&x->p_full[t & 1]);
+      ++kt;
     }
-    if (ok && have) finish();
   }
   __syncthreads();
   if (warp == 8) {

@@ -16,19 +16,33 @@ namespace t2w {
 PagedCut paged_cut(int max_fresh, int q_heads, int kv_heads, int head_dim) {
   const int group = q_heads / kv_heads;
   PagedCut c;
-  c.mma = (int64_t)max_fresh * group > 16;
-  if (c.mma) {
+  if ((int64_t)max_fresh * group <= 16) {
+    c.form = PagedForm::kFew;
+    c.part_rows = 16;
+    c.tq = max_fresh;
+    c.kt = 32;
+    c.workers = few_warps * few_blocks(head_dim, max_fresh * group > 8 ? 2 : 1) * num_sms();
+    c.min_per = 2;
+    c.extra = 4;
+    c.whole = false;
+  } else if (group <= 16 * mid_warps && MIDRULE) {
+    c.form = PagedForm::kMid;
+    c.part_rows = 16 * mid_warps;
+    c.tq = 16 * mid_warps / group;
+    c.kt = 64;
+    c.workers = mid_blocks(head_dim) * num_sms();
+    c.min_per = 2;
+    c.extra = 2;
+    c.whole = true;
+  } else {
+    c.form = PagedForm::kMany;
+    c.part_rows = 128;
     c.tq = 128 / group;
     c.kt = 64;
     c.workers = 2 * num_sms();
     c.min_per = 4;
     c.extra = 2;
-  } else {
-    c.tq = max_fresh;
-    c.kt = 32;
-    c.workers = 4 * few_blocks(head_dim, max_fresh * group > 8 ? 2 : 1) * num_sms();
-    c.min_per = 2;
-    c.extra = 4;
+    c.whole = true;
   }
   return c;
 }
@@ -52,7 +66,7 @@ PlanLayout paged_layout(int64_t requests, int64_t rows, int page, const PagedCut
   l.run_base = take(requests + 1);
   l.tile_base = take(requests + 1);
   l.seg_base = take(requests + 1);
-  l.starts = take(8 * (int64_t)l.max_workers);
+  l.starts = take(8 * ((int64_t)l.max_workers + 1));
   l.runs = take(4 * (int64_t)l.max_runs);
   l.total = at;
   return l;
@@ -132,28 +146,38 @@ T2W_DEV void scatter(const PlanDev& p, const int* q_start, const int* new_base, 
     atomicExch(&head->status, T2W_ERR_INVALID);  // a page that the cache does not have
     return -1;
   };
-  for (int i = i0; i < p.rows; i += step) {
-    if (i >= n_rows) {
-      slot[i] = -1;
-      request[i] = -1;
-      continue;
+  // four rows in a row at a time: they are mostly of one request and one page
+  for (int i = 4 * i0; i < p.rows; i += 4 * step) {
+    int r = i < n_rows ? find(q_start, p.requests, i) : -1, page_at = -1, g = -1;
+    int s[4], o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s[j] = o[j] = -1;
+      if (i + j >= n_rows) continue;
+      while (i + j >= q_start[r + 1]) {
+        ++r;
+        page_at = -1;
+      }
+      o[j] = r;
+      if (!p.free_pages) continue;
+      const int len = kv_len[r] - (q_start[r + 1] - q_start[r]), pos = len + i + j - q_start[r];
+      if (page_at != pos >> p.shift) {
+        page_at = pos >> p.shift;
+        g = page_of(r, page_at, len);
+      }
+      if (g >= 0) s[j] = g * p.page + (pos & (p.page - 1));
     }
-    const int r = find(q_start, p.requests, i);
-    request[i] = r;
-    if (!p.free_pages) {
-      slot[i] = -1;
-      continue;
-    }
-    const int f = q_start[r + 1] - q_start[r], len = kv_len[r] - f, pos = len + i - q_start[r];
-    const int g = page_of(r, pos >> p.shift, len);
-    slot[i] = g < 0 ? -1 : g * p.page + (pos & (p.page - 1));
+    // (each part of the plan begins on a 16-byte boundary and is as long as whole pieces)
+    *reinterpret_cast<int4*>(slot + i) = make_int4(s[0], s[1], s[2], s[3]);
+    *reinterpret_cast<int4*>(request + i) = make_int4(o[0], o[1], o[2], o[3]);
   }
-  for (int i = i0; i < n_pages; i += step) {
+  // (other threads begin here than there: a small step's loads are then all on their way at once)
+  for (int i = (i0 + step - step / 4) % step; i < n_pages; i += step) {
     const int r = find(new_base, p.requests, i);
     const int f = q_start[r + 1] - q_start[r], first = pages_of(kv_len[r] - f, p.shift), b = first + i - new_base[r];
     p.table[(size_t)r * p.table_ld + b] = page_of(r, b, kv_len[r] - f);
   }
-  for (int i = i0; i < n_runs; i += step) {
+  for (int i = (i0 + step / 2) % step; i < n_runs; i += step) {
     const int r = find(run_base, p.requests, i);
     const int f = q_start[r + 1] - q_start[r], len = kv_len[r] - f, b = (len >> p.shift) + i - run_base[r];
     const int from = max(len, b * p.page), to = (int)min((long long)kv_len[r], (long long)(b + 1) * p.page);
@@ -277,11 +301,39 @@ __global__ void __launch_bounds__(1024) k_plan(const PlanDev p) {
       const int mid = (lo + hi) >> 1;
       if (before(mid) <= in) lo = mid; else hi = mid;
     }
+    int place = w * per, kt = in - before(lo) - extra, seg_r = r, seg_h = hk, seg_q = lo, row0 = q_start[r], rows = f, keys = kv;
+    const int nt = seg_tiles(tile_keys(f, kv, p.causal, p.cut.tq, lo), p.cut.kt);
+    if (p.cut.whole && kt > -extra && 5 * (nt + extra) <= 3 * per) {  // a short segment is not cut
+      if (2 * kt < nt) {
+        place -= kt + extra;
+      } else {  // the next one begins the share
+        place += nt - kt;
+        if (++seg_q == nq) {
+          seg_q = 0;
+          if (++seg_h == p.kv_heads) {
+            seg_h = 0;
+            do ++seg_r;
+            while (seg_r < n && q_start[seg_r + 1] == q_start[seg_r]);
+            if (seg_r < n) {
+              row0 = q_start[seg_r];
+              rows = q_start[seg_r + 1] - row0;
+              keys = kv_len[seg_r];
+            }
+          }
+        }
+      }
+      kt = -extra;
+    }
     // request, key head, query tile and key tile (below 0 where the share begins with empty places); then what a worker
-    // would look up for that request
+    // would look up for that request, and the share's first place
     int4* const start = reinterpret_cast<int4*>(p.buf + p.lay.starts) + 2 * w;
-    start[0] = make_int4(r, hk, lo, in - before(lo) - extra);
-    start[1] = make_int4(q_start[r], f, kv, 0);
+    start[0] = make_int4(seg_r, seg_h, seg_q, kt);
+    start[1] = make_int4(row0, rows, keys, place);
+  }
+  if (tid == 0) {  // where the last share ends
+    int4* const start = reinterpret_cast<int4*>(p.buf + p.lay.starts) + 2 * workers;
+    start[0] = make_int4(0, 0, 0, 0);
+    start[1] = make_int4(0, 0, 0, tiles);
   }
   if (!p.scattered)
     scatter(p, q_start, new_base, run_base, kv_len, n_rows, n_pages, n_runs, free_n, tid, blockDim.x);
@@ -295,10 +347,26 @@ __global__ void __launch_bounds__(1024) k_plan(const PlanDev p) {
 __global__ void __launch_bounds__(256) k_plan_rows(const PlanDev p) {
   pdl_wait();
   pdl_launch();
+  __shared__ int held[4][kHeld + 1];
   const PlanHead h = *reinterpret_cast<const PlanHead*>(p.buf);
-  const int n_pages = p.buf[p.lay.new_base + p.requests];
-  scatter(p, p.buf + p.lay.q_start, p.buf + p.lay.new_base, p.buf + p.lay.run_base, p.buf + p.lay.kv_len, h.used,
-          n_pages, h.n_runs, h.free_left + n_pages, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
+  const int n = p.requests, n_pages = p.buf[p.lay.new_base + n];
+  const int *q_start = p.buf + p.lay.q_start, *new_base = p.buf + p.lay.new_base, *run_base = p.buf + p.lay.run_base,
+            *kv_len = p.buf + p.lay.kv_len;
+  if (n <= kHeld) {
+    for (int r = threadIdx.x; r <= n; r += blockDim.x) {
+      held[0][r] = q_start[r];
+      held[1][r] = new_base[r];
+      held[2][r] = run_base[r];
+      if (r < n) held[3][r] = kv_len[r];
+    }
+    __syncthreads();
+    q_start = held[0];
+    new_base = held[1];
+    run_base = held[2];
+    kv_len = held[3];
+  }
+  scatter(p, q_start, new_base, run_base, kv_len, h.used, n_pages, h.n_runs, h.free_left + n_pages,
+          blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
 }
 
 // Pages of finished requests back onto the end of the free list, in request and block order; their lengths become 0.
@@ -409,10 +477,10 @@ extern "C" int t2w_paged_plan(const t2w_paged_plan_args* a, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   p.scattered = a->rows > 4096;
   const bool small = a->rows <= 1024 && a->requests <= 256;
-  cudaError_t e = launch_k(k_plan, dim3(1), dim3(small ? 256 : 1024), 0, st, p);
+  cudaError_t e = launch_k(k_plan, dim3(1), dim3(small ? 512 : 1024), 0, st, p);
   if (e == cudaSuccess && p.scattered) {
-    const int grid = (a->rows + 255) / 256;
-    e = launch_k(k_plan_rows, dim3(grid < 4 * num_sms() ? grid : 4 * num_sms()), dim3(256), 0, st, p);
+    const int grid = (a->rows + 1023) / 1024;
+    e = launch_k(k_plan_rows, dim3(grid < 2 * num_sms() ? grid : 2 * num_sms()), dim3(256), 0, st, p);
   }
   if (e != cudaSuccess) {
     set_cuda_error(e);

@@ -367,7 +367,7 @@ void plan_of(const char* op, const at::Tensor& plan, const at::Tensor& like, int
   i32_of(op, "a plan made for these sizes", plan, like, n);
 }
 
-at::Tensor paged_plan(const at::Tensor& fresh, const at::Tensor& length, at::Tensor& table, int64_t page, int64_t rows,
+std::vector<at::Tensor> paged_plan(const at::Tensor& fresh, const at::Tensor& length, at::Tensor& table, int64_t page, int64_t rows,
                       int64_t max_fresh, int64_t q_heads, int64_t kv_heads, int64_t head_dim, bool causal,
                       const std::optional<at::Tensor>& free_pages, const std::optional<at::Tensor>& free_count,
                       const std::optional<at::Tensor>& kv_len, const std::optional<at::Tensor>& free_left) {
@@ -397,12 +397,14 @@ at::Tensor paged_plan(const at::Tensor& fresh, const at::Tensor& length, at::Ten
   }
   if (kv_len) a.kv_len = const_cast<int32_t*>(i32_of(op, "kv_len", *kv_len, fresh, a.requests));
   if (free_left) a.free_left = const_cast<int32_t*>(i32_of(op, "free_left", *free_left, fresh, 1));
-  const int64_t n = t2w_paged_plan_ints(a.requests, a.rows, a.max_fresh, a.page, a.q_heads, a.kv_heads, a.head_dim, nullptr);
+  int64_t at[4];
+  const int64_t n = t2w_paged_plan_ints(a.requests, a.rows, a.max_fresh, a.page, a.q_heads, a.kv_heads, a.head_dim, at);
   if (n < 0) check("t2w_paged_plan", (int)n);
   at::Tensor plan = at::empty({n}, fresh.options());
   a.plan = plan.data_ptr<int32_t>();
   check("t2w_paged_plan", t2w_paged_plan(&a, stream_of(fresh)));
-  return plan;
+  return {plan, plan.narrow(0, at[0], a.requests + 1), plan.narrow(0, at[1], a.requests), plan.narrow(0, at[2], a.rows),
+          plan.narrow(0, at[3], a.rows), plan.narrow(0, 6, 1)};
 }
 
 void paged_append(const at::Tensor& k, const at::Tensor& v, at::Tensor& k_codes, at::Tensor& v_codes, at::Tensor& k_scale,
@@ -550,7 +552,7 @@ TORCH_LIBRARY(b200t2w, m) {
         &encode);
   m.def("paged_plan(Tensor fresh, Tensor length, Tensor(a!) table, int page, int rows, int max_fresh, int q_heads, "
         "int kv_heads, int head_dim, bool causal, Tensor? free_pages, Tensor? free_count, Tensor? kv_len, "
-        "Tensor? free_left) -> Tensor",
+        "Tensor? free_left) -> Tensor[]",
         &paged_plan);
   m.def("paged_append(Tensor k, Tensor v, Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) k_scale, "
         "Tensor(d!) v_scale, Tensor plan, int requests, int max_fresh, int q_heads) -> ()",
