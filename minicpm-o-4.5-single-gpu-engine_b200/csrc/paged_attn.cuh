@@ -92,9 +92,8 @@ T2W_DEV int row_shift(uint32_t max_bits16) {
 template <bool HALF>
 T2W_DEV uint32_t row_half2(uint32_t u, int shift, bool negate) {
   if constexpr (HALF) return negate ? u ^ 0x80008000u : u;
-  const float f = exp2i(shift);
-  const float a = __uint_as_float(u << 16) * f, b = __uint_as_float(u & 0xffff0000u) * f;
-  return negate ? pack_f16x2(-a, -b) : pack_f16x2(a, b);
+  const float f = negate ? -exp2i(shift) : exp2i(shift);
+  return pack_f16x2(__uint_as_float(u << 16) * f, __uint_as_float(u & 0xffff0000u) * f);
 }
 
 constexpr float kLog2e = 1.4426950408889634f;

@@ -60,7 +60,8 @@ struct Aux {
   int pad;
   // By tile: the scales of its 16-key chunks.  The copies' warp is ahead of the softmax by six tiles at most: tile t is
   // sent for once V of t - RawV (at most 5) has been widened, that is once the product of t - RawV - 2 is done.
-  float ks[8][4], vs[8][4];
+  float ks[8][4], lv[8][4], unit[8][4];  // K's; log2 of V's (0 where that is not finite) and 2^-lv
+  uint32_t odd[8];
   Seg seg[8];                // by segment, as far ahead as the tiles
   int16_t shift[4][kRows];   // by segment: the power of two that a row's queries were multiplied by
 };
@@ -92,9 +93,6 @@ T2W_DEV bool bar_wait(uint64_t* bar, uint32_t parity, int* err) {
   const uint32_t a = smem_u32(bar);
   unsigned long long t0 = 0;
   for (uint32_t i = 1; !mbar_try_wait(a, parity); ++i) {
-#ifdef NS
-    __nanosleep(NS);
-#endif
     if (i & 1023u) continue;
     const unsigned long long now = globaltimer();
     if (t0 == 0) t0 = now;
@@ -116,9 +114,6 @@ T2W_DEV void bulk_load_hint(void* smem_dst, const void* src, uint32_t bytes, uin
       : "memory");
 }
 
-// log2 of a value scale; 0 for one that is not finite.
-T2W_DEV float exponent(float s) { return s < INFINITY ? (float)((int)(__float_as_uint(s) >> 23) - 127) : 0.f; }
-
 // The tile row that a segment's first row has.
 T2W_DEV int base_of(int rows) { return rows <= 64 && 2 * blockIdx.x >= gridDim.x ? 64 : 0; }
 
@@ -131,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
   constexpr int kPanels = HD / 64;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&x->q_full[i], 1);
+      mbar_init(&x->q_full[i], 4);
       mbar_init(&x->q_free[i], 1);
       mbar_init(&x->k_full[i], 4);
       mbar_init(&x->k_empty[i], 1);
@@ -142,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
       mbar_init(&x->o_done[i], 1);
     }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&x->shift_full[i], 1);
+      mbar_init(&x->shift_full[i], 4);
       mbar_init(&x->raw_full[i], 1);
       mbar_init(&x->raw_k_empty[i], 4);
     }
@@ -197,11 +192,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
           if (g) {
             if (!bar_wait(&x->k_full[n % R::K], (n / R::K) & 1, p.status)) break;
             tc_fence_after();
-            const uint32_t q0 = smem_u32(smem + (s % R::Q) * R::q_bytes), k0 = smem_u32(smem + R::k_at + (n % R::K) * R::tile_bytes);
-#pragma unroll 4
+            // (the address field of a descriptor counts 16 bytes)
+            const uint64_t q0 = sdesc_sw128(smem_u32(smem + (s % R::Q) * R::q_bytes), 1024, 16);
+            const uint64_t k0 = sdesc_sw128(smem_u32(smem + R::k_at + (n % R::K) * R::tile_bytes), 1024, 16);
+#pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk)
-              umma_f16(tmem + 64 * (n & 1), sdesc_sw128(q0 + (kk >> 2) * (kRows * 128) + 32 * (kk & 3), 1024, 16),
-                       sdesc_sw128(k0 + (kk >> 2) * (kKeys * 128) + 32 * (kk & 3), 1024, 16), idesc_s, kk ? 1u : 0u);
+              umma_f16(tmem + 64 * (n & 1), q0 + (kk >> 2) * (kRows * 8) + 2 * (kk & 3), k0 + (kk >> 2) * (kKeys * 8) + 2 * (kk & 3),
+                       idesc_s, kk ? 1u : 0u);
             umma_commit(&x->s_full[n & 1]);
             umma_commit(&x->k_empty[n % R::K]);
             if (left == 1) umma_commit(&x->q_free[s % R::Q]);
@@ -212,13 +209,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
             // a segment's first product overwrites O: the softmax has read the previous segment's
             if (first_p && sp > 0 && !bar_wait(&x->o_free, (sp - 1) & 1, p.status)) break;
             tc_fence_after();
-            const uint32_t v0 = smem_u32(smem + R::v_at + (t % R::V) * R::tile_bytes);
+            const uint64_t v0 = sdesc_sw128(smem_u32(smem + R::v_at + (t % R::V) * R::tile_bytes), 1024, 8192);
 #pragma unroll
             for (int c = 0; c < kPanels; ++c)
 #pragma unroll
               for (int kk = 0; kk < kKeys / 16; ++kk)
                 umma_f16_ts(tmem + 128 + 64 * c, tmem + 64 * (t & 1) + 8 * kk,
-                            sdesc_sw128(v0 + c * (kKeys * 128) + kk * 16 * 128, 1024, 8192), idesc_o, !first_p || kk ? 1u : 0u);
+                            v0 + c * (kKeys * 8) + kk * 128, idesc_o, !first_p || kk ? 1u : 0u);
             umma_commit(&x->o_done[t & 1]);
             umma_commit(&x->v_empty[t % R::V]);
           }
@@ -239,7 +236,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
       };
       float scale = 0.f;  // of the tile before, which is on its way while that tile's codes are
       auto publish = [&](int n) {
-        if (lane < 8) (y ? x->vs : x->ks)[n & 7][c] = scale;
+        const bool odd = !(scale < INFINITY);
+        const int e = odd ? 0 : (int)(__float_as_uint(scale) >> 23) - 127;
+        const uint32_t of = __ballot_sync(~0u, lane < 8 && odd);
+        if (lane < 4) x->ks[n & 7][c] = scale;
+        else if (lane < 8) x->lv[n & 7][c] = (float)e, x->unit[n & 7][c] = exp2i(-e);
+        else if (lane == 8) x->odd[n & 7] = (of >> 4 & 15u) | (of & 15u ? 16u : 0u);
         __syncwarp();
         if (lane == 0) mbar_arrive(&x->meta_full[n & 7]);
       };
@@ -293,80 +295,49 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
         more = at.next(p);
       }
       if (ok && t) publish(t - 1);
-    } else if (warp == 11) {
-      // ---------------- queries: copied as they are to where their halves go, all on their way at once, then a lane four rows
-      constexpr int kPieces = HD / 8;  // 16-byte pieces of a row
-      const bool neg = p.scale < 0.f;
-#pragma unroll 1
-      for (int s = 0;; ++s) {
-        const Seg* const g = next_seg(s);
-        if (!g) break;
-        const int qb = s % R::Q, rows = g->rows, base = base_of(rows);
-        const uint32_t dst = smem_u32(smem + qb * R::q_bytes);
-        auto place = [&](int row, int piece) { return (piece >> 3) * (kRows * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4); };
-        if (!(ok = __all_sync(~0u, bar_wait(&x->q_free[qb], ((s / R::Q) & 1) ^ 1u, p.status)))) break;
-#pragma unroll 1
-        for (int i = 0; i < kRows; i += 32) {
-          const int r = i + lane - base;
-          const long long from =
-              r >= 0 && r < rows ? (g->row0 + over_group(p, r)) * p.q_row_ld + (g->head0 + r - group * over_group(p, r)) * p.q_head_ld : -1;
-#pragma unroll 2
-          for (int j = lane; j < 32 * kPieces; j += 32) {
-            const int row = j / kPieces, piece = j % kPieces;
-            const long long q = __shfl_sync(~0u, from, row);
-            if (q >= 0) copy16_plain(dst + place(i + row, piece), static_cast<const uint16_t*>(p.q) + q + 8 * piece);
-          }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncwarp();
-#pragma unroll 1
-        for (int i = lane; i < kRows; i += 32) {
-          const bool has = i >= base && i < base + rows;
-          uint8_t* const at_row = smem + qb * R::q_bytes;
-          uint32_t m = 0;
-#pragma unroll 2
-          for (int c = 0; c < kPieces; ++c) {
-            const uint4 v = has ? *reinterpret_cast<const uint4*>(at_row + place(i, c)) : make_uint4(0, 0, 0, 0);
-            m = __vmaxu2(__vmaxu2(m, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
-            m = __vmaxu2(__vmaxu2(m, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
-          }
-          const int sh = row_shift<HALF>(max(m & 0xffffu, m >> 16));
-#pragma unroll 2
-          for (int c = 0; c < kPieces; ++c) {
-            uint4* const to = reinterpret_cast<uint4*>(at_row + place(i, c));
-            const uint4 v = has ? *to : make_uint4(0, 0, 0, 0);
-            *to = make_uint4(row_half2<HALF>(v.x, sh, neg), row_half2<HALF>(v.y, sh, neg), row_half2<HALF>(v.z, sh, neg),
-                             row_half2<HALF>(v.w, sh, neg));
-          }
-          x->shift[s & 3][i] = (int16_t)sh;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&x->q_full[qb]);
-          mbar_arrive(&x->shift_full[s & 3]);
-        }
-      }
     }
   } else if (warp >= 4) {
     // ---------------- widening: thread i has the 16-byte pieces i, i + 128, ... of a tile's K and of its V codes
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     const int i = threadIdx.x - 128;
     constexpr int kPieces = HD / 16, kN = kKeys * kPieces / 128, kStep = 128 / kPieces;  // pieces a row, a thread; rows between
-    const int row_i = i / kPieces, piece = i % kPieces, c0 = (piece & 3) * 2;
+    // Of 8 threads, whose 16 bytes are read or written together, the even row's four read the pieces of one half of the row
+    // and the odd row's those of the other (HD 128): neither the codes nor the halves meet in a bank.
+    const int row_i = HD == 64 ? i / 4 : 2 * (i / 16) + ((i >> 2) & 1);
+    const int piece = HD == 64 ? i % 4 : (i & 3) + 4 * (((i >> 3) ^ (i >> 2)) & 1), c0 = (piece & 3) * 2;
+    // the queries of a segment that begins at tile t are copied as they are to where their halves go, a thread a row, while
+    // K of tile t is widened
+    constexpr int kQPieces = HD / 8;
+    auto q_place = [&](int c) { return (c >> 3) * (kRows * 128) + i * 128 + (((c & 7) ^ (i & 7)) << 4); };
     // K of tile t, then V of tile t - 1
     int s = 0, kt = 0, left = 0;  // the keys from the tile before's first one on
     const Seg* g = next_seg(0);
     if (g) kt = g->kt0;
 #pragma unroll 1
     for (int t = 0; ok; ++t) {
+      const bool enter = g && kt == g->kt0;
+      const int qb = s % R::Q;
+      uint8_t* const q_row = smem + qb * R::q_bytes;
+      bool has = false, used = false;  // this thread's row, one of its warp's
+      if (enter) {
+        if (!(ok = __all_sync(~0u, bar_wait(&x->q_free[qb], ((s / R::Q) & 1) ^ 1u, p.status)))) break;
+        const int row = i - base_of(g->rows), tok = over_group(p, max(row, 0));
+        has = row >= 0 && row < g->rows;
+        used = __any_sync(~0u, has);
+        if (has) {
+          const uint16_t* const from = static_cast<const uint16_t*>(p.q) + (long long)(g->row0 + tok) * p.q_row_ld +
+                                       (long long)(g->head0 + row - group * tok) * p.q_head_ld;
+#pragma unroll
+          for (int c = 0; c < kQPieces; ++c) copy16_plain(smem_u32(q_row + q_place(c)), from + 8 * c);
+        }
+      }
       if (g && !(ok = bar_wait(&x->raw_full[t % R::RawK], (t / R::RawK) & 1, p.status))) break;
 #pragma unroll 1
       for (int y = g ? 0 : 1; y < (t ? 2 : 1); ++y) {
         const int n = t - y, ring = y ? R::V : R::K, slot = n % ring;
         if (!(ok = bar_wait(y ? &x->v_empty[slot] : &x->k_empty[slot], ((n / ring) & 1) ^ 1u, p.status))) break;
         const uint8_t* const raw =
-            smem + (y ? R::raw_v_at + (n % R::RawV) * R::raw_bytes : R::raw_k_at + (n % R::RawK) * R::raw_bytes) + 16 * i;
+            smem + (y ? R::raw_v_at + (n % R::RawV) * R::raw_bytes : R::raw_k_at + (n % R::RawK) * R::raw_bytes) + row_i * HD + 16 * piece;
         uint8_t* const dst = smem + (y ? R::v_at : R::k_at) + slot * R::tile_bytes + (piece >> 2) * (kKeys * 128) + row_i * 128;
         const int x0 = (c0 ^ (row_i & 7)) << 4;  // (rows kStep apart are the same in the swizzle's 8)
 #pragma unroll
@@ -383,6 +354,34 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
         if (lane == 0) {
           mbar_arrive(y ? &x->v_full[slot] : &x->k_full[slot]);
           mbar_arrive(y ? &x->raw_v_empty[n % R::RawV] : &x->raw_k_empty[n % R::RawK]);
+        }
+        if (enter && y == 0) {
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          if (used) {  // (of a warp without a row nobody reads the scores)
+            uint32_t m = 0;
+#pragma unroll 4
+            for (int c = 0; c < kQPieces; ++c) {
+              const uint4 v = has ? *reinterpret_cast<const uint4*>(q_row + q_place(c)) : make_uint4(0, 0, 0, 0);
+              m = __vmaxu2(__vmaxu2(m, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
+              m = __vmaxu2(__vmaxu2(m, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
+            }
+            const int sh = row_shift<HALF>(max(m & 0xffffu, m >> 16));
+            const bool neg = p.scale < 0.f;
+#pragma unroll 2
+            for (int c = 0; c < kQPieces; ++c) {
+              uint4* const to = reinterpret_cast<uint4*>(q_row + q_place(c));
+              const uint4 v = has ? *to : make_uint4(0, 0, 0, 0);
+              *to = make_uint4(row_half2<HALF>(v.x, sh, neg), row_half2<HALF>(v.y, sh, neg), row_half2<HALF>(v.z, sh, neg),
+                               row_half2<HALF>(v.w, sh, neg));
+            }
+            x->shift[s & 3][i] = (int16_t)sh;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&x->q_full[qb]);
+            mbar_arrive(&x->shift_full[s & 3]);
+          }
         }
       }
       if (!ok || !g) break;
@@ -443,85 +442,78 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
         const uint32_t sbuf = tmem + lanes + 64 * (t & 1);
         const int kb = kt * kKeys;
         const float* const ks = x->ks[t & 7];
-        const float* const vs = x->vs[t & 7];
-        const bool odd = !__all_sync(~0u, ks[lane & 3] < INFINITY && vs[lane & 3] < INFINITY);
-        // scores that their rows do not see, and all of them where a scale is not finite: it may only meet what a row sees
-        if (!__all_sync(~0u, kb + kKeys <= lim) || odd) {
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            float v[16];
-            tmem_ld16(sbuf + 16 * c, v);
-            uint32_t u[16];
+        const uint32_t odd = x->odd[t & 7];  // 1 << c: chunk c's value scale is not finite; 16: a key scale
+        float ck[4], lv[4];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float f = odd ? fmaf(v[i], c_row * ks[c], exponent(vs[c])) : v[i];
-              u[i] = __float_as_uint(kb + 16 * c + i < lim ? f : -INFINITY);
-            }
-            tmem_st16(sbuf + 16 * c, u);
+        for (int c = 0; c < 4; ++c) {
+          ck[c] = c_row * ks[c];
+          if (ck[c] == 0.f) ck[c] = 1.1754944e-38f;  // (-inf times 0)
+          lv[c] = x->lv[t & 7][c];
+        }
+        float w[2][32];
+        tmem_ld32(sbuf, w[0]);
+        tmem_ld32(sbuf + 32, w[1]);
+        uint32_t v[64];  // the scores, then two weights each
+#pragma unroll
+        for (int i = 0; i < 64; ++i) v[i] = __float_as_uint(w[i >> 5][i & 31]);
+        // scores that the row does not see, and all of them where a scale is not finite: it may only meet what a row sees
+        if (!__all_sync(~0u, kb + kKeys <= lim) || odd) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            float f = __uint_as_float(v[i]);
+            if (odd) f = fmaf(f, c_row * ks[i >> 4], lv[i >> 4]);
+            v[i] = __float_as_uint(kb + i < lim ? f : -INFINITY);
           }
-          tmem_st_wait();
+          if (odd) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              ck[c] = 1.f;
+              lv[c] = 0.f;
+            }
+          }
         }
         float mx = -INFINITY;
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          float v[32];
-          tmem_ld32(sbuf + 32 * h, v);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float m = fmax3(v[16 * c], v[16 * c + 1], v[16 * c + 2]);
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t* const u = v + 16 * c;
+          float m = fmax3(__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]));
 #pragma unroll
-            for (int i = 3; i < 15; i += 2) m = fmax3(m, v[16 * c + i], v[16 * c + i + 1]);
-            m = fmaxf(m, v[16 * c + 15]);
-            // (-inf times a scale of 0 is no number, and fmaxf passes over it)
-            mx = fmaxf(mx, odd ? m : fmaf(m, c_row * ks[2 * h + c], exponent(vs[2 * h + c])));
-          }
+          for (int i = 3; i < 15; i += 2) m = fmax3(m, __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
+          mx = fmaxf(mx, fmaf(fmaxf(m, __uint_as_float(u[15])), ck[c], lv[c]));
         }
         const bool raise = mx > M + kRaise;
         const float m_old = M;
         M = raise ? mx - kBelow : M;
         const float ref = M == -INFINITY ? 0.f : M;
         float add = 0.f;
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          float v[32];
-          tmem_ld32(sbuf + 32 * h, v);
-          uint32_t u[16];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float e2 = exponent(vs[2 * h + c]), d = (odd ? 0.f : e2) - ref;
-            float ck = odd ? 1.f : c_row * ks[2 * h + c];
-            ck = ck == 0.f ? 1.1754944e-38f : ck;  // (-inf times 0)
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int c = 2 * h; c < 2 * h + 2; ++c) {
+            const float d = lv[c] - ref;
             float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll
             for (int i = 16 * c; i < 16 * c + 16; i += 4) {
-              const float2 a = __ffma2_rn(make_float2(v[i], v[i + 1]), make_float2(ck, ck), make_float2(d, d));
-              const float2 b = __ffma2_rn(make_float2(v[i + 2], v[i + 3]), make_float2(ck, ck), make_float2(d, d));
+              const float2 a = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), make_float2(ck[c], ck[c]), make_float2(d, d));
+              const float2 b = __ffma2_rn(make_float2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), make_float2(ck[c], ck[c]), make_float2(d, d));
               const float2 ea = make_float2(exp2_approx(a.x), exp2_approx(a.y)), eb = make_float2(exp2_approx(b.x), exp2_approx(b.y));
               s0 = __fadd2_rn(s0, ea);
               s1 = __fadd2_rn(s1, eb);
-              u[i / 2] = pack_f16x2(ea.x, ea.y);
-              u[i / 2 + 1] = pack_f16x2(eb.x, eb.y);
+              v[i / 2] = pack_f16x2(ea.x, ea.y);
+              v[i / 2 + 1] = pack_f16x2(eb.x, eb.y);
             }
-            add = fmaf((s0.x + s1.x) + (s0.y + s1.y), exp2i(-(int)e2), add);
+            add = fmaf((s0.x + s1.x) + (s0.y + s1.y), x->unit[t & 7][c], add);
           }
-          // over the scores of the half that is done with: columns 0-15, then 16-31
-          tmem_st16(sbuf + 16 * h, u);
-        }
-        if (odd) {  // values that are NaN, where the row sees them
-          tmem_st_wait();
-#pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            float v[16];
-            tmem_ld16(sbuf + 16 * h, v);
-            uint32_t u[16];
+          if (odd) {  // values that are NaN, where the row sees them
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int key = kb + 32 * h + 2 * i;
-              u[i] = __float_as_uint(v[i]);
-              if (!(vs[2 * h + (i >> 3)] < INFINITY)) u[i] |= (key < lim ? 0x7fffu : 0u) | (key + 1 < lim ? 0x7fff0000u : 0u);
-            }
-            tmem_st16(sbuf + 16 * h, u);
+            for (int i = 16 * h; i < 16 * h + 16; ++i)
+              if (odd >> (i >> 3) & 1u)
+                v[i] |= (kb + 2 * i < lim ? 0x7fffu : 0u) | (kb + 2 * i + 1 < lim ? 0x7fff0000u : 0u);
           }
+          uint32_t u[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) u[i] = v[16 * h + i];
+          tmem_st16(sbuf + 16 * h, u);
         }
         if (!first && __any_sync(~0u, raise)) {
           // O holds the tiles before relative to the old exponent
