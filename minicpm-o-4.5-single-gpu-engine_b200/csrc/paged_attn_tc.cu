@@ -103,6 +103,12 @@ T2W_DEV bool bar_wait(uint64_t* bar, uint32_t parity, int* err) {
   }
   return true;
 }
+// One lane of a converged warp: said so, the compiler need not expect several lanes' descriptors behind a product.
+T2W_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p;
+}
 T2W_DEV void copy16_plain(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -173,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == 8) {
       // ---------------- S_n, then W V of tile n - 1 (the products of one thread are in order: S_n writes over W_{n-2})
-      if (lane == 0) {
+      if (elect_one()) {
         constexpr uint32_t idesc_s = idesc_half(kRows, kKeys), idesc_o = idesc_half(kRows, 64, true);
         int s = -1, left = 0;              // the segment of S_n, and its tiles from n on
         int sp = 0;                        // the segment of tile n - 1, and whether that tile is its first
