@@ -18,8 +18,8 @@ namespace t2w {
 constexpr int kScaleMin = -64, kScaleMax = 64;
 
 // ---------------------------------------------------------------- a plan's buffer (int32)
-// header, then q_start [B + 1], kv_len [B], slot [rows], request [rows], bases [B + 1] x 4 (new pages, runs, places, segments), starts
-// 2 x int4 [workers], runs int4 [max_runs].  Every part begins on a 16-byte boundary.
+// header, then q_start [B + 1], kv_len [B], slot [rows], request [rows], bases [B + 1] x 4 (new pages, runs, places,
+// segments), starts 2 x int4 [workers], runs int4 [max_runs].  Every part begins on a 16-byte boundary.
 struct PlanHead {
   int n_runs;   // runs of rows that go into one page
   int tiles;    // places of the attention's key tiles (see PagedCut)
@@ -39,11 +39,12 @@ struct PlanLayout {
 // in tiles of `kt`.  The tiles of all segments, in that order, are numbered, and the places are dealt to the workers in
 // equal contiguous shares, so that ragged lengths cost no balance; a segment that is cut by a share's end is finished by
 // k_paged_merge.  Where the worker is a block and a segment is a good deal shorter than a share, the shares end at the
-// nearest segment's end instead (whole segments).  In large calls each segment's first tile has `extra` empty places before it: what it costs a worker to
-// begin a segment, in tiles, so that a share of many short segments is not the one that the others wait for.
+// nearest segment's end instead (whole segments).  In large calls each segment's first tile has `extra` empty places
+// before it: what it costs a worker to begin a segment, in tiles, so that a share of many short segments is not the one
+// that the others wait for.
 enum class PagedForm {
   kFew,   // at most 16 query rows to a key head: a worker is a warp
-  kMid,   // a worker is a block, with tiles of 64 rows
+  kMid,   // at most 64, head_dim 64: a worker is a block, with tiles of 64 rows
   kMany,  // a worker is a block, with tcgen05 tiles of 128 rows
 };
 struct PagedCut {
@@ -60,28 +61,8 @@ struct PagedCut {
 // Blocks of 8 warps that an SM holds of the kernel for few query rows.
 constexpr int few_warps = 8;
 constexpr int few_blocks(int hd, int nq) { return hd == 128 || nq == 2 ? 1 : 2; }
-#ifndef MB64
-#define MB64 4
-#endif
-#ifndef MB128
-#define MB128 3
-#endif
-#ifndef MS
-#define MS 3
-#endif
-#ifndef MW
-#define MW 4
-#endif
-#ifndef MQS
-#define MQS 1
-#endif
-#ifndef MIDRULE
-#define MIDRULE 1
-#endif
-constexpr int mid_blocks(int hd) { return hd == 128 ? MB128 : MB64; }
-constexpr int mid_warps = MW;
-constexpr int mid_stages = MS;
-// 
+// The same of the form for middling numbers of rows (head_dim 64 alone), its warps, and the stages of a block's ring.
+constexpr int mid_blocks = 4, mid_warps = 4, mid_stages = 3;
 constexpr int few_stages = 3;  // tiles of a warp's ring (8 KB each, 4 KB where head_dim is 64): the SM's rings hold 196 KB
 
 inline int64_t round4(int64_t n) { return (n + 3) & ~int64_t(3); }
@@ -90,8 +71,8 @@ PagedCut paged_cut(int max_fresh, int q_heads, int kv_heads, int head_dim);
 PlanLayout paged_layout(int64_t requests, int64_t rows, int page, const PagedCut& cut);
 
 // ---------------------------------------------------------------- tiles of a request (device)
-// sum over i < n of floor((a i + b) / m), a, b >= 0 (the lattice points under a line, by Euclid's algorithm on a and m)
-// (a n + b < 2^32: the arguments are numbers of keys; division by 32 bits is several times faster)
+// sum over i < n of floor((a i + b) / m), a, b >= 0 (the lattice points under a line, by Euclid's algorithm on a and m);
+// a n + b < 2^32, the arguments being numbers of keys: division by 32 bits is several times faster.
 T2W_DEV long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
   long long s = 0;
   while (n > 0) {

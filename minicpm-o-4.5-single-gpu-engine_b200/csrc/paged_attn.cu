@@ -66,89 +66,72 @@ T2W_DEV void stage_places(uint32_t (&put)[2], uint32_t& get_k, uint32_t (&get_v)
 }
 
 // A warp's 8 NQ query rows of a segment: thread (g, t) = (lane / 4, lane % 4) has of rows g, g + 8, ... what the scores'
-// tiles give it, and columns 2t, 2t + 1 (+ 8 ...) of the transposed output.  Where the output alone takes half the
-// registers (QS), the queries' fragments lie in shared memory: 16 bytes of a lane for each 16 rows and step of 16 dims.
-template <int HD, int NQ, bool QS>
+// tiles give it, and columns 2t, 2t + 1 (+ 8 ...) of the transposed output.
+template <int HD, int NQ>
 struct Rows {
-  static constexpr int A = (NQ + 1) / 2;  // tiles of 16 rows
-  uint32_t qa[QS ? 1 : A][QS ? 1 : HD / 16][4];  // queries as halves, as A operands
+  uint32_t qa[HD / 16][4];         // queries as halves, as A operands
   float c[NQ];                     // scale * log2 e / the power of two that the row's queries were multiplied by
   int end[NQ];                     // keys that the row sees
   float M[NQ], l[NQ], o[NQ][HD / 16][4];
 };
 // Rows first .. of the segment that begins at row row0 and has `rows`; the segment's first row's query sees `before` + 1
-// keys where the call is causal.  qs: the warp's place in shared memory (QS).
-template <int HD, bool HALF, int NQ, bool QS>
-T2W_DEV void load_rows(const AttnDev& p, Rows<HD, NQ, QS>& q, uint4* qs, int row0, int first, int rows, int hk, int before, int kv) {
+// keys where the call is causal.
+template <int HD, bool HALF, int NQ>
+T2W_DEV void load_rows(const AttnDev& p, Rows<HD, NQ>& q, int row0, int first, int rows, int hk, int before, int kv) {
   constexpr int kC = HD / 64, kM = HD / 16;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, group = p.group;
 #pragma unroll
-  for (int a = 0; a < (NQ + 1) / 2; ++a) {
-    uint32_t qa[kM][4];
+  for (int n = 0; n < 2; ++n) {
+    if (n >= NQ) {
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      const int n = 2 * a + y;
-      if (n >= NQ) {
+      for (int i = 0; i < kM; ++i) q.qa[i][n] = q.qa[i][2 + n] = 0;
+      continue;
+    }
+    const int row = first + g + 8 * n;
+    uint4 v[kC][2];
+    uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < kM; ++i) qa[i][y] = qa[i][2 + y] = 0;
-        continue;
-      }
-      const int row = first + g + 8 * n;
-      uint4 v[kC][2];
-      uint32_t m = 0;
+    for (int c = 0; c < kC; ++c)
 #pragma unroll
-      for (int c = 0; c < kC; ++c)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          v[c][i] = make_uint4(0, 0, 0, 0);
-          if (row < rows) {
-            const uint16_t* x = static_cast<const uint16_t*>(p.q) + (row0 + over_group(p, row)) * p.q_row_ld +
-                                (hk * group + row - group * over_group(p, row)) * p.q_head_ld;
-            v[c][i] = __ldg(reinterpret_cast<const uint4*>(x + 64 * c + 16 * t + 8 * i));
-          }
-          const uint4 u = v[c][i];
-          m = __vmaxu2(__vmaxu2(m, u.x & 0x7fff7fffu), u.y & 0x7fff7fffu);
-          m = __vmaxu2(__vmaxu2(m, u.z & 0x7fff7fffu), u.w & 0x7fff7fffu);
+      for (int i = 0; i < 2; ++i) {
+        v[c][i] = make_uint4(0, 0, 0, 0);
+        if (row < rows) {
+          const uint16_t* x = static_cast<const uint16_t*>(p.q) + (row0 + over_group(p, row)) * p.q_row_ld +
+                              (hk * group + row - group * over_group(p, row)) * p.q_head_ld;
+          v[c][i] = __ldg(reinterpret_cast<const uint4*>(x + 64 * c + 16 * t + 8 * i));
         }
-      m = max(m & 0xffffu, m >> 16);
-      m = max(m, __shfl_xor_sync(~0u, m, 1));
-      m = max(m, __shfl_xor_sync(~0u, m, 2));
-      const int sh = row_shift<HALF>(m);
-#pragma unroll
-      for (int c = 0; c < kC; ++c) {
-        const uint32_t u[8] = {v[c][0].x, v[c][0].y, v[c][0].z, v[c][0].w, v[c][1].x, v[c][1].y, v[c][1].z, v[c][1].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) qa[4 * c + j][2 * i + y] = row_half2<HALF>(u[2 * j + i], sh, p.scale < 0.f);
+        const uint4 u = v[c][i];
+        m = __vmaxu2(__vmaxu2(m, u.x & 0x7fff7fffu), u.y & 0x7fff7fffu);
+        m = __vmaxu2(__vmaxu2(m, u.z & 0x7fff7fffu), u.w & 0x7fff7fffu);
       }
-      q.c[n] = scaled(fabsf(p.scale) * kLog2e, -sh);
-      q.end[n] = p.causal ? before + over_group(p, row) + 1 : kv;
-      q.M[n] = -INFINITY;
-      q.l[n] = 0.f;
+    m = max(m & 0xffffu, m >> 16);
+    m = max(m, __shfl_xor_sync(~0u, m, 1));
+    m = max(m, __shfl_xor_sync(~0u, m, 2));
+    const int sh = row_shift<HALF>(m);
 #pragma unroll
-      for (int i = 0; i < kM; ++i) q.o[n][i][0] = q.o[n][i][1] = q.o[n][i][2] = q.o[n][i][3] = 0.f;
+    for (int c = 0; c < kC; ++c) {
+      const uint32_t u[8] = {v[c][0].x, v[c][0].y, v[c][0].z, v[c][0].w, v[c][1].x, v[c][1].y, v[c][1].z, v[c][1].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) q.qa[4 * c + j][2 * i + n] = row_half2<HALF>(u[2 * j + i], sh, p.scale < 0.f);
     }
+    q.c[n] = scaled(fabsf(p.scale) * kLog2e, -sh);
+    q.end[n] = p.causal ? before + over_group(p, row) + 1 : kv;
+    q.M[n] = -INFINITY;
+    q.l[n] = 0.f;
 #pragma unroll
-    for (int i = 0; i < kM; ++i) {
-      if constexpr (QS) {
-        qs[(a * kM + i) * 32 + lane] = make_uint4(qa[i][0], qa[i][1], qa[i][2], qa[i][3]);
-      } else {
-#pragma unroll
-        for (int y = 0; y < 4; ++y) q.qa[a][i][y] = qa[i][y];
-      }
-    }
+    for (int i = 0; i < kM; ++i) q.o[n][i][0] = q.o[n][i][1] = q.o[n][i][2] = q.o[n][i][3] = 0.f;
   }
-  if constexpr (QS) __syncwarp();
 }
 // 32 keys from kb on: their scores, weights and products.  get_k, get_v: the lane's places in a stage (stage_places()).
-template <int HD, int NQ, bool QS, bool P16>
-T2W_DEV void tile_step(Rows<HD, NQ, QS>& q, const uint4* qs, const FewStage<HD>& st, uint32_t get_k, const uint32_t (&get_v)[2],
+template <int HD, int NQ, bool P16>
+T2W_DEV void tile_step(Rows<HD, NQ>& q, const FewStage<HD>& st, uint32_t get_k, const uint32_t (&get_v)[2],
                        int kb, int kv, int all_see) {
-  constexpr int kC = HD / 64, kM = HD / 16, kA = (NQ + 1) / 2, kH = P16 ? 2 : 1;  // kH: pages of the tile
-  const int lane = threadIdx.x & 31, t = lane & 3;
+  constexpr int kC = HD / 64, kM = HD / 16, kH = P16 ? 2 : 1;  // kH: pages of the tile
+  const int t = threadIdx.x & 3;
   const uint8_t* const bytes = st.k;
-  float d[kA][4][4] = {};
+  float d[4][4] = {};
 #pragma unroll
   for (int c = 0; c < kC; ++c) {
     uint4 kr[4];
@@ -156,25 +139,11 @@ T2W_DEV void tile_step(Rows<HD, NQ, QS>& q, const uint4* qs, const FewStage<HD>&
     for (int j = 0; j < 4; ++j) kr[j] = *reinterpret_cast<const uint4*>(bytes + 8 * HD * j + (get_k ^ (64 * c)));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint32_t qa[kA][4];
-#pragma unroll
-      for (int a = 0; a < kA; ++a) {
-        if constexpr (QS) {
-          const uint4 u = qs[(a * kM + 4 * c + i) * 32 + lane];
-          qa[a][0] = u.x;
-          qa[a][1] = u.y;
-          qa[a][2] = u.z;
-          qa[a][3] = u.w;
-        } else {
-#pragma unroll
-          for (int y = 0; y < 4; ++y) qa[a][y] = q.qa[a][4 * c + i][y];
-        }
-      }
+      const uint32_t(&qa)[4] = q.qa[4 * c + i];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint2 u = e4m3x4_to_f16x4(i == 0 ? kr[j].x : i == 1 ? kr[j].y : i == 2 ? kr[j].z : kr[j].w);
-#pragma unroll
-        for (int a = 0; a < kA; ++a) mma_f16(d[a][j], qa[a][0], qa[a][1], qa[a][2], qa[a][3], u.x, u.y);
+        mma_f16(d[j], qa[0], qa[1], qa[2], qa[3], u.x, u.y);
       }
     }
   }
@@ -205,7 +174,7 @@ T2W_DEV void tile_step(Rows<HD, NQ, QS>& q, const uint4* qs, const FewStage<HD>&
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) s[j][i] = d[n >> 1][j][2 * (n & 1) + i];
+      for (int i = 0; i < 2; ++i) s[j][i] = d[j][2 * n + i];
     if (part) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -316,8 +285,8 @@ T2W_DEV void tile_step(Rows<HD, NQ, QS>& q, const uint4* qs, const FewStage<HD>&
   }
 }
 // This thread's columns of queries 2t and 2t + 1, HD / 8 in a row: finished rows (part nullptr) or a part's.
-template <int HD, bool HALF, int NQ, bool QS>
-T2W_DEV void store_rows(const AttnDev& p, const Rows<HD, NQ, QS>& q, int row0, int from, int rows, int hk, float* part, int part_rows) {
+template <int HD, bool HALF, int NQ>
+T2W_DEV void store_rows(const AttnDev& p, const Rows<HD, NQ>& q, int row0, int from, int rows, int hk, float* part, int part_rows) {
   constexpr int kM = HD / 16;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, group = p.group;
 #pragma unroll
@@ -364,8 +333,8 @@ T2W_DEV void store_rows(const AttnDev& p, const Rows<HD, NQ, QS>& q, int row0, i
 template <int HD, bool HALF, int NQ, bool P16>
 __global__ void __launch_bounds__(32 * few_warps, few_blocks(HD, NQ)) k_paged_few(const AttnDev p) {
   extern __shared__ __align__(16) uint8_t ring[];
-  constexpr int kC = HD / 64, kM = HD / 16, kS = few_stages;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  constexpr int kS = few_stages;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int w = few_warps * blockIdx.x + warp, group = p.group;
   const FewStage<HD>* const stage = reinterpret_cast<const FewStage<HD>*>(ring) + warp * kS;
   const uint32_t ring0 = smem_u32(stage);
@@ -458,8 +427,8 @@ __global__ void __launch_bounds__(32 * few_warps, few_blocks(HD, NQ)) k_paged_fe
     const int rows = f * group, nt = seg_tiles(kv, 32);
     const int kt0 = max(seg.w, 0), kt1 = min(nt, stop - zero);
     if (kt1 <= kt0) break;
-    Rows<HD, NQ, false> q;
-    load_rows<HD, HALF, NQ, false>(p, q, nullptr, row0, 0, rows, hk, kv - f, kv);
+    Rows<HD, NQ> q;
+    load_rows<HD, HALF, NQ>(p, q, row0, 0, rows, hk, kv - f, kv);
     const int all_see = p.causal ? kv - f + 1 : kv;  // keys that every row sees
     for (int kt = kt0; kt < kt1; ++kt) {
       __syncwarp();  // every lane is done with the stage that is filled again
@@ -467,9 +436,8 @@ __global__ void __launch_bounds__(32 * few_warps, few_blocks(HD, NQ)) k_paged_fe
       asm volatile("cp.async.wait_group %0;" ::"n"(kS - 1) : "memory");
       __syncwarp();
       const FewStage<HD>& st = stage[at];
-      const uint8_t* const bytes = st.k;
       at = at + 1 == kS ? 0 : at + 1;
-      tile_step<HD, NQ, false, P16>(q, nullptr, st, get_k, get_v, kt * 32, kv, all_see);
+      tile_step<HD, NQ, P16>(q, st, get_k, get_v, kt * 32, kv, all_see);
     }
     const bool whole = kt0 == 0 && kt1 == nt;
     float* const part = whole    ? nullptr
@@ -479,7 +447,7 @@ __global__ void __launch_bounds__(32 * few_warps, few_blocks(HD, NQ)) k_paged_fe
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       __syncwarp();  // the warp's ring is read to the end
     }
-    store_rows<HD, HALF, NQ, false>(p, q, row0, 0, rows, hk, part, 16);
+    store_rows<HD, HALF, NQ>(p, q, row0, 0, rows, hk, part, 16);
     if (filled) {  // all the block's warps come here, each with its one segment
       __syncthreads();
       float* const out = part_of(p.ws, 2 * few_warps * blockIdx.x, 16, HD);
@@ -538,11 +506,11 @@ __global__ void __launch_bounds__(32 * few_warps, few_blocks(HD, NQ)) k_paged_fe
 // keys' K or V) into the block's ring and all four read all.  Tiles of 128 rows on tcgen05 (paged_attn_tc.cu) have the
 // faster products, but their hand-overs from copies to widening to products to softmax and back cost a 50-row window more
 // than its work.
-template <int HD, bool HALF, bool P16>
-__global__ void __launch_bounds__(32 * mid_warps, mid_blocks(HD)) k_paged_mid(const AttnDev p) {
+template <bool HALF, bool P16>
+__global__ void __launch_bounds__(32 * mid_warps, mid_blocks) k_paged_mid(const AttnDev p) {
   extern __shared__ __align__(16) uint8_t ring[];
-  constexpr int kS = mid_stages;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  constexpr int HD = 64, kS = mid_stages;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int w = blockIdx.x, group = p.group;
   const FewStage<HD>* const stage = reinterpret_cast<const FewStage<HD>*>(ring);
   const uint64_t policy = l2_policy_evict_first();
@@ -553,41 +521,35 @@ __global__ void __launch_bounds__(32 * mid_warps, mid_blocks(HD)) k_paged_mid(co
   Walk at;
   if (!at.begin(p, w)) return;
 
-  // ---- copies: a tile's quarters are K and V codes of its keys 0-31 and 32-63; a warp has every mid_warps-th
-  constexpr int kOwn = 4 / mid_warps;
+  // ---- copies: a tile's quarters are K and V codes of its keys 0-31 and 32-63, a quarter a warp
+  static_assert(mid_warps == 4, "a quarter a warp");
+  const int half = warp >> 1, x = warp & 1;
   Walk ahead = at;
-  int kt_a = at.kt0, pgA[kOwn], pgB[kOwn];
+  int kt_a = at.kt0, pgA = 0, pgB = 0;
   bool live = true;
   auto look_up = [&]() {
     if (!live) return;
-#pragma unroll
-    for (int u = 0; u < kOwn; ++u) {
-      const int key = kt_a * 64 + 32 * ((warp + u * mid_warps) >> 1);
-      const int* const table = p.table + (size_t)ahead.r * p.table_ld + (key >> p.shift);
-      pgA[u] = key < ahead.kv ? __ldg(table) : -2;  // -2: no keys
-      pgB[u] = P16 && key + 16 < ahead.kv ? __ldg(table + 1) : pgA[u];
-    }
+    const int key = kt_a * 64 + 32 * half;
+    const int* const table = p.table + (size_t)ahead.r * p.table_ld + (key >> p.shift);
+    pgA = key < ahead.kv ? __ldg(table) : -2;  // -2: no keys
+    pgB = P16 && key + 16 < ahead.kv ? __ldg(table + 1) : pgA;
   };
   auto send = [&](int to_stage) {
     if (live) {
-#pragma unroll
-      for (int u = 0; u < kOwn; ++u) {
-        const int half = (warp + u * mid_warps) >> 1, x = (warp + u * mid_warps) & 1;
-        if (pgA[u] == -2) continue;
-        if ((unsigned)pgA[u] >= (unsigned)p.pages || (unsigned)pgB[u] >= (unsigned)p.pages) {
+      if (pgA != -2) {
+        if ((unsigned)pgA >= (unsigned)p.pages || (unsigned)pgB >= (unsigned)p.pages) {
           atomicExch(p.status, T2W_ERR_INVALID);
-          pgA[u] = pgB[u] = 0;
+          pgA = pgB = 0;
         }
         const uint32_t to = smem_u32(ring) + (2 * to_stage + half) * (uint32_t)sizeof(FewStage<HD>);
-        const long long in =
-            ((long long)ahead.hk * p.page + (P16 ? 0 : (kt_a * 64 + 32 * half) & (p.page - 1))) * HD + 16 * lane;
-        const uint8_t* const lo = p.codes[x] + pgA[u] * p.page_ld[x] + in;
-        const uint8_t* const hi = P16 ? p.codes[x] + pgB[u] * p.page_ld[x] + in : lo + 16 * HD;
+        const long long in = ((long long)ahead.hk * p.page + (P16 ? 0 : (kt_a * 64 + 32 * half) & (p.page - 1))) * HD + 16 * lane;
+        const uint8_t* const lo = p.codes[x] + pgA * p.page_ld[x] + in;
+        const uint8_t* const hi = P16 ? p.codes[x] + pgB * p.page_ld[x] + in : lo + 16 * HD;
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i)
           copy16(to + x * 32 * HD + i * 512 + put[i & 1], i < HD / 32 ? lo + i * 512 : hi + (i - HD / 32) * 512, policy);
         if (lane < 2)  // ks or vs
-          copy4(to + 64 * HD + 8 * x + 4 * lane, p.scales[x] + (lane ? pgB[u] : pgA[u]) * p.scale_ld[x] + ahead.hk);
+          copy4(to + 64 * HD + 8 * x + 4 * lane, p.scales[x] + (lane ? pgB : pgA) * p.scale_ld[x] + ahead.hk);
       }
       if (++kt_a == ahead.kt1) {
         live = ahead.next(p);
@@ -609,8 +571,8 @@ __global__ void __launch_bounds__(32 * mid_warps, mid_blocks(HD)) k_paged_mid(co
     // keys that all of the warp's rows see, and that one of them sees
     const int all_see = p.causal ? before + over_group(p, from) + 1 : at.kv;
     const int some_see = p.causal ? before + over_group(p, min(from + 16, rows) - 1) + 1 : at.kv;
-    Rows<HD, 2, false> q;
-    load_rows<HD, HALF, 2, false>(p, q, nullptr, row0, from, rows, at.hk, before, at.kv);
+    Rows<HD, 2> q;
+    load_rows<HD, HALF, 2>(p, q, row0, from, rows, at.hk, before, at.kv);
     for (int kt = at.kt0; kt < at.kt1; ++kt) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kS - 2) : "memory");
       __syncthreads();  // every warp's copies of this tile are there, and nobody reads the stage before it any more
@@ -619,11 +581,11 @@ __global__ void __launch_bounds__(32 * mid_warps, mid_blocks(HD)) k_paged_mid(co
 #pragma unroll 1
         for (int i = 0; i < 2; ++i)
           if (kt * 64 + 32 * i < some_see)
-            tile_step<HD, 2, false, P16>(q, nullptr, stage[2 * st + i], get_k, get_v, kt * 64 + 32 * i, at.kv, all_see);
+            tile_step<HD, 2, P16>(q, stage[2 * st + i], get_k, get_v, kt * 64 + 32 * i, at.kv, all_see);
       st = st + 1 == kS ? 0 : st + 1;
     }
     float* const part = at.kt0 == 0 && at.kt1 == at.nt ? nullptr : part_of(p.ws, 2 * w + (at.first ? 0 : 1), 16 * mid_warps, HD);
-    if (mine) store_rows<HD, HALF, 2, false>(p, q, row0, from, rows, at.hk, part, 16 * mid_warps);
+    if (mine) store_rows<HD, HALF, 2>(p, q, row0, from, rows, at.hk, part, 16 * mid_warps);
   } while (at.next(p));
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -755,7 +717,7 @@ __global__ void __launch_bounds__(256) k_paged_merge(const AttnDev p) {
   if (parts.n <= 4) {  // a thread four columns of a row
     const float* part[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part[i] = parts.at(min(i, parts.n - 1));
+    for (int i = 0; i < 4; ++i) part[i] = parts.at(i);
 #pragma unroll 2
     for (int i = share * 32 + lane; i < rn * (HD / 4); i += 32 * shares) {
       const int row = i / (HD / 4), d = i % (HD / 4) * 4;
@@ -763,9 +725,14 @@ __global__ void __launch_bounds__(256) k_paged_merge(const AttnDev p) {
       float4 v[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        v[x] = __ldcg(reinterpret_cast<const float4*>(part[x] + row * HD + d));
-        m[x] = x < parts.n ? __ldcg(part[x] + p.part_rows * HD + row) : -INFINITY;
-        l[x] = __ldcg(part[x] + p.part_rows * HD + p.part_rows + row);
+        v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+        m[x] = -INFINITY;
+        l[x] = 0.f;
+        if (x < parts.n) {
+          v[x] = __ldcg(reinterpret_cast<const float4*>(part[x] + row * HD + d));
+          m[x] = __ldcg(part[x] + p.part_rows * HD + row);
+          l[x] = __ldcg(part[x] + p.part_rows * HD + p.part_rows + row);
+        }
         top = fmaxf(top, m[x]);
       }
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -804,19 +771,20 @@ cudaError_t launch_paged(const AttnDev& p, const PagedCut& cut, int max_rows, cu
   auto merge = [&](int shares) {
     return launch_k(k_paged_merge<HD, HALF>, dim3((cut.workers + 7) / 8, shares), dim3(256), 0, st, p);
   };
-  if (cut.form == PagedForm::kMid) {
-    constexpr int smem = 2 * mid_stages * (int)sizeof(FewStage<HD>);
-    static std::atomic<uint64_t> done[2];
-    auto mid = [&](auto* k, std::atomic<uint64_t>& d) {
-      const cudaError_t r = smem_attr_once(k, smem, d);
-      return r != cudaSuccess ? r : launch_k(k, dim3(cut.workers), dim3(32 * mid_warps), smem, st, p);
-    };
-    const cudaError_t e = p.page == 16 ? mid(k_paged_mid<HD, HALF, true>, done[0]) : mid(k_paged_mid<HD, HALF, false>, done[1]);
-    return e != cudaSuccess ? e : merge(cut.form == PagedForm::kMany ? 32 : 16);
-  }
+  if constexpr (HD == 64)
+    if (cut.form == PagedForm::kMid) {
+      constexpr int smem = 2 * mid_stages * (int)sizeof(FewStage<HD>);
+      static std::atomic<uint64_t> done[2];
+      auto mid = [&](auto* k, std::atomic<uint64_t>& d) {
+        const cudaError_t r = smem_attr_once(k, smem, d);
+        return r != cudaSuccess ? r : launch_k(k, dim3(cut.workers), dim3(32 * mid_warps), smem, st, p);
+      };
+      const cudaError_t e = p.page == 16 ? mid(k_paged_mid<HALF, true>, done[0]) : mid(k_paged_mid<HALF, false>, done[1]);
+      return e != cudaSuccess ? e : merge(16);
+    }
   if (cut.form == PagedForm::kMany) {
     const cudaError_t e = launch_paged_many(p, cut, HD, HALF, st);
-    return e != cudaSuccess ? e : merge(cut.form == PagedForm::kMany ? 32 : 16);
+    return e != cudaSuccess ? e : merge(16);
   }
   const int nq = max_rows > 8 ? 2 : 1;
   constexpr int smem = few_warps * few_stages * (int)sizeof(FewStage<HD>);

@@ -1,4 +1,4 @@
-// What the two forms of the paged attention share: the arguments, a finished row's store, the queries as halves, and the
+// What the forms of the paged attention share: the arguments, a finished row's store, the queries as halves, and the
 // parts of segments that were cut.
 #pragma once
 
@@ -45,27 +45,6 @@ T2W_DEV void store_row(const AttnDev& p, int row, int head, int hd, int d, float
     p.lse[(size_t)row * p.q_heads + head] = l != 0.f ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
 }
 
-// Eight columns, in one 16-byte store.
-template <bool HALF>
-T2W_DEV void store_row8(const AttnDev& p, int row, int head, int hd, int d, const float* o, float M, float l) {
-  const float inv = l != 0.f ? 1.f / l : 0.f;
-  uint32_t u[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float a = o[2 * i] * inv, b = o[2 * i + 1] * inv;
-    if constexpr (HALF) {
-      const __half2 v = __floats2half2_rn(a, b);
-      u[i] = *reinterpret_cast<const uint32_t*>(&v);
-    } else {
-      u[i] = pack_bf16x2(a, b);
-    }
-  }
-  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + ((size_t)row * p.q_heads + head) * hd + d) =
-      make_uint4(u[0], u[1], u[2], u[3]);
-  if (d == 0 && p.lse)
-    p.lse[(size_t)row * p.q_heads + head] = l != 0.f ? (M + log2f(l)) * 0.6931471805599453f : -INFINITY;
-}
-
 // The cache streams through L2 (evicted first), so that the plan, the tables and the parts stay there.
 T2W_DEV uint64_t l2_policy_evict_first() {
   uint64_t p;
@@ -105,7 +84,7 @@ constexpr float kRaise = 15.f, kBelow = 9.f;
 // A worker's unfinished rows of a segment: O [rows][HD], then the reference exponents [rows] and the sums [rows].
 T2W_DEV float* part_of(float* ws, int slot, int rows, int hd) { return ws + (size_t)slot * rows * (hd + 2); }
 
-// A worker's walk over its segments: every role makes it for itself.
+// A block's walk over its segments.
 struct Walk {
   int r, hk, qt;       // the segment
   int row0, f, kv;     // its request's first row, rows and keys

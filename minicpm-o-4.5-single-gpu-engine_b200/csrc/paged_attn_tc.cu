@@ -14,19 +14,23 @@
 //
 // Two blocks an SM, each three warpgroups.  Warps 0-3 softmax, a thread a row; a segment's output is finished during the
 // next segment's first tile.  Warps 4-7 widen: they write a tile's codes as halves in the 128-byte swizzle that the tensor
-// core reads, K a tile ahead of V.  Warp 8 issues the products, warp 10 walks the segments and sends for the tiles ahead (a
-// bulk copy for each page), warp 11 brings the next segment's queries.  Of the 80 registers that a thread of the block is launched with, the three warpgroups take 128, 64
-// and 48.
+// core reads, K a tile ahead of V, and bring a segment's queries.  Warp 8 issues the products, warp 10 walks the segments
+// and sends for the tiles ahead (a bulk copy for each page).  Of the 80 registers that a thread of the block is launched
+// with, the three warpgroups take 128, 56 and 56.
 //
-// The roles' code is kept short (loops where the trip count is known, one walk over the segments for all): with the first
-// version's 62 KB the softmax warps waited for instructions most of the time.
+// What was in the way, in the order it was found (4 requests of 700 to 1024 tokens over histories to 4096, 16 query and 4
+// key heads, head_dim 128): queries brought by one warp of their own, 20,000 clocks a segment (185 us, of which it was
+// 30); code that does not fit the instruction caches, 62 KB at first, so that what few tiles need is kept in short loops;
+// descriptors made for each product by a lane that the compiler could not know to be alone (150 us before, 147 after);
+// spills of the products' warp (138 to 135).  Without the registers' split (96 for each of 10 warps) it is 158.
 //
 // Segments of at most 64 rows (windows) lie in the upper rows of every other block's tiles: a warp's exponentials run on
 // the SM quarter that its TMEM lanes belong to, and so the two blocks of an SM use all four.
 //
-// What bounds it: for windows of some ten rows HBM (the codes are read once; 8 KB a tile at 64 columns), for longer
-// chunks the exponentials: 16 a clock and SM, 512 clocks a tile, against 256 (head_dim 64) or 512 (128) of the tensor
-// core.
+// What bounds it: a tile takes an SM 1950 clocks.  The exponentials (16 a clock and SM) need 512 of them, the tensor core
+// 256 (head_dim 64) or 512 (128), shared memory about 1100 (the products read queries, keys and values from it, and every
+// code passes through it twice); 900 instructions issue on each of the SM's quarters, from two softmax and two widening
+// warps, which is too few to hide what each waits for.  The chunks above: 135 us, 430 TFLOP/s, 25% of cuBLAS's bf16 rate.
 #include "paged_attn.cuh"
 
 namespace t2w {
@@ -176,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
   };
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 8) {
       // ---------------- S_n, then W V of tile n - 1 (the products of one thread are in order: S_n writes over W_{n-2})
       if (elect_one()) {
@@ -304,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
     }
   } else if (warp >= 4) {
     // ---------------- widening: thread i has the 16-byte pieces i, i + 128, ... of a tile's K and of its V codes
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     const int i = threadIdx.x - 128;
     constexpr int kPieces = HD / 16, kN = kKeys * kPieces / 128, kStep = 128 / kPieces;  // pieces a row, a thread; rows between
     // Of 8 threads, whose 16 bytes are read or written together, the even row's four read the pieces of one half of the row

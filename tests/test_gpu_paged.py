@@ -316,7 +316,7 @@ def test_scale_range(value):
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-@pytest.mark.parametrize("fresh", [1, 40])
+@pytest.mark.parametrize("fresh", [1, 20, 40])
 def test_not_finite(bad, fresh):
     """A page and head given a value that is not finite reads as NaN: in rows that see one of its keys and in no others."""
     page, heads, hd, group = 16, 2, 64, 2
@@ -401,7 +401,7 @@ def test_pitches_and_far_pages(fresh):
     assert bool((big[:, :2] == -1).all()) and bool((big[:, 6:] == -1).all())
 
 
-@pytest.mark.parametrize("fresh", [1, 30])
+@pytest.mark.parametrize("fresh", [1, 30, 70])
 def test_graph_and_streams(fresh):
     """A step captured on a side stream and replayed equals the same steps called one by one, bit for bit."""
     page, heads, hd, n = 16, 2, 64, 3
@@ -505,11 +505,11 @@ def test_void_plans():
             assert torch.equal(a, b)
 
 
-@pytest.mark.parametrize("fresh", [1, 40])
-def test_a_table_entry_that_is_no_page(fresh):
+@pytest.mark.parametrize("fresh,hd", [(1, 64), (40, 64), (40, 128)])
+def test_a_table_entry_that_is_no_page(fresh, hd):
     """An entry outside the pool is not followed: the status tells."""
-    c = paged.B200PagedCache(1, 16, 16, 1, 64, 1, 128)
-    x = torch.ones(40, 1, 64, device="cuda", dtype=torch.bfloat16)
+    c = paged.B200PagedCache(1, 16, 16, 1, hd, 1, 128)
+    x = torch.ones(40, 1, hd, device="cuda", dtype=torch.bfloat16)
     c.append(0, x, x, c.plan(i32([40]), 40, 40))
     p = c.plan(i32([fresh]), fresh, fresh)
     p.check()
