@@ -10,7 +10,9 @@ again for their sum being of unrounded weights, weights under 2^-25 of the large
 up to 128 products in fp32, each addition off by at most 2^-23 of B, and a weight's relative error is its score's error
 (twice, for the weight and the sum).  The log-sum may be off by 2^-16 B + 2^-19 max(1, |lse|)."""
 
+import importlib.util
 import math
+import pathlib
 
 import pytest
 import torch
@@ -570,3 +572,14 @@ def test_refusals():
     assert c.attend(0, q[:0], none).shape == (0, 4, 64)
     c.append(0, k[:0], k[:0], none)
     none.check()
+
+
+def test_the_example():
+    """A layer moves by at most 2^-3 of its values' size times the root of its squared weights' sum (2^-4 each from the
+    rounding of keys and of values): 0.025 over 66 even weights, 0.1 over four layers in step with one another, against
+    outputs of deviation 1 and more; the largest of 1024 is four times that."""
+    path = pathlib.Path(__file__).resolve().parents[1] / "examples" / "paged_stream.py"
+    spec = importlib.util.spec_from_file_location("paged_stream", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    assert module.run(layers=4, requests=3, steps=5, say=lambda s: None) < 0.4
