@@ -591,9 +591,11 @@ __global__ void __launch_bounds__(32 * mid_warps, mid_blocks) k_paged_mid(const 
 }
 
 // ---------------------------------------------------------------- segments that were cut
-// Where worker w's start is the first cut of a segment, a warp (or a few, for the rows' shares) joins the parts of that
-// segment: up to 4 parts a thread four columns of a row, more of them row by row.  The order is fixed, so the bits are too.  What it costs is a chain of loads after the kernel in front of it has ended:
-// so all that the plan tells is read before that, and the parts' rows are sent for together with their exponents.
+// Where worker w's start is the first cut of a segment, that segment's parts are joined: up to 4 parts by the start's
+// warp, a thread four columns of a row, more of them by the 8 warps of the block, a row at a time and every eighth part a
+// warp.  The order is fixed, so the bits are too.  What it costs is a chain of loads after the kernel in front of it has
+// ended: so all that the plan tells is read before that, the parts' rows are sent for together with their exponents, and
+// the blocks are resident at once.
 struct Parts {
   const float* ws;
   int rows_ld, hd;
@@ -618,19 +620,20 @@ T2W_DEV void load_cols(float (&u)[N], const float* v) {
   if constexpr (N == 4) *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(v);
   else *reinterpret_cast<float2*>(u) = *reinterpret_cast<const float2*>(v);
 }
-// A row's parts: a lane holds one part's exponent and sum of 32, and N columns of all of them.
+// A row's parts first, first + 8, ...: a lane holds one part's exponent and sum of 32, and N columns of all of them.
 template <int HD>
-T2W_DEV void join_parts(Joined<HD>& j, const Parts& parts, int row, int lane) {
+T2W_DEV void join_parts(Joined<HD>& j, const Parts& parts, int first, int row, int lane) {
   constexpr int N = HD / 32, K = 8;
+  const int count = (parts.n - first + 7) / 8;
   j.top = -INFINITY;
   j.sum = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) j.acc[i] = 0.f;
-  for (int x0 = 0; x0 < parts.n; x0 += 32) {
-    const int n = min(32, parts.n - x0);
+  for (int x0 = 0; x0 < count; x0 += 32) {
+    const int n = min(32, count - x0);
     float top = -INFINITY, sum = 0.f;
     if (lane < n) {
-      const float* q = parts.at(x0 + lane) + parts.rows_ld * HD + row;
+      const float* q = parts.at(first + 8 * (x0 + lane)) + parts.rows_ld * HD + row;
       top = __ldcg(q);
       sum = __ldcg(q + parts.rows_ld);
     }
@@ -641,7 +644,7 @@ T2W_DEV void join_parts(Joined<HD>& j, const Parts& parts, int row, int lane) {
       for (int i = 0; i < K; ++i) {
 #pragma unroll
         for (int y = 0; y < N; ++y) u[i][y] = 0.f;
-        if (i0 + i < n) load_cols<N>(u[i], parts.at(x0 + i0 + i) + row * HD + lane * N);
+        if (i0 + i < n) load_cols<N>(u[i], parts.at(first + 8 * (x0 + i0 + i)) + row * HD + lane * N);
       }
       if (i0 == 0) {
         m = fmaxf(j.top, top);
@@ -663,18 +666,15 @@ T2W_DEV void join_parts(Joined<HD>& j, const Parts& parts, int row, int lane) {
     }
   }
 }
+struct Long {  // a segment of more than 4 parts
+  Parts parts;
+  int r0, rn, head0;
+};
 template <int HD, bool HALF>
-T2W_DEV void store_joined(const AttnDev& p, const Joined<HD>& j, int row, int head, int lane) {
-  if constexpr (HD == 128) {
-    store_row<HALF>(p, row, head, HD, lane * 4, make_float4(j.acc[0], j.acc[1], j.acc[2], j.acc[3]), j.top, j.sum);
-  } else {
-    const float c = __shfl_down_sync(~0u, j.acc[0], 1), d = __shfl_down_sync(~0u, j.acc[1], 1);
-    if ((lane & 1) == 0) store_row<HALF>(p, row, head, HD, lane * 2, make_float4(j.acc[0], j.acc[1], c, d), j.top, j.sum);
-  }
-}
+__global__ void __launch_bounds__(256, 4) k_paged_merge(const AttnDev p) {
+  __shared__ Long longs[8];
+  __shared__ __align__(16) float joined[2][8][HD + 4];  // by warp: columns, exponent, sum
 
-template <int HD, bool HALF>
-__global__ void __launch_bounds__(256) k_paged_merge(const AttnDev p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = p.group;
   // The plan was complete before the kernel in front of this one began (it waited for it), so it is read ahead of the
   // wait, past this SM's L1.
@@ -685,6 +685,7 @@ __global__ void __launch_bounds__(256) k_paged_merge(const AttnDev p) {
   bool mine = false;
   int r0 = 0, rn = 0, head0 = 0;
   Parts parts;
+  parts.n = 0;
   if (w > 0 && w < workers) {
     const int4 seg = __ldcg(p.starts + 2 * w), of = __ldcg(p.starts + 2 * w + 1);  // of: first row, rows, keys
     const int at = of.w - seg.w, before = __ldcg(p.starts + 2 * w - 1).w;  // the place of the segment's tile 0; where w - 1 begins
@@ -713,8 +714,13 @@ __global__ void __launch_bounds__(256) k_paged_merge(const AttnDev p) {
   for (int row = used + blockIdx.y * gridDim.x + blockIdx.x; row < p.rows; row += gridDim.x * gridDim.y)
     for (int i = threadIdx.x; i < p.q_heads * (HD / 4); i += blockDim.x)
       store_row<HALF>(p, row, i / (HD / 4), HD, i % (HD / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
-  if (!mine) return;
-  if (parts.n <= 4) {  // a thread four columns of a row
+  if (lane == 0) {
+    longs[warp].parts = parts;
+    longs[warp].r0 = r0;
+    longs[warp].rn = mine && parts.n > 4 ? rn : 0;
+    longs[warp].head0 = head0;
+  }
+  if (mine && parts.n <= 4) {  // a thread four columns of a row
     const float* part[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) part[i] = parts.at(i);
@@ -750,12 +756,45 @@ __global__ void __launch_bounds__(256) k_paged_merge(const AttnDev p) {
       }
       store_row<HALF>(p, r0 + over_group(p, row), head0 + row - group * over_group(p, row), HD, d, acc, top, sum);
     }
-    return;
   }
-  for (int row = share; row < rn; row += shares) {
-    Joined<HD> j;
-    join_parts<HD>(j, parts, row, lane);
-    store_joined<HD, HALF>(p, j, r0 + over_group(p, row), head0 + row - group * over_group(p, row), lane);
+  __syncthreads();
+  int turn = 0;
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    const Long& g = longs[i];
+#pragma unroll 1
+    for (int row = share; row < g.rn; row += shares, turn ^= 1) {
+      Joined<HD> j;
+      join_parts<HD>(j, g.parts, warp, row, lane);
+      float* const mine8 = joined[turn][warp];
+#pragma unroll
+      for (int y = 0; y < HD / 32; ++y) mine8[lane * (HD / 32) + y] = j.acc[y];
+      if (lane == 0) {
+        mine8[HD] = j.top;
+        mine8[HD + 1] = j.sum;
+      }
+      __syncthreads();  // (the other turn's buffer is read until the next one)
+      if (threadIdx.x < HD / 4) {
+        const int d = threadIdx.x * 4;
+        float top = -INFINITY, sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) top = fmaxf(top, joined[turn][x][HD]);
+        if (top > -INFINITY) {
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const float e = exp2_approx(joined[turn][x][HD] - top);
+            const float4 v = *reinterpret_cast<const float4*>(&joined[turn][x][d]);
+            acc.x = fmaf(e, v.x, acc.x);
+            acc.y = fmaf(e, v.y, acc.y);
+            acc.z = fmaf(e, v.z, acc.z);
+            acc.w = fmaf(e, v.w, acc.w);
+            sum = fmaf(e, joined[turn][x][HD + 1], sum);
+          }
+        }
+        store_row<HALF>(p, g.r0 + over_group(p, row), g.head0 + row - group * over_group(p, row), HD, d, acc, top, sum);
+      }
+    }
   }
 }
 
@@ -780,11 +819,11 @@ cudaError_t launch_paged(const AttnDev& p, const PagedCut& cut, int max_rows, cu
         return r != cudaSuccess ? r : launch_k(k, dim3(cut.workers), dim3(32 * mid_warps), smem, st, p);
       };
       const cudaError_t e = p.page == 16 ? mid(k_paged_mid<HALF, true>, done[0]) : mid(k_paged_mid<HALF, false>, done[1]);
-      return e != cudaSuccess ? e : merge(16);
+      return e != cudaSuccess ? e : merge(cut.part_rows / 8);
     }
   if (cut.form == PagedForm::kMany) {
     const cudaError_t e = launch_paged_many(p, cut, HD, HALF, st);
-    return e != cudaSuccess ? e : merge(16);
+    return e != cudaSuccess ? e : merge(cut.part_rows / 8);
   }
   const int nq = max_rows > 8 ? 2 : 1;
   constexpr int smem = few_warps * few_stages * (int)sizeof(FewStage<HD>);
