@@ -33,6 +33,13 @@ T2W_DEV void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint3
 // Exponents: key j with scales s_k, s_v of its page weighs 2^(x_j + log2 s_v - M) on its V codes, M a little
 // below the running maximum of x_j + log2 s_v (kBelow): the weights of the largest contributions have all the bits that a
 // half has whatever the scales.  The sum of exponentials is kept in units of 2^M too.
+//
+// Measured: 64 requests of 40 to 4100 keys, 32 query and 8 key heads of 128: 272.6 MB in 58 us, 4.7 TB/s (73% of a copy);
+// 3 requests of 90k to 150k keys, 16 and 2 heads: 184.5 MB in 44 us, 4.2 TB/s.  In the second the stream itself, between a
+// worker's first tile and its last, runs at 7.5 TB/s; the rest is the launch, the plan's and the table's loads ahead of the
+// first tile (5 us), the last workers' ends (3) and the joining (5).  Of the other splits, a block of 8 warps on one
+// segment at a time took 167 and 68 us in its best form (short segments leave most of it idle), fragments loaded straight
+// from global memory 75 and 54, rings of 2 or 6 tiles 66 and 49 or 76 and 52 (this one then 61 and 42 to 46).
 template <int HD>
 struct FewStage {
   uint8_t k[32 * HD], v[32 * HD];
@@ -500,12 +507,16 @@ __global__ void __launch_bounds__(32 * few_warps, few_blocks(HD, NQ)) k_paged_fe
 
 // ---------------------------------------------------------------- 17 to 64 query rows to a key head
 //
-// Windows: what bounds them is still HBM, or close to it the mma pipe (4 HD flops for each key and row), and a segment is
-// a few tiles long, so what counts is that a block begins and ends one cheaply and that other blocks run meanwhile.  A
-// worker is a block of 4 warps with 16 rows each; it takes 64 keys at a time, of which each warp copies a quarter (32
-// keys' K or V) into the block's ring and all four read all.  Tiles of 128 rows on tcgen05 (paged_attn_tc.cu) have the
-// faster products, but their hand-overs from copies to widening to products to softmax and back cost a 50-row window more
-// than its work.
+// A segment is a few tiles long, so what counts is that a block begins and ends one cheaply and that other blocks run
+// meanwhile.  A worker is a block of 4 warps with 16 rows each; it takes 64 keys at a time, of which each warp copies a
+// quarter (32 keys' K or V) into the block's ring and all four read all.  Tiles of 128 rows on tcgen05 (paged_attn_tc.cu)
+// have the faster products, but half of their rows or more would be empty.
+//
+// What bounds it: instructions.  Every warp widens all the codes for its 16 rows, so 1 in 4 instructions is a product; an
+// SM's quarters issue one in 48% of the clocks with 4 warps each, whose tiles are chains from the copies through widening,
+// products and exponentials to products.  Measured: 128 windows of 50 tokens over 400 keys, 8 heads of 64: 65.7 MB and 5.2
+// GFLOP in 54 us, 1.2 TB/s.  Dropped: 32 rows a warp (half the widening, but the output's registers leave 2 blocks an SM):
+// 85 to 99 us.
 template <bool HALF, bool P16>
 __global__ void __launch_bounds__(32 * mid_warps, mid_blocks) k_paged_mid(const AttnDev p) {
   extern __shared__ __align__(16) uint8_t ring[];
@@ -595,7 +606,10 @@ __global__ void __launch_bounds__(32 * mid_warps, mid_blocks) k_paged_mid(const 
 // warp, a thread four columns of a row, more of them by the 8 warps of the block, a row at a time and every eighth part a
 // warp.  The order is fixed, so the bits are too.  What it costs is a chain of loads after the kernel in front of it has
 // ended: so all that the plan tells is read before that, the parts' rows are sent for together with their exponents, and
-// the blocks are resident at once.
+// the blocks are resident at once.  It ends 5 us after that kernel for single tokens (3 requests of 150k keys: 38 parts
+// each; row by row in one warp it was 11), 5 for windows, 11 for chunks (39 MB of parts, from L2).  A share of the rows for
+// each 8 of a part: with twice or half as many the windows take 56.5 or 55.4 us for 54.0, the chunks 160 at a quarter and
+// 142 at half for 132.
 struct Parts {
   const float* ws;
   int rows_ld, hd;
