@@ -57,7 +57,7 @@ struct Seg {
   int kt0, kt1, slot;      // key tiles; the part's slot, or -1 for a whole segment
 };
 struct Aux {
-  uint64_t q_full[2], q_free[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], o_free;
+  uint64_t q_full[2], q_free[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], o_free, idle;
   uint64_t meta_full[8], shift_full[4];  // by tile: ks, vs; by segment: shift
   uint64_t raw_full[4], raw_k_empty[4], raw_v_empty[5], seg_full[8];
   uint32_t tmem;
@@ -157,6 +157,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
       mbar_init(&x->seg_full[i], 1);
     }
     mbar_init(&x->o_free, 4);
+    mbar_init(&x->idle, 1);
     fence_mbar_init();
   }
   pdl_wait();
@@ -233,7 +234,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
           first_p = first_n;
           sp = s;
         }
+        umma_commit(&x->idle);
       }
+      __syncwarp();
+      bar_wait(&x->idle, 0, p.status);  // no product is under way when the block ends, not where a wait gave up either
     } else if (warp == 10) {
       // ---------------- segments, codes and scales: lane x * 4 + c has the c-th page of a tile's K (x 0) or V, and chunk
       // c's scale
@@ -305,6 +309,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
         more = at.next(p);
       }
       if (ok && t) publish(t - 1);
+      // nor is a copy
+      for (int n = max(0, t - R::RawK); n < t; ++n) bar_wait(&x->raw_full[n % R::RawK], (n / R::RawK) & 1, p.status);
     }
   } else if (warp >= 4) {
     // ---------------- widening: thread i has the 16-byte pieces i, i + 128, ... of a tile's K and of its V codes
@@ -401,6 +407,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
         if (g) kt = g->kt0;
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     // ---------------- softmax: thread r has the tile's row r
     asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
