@@ -33,7 +33,7 @@ PagedCut paged_cut(int max_fresh, int q_heads, int kv_heads, int head_dim) {
     // Where one 64-row tile has all of a request's rows and products are short.  Measured (bf16, either form for the same
     // call): 64 requests of 8 tokens, 4 heads to a key head, 40 to 4100 keys: 97 us against 112 to 122 in tiles of 128
     // rows; 128 of 50 tokens, 400 keys: 64 against 66.  With more rows the larger tiles win (32 of 24 tokens, 4 heads, 2000
-    // keys: 90 against 56), and with head_dim 128 always (the calls before: 178 against 130, 102 against 78).
+    // keys: 90 against 56), and with head_dim 128 always (the calls before: 178 against 126, 102 against 77).
     c.form = PagedForm::kMid;
     c.part_rows = 16 * mid_warps;
     c.tq = 16 * mid_warps / group;
