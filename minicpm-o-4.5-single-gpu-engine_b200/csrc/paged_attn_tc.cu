@@ -20,9 +20,10 @@
 //
 // What was in the way, in the order it was found (4 requests of 700 to 1024 tokens over histories to 4096, 16 query and 4
 // key heads, head_dim 128): queries brought by one warp of their own, 20,000 clocks a segment (185 us, of which it was
-// 30); code that does not fit the instruction caches, 62 KB at first, so that what few tiles need is kept in short loops;
-// descriptors made for each product by a lane that the compiler could not know to be alone (150 us before, 147 after);
-// spills of the products' warp (138 to 135).  Without the registers' split (96 for each of 10 warps) it is 158.
+// 30); code that does not fit the instruction caches, 62 KB at first, so that the roles are kept short (16-byte
+// pieces read ahead while widening: 138 to 150); descriptors made for each product by a lane that the compiler could not
+// know to be alone (152 us before, 148 after); spills of the products' warp (138 to 135).  Without the registers' split (96
+// for each of 10 warps) it was 158.
 //
 // Segments of at most 64 rows (windows) lie in the upper rows of every other block's tiles: a warp's exponentials run on
 // the SM quarter that its TMEM lanes belong to, and so the two blocks of an SM use all four.
@@ -30,7 +31,7 @@
 // What bounds it: a tile takes an SM 1950 clocks.  The exponentials (16 a clock and SM) need 512 of them, the tensor core
 // 256 (head_dim 64) or 512 (128), shared memory about 1100 (the products read queries, keys and values from it, and every
 // code passes through it twice); 900 instructions issue on each of the SM's quarters, from two softmax and two widening
-// warps, which is too few to hide what each waits for.  The chunks above: 135 us, 430 TFLOP/s, 25% of cuBLAS's bf16 rate.
+// warps, which is too few to hide what each waits for.  The chunks above: 132 us, 440 TFLOP/s, 26% of cuBLAS's bf16 rate.
 #include "paged_attn.cuh"
 
 namespace t2w {
@@ -57,7 +58,8 @@ struct Seg {
   int kt0, kt1, slot;      // key tiles; the part's slot, or -1 for a whole segment
 };
 struct Aux {
-  uint64_t q_full[2], q_free[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], o_free, idle;
+  uint64_t q_full[2], q_free[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2];
+  uint64_t o_free, idle;
   uint64_t meta_full[8], shift_full[4];  // by tile: ks, vs; by segment: shift
   uint64_t raw_full[4], raw_k_empty[4], raw_v_empty[5], seg_full[8];
   uint32_t tmem;
@@ -511,8 +513,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
             float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll
             for (int i = 16 * c; i < 16 * c + 16; i += 4) {
-              const float2 a = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), make_float2(ck[c], ck[c]), make_float2(d, d));
-              const float2 b = __ffma2_rn(make_float2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), make_float2(ck[c], ck[c]), make_float2(d, d));
+              const float2 a = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])),
+                                          make_float2(ck[c], ck[c]), make_float2(d, d));
+              const float2 b = __ffma2_rn(make_float2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])),
+                                          make_float2(ck[c], ck[c]), make_float2(d, d));
               const float2 ea = make_float2(exp2_approx(a.x), exp2_approx(a.y)), eb = make_float2(exp2_approx(b.x), exp2_approx(b.y));
               s0 = __fadd2_rn(s0, ea);
               s1 = __fadd2_rn(s1, eb);
