@@ -31,7 +31,7 @@
 // What bounds it: a tile takes an SM 1950 clocks.  The exponentials (16 a clock and SM) need 512 of them, the tensor core
 // 256 (head_dim 64) or 512 (128), shared memory about 1100 (the products read queries, keys and values from it, and every
 // code passes through it twice); 900 instructions issue on each of the SM's quarters, from two softmax and two widening
-// warps, which is too few to hide what each waits for.  The chunks above: 132 us, 440 TFLOP/s, 26% of cuBLAS's bf16 rate.
+// warps, which is too few to hide what each waits for.  The chunks above: 130 us, 447 TFLOP/s, 26% of cuBLAS's bf16 rate.
 #include "paged_attn.cuh"
 
 namespace t2w {

@@ -33,7 +33,7 @@ PagedCut paged_cut(int max_fresh, int q_heads, int kv_heads, int head_dim) {
     // Where one 64-row tile has all of a request's rows and products are short.  Measured (bf16, either form for the same
     // call): 64 requests of 8 tokens, 4 heads to a key head, 40 to 4100 keys: 97 us against 112 to 122 in tiles of 128
     // rows; 128 of 50 tokens, 400 keys: 64 against 66.  With more rows the larger tiles win (32 of 24 tokens, 4 heads, 2000
-    // keys: 90 against 56), and with head_dim 128 always (the calls before: 178 against 126, 102 against 77).
+    // keys: 90 against 56), and with head_dim 128 always (the calls before: 178 against 122, 102 against 77).
     c.form = PagedForm::kMid;
     c.part_rows = 16 * mid_warps;
     c.tq = 16 * mid_warps / group;
@@ -49,7 +49,7 @@ PagedCut paged_cut(int max_fresh, int q_heads, int kv_heads, int head_dim) {
     c.kt = 64;
     c.workers = 2 * num_sms();
     c.min_per = 4;
-    c.extra = 2;
+    c.extra = 4;  // (4 chunks of 700 to 1024 tokens over 4096 keys: 136 us with 1, 131 with 2, 130 with 4)
     c.whole = true;
   }
   return c;
