@@ -660,7 +660,8 @@ T2W_API int t2w_paged_release(const int32_t* done, int32_t* length, int32_t* tab
 /* The step's new keys and values [rows][kv_heads][head_dim] (dtype T2W_DT_*, head_dim contiguous, pitches in elements,
  * 16-byte aligned) into their pages.  A page and head's scale is the least power of two by which its largest magnitude
  * fits e4m3; it never falls, and codes written earlier are rounded again where it grows.  A page and head that is given
- * an infinity or a NaN reads as NaN from then on.  A page that is appended to belongs to one request. */
+ * an infinity or a NaN reads as NaN from then on.  A page that is appended to belongs to one request.  Rows whose page
+ * these codes do not have (`pages` less than the free list's) are not written, and the plan's status tells. */
 typedef struct t2w_paged_append_args {
   int32_t requests, rows, max_fresh, page, q_heads, kv_heads, head_dim, pages, dtype;
   const void* k;
@@ -671,7 +672,7 @@ typedef struct t2w_paged_append_args {
   float* k_scale;
   float* v_scale;
   int64_t k_page_ld, v_page_ld, k_scale_ld, v_scale_ld;
-  const int32_t* plan;
+  int32_t* plan;
 } t2w_paged_append_args;
 T2W_API int t2w_paged_append(const t2w_paged_append_args* a, void* stream);
 

@@ -81,7 +81,8 @@ def append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: tor
 
     The scale of a page and head is the least power of two with which the largest magnitude ever given to it fits e4m3
     (at most 448 * 2^64, at least 2^-64).  Where a step's rows raise it, the codes already there are rounded again.  A
-    page and head that is given an infinity or a NaN reads as NaN from then on."""
+    page and head that is given an infinity or a NaN reads as NaN from then on.  Rows whose page these codes do not have
+    (fewer pages than the free stack) are not written, and ``PagedPlan.check`` raises."""
     _fits(plan, k_codes, k, plan.kv_heads)
     O.call("paged_append", k, v, k_codes, v_codes, k_scale, v_scale, plan.buffer, plan.requests, plan.max_fresh, plan.q_heads)
 

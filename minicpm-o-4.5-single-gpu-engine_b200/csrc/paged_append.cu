@@ -24,9 +24,10 @@ struct AppendDev {
   uint8_t* codes[2];  // [pages][heads][page][hd]
   float* scales[2];   // [pages][heads]
   long long page_ld[2], scale_ld[2];
-  int page, heads;
+  int page, heads, pages;
   const PlanHead* head;
   const int4* runs;
+  int* status;
 };
 
 // The largest magnitude of packed 16-bit floats, by their bit patterns (sign off): a pattern from the exponent's all
@@ -59,7 +60,11 @@ __global__ void __launch_bounds__(kThreads) k_append(const AppendDev p) {
   pdl_launch();
   if ((int)blockIdx.x >= p.head->n_runs) return;
   const int4 run = p.runs[blockIdx.x];  // first row, rows, page, place of the first row in the page
-  if (run.z < 0) return;                // the plan has recorded why
+  // The plan's pages come off a free list that may be longer than this layer's codes: what lies past them is not written.
+  if ((unsigned)run.z >= (unsigned)p.pages) {
+    if (tid == 0) atomicExch(p.status, T2W_ERR_INVALID);
+    return;
+  }
   float* const sp = p.scales[w] + run.z * p.scale_ld[w] + h;
   uint8_t* const page = p.codes[w] + run.z * p.page_ld[w] + (size_t)h * p.page * HD;
   const float s_old = run.w > 0 ? *sp : exp2i(kScaleMin);
@@ -153,10 +158,12 @@ extern "C" int t2w_paged_append(const t2w_paged_append_args* a, void* stream) {
   }
   p.page = a->page;
   p.heads = a->kv_heads;
+  p.pages = a->pages;
   const PlanLayout l = paged_layout(a->requests, a->rows, a->page,
                                     paged_cut(a->max_fresh, a->q_heads, a->kv_heads, a->head_dim));
   p.head = reinterpret_cast<const PlanHead*>(a->plan);
   p.runs = reinterpret_cast<const int4*>(a->plan + l.runs);
+  p.status = &reinterpret_cast<PlanHead*>(a->plan)->status;
   if (l.max_runs == 0) return T2W_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool half = a->dtype == T2W_DT_FP16;

@@ -408,7 +408,7 @@ std::vector<at::Tensor> paged_plan(const at::Tensor& fresh, const at::Tensor& le
 }
 
 void paged_append(const at::Tensor& k, const at::Tensor& v, at::Tensor& k_codes, at::Tensor& v_codes, at::Tensor& k_scale,
-                  at::Tensor& v_scale, const at::Tensor& plan, int64_t requests, int64_t max_fresh, int64_t q_heads) {
+                  at::Tensor& v_scale, at::Tensor& plan, int64_t requests, int64_t max_fresh, int64_t q_heads) {
   const char* op = "paged_append";
   const Pages p = pages_of(op, k_codes, v_codes, k_scale, v_scale);
   const c10::DeviceGuard guard(k_codes.device());
@@ -555,7 +555,7 @@ TORCH_LIBRARY(b200t2w, m) {
         "Tensor? free_left) -> Tensor[]",
         &paged_plan);
   m.def("paged_append(Tensor k, Tensor v, Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) k_scale, "
-        "Tensor(d!) v_scale, Tensor plan, int requests, int max_fresh, int q_heads) -> ()",
+        "Tensor(d!) v_scale, Tensor(e!) plan, int requests, int max_fresh, int q_heads) -> ()",
         &paged_append);
   m.def("paged_attn(Tensor q, Tensor k_codes, Tensor v_codes, Tensor k_scale, Tensor v_scale, Tensor table, "
         "Tensor(a!) plan, int requests, int max_fresh, bool causal, float scale, bool lse) -> Tensor[]",
