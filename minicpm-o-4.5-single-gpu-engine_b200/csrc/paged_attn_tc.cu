@@ -57,18 +57,23 @@ struct Seg {
   int before, kv;          // keys ahead of the first token's own (causal), keys
   int kt0, kt1, slot;      // key tiles; the part's slot, or -1 for a whole segment
 };
+constexpr int kMetas = 8, kSegs = 16;  // tiles' scales and segments that the copies' warp may have told (see Aux)
 struct Aux {
   uint64_t q_full[2], q_free[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2];
   uint64_t o_free, idle;
-  uint64_t meta_full[8], shift_full[4];  // by tile: ks, vs; by segment: shift
-  uint64_t raw_full[4], raw_k_empty[4], raw_v_empty[5], seg_full[8];
+  uint64_t meta_full[kMetas], shift_full[4];  // by tile: ks, vs; by segment: shift
+  uint64_t raw_full[4], raw_k_empty[4], raw_v_empty[5], seg_full[kSegs];
   uint32_t tmem;
   int pad;
-  // By tile: the scales of its 16-key chunks.  The copies' warp is ahead of the softmax by six tiles at most: tile t is
-  // sent for once V of t - RawV (at most 5) has been widened, that is once the product of t - RawV - 2 is done.
-  float ks[8][4], lv[8][4], unit[8][4];  // K's; log2 of V's (0 where that is not finite) and 2^-lv
-  uint32_t odd[8];
-  Seg seg[8];                // by segment, as far ahead as the tiles
+  // By tile: the scales of its 16-key chunks.  Tile t is sent for once V of t - RawV has been widened, that is once the
+  // product of t - RawV - V is done and the softmax may read what belongs to the tile behind that.  Tile t - 1's scales are
+  // told then: RawV + V - 2 tiles (5 at most) ahead of it.
+  float ks[kMetas][4], lv[kMetas][4], unit[kMetas][4];  // K's; log2 of V's (0 where that is not finite) and 2^-lv
+  uint32_t odd[kMetas];
+  // By segment.  One that begins with tile t is told before that tile waits for anything, when the product of t - 1 - RawV -
+  // V is done.  The softmax may then still have to look up, for that tile's rows, the segment it ended: where segments are of
+  // one tile, RawV + V + 1 segments (8 where head_dim is 64) lie between the two.
+  Seg seg[kSegs];
   int16_t shift[4][kRows];   // by segment: the power of two that a row's queries were multiplied by
 };
 
@@ -136,6 +141,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
   Aux* const x = reinterpret_cast<Aux*>(smem + R::aux_at);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = blockIdx.x, group = p.group;
   constexpr int kPanels = HD / 64;
+  static_assert(R::RawV + R::V - 2 < kMetas && R::RawV + R::V + 1 < kSegs, "nothing is told over what may still be read");
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&x->q_full[i], 4);
@@ -154,10 +160,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
       mbar_init(&x->raw_k_empty[i], 4);
     }
     for (int i = 0; i < 5; ++i) mbar_init(&x->raw_v_empty[i], 4);
-    for (int i = 0; i < 8; ++i) {
-      mbar_init(&x->meta_full[i], 1);
-      mbar_init(&x->seg_full[i], 1);
-    }
+    for (int i = 0; i < kMetas; ++i) mbar_init(&x->meta_full[i], 1);
+    for (int i = 0; i < kSegs; ++i) mbar_init(&x->seg_full[i], 1);
     mbar_init(&x->o_free, 4);
     mbar_init(&x->idle, 1);
     fence_mbar_init();
@@ -174,11 +178,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
   const uint32_t tmem = x->tmem;
   bool ok = true;
   auto next_seg = [&](int s) -> const Seg* {  // nullptr: none, or the wait gave up
-    if (!bar_wait(&x->seg_full[s & 7], (s >> 3) & 1, p.status)) {
+    if (!bar_wait(&x->seg_full[s & (kSegs - 1)], (s & kSegs) != 0, p.status)) {
       ok = false;
       return nullptr;
     }
-    const Seg* const g = &x->seg[s & 7];
+    const Seg* const g = &x->seg[s & (kSegs - 1)];
     return g->rows ? g : nullptr;
   };
 
@@ -255,11 +259,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
         const bool odd = !(scale < INFINITY);
         const int e = odd ? 0 : (int)(__float_as_uint(scale) >> 23) - 127;
         const uint32_t of = __ballot_sync(~0u, lane < 8 && odd);
-        if (lane < 4) x->ks[n & 7][c] = scale;
-        else if (lane < 8) x->lv[n & 7][c] = (float)e, x->unit[n & 7][c] = exp2i(-e);
-        else if (lane == 8) x->odd[n & 7] = (of >> 4 & 15u) | (of & 15u ? 16u : 0u);
+        if (lane < 4) x->ks[n & (kMetas - 1)][c] = scale;
+        else if (lane < 8) x->lv[n & (kMetas - 1)][c] = (float)e, x->unit[n & (kMetas - 1)][c] = exp2i(-e);
+        else if (lane == 8) x->odd[n & (kMetas - 1)] = (of >> 4 & 15u) | (of & 15u ? 16u : 0u);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&x->meta_full[n & 7]);
+        if (lane == 0) mbar_arrive(&x->meta_full[n & (kMetas - 1)]);
       };
       const uint64_t policy = l2_policy_evict_first();
       Walk at;
@@ -267,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
 #pragma unroll 1
       for (int s = 0;; ++s) {
         if (lane == 0) {
-          Seg* const g = &x->seg[s & 7];
+          Seg* const g = &x->seg[s & (kSegs - 1)];
           g->rows = more ? at.rows(p, group) : 0;
           g->row0 = at.row0 + at.qt * p.tq;
           g->head0 = at.hk * group;
@@ -276,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
           g->kt0 = at.kt0;
           g->kt1 = at.kt1;
           g->slot = at.kt0 == 0 && at.kt1 == at.nt ? -1 : 2 * w + (at.first ? 0 : 1);
-          mbar_arrive(&x->seg_full[s & 7]);
+          mbar_arrive(&x->seg_full[s & (kSegs - 1)]);
         }
         if (!more) break;
 #pragma unroll 1
@@ -453,21 +457,21 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
         }
       }
       if (g) {
-        ok = bar_wait(&x->meta_full[t & 7], (t >> 3) & 1, p.status) && bar_wait(&x->s_full[t & 1], (t >> 1) & 1, p.status);
+        ok = bar_wait(&x->meta_full[t & (kMetas - 1)], (t & kMetas) != 0, p.status) && bar_wait(&x->s_full[t & 1], (t >> 1) & 1, p.status);
         if (!(ok = __all_sync(~0u, ok))) break;
         tc_fence_after();
       }
       if (g && !idle) {
         const uint32_t sbuf = tmem + lanes + 64 * (t & 1);
         const int kb = kt * kKeys;
-        const float* const ks = x->ks[t & 7];
-        const uint32_t odd = x->odd[t & 7];  // 1 << c: chunk c's value scale is not finite; 16: a key scale
+        const float* const ks = x->ks[t & (kMetas - 1)];
+        const uint32_t odd = x->odd[t & (kMetas - 1)];  // 1 << c: chunk c's value scale is not finite; 16: a key scale
         float ck[4], lv[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           ck[c] = c_row * ks[c];
           if (ck[c] == 0.f) ck[c] = 1.1754944e-38f;  // (-inf times 0)
-          lv[c] = x->lv[t & 7][c];
+          lv[c] = x->lv[t & (kMetas - 1)][c];
         }
         float w[2][32];
         tmem_ld32(sbuf, w[0]);
@@ -523,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_paged_many(const AttnDev p) {
               v[i / 2] = pack_f16x2(ea.x, ea.y);
               v[i / 2 + 1] = pack_f16x2(eb.x, eb.y);
             }
-            add = fmaf((s0.x + s1.x) + (s0.y + s1.y), x->unit[t & 7][c], add);
+            add = fmaf((s0.x + s1.x) + (s0.y + s1.y), x->unit[t & (kMetas - 1)][c], add);
           }
           if (odd) {  // values that are NaN, where the row sees them
 #pragma unroll

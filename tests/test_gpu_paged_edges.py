@@ -1,5 +1,13 @@
 """GPU: the paged 8-bit K/V cache where its tables, pools and sizes are at their limits (see ``test_gpu_paged``, whose
-64-bit statement and bounds these tests use)."""
+64-bit statement and bounds these tests use).
+
+Where values hold codes that are exactly 0, a row's bound needs the weights' smallest step too.  A weight is a half in units
+of 2^M, and M is at least 9 below the largest x_j + log2 s_j (s_j: the value scale of key j's page).  Half of a half's
+smallest step is 2^-25, so a weight may be off by 2^-34 max_j 2^(x_j + log2 s_j), and an output column d by
+
+    F = 2^-34 max_j (p_j s_j) sum_j |c_jd|      (p: softmax, c: codes)
+
+beside what ``test_gpu_paged`` allows, whose terms go by sum_j p_j |v_jd| alone."""
 
 import math
 
@@ -51,3 +59,100 @@ def test_append_to_fewer_pages_than_the_free_stack(dtype):
         for g in range(have):
             n = min(page, 40 - g * page)  # request 0's
             assert torch.equal(got[g, :, :n], m.codes[w][g, :, :n]) and torch.equal(scale[g], m.scale[w][g])
+
+
+# ---- many segments and long walks -----------------------------------------------------------------------------------
+
+
+def on_gpu(k, codes, scale_v, q, scale, causal):
+    """``test_gpu_paged.attention`` in 64 bits on the GPU, all rows at once: q [f, hd], k and V's codes [n, hd], V's scales
+    [n] -> out, lse, A, B, F."""
+    f, n = q.shape[0], k.shape[0]
+    s = (q @ k.T) * scale
+    b = (q.abs() @ k.abs().T) * scale
+    see = torch.ones(f, n, device="cuda", dtype=torch.bool)
+    if causal:
+        see = torch.arange(n, device="cuda")[None, :] <= torch.arange(n - f, n, device="cuda")[:, None]
+    s, b = s.masked_fill(~see, -math.inf), b.masked_fill(~see, 0.0)
+    p, v = torch.softmax(s, 1), codes * scale_v[:, None]
+    far = 2.0 ** -34 * (p * scale_v).amax(1, keepdim=True) * (see.double() @ codes.abs())
+    return p @ v, torch.logsumexp(s, 1), p @ v.abs(), b.amax(1), far
+
+
+def held(out, lse, ref):
+    """Whether out [f, hd] and lse [f], of rows that see a key each, are within the bounds of on_gpu()'s ref."""
+    o, l, A, B, far = ref
+    u = 2.0 ** -8 if out.dtype == torch.bfloat16 else 2.0 ** -10
+    d = (out.double() - o).abs() / (u * o.abs() + (2.0 ** -10 + 2.0 ** -15 * B[:, None]) * A + far + 1e-30)
+    assert float(d.max()) <= 1, float(d.max())
+    d = (lse.double() - l).abs() / (2.0 ** -16 * B + 2.0 ** -19 * l.abs().clamp(min=1))
+    assert float(d.max()) <= 1, float(d.max())
+
+
+class Filled:
+    """A layer's pages filled with codes and scales directly, a request's pages in any order, and attention calls that
+    look at them held against 64 bits."""
+
+    def __init__(self, lens, page, heads, hd, seed):
+        self.lens, self.page, self.heads, self.hd = lens, page, heads, hd
+        self.gen = torch.Generator(device="cuda").manual_seed(seed)
+        held = [-(-n // page) for n in lens]
+        pages = sum(held) + 2
+        order = torch.randperm(pages, device="cuda", generator=self.gen).to(torch.int32)
+        self.table = torch.full((len(lens), max(1, max(held))), -1, device="cuda", dtype=torch.int32)
+        self.at, i = [], 0
+        for r, n in enumerate(held):
+            self.table[r, :n] = order[i:i + n]
+            self.at.append(order[i:i + n].long())
+            i += n
+        self.codes, self.scales = [], []
+        for _ in range(2):
+            e = torch.randint(-2, 3, (pages, heads), device="cuda", generator=self.gen)
+            self.scales.append(torch.exp2(e.float()))
+            self.codes.append(torch.randn(pages, heads, page, hd, device="cuda", generator=self.gen).to(torch.float8_e4m3fn))
+        self.length = i32(lens)
+
+    def held_in(self, w, r, h):
+        """Codes [n, hd] and scales [n] of request r's keys."""
+        at, n = self.at[r], self.lens[r]
+        scale = self.scales[w][at, h].double().repeat_interleave(self.page)
+        return self.codes[w][at, h].double().reshape(-1, self.hd)[:n], scale[:n]
+
+    def plan(self, fresh, q_heads, causal):
+        return paged.plan(i32(fresh), self.length, self.table, self.page, rows=sum(fresh), max_fresh=max(fresh),
+                          q_heads=q_heads, kv_heads=self.heads, head_dim=self.hd, causal=causal)
+
+    def attend(self, q, p, **kw):
+        return paged.attend(q, self.codes[0], self.codes[1], self.scales[0], self.scales[1], p, **kw)
+
+    def check(self, fresh, group, causal, requests, dtype=torch.bfloat16):
+        """One call; the rows of ``requests`` are held against 64 bits, every row against a second call's."""
+        heads = self.heads * group
+        p = self.plan(fresh, heads, causal)
+        q = normal(self.gen, sum(fresh), heads, self.hd, dtype=dtype)
+        out, lse = self.attend(q, p, lse=True)
+        p.check()
+        again, lse2 = self.attend(q, p, lse=True)
+        assert torch.equal(out, again) and torch.equal(lse, lse2)
+        for r in requests:
+            a = sum(fresh[:r])
+            if not fresh[r]:
+                continue
+            for h in range(heads):
+                rows = slice(a, a + fresh[r])
+                kc, ks = self.held_in(0, r, h // group)
+                held(out[rows, h], lse[rows, h], on_gpu(kc * ks[:, None], *self.held_in(1, r, h // group),
+                                                        q[rows, h].double(), self.hd ** -0.5, causal))
+        return p
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("lens,group,heads", [((33, 64), 4, 8), ((17, 60), 5, 8), ((64, 64), 2, 16), ((1, 130), 8, 4)])
+def test_many_short_prompts(hd, lens, group, heads):
+    """Causal prompts of a tile of keys or two: a worker walks many segments of one tile each, one right after the other."""
+    n = 300
+    lens = [lens[0] + (7 * r) % (lens[1] - lens[0] + 1) for r in range(n)]
+    c = Filled(lens, 16, heads, hd, hd + group)
+    p = c.check(lens, group, True, range(0, n, 23))
+    workers, segments = int(p.buffer[3]), sum(-(-f // (128 // group)) for f in lens) * heads
+    assert segments >= 9 * workers, (segments, workers)
