@@ -542,12 +542,12 @@ __global__ void __launch_bounds__(32 * mid_warps, mid_blocks) k_paged_mid(const 
     if (!live) return;
     const int key = kt_a * 64 + 32 * half;
     const int* const table = p.table + (size_t)ahead.r * p.table_ld + (key >> p.shift);
-    pgA = key < ahead.kv ? __ldg(table) : -2;  // -2: no keys
+    pgA = key < ahead.kv ? __ldg(table) : 0;
     pgB = P16 && key + 16 < ahead.kv ? __ldg(table + 1) : pgA;
   };
   auto send = [&](int to_stage) {
     if (live) {
-      if (pgA != -2) {
+      if (kt_a * 64 + 32 * half < ahead.kv) {  // there are keys in this half
         if ((unsigned)pgA >= (unsigned)p.pages || (unsigned)pgB >= (unsigned)p.pages) {
           atomicExch(p.status, T2W_ERR_INVALID);
           pgA = pgB = 0;

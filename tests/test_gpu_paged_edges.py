@@ -61,6 +61,29 @@ def test_append_to_fewer_pages_than_the_free_stack(dtype):
             assert torch.equal(got[g, :, :n], m.codes[w][g, :, :n]) and torch.equal(scale[g], m.scale[w][g])
 
 
+@pytest.mark.parametrize("group,fresh,hd", [(1, 1, 64), (4, 4, 128), (1, 40, 64), (2, 30, 64), (1, 40, 128), (2, 70, 64)])
+@pytest.mark.parametrize("entry", [-1, -2, -3, 10, 2 ** 31 - 1, -2 ** 31])
+def test_no_entry_outside_the_pool_passes(group, fresh, hd, entry):
+    """Whatever an entry outside the pool's 10 pages is, and whichever form reads it, the status tells."""
+    c = paged.B200PagedCache(1, 10, 16, 1, hd, 1, 160, q_heads=group)
+    x = torch.ones(80, 1, hd, device="cuda", dtype=torch.bfloat16)
+    c.append(0, x, x, c.plan(i32([80]), 80, 80))
+    p = paged.plan(i32([fresh]), c.length, c.table, 16, rows=fresh, q_heads=group, kv_heads=1, head_dim=hd, max_fresh=fresh,
+                   causal=False)
+    q = torch.ones(fresh, group, hd, device="cuda", dtype=torch.bfloat16)
+    c.attend(0, q, p)
+    p.check()
+    for block in (0, 1, 4):
+        kept = c.table[0, block].clone()
+        c.table[0, block] = entry
+        c.attend(0, q, p)
+        with pytest.raises(L.T2WError) as e:
+            p.check()
+        assert e.value.status == -1
+        c.table[0, block] = kept
+        p.buffer[4] = 0
+
+
 # ---- many segments and long walks -----------------------------------------------------------------------------------
 
 
