@@ -617,7 +617,8 @@ T2W_API int t2w_test_attn_gathered(const void* qkv_bf16, int32_t rows, int32_t h
  * Device pointers are on the current device; every call is asynchronous on `stream` and reads no host memory later, so
  * all of them may be captured in a CUDA graph.  What goes wrong on the GPU (a pool that is used up, lengths that do not
  * fit) makes a plan void: it then has no rows, and the calls that take it write nothing but zeros for their rows;
- * t2w_paged_status tells. */
+ * t2w_paged_status tells.  A page that a call's codes do not have, met in the table or in the plan's new pages, is not
+ * followed and makes the plan void from that call on. */
 #define T2W_DT_BF16 0
 #define T2W_DT_FP16 1
 

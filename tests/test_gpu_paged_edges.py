@@ -84,6 +84,37 @@ def test_no_entry_outside_the_pool_passes(group, fresh, hd, entry):
         p.buffer[4] = 0
 
 
+@pytest.mark.parametrize("group,fresh,hd", [(1, 1, 64), (4, 3, 128), (2, 30, 64), (1, 40, 128), (4, 100, 64)])
+def test_an_entry_outside_the_pool_makes_the_plan_void(group, fresh, hd):
+    """Request 1's table names a page that there is not: no row, of no request, is answered from other pages than its own,
+    neither in that call nor in the plan's next ones."""
+    n, pad = 3, 5
+    c = paged.B200PagedCache(1, 60, 16, 2, hd, n, 320, q_heads=2 * group)
+    gen = torch.Generator(device="cuda").manual_seed(fresh)
+    k = normal(gen, 480, 2, hd)
+    c.append(0, k, k, c.plan(i32([200, 120, 160]), 480, 200))
+    rows = n * fresh + pad
+    p = paged.plan(i32([fresh] * n), c.length, c.table, 16, rows=rows, q_heads=2 * group, kv_heads=2, head_dim=hd,
+                   max_fresh=fresh)
+    q = normal(gen, rows, 2 * group, hd)
+    want = c.attend(0, q, p, lse=True)
+    p.check()
+    kept = c.table[1, 3].clone()
+    c.table[1, 3] = 60
+    for entry in (60, kept):  # once void, void for the next layers too
+        c.table[1, 3] = entry
+        out, lse = c.attend(0, q, p, lse=True)
+        with pytest.raises(L.T2WError) as e:
+            p.check()
+        assert e.value.status == -1
+        assert not out.any() and bool((lse == -math.inf).all())
+    again = paged.plan(i32([fresh] * n), c.length, c.table, 16, rows=rows, q_heads=2 * group, kv_heads=2, head_dim=hd,
+                       max_fresh=fresh)
+    got = c.attend(0, q, again, lse=True)
+    again.check()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ---- many segments and long walks -----------------------------------------------------------------------------------
 
 
