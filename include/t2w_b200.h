@@ -617,8 +617,8 @@ T2W_API int t2w_test_attn_gathered(const void* qkv_bf16, int32_t rows, int32_t h
  * Device pointers are on the current device; every call is asynchronous on `stream` and reads no host memory later, so
  * all of them may be captured in a CUDA graph.  What goes wrong on the GPU (a pool that is used up, lengths that do not
  * fit) makes a plan void: it then has no rows, and the calls that take it write nothing but zeros for their rows;
- * t2w_paged_status tells.  A page that a call's codes do not have, met in the table or in the plan's new pages, is not
- * followed and makes the plan void from that call on. */
+ * t2w_paged_status tells.  A page that a call's own codes do not have is not followed and makes the plan void from that call
+ * on. */
 #define T2W_DT_BF16 0
 #define T2W_DT_FP16 1
 
@@ -632,7 +632,9 @@ T2W_API int64_t t2w_paged_plan_ints(int32_t requests, int32_t rows, int32_t max_
  * = length + fresh, pages that this takes come off the end of the free list (request by request, block by block) into
  * `table`, and slot[i] = page * page_size + place of row i.  Without them the rows only look at what is cached: kv_len =
  * length, slot = -1.  kv_len and free_left (each may be NULL, or the very arrays that `length` and `free_count` are)
- * receive the new lengths and the pages left; with arrays of their own the call may be made again with the same result. */
+ * receive the new lengths and the pages left; with arrays of their own the call may be made again with the same result.
+ * A page number outside [0, pages) among those taken, or in the table where rows go into a page that is begun, makes the
+ * plan void: then table, kv_len (= length) and free_left stay as they were. */
 typedef struct t2w_paged_plan_args {
   int32_t requests, rows, max_fresh, page, q_heads, kv_heads, head_dim, causal;
   int32_t table_ld, max_blocks, pages;

@@ -7,9 +7,9 @@ blocks]``) names the page of each ``page`` tokens of a request and, like the pla
 
 Everything runs on the current stream of the tensors' GPU, reads lengths on the GPU only and never waits for it, so a
 step may be captured in a CUDA graph; tensors that were made on another stream are the caller's to order, as with any
-torch operator.  What only the GPU can find wrong (pages used up, lengths that do not fit) makes the plan void: its calls
-then write zeros for their rows and leave the cache as it was, and ``PagedPlan.check`` raises ``T2WError``.  A call that
-meets a page which its codes do not have, in the table or among the new pages, makes the plan void too, from itself on.
+torch operator.  What only the GPU can find wrong (pages used up, lengths that do not fit, a free stack that names no page)
+makes the plan void: its calls then write zeros for their rows and leave the cache as it was, and ``PagedPlan.check``
+raises ``T2WError``.  A call that meets a page which its own codes do not have makes the plan void from itself on.
 
 Arguments that cannot be right raise at the call: ``T2WError`` for sizes that the kernels do not have (page 16, 32, 64 or
 128; head_dim 64 or 128; at most 128 query heads to a key head), ``RuntimeError`` for tensors of the wrong type, shape,

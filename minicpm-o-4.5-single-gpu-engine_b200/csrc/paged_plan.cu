@@ -12,7 +12,7 @@
 //
 // Measured, on the GPU and as a call (which the host's side bounds below 15 us): 64 single tokens 8.5 and 14.8 us; 128
 // windows of 50 tokens 6.7 us, its rows 2 more behind it, and 17.2; 256 prompts of up to 4095 tokens (4.3 MB of rows) 12.7,
-// its rows 4 more, and 19.0.
+// its rows 4 more, and 19.8 (1.2 of it the look at the 16 thousand pages it takes; 2.7 an entry at a time).
 #include "paged.h"
 
 namespace t2w {
@@ -145,18 +145,15 @@ T2W_DEV void scatter(const PlanDev& p, const int* q_start, const int* new_base, 
                      int n_rows, int n_pages, int n_runs, int free_n, int i0, int step) {
   int* const slot = p.buf + p.lay.slot;
   int* const request = p.buf + p.lay.request;
-  PlanHead* const head = reinterpret_cast<PlanHead*>(p.buf);
-  // page of block b of request r: from the free list where it is new in this step (its table entry may not be written yet)
+  // page of block b of request r: from the free list where it is new in this step (its table entry may not be written yet);
+  // k_plan has looked at both
   auto page_of = [&](int r, int b, int len) {
     const int first = pages_of(len, p.shift);
-    const int g = b < first ? p.table[(size_t)r * p.table_ld + b] : p.free_pages[free_n - 1 - (new_base[r] + b - first)];
-    if ((unsigned)g < (unsigned)p.pages) return g;
-    atomicExch(&head->status, T2W_ERR_INVALID);  // a page that the cache does not have
-    return -1;
+    return b < first ? p.table[(size_t)r * p.table_ld + b] : p.free_pages[free_n - 1 - (new_base[r] + b - first)];
   };
   // four rows in a row at a time: they are mostly of one request and one page
   for (int i = 4 * i0; i < p.rows; i += 4 * step) {
-    int r = i < n_rows ? find(q_start, p.requests, i) : -1, page_at = -1, g = -1;
+    int r = i < n_rows ? find(q_start, p.requests, i) : -1, page_at = -1, g = 0;
     int s[4], o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -173,7 +170,7 @@ T2W_DEV void scatter(const PlanDev& p, const int* q_start, const int* new_base, 
         page_at = pos >> p.shift;
         g = page_of(r, page_at, len);
       }
-      if (g >= 0) s[j] = g * p.page + (pos & (p.page - 1));
+      s[j] = g * p.page + (pos & (p.page - 1));
     }
     // (each part of the plan begins on a 16-byte boundary and is as long as whole pieces)
     *reinterpret_cast<int4*>(slot + i) = make_int4(s[0], s[1], s[2], s[3]);
@@ -212,6 +209,9 @@ __global__ void __launch_bounds__(1024) k_plan(const PlanDev p) {
   int* const seg_base = n <= kHeld ? held[5] : p.buf + p.lay.seg_base;
   int* const kv_len = n <= kHeld ? held[3] : p.buf + p.lay.kv_len;
   const int free_n = p.free_pages ? *p.free_count : 0;
+  // the page that is taken as the tid-th, if as many are: it comes while the sums are made
+  const int nth = p.free_pages && free_n <= p.pages && tid < free_n ? p.free_pages[free_n - 1 - tid] : 0;
+  bool odd = false;  // a page that the cache does not have
   if (tid == 0) {
     bad_s = 0;
     carry_s = Sums{0, 0, 0, 0, 0};
@@ -222,10 +222,12 @@ __global__ void __launch_bounds__(1024) k_plan(const PlanDev p) {
   for (int r0 = 0; r0 < n; r0 += blockDim.x) {
     const int r = r0 + tid;
     Sums mine{0, 0, 0, 0};
-    int f = 0, len = 0;
+    int f = 0, len = 0, begun = 0;
     if (r < n) {
       f = p.fresh[r];
       len = p.length[r];
+      if (p.free_pages && f > 0 && len > 0 && (len & (p.page - 1)) && (len >> p.shift) < p.max_blocks)
+        begun = p.table[(size_t)r * p.table_ld + (len >> p.shift)];  // the page that its rows begin in
       if (!of_request(p, f, len, mine)) bad_s = 1;
     }
     Sums inc = mine;
@@ -256,6 +258,7 @@ __global__ void __launch_bounds__(1024) k_plan(const PlanDev p) {
       seg_base[r] = (int)min(base.segs + inc.segs - mine.segs, 0x7fffffffLL);
       kv_len[r] = p.free_pages ? len + f : len;
     }
+    odd |= (unsigned)begun >= (unsigned)p.pages;
     __syncthreads();
     if (tid == 0) carry_s = add(carry_s, warp_sum[warps - 1]);
     __syncthreads();
@@ -268,6 +271,23 @@ __global__ void __launch_bounds__(1024) k_plan(const PlanDev p) {
   if (bad_s || total.rows > p.rows || total.tiles > 0x7fffffffLL) status = T2W_ERR_INVALID;
   else if (p.free_pages && (free_n < 0 || free_n > p.pages)) status = T2W_ERR_INVALID;
   else if (p.free_pages && total.pages > free_n) status = T2W_ERR_EXHAUSTED;
+  if (status == T2W_OK) {  // (for all threads alike)
+    auto no_page = [&](int g) { return (unsigned)g >= (unsigned)p.pages; };
+    odd |= tid < total.pages && no_page(nth);
+    const int more = (int)total.pages - (int)blockDim.x;  // the first `more` entries from lo on: four at a time, but for the ends
+    if (more > 0) {
+      const int* const lo = p.free_pages + free_n - (int)total.pages;
+      const int head = min(more, (int)(-(reinterpret_cast<intptr_t>(lo) >> 2) & 3)), fours = (more - head) / 4;
+      if (tid < head) odd |= no_page(lo[tid]);
+      if (tid < more - head - 4 * fours) odd |= no_page(lo[head + 4 * fours + tid]);
+#pragma unroll 4
+      for (int i = tid; i < fours; i += blockDim.x) {
+        const int4 g = reinterpret_cast<const int4*>(lo + head)[i];
+        odd |= no_page(g.x) | no_page(g.y) | no_page(g.z) | no_page(g.w);
+      }
+    }
+    if (__syncthreads_or(odd)) status = T2W_ERR_INVALID;
+  }
   __syncthreads();
   if (status != T2W_OK) {  // void: no rows, no pages, the lengths as they were
     total = Sums{0, 0, 0, 0, 0};

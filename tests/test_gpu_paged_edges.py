@@ -115,6 +115,77 @@ def test_an_entry_outside_the_pool_makes_the_plan_void(group, fresh, hd):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("requests,most,page", [(2, 20, 16), (40, 200, 16), (1100, 5, 32), (1700, 9, 16)])
+@pytest.mark.parametrize("where", ["first taken", "last taken", "page begun", "not taken"])
+@pytest.mark.parametrize("entry", [-1, 1 << 20, -2 ** 31])
+def test_plans_of_lists_that_name_no_page(requests, most, page, where, entry):
+    """A free list, or a table's page that rows go into, with an entry that is no page: the plan is void and nothing has
+    changed.  An entry that the step does not take does not matter."""
+    gen = torch.Generator().manual_seed(requests)
+    length = torch.randint(0, 100, (requests,), generator=gen).tolist()
+    fresh = torch.randint(0, most + 1, (requests,), generator=gen).tolist()
+    length[-1], fresh[-1] = page + 1, most
+    blocks = max(-(-(a + b) // page) for a, b in zip(length, fresh))
+    pages = sum(-(-(a + b) // page) for a, b in zip(length, fresh)) + 4
+    m = Model(pages, 1, page, 1, requests, blocks)
+    m.plan(length)
+    count, taken = len(m.free), len(m.free) - 4
+    free, table = m.free + [0] * (pages - count), [list(t) for t in m.table]
+    if where == "first taken":
+        free[count - 1] = entry
+    elif where == "last taken":
+        free[count - taken] = entry
+    elif where == "page begun":
+        table[-1][1] = entry
+    else:
+        free[count - taken - 1] = entry
+        table[-1][0] = entry
+    dev = dict(free=i32(free), table=i32(table), count=i32([count]), length=i32(length), left=i32([count]))
+    before = {k: v.clone() for k, v in dev.items()}
+    rows = sum(fresh) + 3
+    p = paged.plan(i32(fresh), dev["length"], dev["table"], page, rows=rows, q_heads=1, kv_heads=1, head_dim=64, max_fresh=most,
+                   free=dev["free"], free_count=dev["count"], kv_len=dev["length"], free_left=dev["left"])
+    if where == "not taken":
+        p.check()
+        assert p.slot.tolist() == m.plan(fresh)[0] + [-1] * 3 and dev["left"].tolist() == [4]
+        assert dev["length"].tolist() == m.length
+        return
+    with pytest.raises(L.T2WError) as e:
+        p.check()
+    assert e.value.status == -1
+    for k, v in dev.items():
+        assert torch.equal(v, before[k]), k
+    assert p.slot.tolist() == [-1] * rows and p.request.tolist() == [-1] * rows
+    assert p.q_start.tolist() == [0] * (requests + 1) and p.kv_len.tolist() == length and p.free_left.tolist() == [count]
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2, 3])
+@pytest.mark.parametrize("pages", [1023, 1025, 1030, 5000])
+def test_every_page_taken_is_looked_at(offset, pages):
+    """One request takes `pages` pages of a list that lies `offset` entries past a 16-byte boundary: an entry that is no
+    page is found wherever it is, and those beside the taken ones are not looked at."""
+    held = i32([7] * offset + [-1] + list(range(pages)) + [-1] * 3)
+    free, count, one = held[offset:], i32([pages + 1]), i32([pages * 16])
+    table = torch.full((1, pages), -1, device="cuda", dtype=torch.int32)
+
+    def plan():
+        return paged.plan(one, i32([0]), table, 16, rows=pages * 16, q_heads=1, kv_heads=1, head_dim=64, free=free,
+                          free_count=count)
+
+    p = plan()
+    p.check()
+    assert p.free_left.tolist() == [1] and table[0].tolist() == list(range(pages - 1, -1, -1))
+    table.fill_(-1)
+    for at in [1, 2, 3, 4, 5, 6, 7, 8, pages // 2, *range(pages - 1030, pages - 1018), pages - 1, pages]:
+        if at < 1:
+            continue
+        free[at] = pages + 4
+        with pytest.raises(L.T2WError):
+            plan().check()
+        assert bool((table == -1).all())
+        free[at] = at - 1
+
+
 # ---- many segments and long walks -----------------------------------------------------------------------------------
 
 
