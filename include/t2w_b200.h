@@ -654,8 +654,8 @@ T2W_API int t2w_paged_plan(const t2w_paged_plan_args* a, void* stream);
 T2W_API int t2w_paged_status(const int32_t* plan, void* stream);
 
 /* Pages of the requests with done[r] != 0 back onto the end of the free list (request by request, block by block); their
- * table entries become -1 and their lengths 0.  *status (device) becomes T2W_ERR_INVALID, and nothing is given back,
- * where that would make more free pages than there are. */
+ * table entries become -1 and their lengths 0.  *status (device) becomes T2W_ERR_INVALID, and nothing is given back, where
+ * that would make more free pages than there are, or where a length or a table entry of one of them cannot be. */
 T2W_API int t2w_paged_release(const int32_t* done, int32_t* length, int32_t* table, int32_t requests, int32_t page,
                               int32_t table_ld, int32_t max_blocks, int32_t pages, int32_t* free_pages,
                               int32_t* free_count, int32_t* status, void* stream);

@@ -102,7 +102,8 @@ def attend(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scal
 def release(done: torch.Tensor, length: torch.Tensor, table: torch.Tensor, page: int, free: torch.Tensor,
             free_count: torch.Tensor, status: torch.Tensor) -> None:
     """Give the pages of the requests with ``done[r] != 0`` back to the free stack; their lengths become 0.  ``status``
-    (int32 [1]) becomes T2W_ERR_INVALID, and nothing is given back, where more pages would come back than there are."""
+    (int32 [1]) becomes T2W_ERR_INVALID, and nothing is given back, where more pages would come back than there are or a
+    request's length or table names none."""
     O.call("paged_release", done, length, table, page, free, free_count, status)
 
 

@@ -186,6 +186,55 @@ def test_every_page_taken_is_looked_at(offset, pages):
         free[at] = at - 1
 
 
+def table_of(lens, page, blocks, spare=0):
+    """A table that gives each request its pages in order, the free list of the `spare` pages left, and the entries."""
+    table, i = [], 0
+    for n in lens:
+        held = -(-n // page)
+        table.append(list(range(i, i + held)) + [-1] * (blocks - held))
+        i += held
+    return table, list(range(i, i + spare)) + [0] * i, i + spare
+
+
+@pytest.mark.parametrize("lens", [[150001], [0], [17] * 5 + [0, 3000, 1], [1] * 1024, [33] * 1025, [r % 70 for r in range(4097)], [r % 70 for r in range(9000)]])
+def test_release_of_many_pages(lens):
+    """Some requests end, then all of them, some of those without a page; the pages come back in request and block order."""
+    page, n = 16, len(lens)
+    table, free, pages = table_of(lens, page, -(-max(max(lens), 1) // page) + 1, spare=3)
+    dev = dict(length=i32(lens), table=i32(table), free=i32(free), count=i32([3]), status=i32([0]))
+    want, free, left = list(lens), free[:3], [list(t) for t in table]
+    for done in ([int(r % 3 == n % 3) for r in range(n)], [1] * n):
+        paged.release(i32(done), dev["length"], dev["table"], page, dev["free"], dev["count"], dev["status"])
+        for r in range(n):
+            if done[r]:
+                free += [g for g in left[r] if g >= 0]
+                want[r], left[r] = 0, [-1] * len(left[r])
+        assert dev["status"].tolist() == [0] and dev["count"].tolist() == [len(free)]
+        assert dev["free"].tolist()[:len(free)] == free and dev["length"].tolist() == want and dev["table"].tolist() == left
+    assert len(free) == pages
+
+
+@pytest.mark.parametrize("requests", [1, 3, 1024, 1025, 4096, 4097, 9000])
+@pytest.mark.parametrize("what", ["length", "negative", "entry", "count", "twice"])
+def test_release_that_cannot_be_gives_nothing_back(requests, what):
+    """The last request's length or table is wrong, or it alone makes more free pages than there are."""
+    page, lens = 16, [20 + r % 60 for r in range(requests)]
+    table, free, pages = table_of(lens, page, 6, spare=2)
+    if what == "length":
+        lens[-1] = 6 * page + 1
+    elif what == "negative":
+        lens[-1] = -1
+    elif what == "entry":
+        table[-1][1] = pages
+    count = {"count": -1, "twice": 3}.get(what, 2)
+    dev = dict(length=i32(lens), table=i32(table), free=i32(free), count=i32([count]), status=i32([0]))
+    before = {k: v.clone() for k, v in dev.items()}
+    paged.release(i32([1] * requests), dev["length"], dev["table"], page, dev["free"], dev["count"], dev["status"])
+    assert dev["status"].tolist() == [-1]
+    for k in ("length", "table", "free", "count"):
+        assert torch.equal(dev[k], before[k]), k
+
+
 # ---- many segments and long walks -----------------------------------------------------------------------------------
 
 
