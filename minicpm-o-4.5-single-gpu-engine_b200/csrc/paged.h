@@ -71,28 +71,18 @@ PagedCut paged_cut(int max_fresh, int q_heads, int kv_heads, int head_dim);
 PlanLayout paged_layout(int64_t requests, int64_t rows, int page, const PagedCut& cut);
 
 // ---------------------------------------------------------------- tiles of a request (device)
-// sum over i < n of floor((a i + b) / m), a, b >= 0 (the lattice points under a line, by Euclid's algorithm on a and m);
-// a n + b < 2^32, the arguments being numbers of keys: division by 32 bits is several times faster.
-T2W_DEV long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
-  long long s = 0;
-  while (n > 0) {
-    if (a >= m) {
-      s += (long long)n * (n - 1) / 2 * (a / m);
-      a %= m;
-    }
-    if (b >= m) {
-      s += (long long)n * (b / m);
-      b %= m;
-    }
-    const unsigned top = a * n + b;
-    if (top < m) break;
-    n = top / m;
-    b = top % m;
-    const unsigned t = m;
-    m = a;
-    a = t;
-  }
-  return s;
+// sum over i < n of floor((a i + b) / m), m a power of two (a key tile), a >= 1, b >= 0, a n + b < 2^32: the sum of the
+// a i + b less that of their remainders, over m.  With g the largest power of two that divides a and m, the remainders come
+// again after m / g terms, and until then each of b mod g, b mod g + g, .. below m comes once; only what is left of n after
+// whole periods is gone through.  (a is the tokens of a query tile: where the heads to a key head are a power of two a period
+// is 4 terms at most, else 64.)
+T2W_DEV long long sum_of_quotients(unsigned n, unsigned m, unsigned a, unsigned b) {
+  const int lm = __ffs(m) - 1, lg = min(__ffs(a) - 1, lm), lp = lm - lg;  // m = 2^lm, g = 2^lg, m / g = 2^lp
+  const unsigned g = 1u << lg, period = 1u << lp, left = n & (period - 1);
+  const unsigned one = (b & (g - 1)) * period + g * (period * (period - 1) / 2);  // the remainders of a period
+  long long sum = (long long)a * ((unsigned long long)n * (n - 1) / 2) + (long long)b * n - (long long)(n >> lp) * one;
+  for (unsigned i = n - left; i < n; ++i) sum -= (a * i + b) & (m - 1);
+  return sum >> lm;
 }
 // Keys that the last query of query tile qt sees.
 T2W_DEV int tile_keys(int f, int kv, int causal, int tq, int qt) {
@@ -111,7 +101,7 @@ T2W_DEV long long tiles_before(int f, int kv, int causal, int tq, int kt, int x)
   if (none > x) none = x;
   long long s = none;
   if (none < x) {
-    s += floor_sum(x - none, kt, tq, c + none * tq + kt - 1);
+    s += sum_of_quotients(x - none, kt, tq, c + none * tq + kt - 1);
     const long long last = (long long)c + (long long)(x - 1) * tq;
     if (last > kv) s += seg_tiles(kv, kt) - (int)((last + kt - 1) / kt);
   }

@@ -11,8 +11,9 @@
 // the sums from the plan.
 //
 // Measured, on the GPU and as a call (which the host's side bounds below 15 us): 64 single tokens 8.5 and 14.8 us; 128
-// windows of 50 tokens 6.7 us, its rows 2 more behind it, and 17.2; 256 prompts of up to 4095 tokens (4.3 MB of rows) 12.7,
-// its rows 4 more, and 19.8 (1.2 of it the look at the 16 thousand pages it takes; 2.7 an entry at a time).
+// windows of 50 tokens 6.7 us, its rows 2 more behind it, and 17.2; 256 prompts of up to 4095 tokens (4.3 MB of rows) 17.7
+// as a call, 1.2 of it the look at the 16 thousand pages it takes (2.7 an entry at a time).  The tile sums of such prompts
+// count too: with 1, 4, 5 and 25 query heads to a key head the plan takes 17, 17, 24 and 26 us on the GPU.
 #include "paged.h"
 
 namespace t2w {

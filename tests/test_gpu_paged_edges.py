@@ -320,6 +320,44 @@ class Filled:
         return p
 
 
+def form_of(most, group, hd):
+    """Query tokens and keys of a tile, workers of an SM and the tiles that a segment's start counts, by the rows that a
+    request has for a key head at most."""
+    if most * group <= 16:
+        return most, 32, 8 * (1 if hd == 128 or most * group > 8 else 2), 4
+    if hd == 64 and most * group <= 64:
+        return 64 // group, 64, 4, 2
+    return 128 // group, 64, 2, 4
+
+
+def segments(fresh, lens, heads, causal, tq, kt):
+    """(request, key head, query tile, key tiles) of every segment in order."""
+    for r, (f, n) in enumerate(zip(fresh, lens)):
+        for h in range(heads):
+            for q in range(-(-f // tq)):
+                sees = max(0, n - max(0, f - (q + 1) * tq)) if causal else n
+                yield r, h, q, max(1, -(-sees // kt))
+
+
+@pytest.mark.parametrize("hd,group,most", [(64, 1, 4000), (64, 2, 900), (128, 3, 2000), (128, 5, 700), (128, 7, 900), (64, 8, 300),
+                                           (128, 16, 700), (64, 100, 50), (128, 128, 40), (64, 3, 21), (64, 1, 40), (128, 2, 8)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_tiles_of_a_plan(hd, group, most, causal):
+    """The plan's number of key tiles, for requests that are longer than their rows, shorter, and empty."""
+    gen = torch.Generator().manual_seed(group)
+    n, heads = 60, 3
+    fresh = torch.randint(0, most + 1, (n,), generator=gen).tolist()
+    lens = [torch.randint(0, top, (1,), generator=gen).item() for top in (1, 70, most + 1, 3 * most, 20000) for _ in range(12)]
+    fresh[5] = most
+    table = torch.full((n, -(-max(lens) // 16)), -1, device="cuda", dtype=torch.int32)
+    p = paged.plan(i32(fresh), i32(lens), table, 16, rows=sum(fresh), max_fresh=most, q_heads=heads * group, kv_heads=heads,
+                   head_dim=hd, causal=causal)
+    p.check()
+    tq, kt = form_of(most, group, hd)[:2]
+    all_of = list(segments(fresh, lens, heads, causal, tq, kt))
+    assert int(p.buffer[1]) == sum(s[3] for s in all_of) + int(p.buffer[7]) * len(all_of)
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("lens,group,heads", [((33, 64), 4, 8), ((17, 60), 5, 8), ((64, 64), 2, 16), ((1, 130), 8, 4)])
 def test_many_short_prompts(hd, lens, group, heads):
