@@ -9,6 +9,7 @@ smallest step is 2^-25, so a weight may be off by 2^-34 max_j 2^(x_j + log2 s_j)
 
 beside what ``test_gpu_paged`` allows, whose terms go by sum_j p_j |v_jd| alone."""
 
+import ctypes
 import math
 
 import pytest
@@ -312,6 +313,9 @@ class Filled:
             a = sum(fresh[:r])
             if not fresh[r]:
                 continue
+            if not self.lens[r]:
+                assert not out[a:a + fresh[r]].any() and bool((lse[a:a + fresh[r]] == -math.inf).all())
+                continue
             for h in range(heads):
                 rows = slice(a, a + fresh[r])
                 kc, ks = self.held_in(0, r, h // group)
@@ -368,3 +372,132 @@ def test_many_short_prompts(hd, lens, group, heads):
     p = c.check(lens, group, True, range(0, n, 23))
     workers, segments = int(p.buffer[3]), sum(-(-f // (128 // group)) for f in lens) * heads
     assert segments >= 9 * workers, (segments, workers)
+
+
+def starts_of(p):
+    """A plan's workers' starts: [[request, head, query tile, key tile, first row, rows, keys, place], ..] and the last place."""
+    at = (ctypes.c_int64 * 4)()
+    assert L.load().t2w_paged_plan_ints(p.requests, p.rows, p.max_fresh, p.page, p.q_heads, p.kv_heads, p.head_dim, at) > 0
+    up = lambda n: -(-n // 4) * 4  # noqa: E731
+    begin = at[3] + up(p.rows) + 4 * up(p.requests + 1)
+    workers = int(p.buffer[3])
+    return p.buffer[begin:begin + 8 * (workers + 1)].view(-1, 8).tolist()
+
+
+def walk(p, fresh, lens, sms):
+    """Goes through a plan's split as the workers and the joining do, and checks that every key tile has one worker and that
+    of each cut segment the parts are read that were written, once.  Returns how many segments were cut."""
+    group = p.q_heads // p.kv_heads
+    tq, kt, per_sm, extra_at_most = form_of(p.max_fresh, group, p.head_dim)
+    few = p.max_fresh * group <= 16
+    tiles, per, workers, extra = int(p.buffer[1]), int(p.buffer[2]), int(p.buffer[3]), int(p.buffer[7])
+    assert extra in (0, extra_at_most) and workers <= per_sm * sms
+    row0 = [0]
+    for n in fresh:
+        row0.append(row0[-1] + n)
+    segs, place = [], 0
+    for r, h, q, nt in segments(fresh, lens, p.kv_heads, p.causal, tq, kt):
+        segs.append((r, h, q, nt, place + extra))
+        place += nt + extra
+    assert place == tiles
+    at = {s[:3]: i for i, s in enumerate(segs)}
+    starts = starts_of(p)
+    places = [s[7] for s in starts]
+    assert places[0] == 0 and places[-1] == tiles and all(a <= b for a, b in zip(places, places[1:]))
+    if few:
+        assert places[:-1] == [w * per for w in range(workers)]
+    bw = 8 if few else 1
+    written = {}  # by segment: the parts' slots in the order of their keys
+    for w in range(workers):
+        r, h, q, k, first, rows, keys, begin = starts[w]
+        if begin == tiles:  # (moved to the end: nothing is left)
+            continue
+        i = at[r, h, q]
+        assert (first, rows, keys) == (row0[r], fresh[r], lens[r]) and segs[i][4] + k == begin and -extra <= k < segs[i][3]
+        j, stop = i, places[w + 1]
+        while j < len(segs) and segs[j][4] < stop:
+            nt, zero = segs[j][3:]
+            lo, hi = max(0, begin - zero), min(nt, stop - zero)
+            assert lo < hi
+            if hi - lo < nt:
+                b = w // bw
+                full = bw > 1 and (b + 1) * bw <= workers and zero <= b * bw * per and zero + nt >= (b + 1) * bw * per
+                if not full:
+                    written.setdefault(j, []).append(2 * w + (j != i))
+                elif w % bw == 0:
+                    written.setdefault(j, []).append(2 * w)
+            j += 1
+    joined = {}
+    for w in range(1, workers):
+        r, h, q, k, first, rows, keys, begin = starts[w]
+        zero, before = begin - k, places[w - 1]
+        if not (k > 0 and zero >= before):
+            continue
+        i = at[r, h, q]
+        end = zero + segs[i][3]
+        w0, last = w - 1, (end - 1) // per
+        b0, b1 = -(-zero // (bw * per)), end // (bw * per)
+        mid = b1 - b0 if bw > 1 and b1 > b0 else 0
+        lead = b0 * bw - w0 if mid else last - w0 + 1
+        slots = [2 * (w0 + x) + (x == 0 and zero - extra > before) for x in range(lead)]
+        slots += [2 * bw * (b0 + x) for x in range(mid)]
+        if mid:
+            slots += [2 * x for x in range(b1 * bw, last + 1)]
+        assert i not in joined
+        joined[i] = slots
+    assert joined == written
+    return len(joined)
+
+
+LONG = [
+    # head_dim, key heads, query heads to each, most rows, causal, page, requests' keys, dtype
+    (64, 8, 1, 1, True, 16, (64, 40, 4000), torch.bfloat16),
+    (64, 8, 1, 1, True, 32, (64, 40, 1500, 40000), torch.float16),
+    (64, 8, 2, 5, True, 64, (64, 40, 3000), torch.bfloat16),
+    (128, 8, 4, 1, True, 32, (64, 40, 3000), torch.float16),
+    (128, 4, 8, 2, False, 16, (96, 2, 3000), torch.bfloat16),
+    (128, 4, 3, 4, True, 128, (128, 4, 900, 30000), torch.bfloat16),
+    (64, 8, 1, 50, False, 64, (128, 50, 700), torch.bfloat16),
+    (64, 8, 1, 60, True, 16, (100, 60, 900), torch.float16),
+    (64, 5, 3, 20, True, 32, (128, 20, 900, 9000), torch.bfloat16),
+    (64, 4, 2, 100, True, 16, (64, 100, 1200), torch.bfloat16),
+    (64, 8, 4, 33, False, 128, (100, 33, 300, 9000), torch.float16),
+    (128, 4, 4, 60, True, 64, (64, 60, 1200), torch.bfloat16),
+    (128, 1, 128, 2, True, 32, (300, 2, 900, 9000), torch.float16),
+    (128, 3, 5, 90, False, 16, (64, 90, 500), torch.bfloat16),
+]
+
+
+@pytest.mark.parametrize("hd,heads,group,most,causal,page,keys,dtype", LONG)
+def test_calls_with_many_tiles_for_a_worker(hd, heads, group, most, causal, page, keys, dtype):
+    """Every form where a worker walks several segments and each segment's start counts places: ragged lengths, requests
+    without rows and without keys, here and there one that is far longer than the others."""
+    n, lo, hi = keys[:3]
+    gen = torch.Generator().manual_seed(hd + group + most)
+    lens = [max(most, x) for x in torch.randint(lo, hi + 1, (n,), generator=gen).tolist()]
+    fresh = torch.randint(max(1, most // 2), most + 1, (n,), generator=gen).tolist()
+    for r in (0, 7, n // 2, n - 1):
+        fresh[r] = 0
+    for r in (3, 11, n - 2):
+        lens[r] = 0
+    fresh[5] = most
+    lens[9:10] = keys[3:] or lens[9:10]
+    c = Filled(lens, page, heads, hd, most)
+    p = c.check(fresh, group, causal, [1, 2, 3, 5, 9, n // 2 + 1, n - 2], dtype=dtype)
+    assert int(p.buffer[7]) > 0
+    assert walk(p, fresh, lens, torch.cuda.get_device_properties(0).multi_processor_count) > 0
+
+
+@pytest.mark.parametrize("hd,heads,group,most,lens", [
+    (64, 2, 1, 1, [5000, 1, 64, 900]), (64, 1, 4, 4, [9000]), (128, 1, 1, 1, [30, 33, 31]), (128, 2, 2, 8, [700, 6011]),
+    (64, 2, 2, 30, [900, 64, 65, 3000]), (64, 1, 1, 40, [40]), (64, 2, 2, 70, [900, 4000, 70]), (128, 1, 4, 200, [200, 1000]),
+    (128, 2, 3, 300, [300, 5000])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_calls_with_few_tiles_for_a_worker(hd, heads, group, most, lens, causal):
+    """The same walk where starts count nothing."""
+    fresh = [max(1, most - r) for r in range(len(lens))]
+    lens = [max(a, b) for a, b in zip(lens, fresh)]
+    c = Filled(lens, 16, heads, hd, most)
+    p = c.check(fresh, group, causal, range(len(lens)))
+    assert int(p.buffer[7]) == 0
+    walk(p, fresh, lens, torch.cuda.get_device_properties(0).multi_processor_count)
