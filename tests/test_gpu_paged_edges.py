@@ -197,7 +197,8 @@ def table_of(lens, page, blocks, spare=0):
     return table, list(range(i, i + spare)) + [0] * i, i + spare
 
 
-@pytest.mark.parametrize("lens", [[150001], [0], [17] * 5 + [0, 3000, 1], [1] * 1024, [33] * 1025, [r % 70 for r in range(4097)], [r % 70 for r in range(9000)]])
+@pytest.mark.parametrize("lens", [[150001], [0], [17] * 5 + [0, 3000, 1], [1] * 1024, [33] * 1025,
+                                  [r % 70 for r in range(4097)], [r % 70 for r in range(9000)]])
 def test_release_of_many_pages(lens):
     """Some requests end, then all of them, some of those without a page; the pages come back in request and block order."""
     page, n = 16, len(lens)
@@ -343,8 +344,9 @@ def segments(fresh, lens, heads, causal, tq, kt):
                 yield r, h, q, max(1, -(-sees // kt))
 
 
-@pytest.mark.parametrize("hd,group,most", [(64, 1, 4000), (64, 2, 900), (128, 3, 2000), (128, 5, 700), (128, 7, 900), (64, 8, 300),
-                                           (128, 16, 700), (64, 100, 50), (128, 128, 40), (64, 3, 21), (64, 1, 40), (128, 2, 8)])
+@pytest.mark.parametrize("hd,group,most", [
+    (64, 1, 4000), (64, 2, 900), (128, 3, 2000), (128, 5, 700), (128, 7, 900), (64, 8, 300), (128, 16, 700), (64, 100, 50),
+    (128, 128, 40), (64, 3, 21), (64, 1, 40), (128, 2, 8)])
 @pytest.mark.parametrize("causal", [True, False])
 def test_tiles_of_a_plan(hd, group, most, causal):
     """The plan's number of key tiles, for requests that are longer than their rows, shorter, and empty."""
@@ -447,6 +449,20 @@ def walk(p, fresh, lens, sms):
         joined[i] = slots
     assert joined == written
     return len(joined)
+
+
+@pytest.mark.parametrize("hd,group,fresh", [(64, 1, 1), (128, 4, 3), (64, 1, 40), (64, 2, 70), (128, 2, 100)])
+@pytest.mark.parametrize("zeros", ["first", "last", "every other"])
+def test_pages_of_zeros_beside_large_values(hd, group, fresh, zeros):
+    """Pages whose values are all 0 have the least scale, 2^-64: beside values of a scale up to 2^26, the other end of what the
+    sums of weights hold in full, they still count in the sums."""
+    c = Filled([600], 16, 1, hd, fresh)
+    for i, g in enumerate(c.at[0].tolist()):
+        none = {"first": i < 19, "last": i >= 19, "every other": i % 2 == 0}[zeros]
+        c.scales[1][g] = 2.0 ** -64 if none else 2.0 ** 26
+        if none:
+            c.codes[1].view(torch.uint8)[g] = 0
+    c.check([fresh], group, True, [0])
 
 
 LONG = [
