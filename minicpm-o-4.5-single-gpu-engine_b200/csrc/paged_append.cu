@@ -9,8 +9,8 @@
 //
 // Bound: HBM for prompts (two bytes read for each element and one written; one read of the rows, which stay in
 // registers between the search for the largest magnitude and the rounding), latency for single tokens.  Measured: 16 prompts
-// of 1900 to 6300 rows, 8 heads of 128: 404 MB in 63.4 us, 6.4 TB/s, what a plain copy reaches; 128 windows of 50 rows, 8
-// heads of 64: 23.9 MB in 7.7 us; 4 single rows 7.5 us, which is what the call costs on the host.
+// of 1900 to 6300 rows, 8 heads of 128: 404 MB in 63.3 us, 6.4 TB/s, what a plain copy reaches; 128 windows of 50 rows, 8
+// heads of 64: 23.9 MB in 7.3 us; 4 single rows 7.3 us, which is what the call costs on the host.
 #include "paged.h"
 
 namespace t2w {

@@ -34,10 +34,10 @@ T2W_DEV void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint3
 // below the running maximum of x_j + log2 s_v (kBelow): the weights of the largest contributions have all the bits that a
 // half has whatever the scales.  The sum of exponentials is kept in units of 2^M too.
 //
-// Measured: 64 requests of 40 to 4100 keys, 32 query and 8 key heads of 128: 272.6 MB in 58 us, 4.7 TB/s (73% of a copy);
-// 3 requests of 90k to 150k keys, 16 and 2 heads: 184.5 MB in 44 us, 4.2 TB/s.  In the second the stream itself, between a
+// Measured: 64 requests of 40 to 4100 keys, 32 query and 8 key heads of 128: 272.6 MB in 59 us, 4.6 TB/s (72% of a copy);
+// 3 requests of 90k to 150k keys, 16 and 2 heads: 184.5 MB in 45 us, 4.1 TB/s.  In the second the stream itself, between a
 // worker's first tile and its last, runs at 7.5 TB/s; the rest is the launch, the plan's and the table's loads ahead of the
-// first tile (5 us), the last workers' ends (3) and the joining (5).  Of the other splits, a block of 8 warps on one
+// first tile (5 us), the last workers' ends (3) and the joining (6).  Of the other splits, a block of 8 warps on one
 // segment at a time took 167 and 68 us in its best form (short segments leave most of it idle), fragments loaded straight
 // from global memory 75 and 54, rings of 2 or 6 tiles 66 and 49 or 76 and 52 (this one then 61 and 42 to 46).
 template <int HD>
@@ -606,8 +606,8 @@ __global__ void __launch_bounds__(32 * mid_warps, mid_blocks) k_paged_mid(const 
 // warp, a thread four columns of a row, more of them by the 8 warps of the block, a row at a time and every eighth part a
 // warp.  The order is fixed, so the bits are too.  What it costs is a chain of loads after the kernel in front of it has
 // ended: so all that the plan tells is read before that, the parts' rows are sent for together with their exponents, and
-// the blocks are resident at once.  It ends 5 us after that kernel for single tokens (3 requests of 150k keys: 38 parts
-// each; row by row in one warp it was 11), 5 for windows, 11 for chunks (39 MB of parts, from L2).  A share of the rows for
+// the blocks are resident at once.  It ends 6 us after that kernel for single tokens (3 requests of 150k keys: 38 parts
+// each; row by row in one warp it was 11), 5 for windows, 12 for chunks (39 MB of parts, from L2).  A share of the rows for
 // each 8 of a part: with twice or half as many the windows take 56.5 or 55.4 us for 54.0, the chunks 160 at a quarter and
 // 142 at half for 132.
 struct Parts {

@@ -10,10 +10,10 @@
 // and no second launch waits for them.  A large step's rows are written by a second launch over many blocks, which reads
 // the sums from the plan.
 //
-// Measured, on the GPU and as a call (which the host's side bounds below 15 us): 64 single tokens 8.5 and 14.8 us; 128
-// windows of 50 tokens 6.7 us, its rows 2 more behind it, and 17.2; 256 prompts of up to 4095 tokens (4.3 MB of rows) 17.7
-// as a call, 1.2 of it the look at the 16 thousand pages it takes (2.7 an entry at a time).  The tile sums of such prompts
-// count too: with 1, 4, 5 and 25 query heads to a key head the plan takes 17, 17, 24 and 26 us on the GPU.
+// Measured, on the GPU and as a call (which the host's side bounds below 15 us): 64 single tokens 8.9 and 14.9 us; 128
+// windows of 50 tokens 7.0 us, its rows 3.6 more behind it, and 17.4; 256 prompts of up to 4095 tokens (4.3 MB of rows) 11.1,
+// its rows 6 more, and 17.2, of which the look at the 16 thousand pages they take is 1.2 (2.7 an entry at a time).  With 1, 4,
+// 5 and 25 query heads to a key head such prompts' plans take 17, 17, 24 and 26 us on the GPU: their tile sums' periods.
 #include "paged.h"
 
 namespace t2w {
