@@ -704,6 +704,76 @@ typedef struct t2w_paged_attn_args {
 T2W_API size_t t2w_paged_workspace_bytes(int32_t max_fresh, int32_t q_heads, int32_t kv_heads, int32_t head_dim);
 T2W_API int t2w_paged_attn(const t2w_paged_attn_args* a, void* stream);
 
+/* ---- Products with 4-bit weights (no reference counterpart: the reference's weights are 16-bit).  W[n][k] = (code - zero)
+ * * scale: codes 0 .. 15, one scale (bf16 or fp16) and one zero (0 .. 15; 8 for a weight without zeros) for each row and
+ * `group` consecutive k.  group is 32, 64 or 128 and divides k.
+ * A weight is laid out once by t2w_w4_pack into `buffer` (t2w_w4_bytes, 128-byte aligned, on the current device); a gated
+ * weight holds two matrices [n][k], the gate's and the up projection's.  Products read the buffer before the kernel ahead of them in the stream
+ * has ended, so whatever writes it (packing, a copy) has to be complete, by an event or a synchronisation that the host has
+ * seen, before the first product with it is enqueued.  Calls are asynchronous on `stream`, keep nothing between them and need
+ * no workspace; they may be captured, and may run at once with one weight. */
+#define T2W_ACT_SILU 0
+#define T2W_ACT_GELU_TANH 1
+
+typedef struct t2w_w4_weight {
+  int32_t n, k, group, scale_dtype /* T2W_DT_* */, zeros, gated;
+  void* buffer;
+} t2w_w4_weight;
+typedef struct t2w_w4_source {
+  const void* codes;  /* device uint8 [n][k], pitch code_ld */
+  const void* scales; /* device scale_dtype [n][k / group], pitch scale_ld */
+  const void* zeros;  /* device uint8 [n][k / group], pitch zero_ld, or NULL */
+  int64_t code_ld, scale_ld, zero_ld;
+} t2w_w4_source;
+
+/* Bytes of a weight's buffer (negative: a status). */
+T2W_API int64_t t2w_w4_bytes(int32_t n, int32_t k, int32_t group, int32_t zeros, int32_t gated);
+/* Lay `a` (gated: the gate `a` and the up projection `b`) out into w->buffer.  Codes and zeros are taken modulo 16. */
+T2W_API int t2w_w4_pack(const t2w_w4_weight* w, const t2w_w4_source* a, const t2w_w4_source* b, void* stream);
+/* The values (code - zero) * scale, exact, into fp32 [n][k] matrices at these pitches (b: the up projection's). */
+T2W_API int t2w_w4_unpack(const t2w_w4_weight* w, float* a, int64_t a_ld, float* b, int64_t b_ld, void* stream);
+/* What a product with this weight recorded (T2W_OK or T2W_ERR_TIMEOUT, then that call's outputs are void), by a copy on
+ * `stream` that this call waits for. */
+T2W_API int t2w_w4_status(const t2w_w4_weight* w, void* stream);
+
+/* out[rows][n] = x[rows][k] W^T (+ bias [n]) (+ residual [rows][n]), or for a gated weight act(x Wgate^T) * (x Wup^T)
+ * (neither bias nor residual).  x, bias, residual and out are of `dtype`; x lies at a pitch of x_ld elements, on
+ * 16-byte boundaries (x_ld a multiple of 8), residual at res_ld; out is contiguous.  Sums are fp32 over (code - zero) x, group
+ * by group times the scale, rounded once at the end. */
+typedef struct t2w_w4_linear_args {
+  t2w_w4_weight w;
+  int32_t rows, dtype, act;
+  const void* x;
+  int64_t x_ld;
+  const void* bias;
+  const void* residual;
+  int64_t res_ld;
+  void* out;
+} t2w_w4_linear_args;
+T2W_API int t2w_w4_linear(const t2w_w4_linear_args* a, void* stream);
+
+/* ---- Rotary positions with several axes (no reference counterpart).  Pair i of every head of q and k, i < rotary_dim / 2,
+ * turns by positions[axis_i][row] * f_i (by its negative with `inverse`, which undoes it and is its gradient): (x, y) -> (x
+ * cos - y sin, y cos + x sin).  A pair is values i and i + rotary_dim / 2 of the head, or with `adjacent` 2 i and 2 i + 1; values
+ * past rotary_dim stay.
+ * table: device uint64 [rotary_dim / 2] with f_i / (2 pi) * 2^64 rounded, then as many axis numbers (0 .. axes - 1).
+ * positions: int32, or int64 with wide_positions, [axes][rows] at a pitch of pos_ld, of either sign.
+ * Rows [rows][heads][head_dim] of `dtype`, head_dim contiguous, on 16-byte boundaries (pitches multiples of 8); out may be
+ * `in` itself, with its pitches, and may not overlap otherwise.  head_dim is a multiple of 8, rotary_dim of 16. */
+typedef struct t2w_rotary_rows {
+  const void* in;
+  void* out;
+  int64_t in_row_ld, in_head_ld, out_row_ld, out_head_ld;
+} t2w_rotary_rows;
+typedef struct t2w_rotary_args {
+  int32_t rows, q_heads, k_heads, head_dim, rotary_dim, axes, adjacent, inverse, wide_positions, dtype;
+  t2w_rotary_rows q, k;
+  const void* positions;
+  int64_t pos_ld;
+  const void* table;
+} t2w_rotary_args;
+T2W_API int t2w_rotary(const t2w_rotary_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

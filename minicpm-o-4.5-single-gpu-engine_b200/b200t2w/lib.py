@@ -151,6 +151,33 @@ class PagedAttnArgs(ctypes.Structure):
                [("workspace_bytes", ctypes.c_size_t)]
 
 
+class W4Weight(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("n", "k", "group", "scale_dtype", "zeros", "gated")] + [("buffer", ctypes.c_void_p)]
+
+
+class W4Source(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("codes", "scales", "zeros")] + \
+               [(n, ctypes.c_int64) for n in ("code_ld", "scale_ld", "zero_ld")]
+
+
+class W4LinearArgs(ctypes.Structure):
+    _fields_ = [("w", W4Weight)] + [(n, ctypes.c_int32) for n in ("rows", "dtype", "act")] + \
+               [("x", ctypes.c_void_p), ("x_ld", ctypes.c_int64), ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+                ("res_ld", ctypes.c_int64), ("out", ctypes.c_void_p)]
+
+
+class RotaryRows(ctypes.Structure):
+    _fields_ = [("in", ctypes.c_void_p), ("out", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int64) for n in ("in_row_ld", "in_head_ld", "out_row_ld", "out_head_ld")]
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("rows", "q_heads", "k_heads", "head_dim", "rotary_dim", "axes", "adjacent",
+                                              "inverse", "wide_positions", "dtype")] + \
+               [("q", RotaryRows), ("k", RotaryRows), ("positions", ctypes.c_void_p), ("pos_ld", ctypes.c_int64),
+                ("table", ctypes.c_void_p)]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
 _F = ctypes.c_float
@@ -240,6 +267,12 @@ _SIGS = {
     "t2w_paged_append": ([ctypes.POINTER(PagedAppendArgs), _P], ctypes.c_int),
     "t2w_paged_workspace_bytes": ([_I, _I, _I, _I], ctypes.c_size_t),
     "t2w_paged_attn": ([ctypes.POINTER(PagedAttnArgs), _P], ctypes.c_int),
+    "t2w_w4_bytes": ([_I, _I, _I, _I, _I], ctypes.c_int64),
+    "t2w_w4_pack": ([ctypes.POINTER(W4Weight), ctypes.POINTER(W4Source), ctypes.POINTER(W4Source), _P], ctypes.c_int),
+    "t2w_w4_unpack": ([ctypes.POINTER(W4Weight), _P, ctypes.c_int64, _P, ctypes.c_int64, _P], ctypes.c_int),
+    "t2w_w4_status": ([ctypes.POINTER(W4Weight), _P], ctypes.c_int),
+    "t2w_w4_linear": ([ctypes.POINTER(W4LinearArgs), _P], ctypes.c_int),
+    "t2w_rotary": ([ctypes.POINTER(RotaryArgs), _P], ctypes.c_int),
     "t2w_gemm_e4m3": ([_P, _I, _I, _P, _I, ctypes.c_int64, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _I, _P,
                        ctypes.POINTER(_P), _F, _P], ctypes.c_int),
 }

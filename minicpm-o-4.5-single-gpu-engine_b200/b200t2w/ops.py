@@ -51,4 +51,5 @@ def call(name: str, *args):
 
 OPS = ("create", "destroy", "workspace_bytes", "solve_packed", "slots_create", "slots_destroy", "cached_workspace_bytes",
        "solve_cached", "solve_slots", "ln_mod", "add_ln_mod", "ln_mish", "gemm", "attn_varlen", "euler_cfg",
-       "enc_workspace_bytes", "encode", "paged_plan", "paged_append", "paged_attn", "paged_release", "paged_status")
+       "enc_workspace_bytes", "encode", "paged_plan", "paged_append", "paged_attn", "paged_release", "paged_status", "w4_pack",
+       "w4_unpack", "w4_status", "w4_linear", "w4_gated", "rotary", "rotary_")

@@ -513,6 +513,195 @@ int64_t paged_status(const at::Tensor& plan) {
   return t2w_paged_status(i32_of("paged_status", "plan", plan, plan), stream_of(plan));
 }
 
+// ---- products with 4-bit weights --------------------------------------------------------------------------------------
+// A weight crosses as its buffer (uint8, t2w_w4_bytes), its sizes and its kind: 1 zeros, 2 gated, 4 fp16 scales.
+
+t2w_w4_weight weight_of(const char* op, const at::Tensor& buffer, int64_t n, int64_t k, int64_t group, int64_t kind) {
+  TORCH_CHECK(buffer.is_cuda() && buffer.scalar_type() == at::kByte && buffer.dim() == 1 && buffer.is_contiguous(),
+              op, ": a weight's buffer is contiguous uint8 on the GPU");
+  t2w_w4_weight w{};
+  w.n = to_i32(op, "n", n);
+  w.k = to_i32(op, "k", k);
+  w.group = to_i32(op, "group", group);
+  w.zeros = (kind & 1) != 0;
+  w.gated = (kind & 2) != 0;
+  w.scale_dtype = kind & 4 ? T2W_DT_FP16 : T2W_DT_BF16;
+  const int64_t bytes = t2w_w4_bytes(w.n, w.k, w.group, w.zeros, w.gated);
+  if (bytes < 0) check("t2w_w4_bytes", (int)bytes);
+  TORCH_CHECK(buffer.numel() == bytes, op, ": a weight of these sizes has ", bytes, " bytes, not ", buffer.numel());
+  w.buffer = buffer.data_ptr();
+  return w;
+}
+
+t2w_w4_source source_of(const char* op, const t2w_w4_weight& w, const at::Tensor& buffer, const at::Tensor& codes,
+                        const at::Tensor& scales, const std::optional<at::Tensor>& zeros) {
+  const int64_t groups = w.k / w.group;
+  auto fits = [&](const at::Tensor& t, at::ScalarType type, int64_t cols) {
+    return t.dim() == 2 && t.scalar_type() == type && t.size(0) == w.n && t.size(1) == cols &&
+           (cols == 1 || t.stride(1) == 1) && t.stride(0) >= 0 && t.device() == buffer.device();
+  };
+  TORCH_CHECK(fits(codes, at::kByte, w.k), op, ": codes are uint8 [n, k] with contiguous rows on ", buffer.device().str());
+  TORCH_CHECK(fits(scales, w.scale_dtype == T2W_DT_FP16 ? at::kHalf : at::kBFloat16, groups), op,
+              ": scales are bf16 or fp16 [n, k / group] with contiguous rows on ", buffer.device().str());
+  TORCH_CHECK(zeros.has_value() == (w.zeros != 0), op, ": zeros come where the weight has them");
+  t2w_w4_source s{};
+  s.codes = codes.data_ptr();
+  s.scales = scales.data_ptr();
+  s.code_ld = codes.stride(0);
+  s.scale_ld = scales.stride(0);
+  if (zeros) {
+    TORCH_CHECK(fits(*zeros, at::kByte, groups), op, ": zeros are uint8 [n, k / group] with contiguous rows on ",
+                buffer.device().str());
+    s.zeros = zeros->data_ptr();
+    s.zero_ld = zeros->stride(0);
+  }
+  return s;
+}
+
+void w4_pack(at::Tensor& buffer, int64_t n, int64_t k, int64_t group, int64_t kind, const at::Tensor& codes,
+             const at::Tensor& scales, const std::optional<at::Tensor>& zeros, const std::optional<at::Tensor>& up_codes,
+             const std::optional<at::Tensor>& up_scales, const std::optional<at::Tensor>& up_zeros) {
+  const char* op = "w4_pack";
+  const t2w_w4_weight w = weight_of(op, buffer, n, k, group, kind);
+  const c10::DeviceGuard guard(buffer.device());
+  TORCH_CHECK((w.gated != 0) == up_codes.has_value() && up_codes.has_value() == up_scales.has_value(), op,
+              ": a gated weight has the up projection's codes and scales too");
+  const t2w_w4_source a = source_of(op, w, buffer, codes, scales, zeros);
+  t2w_w4_source b{};
+  if (w.gated) b = source_of(op, w, buffer, *up_codes, *up_scales, up_zeros);
+  check("t2w_w4_pack", t2w_w4_pack(&w, &a, w.gated ? &b : nullptr, stream_of(buffer)));
+}
+
+std::vector<at::Tensor> w4_unpack(const at::Tensor& buffer, int64_t n, int64_t k, int64_t group, int64_t kind) {
+  const t2w_w4_weight w = weight_of("w4_unpack", buffer, n, k, group, kind);
+  const c10::DeviceGuard guard(buffer.device());
+  std::vector<at::Tensor> r;
+  for (int i = 0; i < (w.gated ? 2 : 1); ++i) r.push_back(at::empty({n, k}, buffer.options().dtype(at::kFloat)));
+  check("t2w_w4_unpack", t2w_w4_unpack(&w, r[0].data_ptr<float>(), k, w.gated ? r[1].data_ptr<float>() : nullptr, k,
+                                       stream_of(buffer)));
+  return r;
+}
+
+int64_t w4_status(const at::Tensor& buffer, int64_t n, int64_t k, int64_t group, int64_t kind) {
+  const t2w_w4_weight w = weight_of("w4_status", buffer, n, k, group, kind);
+  const c10::DeviceGuard guard(buffer.device());
+  return t2w_w4_status(&w, stream_of(buffer));
+}
+
+at::Tensor w4_product(const char* op, const at::Tensor& x, const at::Tensor& buffer, const t2w_w4_weight& w, int64_t act,
+                      const std::optional<at::Tensor>& bias, const std::optional<at::Tensor>& residual) {
+  const c10::DeviceGuard guard(buffer.device());
+  t2w_w4_linear_args a{};
+  a.w = w;
+  a.dtype = dtype_of(op, x);
+  a.act = (int32_t)act;
+  TORCH_CHECK(x.dim() == 2 && x.size(1) == w.k && x.stride(1) == 1 && x.device() == buffer.device(), op, ": x is [rows, ", w.k,
+              "] with contiguous rows on ", buffer.device().str());
+  TORCH_CHECK(!x.requires_grad() || !at::GradMode::is_enabled(), op, ": has no gradient");
+  a.rows = to_i32(op, "rows", x.size(0));
+  a.x_ld = a.rows > 1 ? x.stride(0) : w.k;
+  TORCH_CHECK(a.x_ld >= w.k && a.x_ld % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0, op,
+              ": x lies on 16-byte boundaries (a pitch of a multiple of 8 elements, at least k)");
+  a.x = x.data_ptr();
+  if (bias) {
+    TORCH_CHECK(bias->dim() == 1 && bias->numel() == w.n && (w.n == 1 || bias->stride(0) == 1) &&
+                    bias->scalar_type() == x.scalar_type() && bias->device() == x.device(),
+                op, ": bias is contiguous [", w.n, "] of x's type and device");
+    a.bias = bias->data_ptr();
+  }
+  if (residual) {
+    TORCH_CHECK(residual->dim() == 2 && residual->size(0) == a.rows && residual->size(1) == w.n &&
+                    (w.n == 1 || residual->stride(1) == 1) && (a.rows <= 1 || residual->stride(0) >= w.n) &&
+                    residual->scalar_type() == x.scalar_type() && residual->device() == x.device(),
+                op, ": residual is [", a.rows, ", ", w.n, "] with contiguous rows of x's type and device");
+    a.residual = residual->data_ptr();
+    a.res_ld = a.rows > 1 ? residual->stride(0) : w.n;
+  }
+  at::Tensor out = at::empty({a.rows, w.n}, x.options());
+  if (a.rows == 0) return out;
+  a.out = out.data_ptr();
+  check("t2w_w4_linear", t2w_w4_linear(&a, stream_of(buffer)));
+  return out;
+}
+
+at::Tensor w4_linear(const at::Tensor& x, const at::Tensor& buffer, int64_t n, int64_t k, int64_t group, int64_t kind,
+                     const std::optional<at::Tensor>& bias, const std::optional<at::Tensor>& residual) {
+  const t2w_w4_weight w = weight_of("w4_linear", buffer, n, k, group, kind);
+  TORCH_CHECK(!w.gated, "w4_linear: the weight is a gated pair");
+  return w4_product("w4_linear", x, buffer, w, T2W_ACT_SILU, bias, residual);
+}
+
+at::Tensor w4_gated(const at::Tensor& x, const at::Tensor& buffer, int64_t n, int64_t k, int64_t group, int64_t kind,
+                    int64_t act) {
+  const t2w_w4_weight w = weight_of("w4_gated", buffer, n, k, group, kind);
+  TORCH_CHECK(w.gated, "w4_gated: the weight is not a gated pair");
+  return w4_product("w4_gated", x, buffer, w, act, std::nullopt, std::nullopt);
+}
+
+// ---- rotary positions -------------------------------------------------------------------------------------------------
+
+std::vector<at::Tensor> rotate(const char* op, const at::Tensor& q, const std::optional<at::Tensor>& k, const at::Tensor& positions,
+                               const at::Tensor& table, int64_t rotary_dim, int64_t axes, bool adjacent, bool inverse,
+                               bool in_place) {
+  TORCH_CHECK(q.is_cuda(), "b200t2w ops take CUDA tensors");
+  const c10::DeviceGuard guard(q.device());
+  TORCH_CHECK(q.dim() == 3, op, ": q is [rows, heads, head_dim]");
+  t2w_rotary_args a{};
+  a.rows = to_i32(op, "rows", q.size(0));
+  a.head_dim = to_i32(op, "head_dim", q.size(2));
+  a.rotary_dim = to_i32(op, "rotary_dim", rotary_dim);
+  a.axes = to_i32(op, "axes", axes);
+  a.adjacent = adjacent;
+  a.inverse = inverse;
+  a.dtype = dtype_of(op, q);
+  TORCH_CHECK(table.scalar_type() == at::kLong && table.dim() == 1 && table.is_contiguous() && table.numel() == rotary_dim &&
+                  table.device() == q.device(),
+              op, ": the table is int64 [rotary_dim] on ", q.device().str());
+  a.table = table.data_ptr();
+  const bool wide = positions.scalar_type() == at::kLong;
+  TORCH_CHECK(wide || positions.scalar_type() == at::kInt, op, ": positions are int32 or int64");
+  const bool flat = positions.dim() == 1 && axes == 1;
+  TORCH_CHECK((flat || (positions.dim() == 2 && positions.size(0) == axes)) && positions.size(flat ? 0 : 1) == a.rows &&
+                  (a.rows <= 1 || positions.stride(flat ? 0 : 1) == 1) && positions.device() == q.device(),
+              op, ": positions are [", axes, ", ", a.rows, "] with contiguous rows on ", q.device().str());
+  a.wide_positions = wide;
+  a.pos_ld = flat || axes == 1 ? a.rows : positions.stride(0);
+  TORCH_CHECK(a.pos_ld >= a.rows, op, ": the axes of positions do not overlap");
+  a.positions = positions.data_ptr();
+  std::vector<at::Tensor> r;
+  auto fill = [&](const char* name, const at::Tensor& x, int32_t& heads, t2w_rotary_rows& rows) {
+    TORCH_CHECK(x.dim() == 3 && x.scalar_type() == q.scalar_type(), op, ": q and k are [rows, heads, head_dim] of one type");
+    TORCH_CHECK(!x.requires_grad() || !at::GradMode::is_enabled(), op, ": no gradient is recorded (`inverse` is the gradient)");
+    heads = to_i32(op, "heads", x.size(1));
+    if (heads == 0 || a.rows == 0) {
+      TORCH_CHECK(x.size(0) == a.rows && x.size(2) == a.head_dim, op, ": q and k have the same rows and head_dim");
+      r.push_back(in_place ? x : at::empty_like(x));
+      return;
+    }
+    rows_of(op, name, x, q, a.rows, heads, a.head_dim, rows.in_row_ld, rows.in_head_ld);
+    r.push_back(in_place ? x : at::empty({a.rows, heads, a.head_dim}, x.options()));
+    rows.in = x.data_ptr();
+    rows.out = r.back().data_ptr();
+    rows.out_row_ld = in_place ? rows.in_row_ld : (int64_t)heads * a.head_dim;
+    rows.out_head_ld = in_place ? rows.in_head_ld : a.head_dim;
+  };
+  fill("q", q, a.q_heads, a.q);
+  if (k) fill("k", *k, a.k_heads, a.k);
+  if (in_place && k && a.rows && a.q_heads && a.k_heads)
+    TORCH_CHECK(q.data_ptr() != k->data_ptr(), op, ": q and k are one tensor");
+  check("t2w_rotary", t2w_rotary(&a, stream_of(q)));
+  return r;
+}
+
+std::vector<at::Tensor> rotary(const at::Tensor& q, const std::optional<at::Tensor>& k, const at::Tensor& positions,
+                               const at::Tensor& table, int64_t rotary_dim, int64_t axes, bool adjacent, bool inverse) {
+  return rotate("rotary", q, k, positions, table, rotary_dim, axes, adjacent, inverse, false);
+}
+void rotary_(at::Tensor& q, const std::optional<at::Tensor>& k, const at::Tensor& positions, const at::Tensor& table,
+             int64_t rotary_dim, int64_t axes, bool adjacent, bool inverse) {
+  rotate("rotary_", q, k, positions, table, rotary_dim, axes, adjacent, inverse, true);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(b200t2w, m) {
@@ -564,4 +753,18 @@ TORCH_LIBRARY(b200t2w, m) {
         "Tensor(d!) free_count, Tensor(e!) status) -> ()",
         &paged_release);
   m.def("paged_status(Tensor plan) -> int", &paged_status);
+  m.def("w4_pack(Tensor(a!) buffer, int n, int k, int group, int kind, Tensor codes, Tensor scales, Tensor? zeros, "
+        "Tensor? up_codes, Tensor? up_scales, Tensor? up_zeros) -> ()",
+        &w4_pack);
+  m.def("w4_unpack(Tensor buffer, int n, int k, int group, int kind) -> Tensor[]", &w4_unpack);
+  m.def("w4_status(Tensor buffer, int n, int k, int group, int kind) -> int", &w4_status);
+  m.def("w4_linear(Tensor x, Tensor buffer, int n, int k, int group, int kind, Tensor? bias, Tensor? residual) -> Tensor",
+        &w4_linear);
+  m.def("w4_gated(Tensor x, Tensor buffer, int n, int k, int group, int kind, int act) -> Tensor", &w4_gated);
+  m.def("rotary(Tensor q, Tensor? k, Tensor positions, Tensor table, int rotary_dim, int axes, bool adjacent, bool inverse) "
+        "-> Tensor[]",
+        &rotary);
+  m.def("rotary_(Tensor(a!) q, Tensor(b!)? k, Tensor positions, Tensor table, int rotary_dim, int axes, bool adjacent, "
+        "bool inverse) -> ()",
+        &rotary_);
 }
