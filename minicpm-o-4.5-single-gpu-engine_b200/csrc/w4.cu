@@ -198,5 +198,6 @@ extern "C" int t2w_w4_linear(const t2w_w4_linear_args* a, void* stream) {
   p.residual = a->residual;
   p.res_ld = a->res_ld;
   p.out = a->out;
-  return done(launch_w4_few(p, w.group, w.has_zeros, w.gated, a->dtype == T2W_DT_FP16, static_cast<cudaStream_t>(stream)));
+  const auto launch = a->rows <= 16 ? launch_w4_few : launch_w4_many;
+  return done(launch(p, w.group, w.has_zeros, w.gated, a->dtype == T2W_DT_FP16, static_cast<cudaStream_t>(stream)));
 }
