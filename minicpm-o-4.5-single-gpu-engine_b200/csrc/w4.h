@@ -59,6 +59,39 @@ struct W4Dev {
 cudaError_t launch_w4_few(const W4Dev& p, int group, bool zeros, bool gated, bool half, cudaStream_t st);
 cudaError_t launch_w4_many(const W4Dev& p, int group, bool zeros, bool gated, bool half, cudaStream_t st);
 
+// ---------------------------------------------------------------- waiting
+// mbar_wait without its look at %globaltimer, which costs about a microsecond: these kernels hand over every few hundred
+// clocks, and most waits are not met at once.  The limit is in SM clocks.
+T2W_DEV bool w4_wait(uint64_t* bar, uint32_t parity, int* err) {
+  const uint32_t at = smem_u32(bar);
+  if (mbar_try_wait(at, parity)) return true;
+  const long long t0 = clock64();
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(at, parity)) return true;
+    if ((i & 63u) == 0 && clock64() - t0 > kWaitLimitCycles) {
+      atomicExch(err, T2W_ERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+
+// The same by a whole warp, with one answer.  The first polls are one asm block: control flow that the compiler does not
+// see as divergent, so that what a warp computes around its waits stays in uniform registers.
+T2W_DEV bool w4_wait_warp(uint64_t* bar, uint32_t parity, int* err) {
+  const uint32_t at = smem_u32(bar);
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n\t"
+      "AGAIN:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE;\n\t"
+      "add.u32 n, n, 1;\n\tsetp.lt.u32 q, n, 64;\n\t@q bra AGAIN;\n\t"
+      "DONE:\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(at), "r"(parity)
+      : "memory");
+  if (__all_sync(0xffffffffu, ok)) return true;
+  return __all_sync(0xffffffffu, w4_wait(bar, parity, err));
+}
+
 // ---------------------------------------------------------------- clusters
 T2W_DEV uint32_t cluster_rank() {
   uint32_t r;
@@ -67,12 +100,34 @@ T2W_DEV uint32_t cluster_rank() {
 }
 T2W_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 T2W_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-T2W_DEV float ld_cluster(uint32_t addr, uint32_t rank) {
+T2W_DEV uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
   uint32_t a;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+T2W_DEV float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
+}
+// The sum over the cluster's blocks (1, 2, 4 or 8), in their order, of four values at one place of each; four reads are under
+// way at once.
+T2W_DEV float4 cluster_sum4(uint32_t addr, int split) {
+  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int s0 = 0; s0 < split; s0 += 4) {
+    float4 v[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) v[s] = s0 + s < split ? ld_cluster4(cluster_addr(addr, s0 + s)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      r.x += v[s].x;
+      r.y += v[s].y;
+      r.z += v[s].z;
+      r.w += v[s].w;
+    }
+  }
+  return r;
 }
 
 // ---------------------------------------------------------------- codes to operands
@@ -114,16 +169,50 @@ T2W_DEV void w4_widen(uint32_t w, uint32_t zlo, uint32_t zhi, uint32_t (&a)[4]) 
     a[i] = W4Num<HALF>::sub(v, (i & 1) ? zhi : zlo);
   }
 }
+// Four consecutive outputs of a row, as far as there are any: one store where they lie on 8 bytes.
+T2W_DEV void w4_store4(uint16_t* out, const uint16_t (&v)[4], int count) {
+  if (count >= 4 && (reinterpret_cast<uintptr_t>(out) & 7) == 0) {
+    *reinterpret_cast<uint2*>(out) = make_uint2(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < count) out[i] = v[i];
+  }
+}
 T2W_DEV float w4_scale(uint16_t v, int half) { return half ? W4Num<true>::to_float(v) : W4Num<false>::to_float(v); }
 
 // ---------------------------------------------------------------- activations (fp32, relative error of a few 2^-22)
-// y sigmoid(y); the quotient is kept off __fdividef, whose result is 0 for divisors above 2^126: y / (1 + e^-y) is that
-// small there that fp32 holds it as a subnormal or 0, and +-inf and NaN go as in the formula
-T2W_DEV float w4_sigmoid_mul(float y, float s) { return y / (1.f + __expf(-s)); }
+// y sigmoid(s) = y / (1 + e^-s) by the reciprocal (rcp.approx, which has subnormal results where __fdividef gives 0: for
+// divisors above 2^126); e^-s = inf gives y * 0, +-inf and NaN go as in the formula.
+T2W_DEV float w4_sigmoid_mul(float y, float s) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-s)));
+  return y * r;
+}
 T2W_DEV float w4_act(float g, int act) {
   if (act == T2W_ACT_SILU) return w4_sigmoid_mul(g, g);
   // GELU in its tanh form: g (1 + tanh t) / 2 = g sigmoid(2 t), t = sqrt(2 / pi) (g + 0.044715 g^3)
   return w4_sigmoid_mul(g, 1.5957691216057308f * (g + 0.044715f * g * g * g));
+}
+
+// Outputs n .. n + 3 of row m from their sums (gated: gate and up), as far as n < p.n.
+template <bool HALF, bool GATED>
+T2W_DEV void w4_finish4(const W4Dev& p, int m, int64_t n, float4 sum, float4 up) {
+  float v[4] = {sum.x, sum.y, sum.z, sum.w};
+  const float u[4] = {up.x, up.y, up.z, up.w};
+  const int count = (int)min((int64_t)4, p.n - n);
+  uint16_t out[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (GATED) {
+      v[i] = w4_act(v[i], p.act) * u[i];
+    } else if (i < count) {
+      if (p.bias) v[i] += W4Num<HALF>::to_float(static_cast<const uint16_t*>(p.bias)[n + i]);
+      if (p.residual) v[i] += W4Num<HALF>::to_float(static_cast<const uint16_t*>(p.residual)[(int64_t)m * p.res_ld + n + i]);
+    }
+    out[i] = W4Num<HALF>::from_float(v[i]);
+  }
+  w4_store4(static_cast<uint16_t*>(p.out) + (int64_t)m * p.n + n, out, count);
 }
 
 }  // namespace t2w

@@ -15,6 +15,7 @@ namespace t2w {
 namespace {
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps, kMaxStages = 3;
+constexpr int kPitch = 68;  // of a column of 64 sums: on 16 bytes, and 8 columns apart in the banks
 
 template <bool HALF>
 T2W_DEV void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -57,8 +58,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int split
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem);  // [warp][stage]
-  float* part = reinterpret_cast<float*>(smem + kWarps * kMaxStages * 8);  // the block's sums [column of x][64 + 1]
-  constexpr int kPart = (kWarps * kMaxStages * 8 + kCols * 65 * 4 + 127) / 128 * 128;
+  float* part = reinterpret_cast<float*>(smem + kWarps * kMaxStages * 8);  // the block's sums [column of x][kPitch]
+  constexpr int kPart = (kWarps * kMaxStages * 8 + kCols * kPitch * 4 + 127) / 128 * 128;
   uint8_t* ring = smem + kPart + warp * stages * kTile;
   uint64_t* full = bars + warp * kMaxStages;
 
@@ -92,14 +93,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int split
   int stage = 0;
   uint32_t phase = 0;
   for (; tile < k_end; tile += kWarps) {
-    if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, p.status))) {
+    if (!w4_wait_warp(&full[stage], phase, p.status)) {
       // The status tells that the outputs are void.  What else is under way lands (or is given up) before the ring is used.
       for (int i = 1; i < stages && tile + i * kWarps < k_end; ++i) {
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
-        mbar_wait(&full[stage], phase, p.status);
+        w4_wait(&full[stage], phase, p.status);
       }
       break;
     }
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int split
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) v += all[w * 64 * kCols + e];
-    part[(e % kCols) * 65 + e / kCols] = v;
+    part[(e % kCols) * kPitch + e / kCols] = v;
   }
   if (split > 1) {
     cluster_arrive();
@@ -180,29 +181,24 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int split
   } else {
     __syncthreads();
   }
-  // This block's share of the outputs, along n in a warp.
-  constexpr int kOut = GATED ? 32 : 64;
+  // This block's share of the outputs, four along n to a thread.
+  constexpr int kQuads = GATED ? 8 : 16;
   const int cols = min(kCols, p.rows - m0);
   const uint32_t base = smem_u32(part);
-  for (int e = rank * (kOut * kCols / split) + threadIdx.x; e < (rank + 1) * (kOut * kCols / split); e += kThreads) {
-    const int m = e / kOut, o = e % kOut, n = rb * kOut + o;
+  for (int e = rank * (kQuads * kCols / split) + threadIdx.x; e < (rank + 1) * (kQuads * kCols / split); e += kThreads) {
+    const int m = e / kQuads, o = e % kQuads * 4;
+    const int64_t n = (int64_t)rb * (GATED ? 32 : 64) + o;
     if (m >= cols || n >= p.n) continue;
-    const int row = GATED ? (o >> 3) * 16 + (o & 7) : o;
-    float v = 0.f, u = 0.f;
-    for (int s = 0; s < split; ++s) {
-      const uint32_t at = base + (m * 65 + row) * 4;
-      v += split > 1 ? ld_cluster(at, s) : part[m * 65 + row];
-      if constexpr (GATED) u += split > 1 ? ld_cluster(at + 32, s) : part[m * 65 + row + 8];
-    }
-    const int64_t at = (int64_t)(m0 + m) * p.n + n;
-    if constexpr (GATED) {
-      v = w4_act(v, p.act) * u;
+    const int at = m * kPitch + (GATED ? (o >> 3) * 16 + (o & 7) : o);
+    float4 v, u = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (split > 1) {
+      v = cluster_sum4(base + at * 4, split);
+      if constexpr (GATED) u = cluster_sum4(base + at * 4 + 32, split);
     } else {
-      if (p.bias) v += W4Num<HALF>::to_float(static_cast<const uint16_t*>(p.bias)[n]);
-      if (p.residual)
-        v += W4Num<HALF>::to_float(static_cast<const uint16_t*>(p.residual)[(int64_t)(m0 + m) * p.res_ld + n]);
+      v = *reinterpret_cast<const float4*>(part + at);
+      if constexpr (GATED) u = *reinterpret_cast<const float4*>(part + at + 8);
     }
-    static_cast<uint16_t*>(p.out)[at] = W4Num<HALF>::from_float(v);
+    w4_finish4<HALF, GATED>(p, m0 + m, n, v, u);
   }
   if (split > 1) {  // no block leaves while another reads its sums
     cluster_arrive();
@@ -213,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int split
 template <bool HALF, int NT, int G, bool ZEROS, bool GATED>
 cudaError_t launch(const W4Dev& p, cudaStream_t st) {
   constexpr int kTile = w4_tile_bytes(G, ZEROS), kCols = 8 * NT;
-  constexpr int kPart = (kWarps * kMaxStages * 8 + kCols * 65 * 4 + 127) / 128 * 128;
+  constexpr int kPart = (kWarps * kMaxStages * 8 + kCols * kPitch * 4 + 127) / 128 * 128;
   const int chunks = (p.rows + kCols - 1) / kCols;
   int split = 1;
   while (split < 8 && (int64_t)p.blocks * chunks * split < num_sms() && p.tiles_k >= 2 * split) split *= 2;
