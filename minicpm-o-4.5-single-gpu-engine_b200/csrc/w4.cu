@@ -36,13 +36,13 @@ __global__ void __launch_bounds__(256) k_w4_pack(const PackDev p) {
   if (tile == 0 && threadIdx.x < kW4Header / 4) reinterpret_cast<uint32_t*>(p.buffer)[threadIdx.x] = 0;
   for (int w = threadIdx.x; w < kW4Codes / 4; w += 256) {
     const int j = w & 3, lane = (w >> 2) & 31, kb = (w >> 7) & 1, strip = w >> 8;
-    const int g = lane >> 2, t = lane & 3, q = j >> 1, h = j & 1;
+    const int g = lane >> 2, t = lane & 3;
     uint32_t word = 0;
     for (int i = 0; i < 4; ++i) {
       int which;
       int64_t row;
       source_of(p, rb * kW4Rows + strip * 16 + (i & 1) * 8 + g, which, row);
-      const int k = k0 + kb * 64 + q * 32 + 8 * t + 4 * h + (i >> 1) * 2;
+      const int k = k0 + kb * 64 + 16 * j + 4 * t + (i >> 1) * 2;
       for (int e = 0; e < 2; ++e) {
         uint32_t c = p.has_zeros ? 0u : 8u;
         if (row >= 0 && k + e < p.k) c = p.codes[which][row * p.code_ld[which] + k + e] & 15u;
@@ -79,9 +79,9 @@ __global__ void __launch_bounds__(256) k_w4_unpack(const PackDev p) {
     int64_t row;
     source_of(p, rb * kW4Rows + r, which, row);
     if (row < 0 || k0 + k >= p.k) continue;
-    const int kb = k >> 6, q = (k >> 5) & 1, t = (k >> 3) & 3, h = (k >> 2) & 1, strip = r >> 4, g = r & 7;
+    const int kb = k >> 6, j = (k >> 4) & 3, t = (k >> 2) & 3, strip = r >> 4, g = r & 7;
     const int i = ((k >> 1) & 1) * 2 + ((r >> 3) & 1);
-    const uint32_t word = reinterpret_cast<const uint32_t*>(in)[((strip * 2 + kb) * 32 + g * 4 + t) * 4 + q * 2 + h];
+    const uint32_t word = reinterpret_cast<const uint32_t*>(in)[((strip * 2 + kb) * 32 + g * 4 + t) * 4 + j];
     const int code = (word >> (4 * i + 16 * (k & 1))) & 15, gr = k / p.group;
     const int zero = p.has_zeros ? in[kW4Codes + groups * 128 + gr * kW4Rows + w4_place(r)] : 8;
     const float s = w4_scale(reinterpret_cast<const uint16_t*>(in + kW4Codes)[gr * kW4Rows + w4_place(r)], p.scale_half);

@@ -10,11 +10,11 @@
 //
 // Layout: a header of 128 bytes (int32 status, the rest zero), then tiles of 64 rows x 128 k, [row block][k tile], each
 // one contiguous piece that one bulk copy brings:
-//   codes   [4 strips of 16 rows][2 blocks of 64 k][32 lanes][4 words]: a lane's 16 bytes are what it feeds to four
-//           m16n8k16 products.  Lane (g, t) = (lane / 4, lane % 4), word j = 2 q + h: rows g and g + 8 of the strip, k =
-//           32 q + 8 t + 4 h + 0 .. 3 of the block.  Nibble i and i + 4 of the word are register i of the A fragment: rows
-//           g, g + 8, g, g + 8; k + 0, 1 for i < 2 and k + 2, 3 for the others.  So 8 consecutive k of x are one 16-byte piece of a
-//           lane's B fragments, and no product reaches over a group of 32.
+//   codes   [4 strips of 16 rows][2 blocks of 64 k][32 lanes][4 words]: a word is a lane's A fragment of an m16n8k16 product
+//           of 16 k, j of the block.  Lane (g, t) = (lane / 4, lane % 4) has rows g and g + 8 of the strip and k = 16 j + 4 t + 0 .. 3:
+//           nibbles i and i + 4 are register i, rows g, g + 8, g, g + 8; k + 0, 1 for i < 2 and k + 2, 3 for the others.  So
+//           a lane's part of x is 8 consecutive bytes, widened registers are what tcgen05.st 16x256b takes, and no product reaches
+//           over a group.
 //   scales  [128 / group][64] 16-bit, then zeros [128 / group][64] bytes where there are any: place g * 8 + strip * 2 + half
 //           for row strip * 16 + half * 8 + g, so that a lane finds the eight rows it holds in one piece.
 // Rows and k past the weight's are codes that equal their zero, with scale 0.  A gated pair (gate, up) is one weight whose
@@ -75,20 +75,10 @@ T2W_DEV bool w4_wait(uint64_t* bar, uint32_t parity, int* err) {
   }
 }
 
-// The same by a whole warp, with one answer.  The first polls are one asm block: control flow that the compiler does not
-// see as divergent, so that what a warp computes around its waits stays in uniform registers.
-T2W_DEV bool w4_wait_warp(uint64_t* bar, uint32_t parity, int* err) {
-  const uint32_t at = smem_u32(bar);
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n\t"
-      "AGAIN:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE;\n\t"
-      "add.u32 n, n, 1;\n\tsetp.lt.u32 q, n, 64;\n\t@q bra AGAIN;\n\t"
-      "DONE:\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(at), "r"(parity)
-      : "memory");
-  if (__all_sync(0xffffffffu, ok)) return true;
+// The same by a whole warp, with one answer; `ready` is what a look at the barrier, taken ahead of other work, has said.  (A wait
+// for a barrier that is ready costs about 150 clocks, a look whose answer is not needed at once next to none.)
+T2W_DEV bool w4_wait_warp(uint64_t* bar, uint32_t parity, int* err, bool ready = false) {
+  if (__all_sync(0xffffffffu, ready)) return true;
   return __all_sync(0xffffffffu, w4_wait(bar, parity, err));
 }
 

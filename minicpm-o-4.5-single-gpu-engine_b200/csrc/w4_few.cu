@@ -31,24 +31,20 @@ T2W_DEV void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32
 
 template <int NT>
 struct XFrag {
-  uint4 v[NT][2][2];  // [8 rows of x][block of 64 k][half of it]: 8 consecutive k each
+  uint2 v[NT][8];  // [8 rows of x][16 k]: 4 consecutive k each
 };
 
-// A lane's pieces of x for a k tile: row m0 + 8 nt + g, k = 128 tile + 64 kb + 32 q + 8 t; zeros past either end (k is
-// a multiple of 32, so a piece lies inside or outside).
+// A lane's pieces of x for a k tile: row m0 + 8 nt + g, k = 128 tile + 16 j + 4 t; zeros past either end (k is a multiple
+// of 32, so a piece lies inside or outside).
 template <int NT>
 T2W_DEV void load_x(XFrag<NT>& f, const W4Dev& p, int m0, int tile, int g, int t) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int m = m0 + 8 * nt + g;
-    const uint16_t* row = static_cast<const uint16_t*>(p.x) + (int64_t)m * p.x_ld;
+    const int m = m0 + 8 * nt + g, k0 = tile * kW4K + 4 * t;
+    const uint16_t* row = static_cast<const uint16_t*>(p.x) + (int64_t)m * p.x_ld + k0;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int k = tile * kW4K + kb * 64 + q * 32 + 8 * t;
-        f.v[nt][kb][q] = (m < p.rows && k < p.k) ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
-      }
+    for (int j = 0; j < 8; ++j)
+      f.v[nt][j] = (m < p.rows && k0 + 16 * j < p.k) ? *reinterpret_cast<const uint2*>(row + 16 * j) : make_uint2(0, 0);
   }
 }
 
@@ -127,13 +123,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int split
         const uint32_t zlo = w4_zero<HALF>(ZEROS ? zero[i][2 * r] : 8u), zhi = w4_zero<HALF>(ZEROS ? zero[i][2 * r + 1] : 8u);
 #pragma unroll
         for (int s = 0; s < G / 16; ++s) {  // products of 16 k
-          const int j = i * (G / 16) + s, kb = j >> 2, q = (j >> 1) & 1, h = j & 1;
-          const uint32_t w = (&code[kb].x)[j & 3];
+          const int j = i * (G / 16) + s;
+          const uint32_t w = (&code[j >> 2].x)[j & 3];
           uint32_t a[4];
           w4_widen<HALF>(w, zlo, zhi, a);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            mma16816<HALF>(sum[nt], a, (&cur.v[nt][kb][q].x)[2 * h], (&cur.v[nt][kb][q].x)[2 * h + 1]);
+            mma16816<HALF>(sum[nt], a, cur.v[nt][j].x, cur.v[nt][j].y);
         }
         const float slo = w4_scale(scale[i][2 * r], p.scale_half), shi = w4_scale(scale[i][2 * r + 1], p.scale_half);
 #pragma unroll

@@ -1,17 +1,20 @@
 // Products with 4-bit weights for many rows of x on tcgen05: D[128 rows of W][NX rows of x] = (W - zero) x^T, one
 // accumulator for each group of k, scaled and summed in registers.
 //
-// A persistent block an SM:
-//   warp 0       x: TMA, 128-byte swizzle, stages of 64 k (NX = 256) or 128 k
-//   warp 1       TMEM, and tcgen05.mma from one lane (M = 128, N = NX, K = 16)
+// A persistent block an SM takes tiles of 128 k, each in H halves of U = NX / H rows of x:
+//   warp 0       x: TMA, 128-byte swizzle, one stage (128 k x U rows) for each half
+//   warp 1       TMEM, and tcgen05.mma from one lane (M = 128, N = U, K = 16), A from TMEM
 //   warp 2       packed tiles of W (128 rows x 128 k), bulk copies into a ring of their own
-//   2 x 4 warps  widen codes to whole 16-bit numbers and write them as a stage's A operand (K-major, 128-byte swizzle); the
-//                warpgroups take the stages in turn
-//   NA x 4 warps take a group's accumulator out of TMEM (two take turns), each lane one row of W: acc += scale * sum, so the
+//   2 x 4 warps  widen codes to whole 16-bit numbers and store them in TMEM, where they are the A operand; the warpgroups take
+//                the tiles in turn
+//   H x 4 warps  take a group's accumulator out of TMEM (a few take turns), each lane one row of W: acc += scale * sum, so the
 //                scale is a register and no weight is rounded; at a tile's end they write the outputs
+//
+// The weights go through TMEM because shared memory is what such a kernel runs out of: 128 bytes a clock, of which 128 k of
+// widened weights would take 256 clocks to write and 256 to read, where the products take 4 NX clocks.
 // What a hand-over costs decides the rest: passing an mbarrier that is ready takes about 100 clocks, a commit 80, the
-// issue of 4 products 65.  So with groups of 128 one barrier tells the products' warp everything that a tile waits for (x,
-// weights, a free accumulator), and one commit tells that its stage is free and its accumulator full.
+// issue of 4 products 65.  So with groups of 128 one barrier tells the products' warp what a half waits for (x and a free
+// accumulator; the weights too where there is one half), and one commit tells that its stage is free and its accumulator full.
 // With few tiles k is split over a cluster, whose blocks add their sums through distributed shared memory in a fixed order.
 // The first tiles of W come before the kernel waits for the one ahead of it in the stream.  No TMA multicast.
 #include "common.cuh"
@@ -21,35 +24,37 @@
 namespace t2w {
 namespace {
 
-constexpr int kM = 128;              // rows of W of a tile
-constexpr int kABlock = kM * 64 * 2;  // widened weights of 64 k
-constexpr int kMaxCodes = 8;         // packed tile pairs under way
+constexpr int kM = 128;        // rows of W of a tile
+constexpr int kMaxCodes = 12;  // packed tile pairs under way
 constexpr int kMaxSmem = 232448;
-constexpr int kWiden = 8;             // widening warps
-constexpr int kChunk = 16;            // columns that the end of a tile takes at a time
+constexpr int kACols = 64;     // TMEM columns of a tile's widened weights
+constexpr int kChunk = 8;      // columns that the end of a tile takes at a time
 
 template <int NX>
 struct Cfg {
-  static constexpr int NA = NX == 256 ? 2 : 1;    // accumulating warpgroups
-  static constexpr int CA = NX / NA;              // columns of an accumulating warpgroup
-  static constexpr int KB = NX == 256 ? 1 : 2;    // blocks of 64 k in a stage
-  static constexpr int THREADS = 128 * (3 + NA);
-  static constexpr int A_BYTES = KB * kABlock, B_BYTES = KB * NX * 128;
-  static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = NX == 256 ? 4 : 3;
-  static constexpr int SLOTS = STAGES * KB / 2 + 2;  // tiles whose scales are kept (see the widening warps)
-  static constexpr int TMEM = 2 * NX;
-  // Registers: CA = 128 sums need more than an even split has, which the other warps give.  The sum of the warpgroups'
-  // shares is at most what the kernel is launched with: 96 each of 640 threads, 128 each of 512.
-  static constexpr bool SHIFT = CA == 128;
-  static constexpr int LAUNCH = NX == 256 ? 96 : 128;
-  static constexpr int R_ROLES = 48, R_WIDEN = NX == 256 ? 48 : 104, R_SUM = NX == 256 ? 168 : 184;
-  static_assert(R_ROLES + 2 * R_WIDEN + NA * R_SUM <= (3 + NA) * LAUNCH, "registers");
+  static constexpr int H = NX == 256 ? 2 : 1;  // halves of a tile, and accumulating warpgroups
+  static constexpr int U = NX / H;             // rows of x of a half
+  static constexpr int TURNS = NX == 256 ? 2 : 4;  // widening warpgroups
+  static constexpr int WIDEN = 4 * TURNS;          // widening warps
+  static constexpr int THREADS = 128 * (1 + TURNS + H);
+  static constexpr int B_BYTES = U * kW4K * 2;
+  static constexpr int STAGES = NX == 256 ? 5 : NX == 128 ? 4 : 6;  // of x
+  static constexpr int A_TILES = NX == 256 ? 2 : STAGES;            // widened tiles
+  static constexpr int ACCS = NX == 256 ? 3 : 2;                    // accumulators
+  static constexpr int SLOTS = A_TILES + 2;                         // tiles whose scales are kept (see the widening warps)
+  static constexpr int A_AT = ACCS * U;                             // TMEM column of the first widened tile
+  static constexpr int TMEM = 512;
+  static_assert(A_AT + A_TILES * kACols <= TMEM, "tensor memory");
+  static_assert(H == 2 || A_TILES == STAGES, "one barrier for both operands");
+  // Registers: the sums need more than an even split has, which the other warps give.  The sum of the warpgroups' shares is at
+  // most what the kernel is launched with: 96 each of 640 threads, 80 each of 768.
+  static constexpr int LAUNCH = NX == 256 ? 96 : 80;
+  static constexpr int R_ROLES = NX == 256 ? 48 : 56, R_WIDEN = NX == 256 ? 48 : 64, R_SUM = 168;
+  static_assert(R_ROLES + TURNS * R_WIDEN + H * R_SUM <= (1 + TURNS + H) * LAUNCH, "registers");
   static constexpr int fixed(int group) {  // shared memory besides the ring of packed tiles
-    return STAGES * STAGE + SLOTS * (kW4K / group) * 256 + 8 * (2 * STAGES + 2 * kMaxCodes + 5) + 16;
+    return STAGES * B_BYTES + SLOTS * (kW4K / group) * 256 + 8 * (2 * STAGES + 2 * A_TILES + 2 * kMaxCodes + (H + 1) * ACCS + 2) + 16;
   }
 };
-static_assert(Cfg<256>::STAGES % 2 == 0, "a tile's two stages are always the same two kinds");
 
 struct ManyArgs {
   W4Dev p;
@@ -89,6 +94,44 @@ T2W_DEV void tmem_st32(uint32_t taddr, const float* v) {
       "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]),
       "f"(v[31])
       : "memory");
+}
+// A strip of 16 rows, 64 k: four m16n8k16 A fragments side by side.
+T2W_DEV void tmem_st_frags(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+// D (+)= A B with A from TMEM (two numbers to a 32-bit column) and B from shared memory.
+T2W_DEV void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+T2W_DEV void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+T2W_DEV void tmem_ld8(uint32_t taddr, float (&v)[8]) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
 }
 T2W_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -150,19 +193,20 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
   const W4Dev& p = a.p;
   extern __shared__ __align__(1024) uint8_t smem[];
   constexpr int groups = kW4K / G, slot_bytes = groups * 2 * 128;
-  // One barrier for all that a tile's products wait for, and one commit for all that wait for them: where a group is a tile.
+  // One barrier for what a half's products wait for, and one commit for all that wait for them: where a group is a tile.
   constexpr bool kOne = G == kW4K;
-  constexpr int kPerTile = 2 / C::KB;  // stages of a tile
   const int code_bytes = 2 * a.tile_bytes;
-  uint8_t* scales = smem + C::STAGES * C::STAGE;  // [slot][half][group][64]
-  uint64_t* full = reinterpret_cast<uint64_t*>(scales + C::SLOTS * slot_bytes);
-  uint64_t* empty = full + C::STAGES;  // the stage's products have ended
-  uint64_t* cfull = empty + C::STAGES;
+  uint8_t* scales = smem + C::STAGES * C::B_BYTES;  // [slot][half][group][64]
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + C::SLOTS * slot_bytes);  // x of a half (and with H = 1 the weights)
+  uint64_t* empty = full + C::STAGES;                                          // the half's products have ended
+  uint64_t* afull = empty + C::STAGES;                                         // H = 2: the weights
+  uint64_t* aempty = afull + C::A_TILES;
+  uint64_t* cfull = aempty + C::A_TILES;
   uint64_t* cempty = cfull + kMaxCodes;
-  uint64_t* dfull = cempty + kMaxCodes;  // (not kOne)
-  uint64_t* dempty = dfull + 2;
-  uint64_t* drain = dempty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* dfull = cempty + kMaxCodes;  // (not kOne) [half][accumulator]: a warpgroup waits for its own phases alone
+  uint64_t* dempty = dfull + C::H * C::ACCS;
+  uint64_t* drain = dempty + C::ACCS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   uint8_t* codes = smem + (C::fixed(G) + 127) / 128 * 128;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -171,26 +215,62 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
   const Span span = span_of(p.tiles_k, rank, a.split);
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
-      // x, the four warps that widen it, and with the tile's first stage the warps that take accumulators
-      mbar_init(&full[s], 1 + 4 + (kOne && s % kPerTile == 0 ? 4 * C::NA : 0));
+      // x, the four warps that give the accumulator back, and with one half the four that widen
+      mbar_init(&full[s], 1 + (kOne ? 4 : 0) + (C::H == 1 ? 4 : 0));
       mbar_init(&empty[s], 1);
     }
-    for (int s = 0; s < a.code_stages; ++s) {
-      mbar_init(&cfull[s], 1);
-      mbar_init(&cempty[s], kWiden / C::KB);
+    for (int s = 0; s < C::A_TILES; ++s) {
+      mbar_init(&afull[s], 4);
+      mbar_init(&aempty[s], kOne ? C::H : 1);  // a commit of each warp that issued its products
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&dfull[s], 1);
-      mbar_init(&dempty[s], 4 * C::NA);
+    for (int s = 0; s < C::ACCS; ++s) {
+      for (int h = 0; h < C::H; ++h) mbar_init(&dfull[h * C::ACCS + s], 1);
+      mbar_init(&dempty[s], 4);
     }
-    mbar_init(drain, 1);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     fence_mbar_init();
     tma_prefetch_desc(&tmX);
   }
+  // Packed tiles: one lane of warp 2 issues their copies, the first ones before anything is waited for.
+  struct {
+    int tile, kt, issued;
+    Ring r;
+  } next = {first_tile, span.first, 0, {}};
+  auto copy_codes = [&]() {
+    const int rb = (next.tile % a.tiles_n) * 2, halves = rb + 1 < p.blocks ? 2 : 1;
+    mbar_expect_tx(&cfull[next.r.stage], halves * a.tile_bytes);
+    for (int h = 0; h < halves; ++h)
+      bulk_load(codes + next.r.stage * code_bytes + h * a.tile_bytes,
+                p.tiles + ((int64_t)(rb + h) * p.tiles_k + next.kt) * a.tile_bytes, a.tile_bytes, &cfull[next.r.stage]);
+    ++next.issued;
+    next.r.next(a.code_stages);
+    if (++next.kt == span.end) {
+      next.kt = span.first;
+      next.tile += tile_step;
+    }
+  };
+  if (threadIdx.x == 64) {
+    for (int s = 0; s < a.code_stages; ++s) {
+      mbar_init(&cfull[s], 1);
+      mbar_init(&cempty[s], 4);
+    }
+    fence_mbar_init();
+    for (int s = 0; s < a.code_stages && next.tile < a.tiles; ++s) copy_codes();
+  }
+  __syncwarp();
+  if (warp == 1) {
+    pdl_wait();  // (the kernel before may hold tensor memory)
+    tmem_alloc(tmem_slot, C::TMEM);
+    tmem_relinquish();
+  }
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
 
   if (warp < 4) {
-    if constexpr (C::SHIFT) regs_dec<C::R_ROLES>();
+    regs_dec<C::R_ROLES>();
     if (warp == 0) {
       pdl_wait();
       if (elect_one()) {
@@ -199,12 +279,13 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
         bool ok = true;
         for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
           const int m0 = (tile / a.tiles_n) * NX;
-          for (int kb = 2 * span.first; kb < 2 * span.end; kb += C::KB) {
+          for (int u = span.first * C::H; u < span.end * C::H; ++u) {
             if (!(ok = w4_wait(&empty[r.stage], r.phase ^ 1u, p.status))) break;
-            uint8_t* to = smem + r.stage * C::STAGE + C::A_BYTES;
+            uint8_t* to = smem + r.stage * C::B_BYTES;
+            const int k = u / C::H * kW4K, m = m0 + u % C::H * C::U;
             mbar_expect_tx(&full[r.stage], C::B_BYTES);
-#pragma unroll
-            for (int b = 0; b < C::KB; ++b) tma_load_2d(to + b * NX * 128, &tmX, (kb + b) * 64, m0, &full[r.stage]);
+            tma_load_2d(to, &tmX, k, m, &full[r.stage]);
+            tma_load_2d(to + C::B_BYTES / 2, &tmX, k + 64, m, &full[r.stage]);
             ++issued;
             r.next(C::STAGES);
           }
@@ -216,161 +297,184 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
       }
       __syncwarp();
     } else if (warp == 2) {
-      if (elect_one()) {
-        Ring r;
-        int issued = 0;
+      if (lane == 0) {  // (which issued the first)
         bool ok = true;
-        for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
-          const int rb = (tile % a.tiles_n) * 2, halves = rb + 1 < p.blocks ? 2 : 1;
-          for (int kt = span.first; kt < span.end; ++kt) {
-            if (!(ok = w4_wait(&cempty[r.stage], r.phase ^ 1u, p.status))) break;
-            mbar_expect_tx(&cfull[r.stage], halves * a.tile_bytes);
-            for (int h = 0; h < halves; ++h)
-              bulk_load(codes + r.stage * code_bytes + h * a.tile_bytes,
-                        p.tiles + ((int64_t)(rb + h) * p.tiles_k + kt) * a.tile_bytes, a.tile_bytes, &cfull[r.stage]);
-            ++issued;
-            r.next(a.code_stages);
-          }
-        }
+        while (next.tile < a.tiles && (ok = w4_wait(&cempty[next.r.stage], next.r.phase ^ 1u, p.status))) copy_codes();
         if (!ok)
-          for (int i = issued > a.code_stages ? issued - a.code_stages : 0; i < issued; ++i)
+          for (int i = next.issued - a.code_stages; i < next.issued; ++i)
             w4_wait(&cfull[i % a.code_stages], (i / a.code_stages) & 1, p.status);
       }
       __syncwarp();
-    } else if (warp == 1) {
-      pdl_wait();
-      tmem_alloc(tmem_slot, C::TMEM);
-      tmem_relinquish();
-      pdl_launch();
-      tc_fence_before();
-      named_sync(1, 32 + 128 * C::NA);
-      tc_fence_after();
-      const uint32_t tmem = *tmem_slot;
+    } else if (warp == 1 || kOne) {
+      if (warp == 1) pdl_launch();
       // The whole warp goes through the loop, so that descriptors and addresses stay in uniform registers; one lane issues.
-      constexpr uint32_t idesc = idesc_16(kM, NX, HALF);
-      // Operands' descriptors, stage 0: 32 bytes further for each 16 k, a block further for each 64, a stage for each stage.
-      const uint64_t adesc = sdesc_sw128(smem_u32(smem), 1024, 16), bdesc = sdesc_sw128(smem_u32(smem) + C::A_BYTES, 1024, 16);
-      constexpr int kStageSteps = 4 * C::KB;                                      // products of a stage
-      constexpr int kSteps = G / 16 < kStageSteps ? G / 16 : kStageSteps;  // of a group in it
-      Ring sr, dr;
-      bool ok = true;
-      for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step)
-        for (int kb = 2 * span.first; kb < 2 * span.end; kb += C::KB) {
-          if (!(ok = w4_wait_warp(&full[sr.stage], sr.phase, p.status))) break;
-          const uint64_t ad = adesc + sr.stage * (C::STAGE >> 4), bd = bdesc + sr.stage * (C::STAGE >> 4);
+      // With groups of 128 two warps take the halves (the tiles) in turn: one waits while the other's products run.  A wait
+      // for a stage's barrier cannot take the phase before for its own: the last one this warp saw complete needed an
+      // accumulator back that was filled from that phase or a later one.
+      constexpr int kIssuers = kOne ? 2 : 1;
+      const int me = kOne ? warp >> 1 : 0;
+      constexpr uint32_t idesc = idesc_16(kM, C::U, HALF);
+      // x's descriptor, stage 0: 32 bytes further for each 16 k, a block further for each 64, a stage for each stage.
+      const uint64_t bdesc = sdesc_sw128(smem_u32(smem), 1024, 16);
+      constexpr int kSteps = G / 16;  // products of a group
+      Ring sr, ar, dr;
+      sr.stage = dr.stage = me;
+      bool ok = true, x_ready = false, a_ready = false;
+      // this warp's first k tile, and how far the next one is
+      const int len = span.end - span.first, from = C::H == 1 ? me : 0, by = C::H == 1 ? kIssuers : 1;
+      const int tiles = (a.tiles - first_tile + tile_step - 1) / tile_step;
+      for (int64_t it = from, all = (int64_t)tiles * len; it < all; it += by) {
+        if (C::H == 2 && !(ok = w4_wait_warp(&afull[ar.stage], ar.phase, p.status, a_ready))) break;
 #pragma unroll
-          for (int j = 0; j < kStageSteps / kSteps; ++j) {
-            const bool fresh = C::KB == 2 || G < 128 || (kb & 1) == 0, last = C::KB == 2 || G < 128 || (kb & 1) != 0;
+        for (int h = 0; h < C::H; ++h) {
+          if (C::H == 2 && kOne && h != me) continue;
+          if (!(ok = w4_wait_warp(&full[sr.stage], sr.phase, p.status, x_ready))) break;
+          {
+            Ring then = sr;
+            then.next(C::STAGES, kIssuers);
+            x_ready = mbar_test(smem_u32(&full[then.stage]), then.phase);
+            if (C::H == 2) {
+              then = ar;
+              then.next(C::A_TILES);
+              a_ready = mbar_test(smem_u32(&afull[then.stage]), then.phase);
+            }
+          }
+          const uint64_t bd = bdesc + sr.stage * (C::B_BYTES >> 4);
+          const uint32_t ad = tmem + C::A_AT + (C::H == 2 ? ar.stage : sr.stage) * kACols;
+#pragma unroll
+          for (int j = 0; j < groups; ++j) {
             if (!kOne && !(ok = w4_wait_warp(&dempty[dr.stage], dr.phase ^ 1u, p.status))) break;
             tc_fence_after();
-            const uint32_t d = tmem + dr.stage * NX;
+            const uint32_t d = tmem + dr.stage * C::U;
             if (elect_one()) {
 #pragma unroll
               for (int i = 0; i < kSteps; ++i) {
                 const int k = j * kSteps + i;
-                umma_f16(d, ad + (k >> 2) * (kABlock >> 4) + (k & 3) * 2, bd + (k >> 2) * (NX * 128 >> 4) + (k & 3) * 2, idesc,
-                         i == 0 && fresh ? 0u : 1u);
+                umma_ts(d, ad + k * 8, bd + (k >> 2) * (C::B_BYTES / 2 >> 4) + (k & 3) * 2, idesc, i != 0);
               }
-              if (!kOne) umma_commit(&dfull[dr.stage]);
-              if (j == kStageSteps / kSteps - 1) umma_commit(&empty[sr.stage]);
+              if (!kOne) umma_commit(&dfull[h * C::ACCS + dr.stage]);
+              if (j == groups - 1) {
+                umma_commit(&empty[sr.stage]);
+                if (C::H == 2 && (kOne || h == 1)) umma_commit(&aempty[ar.stage]);
+              }
             }
             __syncwarp();
-            if (last) dr.next(2);
+            dr.next(C::ACCS, kIssuers);
           }
           if (!ok) break;
-          sr.next(C::STAGES);
+          sr.next(C::STAGES, kIssuers);
         }
-      if (!ok) {  // TMEM is not given back with a product under way
-        if (elect_one()) umma_commit(drain);
-        __syncwarp();
-        w4_wait_warp(drain, 0, p.status);
+        if (!ok) break;
+        ar.next(C::A_TILES);
       }
+      if (!ok) {  // TMEM is not given back with a product under way
+        if (elect_one()) umma_commit(&drain[me]);
+        __syncwarp();
+        w4_wait_warp(&drain[me], 0, p.status);
+      }
+      if (kOne && warp == 3) named_sync(3, 64);
+      if (kOne && warp == 1) named_sync(3, 64);
     }
     if (a.split > 1) cluster_pass();
     if (warp == 1) {
-      named_sync(1, 32 + 128 * C::NA);
+      named_sync(1, 32 + 128 * C::H);
       tc_fence_after();
-      tmem_dealloc(*tmem_slot, C::TMEM);
+      tmem_dealloc(tmem, C::TMEM);
     }
-  } else if (warp < 4 + kWiden) {
-    if constexpr (C::SHIFT) regs_dec<C::R_WIDEN>();
-    // The warpgroups take the stages in turn: with stages of 64 k each its half of every tile, else every other tile.
-    const int w = (warp - 4) & 3, mine = (warp - 4) >> 2, g = lane >> 2, t = lane & 3, odd = g & 1;
-    const int my_codes = (w * 64 + lane) * 16, my_zeros = kW4Codes + groups * 128 + g * 8 + w * 2;
-    const int my_row = (w * 16 + g) * 128, chunk0 = ((4 * odd + t) ^ g) << 4, chunk1 = ((4 * (1 - odd) + t) ^ g) << 4;
-    Ring cr, sr;
-    sr.stage = mine;
-    int slot = 0, turn = 0;
-    bool ok = true;
-    for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
-      const int halves = (tile % a.tiles_n) * 2 + 1 < p.blocks ? 2 : 1;
-      for (int kt = span.first; kt < span.end; ++kt) {
-        if (C::KB == 1 || turn == mine) {
-          if (!(ok = w4_wait_warp(&cfull[cr.stage], cr.phase, p.status))) break;
-          const uint8_t* in = codes + cr.stage * code_bytes;
-          // 16 rows x 64 k at a time; warp w has strip w of both halves.  Odd rows take (and write) their halves of the k in
-          // the other order, so that eight lanes' 16 bytes of the operand lie in eight groups of banks.
-          uint2 c[C::KB][2][2];
-          uint32_t z[C::KB][2][2];
-#pragma unroll
-          for (int b = 0; b < C::KB; ++b)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (h >= halves) break;
-              const uint8_t* src = in + h * a.tile_bytes;
-              const int kb = C::KB == 1 ? mine : b;
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                c[b][h][i] = *reinterpret_cast<const uint2*>(src + my_codes + kb * 512 + (i ^ odd) * 8);
-                z[b][h][i] = 0x0808;
-                if (a.zeros) {
-                  const int group = G == 32 ? kb * 2 + (i ^ odd) : kb * 64 / G;
-                  z[b][h][i] = *reinterpret_cast<const uint16_t*>(src + my_zeros + group * 64);
-                }
-              }
-            }
-          if (!(ok = w4_wait_warp(&empty[sr.stage], sr.phase ^ 1u, p.status))) break;
-          uint8_t* out = smem + sr.stage * C::STAGE + my_row;
-          // The scales move to a slot of their own.  The slot's last tile was SLOTS tiles ago, 2 more than the stages hold; the
-          // products of the tile that had this stage have ended (`empty`), so an accumulator was free when they began, so
-          // the sums of the group 2 before theirs, and of every tile at least 2 before, are taken.
-          if (C::KB == 2 || kW4K == G * 2 || mine == 0 || G < 64) {
-            // with stages of 64 k each warpgroup moves the groups that begin in its half
-            constexpr int kOwn = C::KB == 2 ? groups : (groups + 1) / 2;
-            const int from = C::KB == 1 ? mine * kOwn * 8 : 0;
-            const int i = w * 32 + lane, h = i / (kOwn * 8), j = i % (kOwn * 8);
-            if (h < halves)
-              reinterpret_cast<uint4*>(scales + slot * slot_bytes + h * groups * 128)[from + j] =
-                  reinterpret_cast<const uint4*>(in + h * a.tile_bytes + kW4Codes)[from + j];
-          }
-#pragma unroll
-          for (int b = 0; b < C::KB; ++b)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (h >= halves) break;
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t zlo = w4_zero<HALF>(z[b][h][i] & 255), zhi = w4_zero<HALF>(z[b][h][i] >> 8);
-                uint32_t x[4], y[4];
-                w4_widen<HALF>(c[b][h][i].x, zlo, zhi, x);
-                w4_widen<HALF>(c[b][h][i].y, zlo, zhi, y);
-                const int chunk = b * kABlock + h * 64 * 128 + (i ? chunk1 : chunk0);
-                *reinterpret_cast<uint4*>(out + chunk) = make_uint4(x[0], x[2], y[0], y[2]);
-                *reinterpret_cast<uint4*>(out + 8 * 128 + chunk) = make_uint4(x[1], x[3], y[1], y[3]);
-              }
-            }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&full[sr.stage]);
-            mbar_arrive(&cempty[cr.stage]);
-          }
-          sr.next(C::STAGES, 2);
-        }
-        turn ^= 1;
-        cr.next(a.code_stages);
-        if (++slot == C::SLOTS) slot = 0;
+  } else if (warp < 4 + C::WIDEN) {
+    regs_dec<C::R_WIDEN>();
+    // The warpgroups take the tiles in turn; warp w has lanes 32 w .. 32 w + 31 of TMEM: strips 2 w and 2 w + 1 of the 128 rows.
+    const int w = (warp - 4) & 3, mine = (warp - 4) >> 2, g = lane >> 2, half = w >> 1;
+    const int my_codes = half * a.tile_bytes + (w & 1) * 2048 + lane * 16;
+    const int my_zeros = half * a.tile_bytes + kW4Codes + groups * 128 + g * 8 + (w & 1) * 4;
+    const uint32_t to = tmem + C::A_AT + ((uint32_t)(w * 32) << 16);
+    uint64_t* free_a = C::H == 2 ? aempty : empty;
+    uint64_t* told = C::H == 2 ? afull : full;
+    Ring cr, ar;
+    int slot = mine % C::SLOTS, tile = first_tile, kt = span.first;
+    auto go_on = [&](int n) {  // n k tiles further
+      kt += n;
+      while (kt >= span.end) {
+        kt -= span.end - span.first;
+        tile += tile_step;
       }
+    };
+    go_on(mine);
+    for (int i = 0; i < mine; ++i) {
+      cr.next(a.code_stages);
+      ar.next(C::A_TILES);
+    }
+    auto next_c = [&](Ring& r) { r.next(a.code_stages, C::TURNS); };
+    auto next_a = [&](Ring& r) { r.next(C::A_TILES, C::TURNS); };
+    bool ok = true, c_ready = false, a_ready = false;
+    for (; tile < a.tiles; go_on(C::TURNS)) {
+      const int halves = (tile % a.tiles_n) * 2 + 1 < p.blocks ? 2 : 1;
+      if (!(ok = w4_wait_warp(&cfull[cr.stage], cr.phase, p.status, c_ready))) break;
+      const uint8_t* in = codes + cr.stage * code_bytes;
+      // Read before it is widened, where there are registers for it: a strip of 16 rows x 64 k is 16 bytes of a lane.
+      constexpr bool kAhead = NX != 256;
+      uint4 c[2][2];
+      uint32_t z[2][groups];
+      if (half < halves) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            if (kAhead) c[s][b] = *reinterpret_cast<const uint4*>(in + my_codes + s * 1024 + b * 512);
+#pragma unroll
+          for (int i = 0; i < groups; ++i)
+            z[s][i] = a.zeros ? *reinterpret_cast<const uint16_t*>(in + my_zeros + s * 2 + i * 64) : 0x0808;
+        }
+      }
+      if (!(ok = w4_wait_warp(&free_a[ar.stage], ar.phase ^ 1u, p.status, a_ready))) break;
+      tc_fence_after();
+      {  // a look at what this warpgroup's next tile waits for
+        Ring then = cr;
+        next_c(then);
+        c_ready = mbar_test(smem_u32(&cfull[then.stage]), then.phase);
+        then = ar;
+        next_a(then);
+        a_ready = mbar_test(smem_u32(&free_a[then.stage]), then.phase ^ 1u);
+      }
+      // The scales move to a slot of their own.  The slot's last tile was SLOTS = A_TILES + 2 tiles ago; the products of the
+      // tile that had this place have ended, so an accumulator was free when the last of them began, so the
+      // sums of every tile at least 2 before it are taken.
+      {
+        const int i = w * 32 + lane, h = i / (groups * 8), j = i % (groups * 8);
+        if (h < halves)
+          reinterpret_cast<uint4*>(scales + slot * slot_bytes + h * groups * 128)[j] =
+              reinterpret_cast<const uint4*>(in + h * a.tile_bytes + kW4Codes)[j];
+      }
+      if (half < halves) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            if (!kAhead) c[s][b] = *reinterpret_cast<const uint4*>(in + my_codes + s * 1024 + b * 512);
+            uint32_t v[16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t zz = z[s][(b * 64 + j * 16) / G];
+              uint32_t x[4];
+              w4_widen<HALF>((&c[s][b].x)[j], w4_zero<HALF>(zz & 255), w4_zero<HALF>(zz >> 8), x);
+              v[4 * j] = x[0];  // row g, k and k + 2; row g + 8
+              v[4 * j + 1] = x[2];
+              v[4 * j + 2] = x[1];
+              v[4 * j + 3] = x[3];
+            }
+            tmem_st_frags(to + ar.stage * kACols + ((uint32_t)(s * 16) << 16) + b * 32, v);
+          }
+        tmem_st_wait();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&told[ar.stage]);
+        mbar_arrive(&cempty[cr.stage]);
+      }
+      next_a(ar);
+      next_c(cr);
+      if ((slot += C::TURNS) >= C::SLOTS) slot -= C::SLOTS;
     }
     if (a.split > 1) {
       if constexpr (NX == 256) {
@@ -379,91 +483,111 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
         __syncwarp();
         cluster_arrive();
         cluster_wait();
-        finish_cluster<HALF, NX>(a, smem, first_tile, rank, threadIdx.x - 128, 128 * (2 + C::NA));
+        finish_cluster<HALF, NX>(a, smem, first_tile, rank, threadIdx.x - 128, 128 * (C::TURNS + C::H));
         __syncwarp();
         cluster_arrive();
         cluster_wait();
       }
     }
   } else {
-    if constexpr (C::SHIFT) regs_inc<C::R_SUM>();
-    const int w = warp - 4 - kWiden, part = w >> 2, r = (warp & 3) * 32 + lane;  // row of W in the tile
-    if (kOne && lane == 0) {  // both accumulators are free
-      mbar_arrive(&full[0]);
-      mbar_arrive(&full[kPerTile]);
+    regs_inc<C::R_SUM>();
+    const int w = warp - 4 - C::WIDEN, part = w >> 2, r = (warp & 3) * 32 + lane;  // half of the tile, row of W in it
+    // kOne: a half's accumulator is full when its products have ended, and is free for the one ACCS halves later, whose
+    // barrier is told; the first ACCS have theirs from the start (from the warpgroup whose turn it would have been).
+    if (kOne && lane == 0) {
+#pragma unroll
+      for (int u = 0; u < C::ACCS; ++u)
+        if ((u + C::ACCS) % C::H == part) mbar_arrive(&full[u]);
     }
     pdl_wait();
-    named_sync(1, 32 + 128 * C::NA);
-    tc_fence_after();
-    const uint32_t taddr = *tmem_slot + ((uint32_t)((warp & 3) * 32) << 16) + part * C::CA;
+    const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint16_t* my_scales = reinterpret_cast<const uint16_t*>(scales + (r >> 6) * groups * 128) + w4_place(r & 63);
-    // kOne: a tile's accumulator is full when its last stage's products have ended, and free for the tile 2 later, whose
-    // first stage's barrier is told.
     Ring dr, er;
-    er.stage = kPerTile - 1;
-    int tell = 2 * kPerTile % C::STAGES, slot = 0;
+    er.stage = part;
+    dr.stage = part * groups % C::ACCS;
+    uint32_t dphase = 0;  // a bit for each accumulator: the next phase of this warpgroup's barrier
+    int tell = (part + C::ACCS) % C::STAGES, slot = 0;
     auto give_back = [&](int d) {  // accumulator d has been taken
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(kOne ? &full[tell] : &dempty[d]);
-      if ((tell += kPerTile) >= C::STAGES) tell -= C::STAGES;
+      if ((tell += C::H) >= C::STAGES) tell -= C::STAGES;
     };
-    bool ok = true;
+    bool ok = true, ready = false;
     for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
-      const int m0 = (tile / a.tiles_n) * NX + part * C::CA;
+      const int m0 = (tile / a.tiles_n) * NX + part * C::U;
       const int64_t packed = (int64_t)(tile % a.tiles_n) * kM + r;  // row of the packed weight
-      float acc[C::CA];
+      float acc[C::U];
       int held = 0;  // the last group's accumulator
 #pragma unroll
-      for (int c = 0; c < C::CA; ++c) acc[c] = 0.f;
+      for (int c = 0; c < C::U; ++c) acc[c] = 0.f;
       for (int kt = span.first; kt < span.end && ok; ++kt) {
         for (int gr = 0; gr < groups; ++gr) {
+          // (with a look at the next one's barrier)
           if (kOne) {
-            if (!(ok = w4_wait_warp(&empty[er.stage], er.phase, p.status))) break;
-            er.next(C::STAGES, kPerTile);
+            if (!(ok = w4_wait_warp(&empty[er.stage], er.phase, p.status, ready))) break;
+            er.next(C::STAGES, C::H);
+            ready = mbar_test(smem_u32(&empty[er.stage]), er.phase);
           } else {
-            if (!(ok = w4_wait_warp(&dfull[dr.stage], dr.phase, p.status))) break;
+            if (!(ok = w4_wait_warp(&dfull[part * C::ACCS + dr.stage], dphase >> dr.stage & 1, p.status, ready))) break;
+            dphase ^= 1u << dr.stage;
+            Ring then = dr;
+            then.next(C::ACCS);
+            ready = (C::H == 1 || gr + 1 < groups) &&
+                    mbar_test(smem_u32(&dfull[part * C::ACCS + then.stage]), dphase >> then.stage & 1);
           }
           tc_fence_after();
           const float s = w4_scale(my_scales[slot * (slot_bytes / 2) + gr * 64], p.scale_half);
           const float2 s2 = make_float2(s, s);
+          constexpr int kLoad = C::U == 64 ? 64 : 32;
 #pragma unroll
-          for (int c = 0; c < C::CA; c += 32) {
-            float v[32];
-            tmem_ld32(taddr + dr.stage * NX + c, v);
+          for (int c = 0; c < C::U; c += kLoad) {
+            float v[kLoad];
+            if constexpr (kLoad == 64) {
+              uint32_t raw[2][32];  // (one instruction for 64 would need more registers than the kernel begins with)
+              tmem_ld32_nowait(taddr + dr.stage * C::U, raw[0]);
+              tmem_ld32_nowait(taddr + dr.stage * C::U + 32, raw[1]);
+              tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
+              for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(raw[i / 32][i % 32]);
+            } else {
+              tmem_ld32(taddr + dr.stage * C::U + c, v);
+            }
+#pragma unroll
+            for (int i = 0; i < kLoad; i += 2) {
               const float2 q = fma2(s2, make_float2(v[i], v[i + 1]), make_float2(acc[c + i], acc[c + i + 1]));
               acc[c + i] = q.x;
               acc[c + i + 1] = q.y;
             }
           }
           held = dr.stage;
-          if (kt + 1 < span.end || gr + 1 < groups) give_back(held);
-          dr.next(2);
+          if (a.split > 1 || kt + 1 < span.end || gr + 1 < groups) give_back(held);
+          // (the other half's groups lie between two tiles of this one)
+          dr.next(C::ACCS);
+          if (C::H == 2 && gr + 1 == groups) {
+#pragma unroll
+            for (int i = 0; i < groups; ++i) dr.next(C::ACCS);
+          }
         }
         if (++slot == C::SLOTS) slot = 0;
+      }
+      const int cols = min(C::U, p.rows - m0);
+      if (a.split > 1) {  // one tile a cluster
+        // [column][row] in the stages' place: every product and copy of this block is complete (of both halves, once both
+        // warpgroups are here; each comes, also where a wait gave up, and waits for nothing that the other has to give).
+        if (C::H == 2) named_sync(2, 128 * C::H);
+        float* sums = reinterpret_cast<float*>(smem) + part * C::U * kM + r;
+#pragma unroll
+        for (int c = 0; c < C::U; ++c) sums[c * kM] = acc[c];
+        break;
       }
       if (!ok) break;
       // The sums go into the accumulator taken last and come back a few columns at a time: what follows is a short loop
       // then, where all columns in a row would be ten thousand bytes of code that no instruction cache has in time.
-      const uint32_t own = taddr + held * NX;
+      const uint32_t own = taddr + held * C::U;
 #pragma unroll
-      for (int c = 0; c < C::CA; c += 32) tmem_st32(own + c, acc + c);
+      for (int c = 0; c < C::U; c += 32) tmem_st32(own + c, acc + c);
       tmem_st_wait();
-      const int cols = min(C::CA, p.rows - m0);
-      if (a.split > 1) {
-        // [column][row] in the stages' place: every product and copy of this block is complete.
-        float* sums = reinterpret_cast<float*>(smem) + part * C::CA * kM + r;
-#pragma unroll 1
-        for (int c0 = 0; c0 < C::CA; c0 += kChunk) {
-          float v[kChunk];
-          tmem_ld16(own + c0, v);
-#pragma unroll
-          for (int c = 0; c < kChunk; ++c) sums[(c0 + c) * kM] = v[c];
-        }
-        break;  // one tile a cluster
-      }
       uint16_t* out = static_cast<uint16_t*>(p.out) + (int64_t)m0 * p.n;
       if (!a.gated) {
         const bool in = packed < p.n;
@@ -477,9 +601,9 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
 #pragma unroll
         for (int c = 0; c < kChunk; ++c) next[c] = res && c < count ? res[(int64_t)c * p.res_ld] : (uint16_t)0;
 #pragma unroll 1
-        for (int c0 = 0; c0 < C::CA; c0 += kChunk) {
+        for (int c0 = 0; c0 < C::U; c0 += kChunk) {
           float v[kChunk];
-          tmem_ld16(own + c0, v);
+          tmem_ld8(own + c0, v);
           if (res) {
             res += kChunk * p.res_ld;
 #pragma unroll
@@ -500,9 +624,9 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
         out += n + (up ? p.n : 0);
         const int count = n < p.n ? cols - (up ? 1 : 0) : 0;
 #pragma unroll 1
-        for (int c0 = 0; c0 < C::CA; c0 += kChunk) {
+        for (int c0 = 0; c0 < C::U; c0 += kChunk) {
           float v[kChunk];
-          tmem_ld16(own + c0, v);
+          tmem_ld8(own + c0, v);
 #pragma unroll
           for (int c = 0; c < kChunk; c += 2) {
             const float other = __shfl_xor_sync(0xffffffffu, up ? v[c] : v[c + 1], 8);
@@ -517,14 +641,14 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
       __syncwarp();
       cluster_arrive();
       cluster_wait();
-      constexpr int kThreads = NX == 256 ? 128 * C::NA : 128 * (2 + C::NA);  // the widening warps help where they have registers
+      constexpr int kThreads = NX == 256 ? 128 * C::H : 128 * (C::TURNS + C::H);  // the widening warps help where they have registers
       finish_cluster<HALF, NX>(a, smem, first_tile, rank, (int)threadIdx.x - (C::THREADS - kThreads), kThreads);
       __syncwarp();
       cluster_arrive();  // no block leaves while another reads its sums
       cluster_wait();
     }
     tc_fence_before();
-    named_sync(1, 32 + 128 * C::NA);
+    named_sync(1, 32 + 128 * C::H);
   }
 }
 
@@ -542,10 +666,10 @@ cudaError_t launch(const W4Dev& p, bool zeros, bool gated, int split, cudaStream
   a.tiles = (int)tiles;
   a.split = split;
   CUtensorMap map;
-  if (!make_tmap_2d(&map, p.x, 2, p.rows, p.k, (uint64_t)p.x_ld * 2, NX, 64)) return cudaErrorInvalidValue;
-  // as many packed tiles under way as there is room for
+  if (!make_tmap_2d(&map, p.x, 2, p.rows, p.k, (uint64_t)p.x_ld * 2, C::U, 64)) return cudaErrorInvalidValue;
+  // as many packed tiles under way as there is room for, in whole turns: so each has its warpgroup, which sees all its phases
   const int fixed = (C::fixed(G) + 127) / 128 * 128, room = (kMaxSmem - fixed) / (2 * a.tile_bytes);
-  a.code_stages = room < kMaxCodes ? room : kMaxCodes;
+  a.code_stages = (room < kMaxCodes ? room : kMaxCodes) / C::TURNS * C::TURNS;
   const int smem = fixed + a.code_stages * 2 * a.tile_bytes;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = smem_attr_once(k_w4_many<HALF, NX, G>, kMaxSmem, done);
