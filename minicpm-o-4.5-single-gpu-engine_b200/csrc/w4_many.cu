@@ -2,18 +2,19 @@
 // accumulator for each group of k, scaled and summed in registers.
 //
 // A persistent block an SM takes tiles of 128 k, each in H halves of U = NX / H rows of x:
-//   warp 0       x: TMA, 128-byte swizzle, one stage (128 k x U rows) for each half
-//   warp 1       TMEM, and tcgen05.mma from one lane (M = 128, N = U, K = 16), A from TMEM
-//   warp 2       packed tiles of W (128 rows x 128 k), bulk copies into a ring of their own
-//   2 x 4 warps  widen codes to whole 16-bit numbers and store them in TMEM, where they are the A operand; the warpgroups take
-//                the tiles in turn
+//   warps 0, 2   x: TMA, 128-byte swizzle, one stage (128 k x U rows) for each half, in turn (with NX = 256 warp 0 alone)
+//   warps 1, 3   TMEM, and tcgen05.mma from one lane (M = 128, N = U, K = 16), A from TMEM
+//   2 or 4 x 4   warps widen codes to whole 16-bit numbers and store them in TMEM, where they are the A operand; the
+//                warpgroups take the tiles in turn, and the first lane of each copies its packed tiles, 128 rows x 128 k (with
+//                NX = 256, where widening has no registers to spare, warp 2 does: 461 us for 505 in the largest case measured)
 //   H x 4 warps  take a group's accumulator out of TMEM (a few take turns), each lane one row of W: acc += scale * sum, so the
 //                scale is a register and no weight is rounded; at a tile's end they write the outputs
 //
 // The weights go through TMEM because shared memory is what such a kernel runs out of: 128 bytes a clock, of which 128 k of
 // widened weights would take 256 clocks to write and 256 to read, where the products take 4 NX clocks.
 // What a hand-over costs decides the rest: passing an mbarrier that is ready takes about 100 clocks, a commit 80, the
-// issue of 4 products 65.  So with groups of 128 one barrier tells the products' warp what a half waits for (x and a free
+// issue of 4 products 65, a round of waiting, expecting and two copies 650 (one thread brings 23 GB/s in pieces of 4 KB).  So
+// copies and products are issued by several warps in turn, and with groups of 128 one barrier tells the products' warp what a half waits for (x and a free
 // accumulator; the weights too where there is one half), and one commit tells that its stage is free and its accumulator full.
 // With few tiles k is split over a cluster, whose blocks add their sums through distributed shared memory in a fixed order.
 // The first tiles of W come before the kernel waits for the one ahead of it in the stream.  No TMA multicast.
@@ -44,12 +45,13 @@ struct Cfg {
   static constexpr int SLOTS = A_TILES + 2;                         // tiles whose scales are kept (see the widening warps)
   static constexpr int A_AT = ACCS * U;                             // TMEM column of the first widened tile
   static constexpr int TMEM = 512;
+  static constexpr bool LEADS = NX != 256;  // widening warpgroups copy their packed tiles
   static_assert(A_AT + A_TILES * kACols <= TMEM, "tensor memory");
   static_assert(H == 2 || A_TILES == STAGES, "one barrier for both operands");
   // Registers: the sums need more than an even split has, which the other warps give.  The sum of the warpgroups' shares is at
   // most what the kernel is launched with: 96 each of 640 threads, 80 each of 768.
   static constexpr int LAUNCH = NX == 256 ? 96 : 80;
-  static constexpr int R_ROLES = NX == 256 ? 48 : 56, R_WIDEN = NX == 256 ? 48 : 64, R_SUM = 168;
+  static constexpr int R_ROLES = 48, R_WIDEN = NX == 256 ? 48 : NX == 128 ? 64 : 72, R_SUM = NX == 256 ? 168 : NX == 128 ? 176 : 144;
   static_assert(R_ROLES + TURNS * R_WIDEN + H * R_SUM <= (1 + TURNS + H) * LAUNCH, "registers");
   static constexpr int fixed(int group) {  // shared memory besides the ring of packed tiles
     return STAGES * B_BYTES + SLOTS * (kW4K / group) * 256 + 8 * (2 * STAGES + 2 * A_TILES + 2 * kMaxCodes + (H + 1) * ACCS + 2) + 16;
@@ -232,31 +234,38 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
     fence_mbar_init();
     tma_prefetch_desc(&tmX);
   }
-  // Packed tiles: one lane of warp 2 issues their copies, the first ones before anything is waited for.
-  struct {
-    int tile, kt, issued;
-    Ring r;
-  } next = {first_tile, span.first, 0, {}};
-  auto copy_codes = [&]() {
-    const int rb = (next.tile % a.tiles_n) * 2, halves = rb + 1 < p.blocks ? 2 : 1;
-    mbar_expect_tx(&cfull[next.r.stage], halves * a.tile_bytes);
-    for (int h = 0; h < halves; ++h)
-      bulk_load(codes + next.r.stage * code_bytes + h * a.tile_bytes,
-                p.tiles + ((int64_t)(rb + h) * p.tiles_k + next.kt) * a.tile_bytes, a.tile_bytes, &cfull[next.r.stage]);
-    ++next.issued;
-    next.r.next(a.code_stages);
-    if (++next.kt == span.end) {
-      next.kt = span.first;
-      next.tile += tile_step;
+  // Packed tiles are copied by a widening warpgroup's first lane for that group, or by one lane for all; as many as there is
+  // room for before anything is waited for.
+  const int len = span.end - span.first, my_turn = (warp - 4) >> 2;
+  auto further = [&](int& tile, int& kt, int n) {  // n k tiles on
+    kt += n;
+    while (kt >= span.end) {
+      kt -= len;
+      tile += tile_step;
     }
   };
-  if (threadIdx.x == 64) {
-    for (int s = 0; s < a.code_stages; ++s) {
+  auto copy_codes = [&](int tile, int kt, int stage) {
+    const int rb = (tile % a.tiles_n) * 2, halves = rb + 1 < p.blocks ? 2 : 1;
+    mbar_expect_tx(&cfull[stage], halves * a.tile_bytes);
+    for (int h = 0; h < halves; ++h)
+      bulk_load(codes + stage * code_bytes + h * a.tile_bytes, p.tiles + ((int64_t)(rb + h) * p.tiles_k + kt) * a.tile_bytes,
+                a.tile_bytes, &cfull[stage]);
+  };
+  const bool leads = C::LEADS && warp >= 4 && warp < 4 + C::WIDEN && (threadIdx.x & 127) == 0;
+  constexpr int kCopyStep = C::LEADS ? C::TURNS : 1;
+  if (C::LEADS ? leads : threadIdx.x == 64) {
+    const int from = C::LEADS ? my_turn : 0;
+    for (int s = from; s < a.code_stages; s += kCopyStep) {
       mbar_init(&cfull[s], 1);
       mbar_init(&cempty[s], 4);
     }
     fence_mbar_init();
-    for (int s = 0; s < a.code_stages && next.tile < a.tiles; ++s) copy_codes();
+    int tile = first_tile, kt = span.first;
+    further(tile, kt, from);
+    for (int s = from; s < a.code_stages && tile < a.tiles; s += kCopyStep) {
+      copy_codes(tile, kt, s);
+      further(tile, kt, kCopyStep);
+    }
   }
   __syncwarp();
   if (warp == 1) {
@@ -271,38 +280,48 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
 
   if (warp < 4) {
     regs_dec<C::R_ROLES>();
-    if (warp == 0) {
+    if (!C::LEADS && warp == 2) {
+      if (lane == 0) {  // (which copied the first)
+        Ring r;
+        int tile = first_tile, kt = span.first, t = tile, k = kt;
+        further(t, k, a.code_stages);
+        bool ok = true;
+        for (; t < a.tiles && (ok = w4_wait(&cempty[r.stage], r.phase, p.status)); r.next(a.code_stages)) {
+          copy_codes(t, k, r.stage);
+          further(t, k, 1);
+        }
+        if (!ok)  // the stages from this one on are under way, or long since full
+          for (int i = 0; i < a.code_stages; ++i, r.next(a.code_stages)) w4_wait(&cfull[r.stage], r.phase, p.status);
+      }
+      __syncwarp();
+    } else if ((warp & 1) == 0) {
       pdl_wait();
       if (elect_one()) {
+        constexpr int kBy = C::LEADS ? 2 : 1;
+        const int me = warp >> 1;
         Ring r;
-        int issued = 0;
+        r.stage = me;
+        int issued = 0, unit = me;  // halves of the block's tiles of 128 k
         bool ok = true;
-        for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
+        for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, unit -= len * C::H) {
           const int m0 = (tile / a.tiles_n) * NX;
-          for (int u = span.first * C::H; u < span.end * C::H; ++u) {
+          for (; unit < len * C::H; unit += kBy) {
             if (!(ok = w4_wait(&empty[r.stage], r.phase ^ 1u, p.status))) break;
             uint8_t* to = smem + r.stage * C::B_BYTES;
-            const int k = u / C::H * kW4K, m = m0 + u % C::H * C::U;
+            const int k = (span.first + unit / C::H) * kW4K, m = m0 + unit % C::H * C::U;
             mbar_expect_tx(&full[r.stage], C::B_BYTES);
             tma_load_2d(to, &tmX, k, m, &full[r.stage]);
             tma_load_2d(to + C::B_BYTES / 2, &tmX, k + 64, m, &full[r.stage]);
             ++issued;
-            r.next(C::STAGES);
+            r.next(C::STAGES, kBy);
           }
         }
         // The block does not end, nor is its shared memory used for sums, with a copy under way (where a wait gave up).
         if (!ok)
-          for (int i = issued > C::STAGES ? issued - C::STAGES : 0; i < issued; ++i)
-            w4_wait(&full[i % C::STAGES], (i / C::STAGES) & 1, p.status);
-      }
-      __syncwarp();
-    } else if (warp == 2) {
-      if (lane == 0) {  // (which issued the first)
-        bool ok = true;
-        while (next.tile < a.tiles && (ok = w4_wait(&cempty[next.r.stage], next.r.phase ^ 1u, p.status))) copy_codes();
-        if (!ok)
-          for (int i = next.issued - a.code_stages; i < next.issued; ++i)
-            w4_wait(&cfull[i % a.code_stages], (i / a.code_stages) & 1, p.status);
+          for (int i = issued > C::STAGES ? issued - C::STAGES : 0; i < issued; ++i) {
+            const int u = me + kBy * i;
+            w4_wait(&full[u % C::STAGES], (u / C::STAGES) & 1, p.status);
+          }
       }
       __syncwarp();
     } else if (warp == 1 || kOne) {
@@ -321,7 +340,7 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
       sr.stage = dr.stage = me;
       bool ok = true, x_ready = false, a_ready = false;
       // this warp's first k tile, and how far the next one is
-      const int len = span.end - span.first, from = C::H == 1 ? me : 0, by = C::H == 1 ? kIssuers : 1;
+      const int from = C::H == 1 ? me : 0, by = C::H == 1 ? kIssuers : 1;
       const int tiles = (a.tiles - first_tile + tile_step - 1) / tile_step;
       for (int64_t it = from, all = (int64_t)tiles * len; it < all; it += by) {
         if (C::H == 2 && !(ok = w4_wait_warp(&afull[ar.stage], ar.phase, p.status, a_ready))) break;
@@ -384,7 +403,7 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
   } else if (warp < 4 + C::WIDEN) {
     regs_dec<C::R_WIDEN>();
     // The warpgroups take the tiles in turn; warp w has lanes 32 w .. 32 w + 31 of TMEM: strips 2 w and 2 w + 1 of the 128 rows.
-    const int w = (warp - 4) & 3, mine = (warp - 4) >> 2, g = lane >> 2, half = w >> 1;
+    const int w = (warp - 4) & 3, mine = my_turn, g = lane >> 2, half = w >> 1;
     const int my_codes = half * a.tile_bytes + (w & 1) * 2048 + lane * 16;
     const int my_zeros = half * a.tile_bytes + kW4Codes + groups * 128 + g * 8 + (w & 1) * 4;
     const uint32_t to = tmem + C::A_AT + ((uint32_t)(w * 32) << 16);
@@ -392,14 +411,7 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
     uint64_t* told = C::H == 2 ? afull : full;
     Ring cr, ar;
     int slot = mine % C::SLOTS, tile = first_tile, kt = span.first;
-    auto go_on = [&](int n) {  // n k tiles further
-      kt += n;
-      while (kt >= span.end) {
-        kt -= span.end - span.first;
-        tile += tile_step;
-      }
-    };
-    go_on(mine);
+    further(tile, kt, mine);
     for (int i = 0; i < mine; ++i) {
       cr.next(a.code_stages);
       ar.next(C::A_TILES);
@@ -407,7 +419,7 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
     auto next_c = [&](Ring& r) { r.next(a.code_stages, C::TURNS); };
     auto next_a = [&](Ring& r) { r.next(C::A_TILES, C::TURNS); };
     bool ok = true, c_ready = false, a_ready = false;
-    for (; tile < a.tiles; go_on(C::TURNS)) {
+    for (; tile < a.tiles; further(tile, kt, C::TURNS)) {
       const int halves = (tile % a.tiles_n) * 2 + 1 < p.blocks ? 2 : 1;
       if (!(ok = w4_wait_warp(&cfull[cr.stage], cr.phase, p.status, c_ready))) break;
       const uint8_t* in = codes + cr.stage * code_bytes;
@@ -445,6 +457,10 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
           reinterpret_cast<uint4*>(scales + slot * slot_bytes + h * groups * 128)[j] =
               reinterpret_cast<const uint4*>(in + h * a.tile_bytes + kW4Codes)[j];
       }
+      if (kAhead) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&cempty[cr.stage]);
+      }
       if (half < halves) {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -470,12 +486,22 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&told[ar.stage]);
-        mbar_arrive(&cempty[cr.stage]);
+        if (!kAhead) mbar_arrive(&cempty[cr.stage]);
       }
+      if (C::LEADS && leads) {  // the tile's place is filled again once all four warps have read it
+        int t = tile, k = kt;
+        further(t, k, a.code_stages);
+        if (t < a.tiles && (ok = w4_wait(&cempty[cr.stage], cr.phase, p.status))) copy_codes(t, k, cr.stage);
+      }
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
       next_a(ar);
       next_c(cr);
       if ((slot += C::TURNS) >= C::SLOTS) slot -= C::SLOTS;
     }
+    if (C::LEADS && !ok && leads)  // no copy is under way when the block ends (where a wait gave up)
+      for (int i = 0; i < a.code_stages && tile < a.tiles; i += C::TURNS, next_c(cr), further(tile, kt, C::TURNS))
+        w4_wait(&cfull[cr.stage], cr.phase, p.status);
+    __syncwarp();
     if (a.split > 1) {
       if constexpr (NX == 256) {
         cluster_pass();
@@ -670,6 +696,7 @@ cudaError_t launch(const W4Dev& p, bool zeros, bool gated, int split, cudaStream
   // as many packed tiles under way as there is room for, in whole turns: so each has its warpgroup, which sees all its phases
   const int fixed = (C::fixed(G) + 127) / 128 * 128, room = (kMaxSmem - fixed) / (2 * a.tile_bytes);
   a.code_stages = (room < kMaxCodes ? room : kMaxCodes) / C::TURNS * C::TURNS;
+  if (a.code_stages < 2 * C::TURNS) return cudaErrorInvalidValue;
   const int smem = fixed + a.code_stages * 2 * a.tile_bytes;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = smem_attr_once(k_w4_many<HALF, NX, G>, kMaxSmem, done);
