@@ -54,7 +54,7 @@ struct Cfg {
   static constexpr int R_ROLES = 48, R_WIDEN = NX == 256 ? 48 : NX == 128 ? 64 : 72, R_SUM = NX == 256 ? 168 : NX == 128 ? 176 : 144;
   static_assert(R_ROLES + TURNS * R_WIDEN + H * R_SUM <= (1 + TURNS + H) * LAUNCH, "registers");
   static constexpr int fixed(int group) {  // shared memory besides the ring of packed tiles
-    return STAGES * B_BYTES + SLOTS * (kW4K / group) * 256 + 8 * (2 * STAGES + 2 * A_TILES + 2 * kMaxCodes + (H + 1) * ACCS + 2) + 16;
+    return STAGES * B_BYTES + SLOTS * (kW4K / group) * 256 + 8 * (2 * STAGES + 2 * A_TILES + 2 * kMaxCodes + H * ACCS + 2 * ACCS + 2) + 16;
   }
 };
 
@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
   constexpr int groups = kW4K / G, slot_bytes = groups * 2 * 128;
   // One barrier for what a half's products wait for, and one commit for all that wait for them: where a group is a tile.
   constexpr bool kOne = G == kW4K;
+  constexpr int kFree = 2 * C::ACCS;  // barriers that tell of a free accumulator, taken in turn (see the issuing warps)
   const int code_bytes = 2 * a.tile_bytes;
   uint8_t* scales = smem + C::STAGES * C::B_BYTES;  // [slot][half][group][64]
   uint64_t* full = reinterpret_cast<uint64_t*>(scales + C::SLOTS * slot_bytes);  // x of a half (and with H = 1 the weights)
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
   uint64_t* cempty = cfull + kMaxCodes;
   uint64_t* dfull = cempty + kMaxCodes;  // (not kOne) [half][accumulator]: a warpgroup waits for its own phases alone
   uint64_t* dempty = dfull + C::H * C::ACCS;
-  uint64_t* drain = dempty + C::ACCS;
+  uint64_t* drain = dempty + kFree;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   uint8_t* codes = smem + (C::fixed(G) + 127) / 128 * 128;
 
@@ -223,11 +224,12 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
     }
     for (int s = 0; s < C::A_TILES; ++s) {
       mbar_init(&afull[s], 4);
-      mbar_init(&aempty[s], kOne ? C::H : 1);  // a commit of each warp that issued its products
+      mbar_init(&aempty[s], C::H);  // a commit of each warp that issued its products
     }
     for (int s = 0; s < C::ACCS; ++s) {
       for (int h = 0; h < C::H; ++h) mbar_init(&dfull[h * C::ACCS + s], 1);
       mbar_init(&dempty[s], 4);
+      mbar_init(&dempty[C::ACCS + s], 4);
     }
     mbar_init(&drain[0], 1);
     mbar_init(&drain[1], 1);
@@ -324,65 +326,64 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
           }
       }
       __syncwarp();
-    } else if (warp == 1 || kOne) {
+    } else if (warp == 1 || C::H == 2 || kOne) {
       if (warp == 1) pdl_launch();
       // The whole warp goes through the loop, so that descriptors and addresses stay in uniform registers; one lane issues.
-      // With groups of 128 two warps take the halves (the tiles) in turn: one waits while the other's products run.  A wait
-      // for a stage's barrier cannot take the phase before for its own: the last one this warp saw complete needed an
-      // accumulator back that was filled from that phase or a later one.
-      constexpr int kIssuers = kOne ? 2 : 1;
-      const int me = kOne ? warp >> 1 : 0;
+      // Two warps take the halves in turn (with one half and groups of 128 the tiles): one waits while the other's products
+      // run.  Groups are numbered in the order (tile, group, half); number v has accumulator v % ACCS, free once v - ACCS has
+      // been taken, which barrier v % kFree tells (with kOne the half's own).  A wait cannot take a phase before for its own:
+      // the last number this warp issued needed one back that was filled later than what the barrier told before.
+      constexpr int kIssuers = C::H == 2 || kOne ? 2 : 1;
+      const int me = kIssuers == 2 ? warp >> 1 : 0;
       constexpr uint32_t idesc = idesc_16(kM, C::U, HALF);
       // x's descriptor, stage 0: 32 bytes further for each 16 k, a block further for each 64, a stage for each stage.
       const uint64_t bdesc = sdesc_sw128(smem_u32(smem), 1024, 16);
       constexpr int kSteps = G / 16;  // products of a group
-      Ring sr, ar, dr;
-      sr.stage = dr.stage = me;
+      Ring sr, ar, dr, fr, pr;
+      sr.stage = dr.stage = fr.stage = me;
       bool ok = true, x_ready = false, a_ready = false;
       // this warp's first k tile, and how far the next one is
       const int from = C::H == 1 ? me : 0, by = C::H == 1 ? kIssuers : 1;
       const int tiles = (a.tiles - first_tile + tile_step - 1) / tile_step;
       for (int64_t it = from, all = (int64_t)tiles * len; it < all; it += by) {
         if (C::H == 2 && !(ok = w4_wait_warp(&afull[ar.stage], ar.phase, p.status, a_ready))) break;
-#pragma unroll
-        for (int h = 0; h < C::H; ++h) {
-          if (C::H == 2 && kOne && h != me) continue;
-          if (!(ok = w4_wait_warp(&full[sr.stage], sr.phase, p.status, x_ready))) break;
-          {
-            Ring then = sr;
-            then.next(C::STAGES, kIssuers);
-            x_ready = mbar_test(smem_u32(&full[then.stage]), then.phase);
-            if (C::H == 2) {
-              then = ar;
-              then.next(C::A_TILES);
-              a_ready = mbar_test(smem_u32(&afull[then.stage]), then.phase);
-            }
+        if (!(ok = w4_wait_warp(&full[sr.stage], sr.phase, p.status, x_ready))) break;
+        {
+          Ring then = sr;
+          then.next(C::STAGES, kIssuers);
+          x_ready = mbar_test(smem_u32(&full[then.stage]), then.phase);
+          if (C::H == 2) {
+            then = ar;
+            then.next(C::A_TILES);
+            a_ready = mbar_test(smem_u32(&afull[then.stage]), then.phase);
           }
-          const uint64_t bd = bdesc + sr.stage * (C::B_BYTES >> 4);
-          const uint32_t ad = tmem + C::A_AT + (C::H == 2 ? ar.stage : sr.stage) * kACols;
-#pragma unroll
-          for (int j = 0; j < groups; ++j) {
-            if (!kOne && !(ok = w4_wait_warp(&dempty[dr.stage], dr.phase ^ 1u, p.status))) break;
-            tc_fence_after();
-            const uint32_t d = tmem + dr.stage * C::U;
-            if (elect_one()) {
-#pragma unroll
-              for (int i = 0; i < kSteps; ++i) {
-                const int k = j * kSteps + i;
-                umma_ts(d, ad + k * 8, bd + (k >> 2) * (C::B_BYTES / 2 >> 4) + (k & 3) * 2, idesc, i != 0);
-              }
-              if (!kOne) umma_commit(&dfull[h * C::ACCS + dr.stage]);
-              if (j == groups - 1) {
-                umma_commit(&empty[sr.stage]);
-                if (C::H == 2 && (kOne || h == 1)) umma_commit(&aempty[ar.stage]);
-              }
-            }
-            __syncwarp();
-            dr.next(C::ACCS, kIssuers);
-          }
-          if (!ok) break;
-          sr.next(C::STAGES, kIssuers);
         }
+        const uint64_t bd = bdesc + sr.stage * (C::B_BYTES >> 4);
+        const uint32_t ad = tmem + C::A_AT + (C::H == 2 ? ar.stage : sr.stage) * kACols;
+#pragma unroll
+        for (int j = 0; j < groups; ++j) {
+          if (!kOne && !(ok = w4_wait_warp(&dempty[fr.stage], fr.phase, p.status))) break;
+          tc_fence_after();
+          const uint32_t d = tmem + dr.stage * C::U;
+          if (elect_one()) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+              const int k = j * kSteps + i;
+              umma_ts(d, ad + k * 8, bd + (k >> 2) * (C::B_BYTES / 2 >> 4) + (k & 3) * 2, idesc, i != 0);
+            }
+            if (!kOne) umma_commit(&dfull[me * C::ACCS + pr.stage]);
+            if (j == groups - 1) {
+              umma_commit(&empty[sr.stage]);
+              if (C::H == 2) umma_commit(&aempty[ar.stage]);
+            }
+          }
+          __syncwarp();
+          dr.next(C::ACCS, kIssuers);
+          fr.next(kFree, kIssuers);
+          pr.next(C::ACCS);
+        }
+        if (!ok) break;
+        sr.next(C::STAGES, kIssuers);
         if (!ok) break;
         ar.next(C::A_TILES);
       }
@@ -391,8 +392,7 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
         __syncwarp();
         w4_wait_warp(&drain[me], 0, p.status);
       }
-      if (kOne && warp == 3) named_sync(3, 64);
-      if (kOne && warp == 1) named_sync(3, 64);
+      if (kIssuers == 2) named_sync(3, 64);
     }
     if (a.split > 1) cluster_pass();
     if (warp == 1) {
@@ -518,26 +518,26 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
   } else {
     regs_inc<C::R_SUM>();
     const int w = warp - 4 - C::WIDEN, part = w >> 2, r = (warp & 3) * 32 + lane;  // half of the tile, row of W in it
-    // kOne: a half's accumulator is full when its products have ended, and is free for the one ACCS halves later, whose
-    // barrier is told; the first ACCS have theirs from the start (from the warpgroup whose turn it would have been).
-    if (kOne && lane == 0) {
+    // With kOne a half's accumulator is full when its products have ended.  One that has been taken is free for the number
+    // ACCS later, whose barrier is told; the first ACCS are free from the start (told by the warpgroup whose turn it would be).
+    constexpr int kTold = kOne ? C::STAGES : kFree;
+    uint64_t* told = kOne ? full : dempty;
+    if (lane == 0) {
 #pragma unroll
-      for (int u = 0; u < C::ACCS; ++u)
-        if ((u + C::ACCS) % C::H == part) mbar_arrive(&full[u]);
+      for (int v = 0; v < C::ACCS; ++v)
+        if ((v + C::ACCS) % C::H == part) mbar_arrive(&told[v]);
     }
     pdl_wait();
     const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint16_t* my_scales = reinterpret_cast<const uint16_t*>(scales + (r >> 6) * groups * 128) + w4_place(r & 63);
-    Ring dr, er;
-    er.stage = part;
-    dr.stage = part * groups % C::ACCS;
-    uint32_t dphase = 0;  // a bit for each accumulator: the next phase of this warpgroup's barrier
-    int tell = (part + C::ACCS) % C::STAGES, slot = 0;
-    auto give_back = [&](int d) {  // accumulator d has been taken
+    Ring dr, er, pr;
+    er.stage = dr.stage = part;
+    int tell = (part + C::ACCS) % kTold, slot = 0;
+    auto give_back = [&]() {  // the accumulator taken last
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(kOne ? &full[tell] : &dempty[d]);
-      if ((tell += C::H) >= C::STAGES) tell -= C::STAGES;
+      if (lane == 0) mbar_arrive(&told[tell]);
+      if ((tell += C::H) >= kTold) tell -= kTold;
     };
     bool ok = true, ready = false;
     for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
@@ -555,12 +555,9 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
             er.next(C::STAGES, C::H);
             ready = mbar_test(smem_u32(&empty[er.stage]), er.phase);
           } else {
-            if (!(ok = w4_wait_warp(&dfull[part * C::ACCS + dr.stage], dphase >> dr.stage & 1, p.status, ready))) break;
-            dphase ^= 1u << dr.stage;
-            Ring then = dr;
-            then.next(C::ACCS);
-            ready = (C::H == 1 || gr + 1 < groups) &&
-                    mbar_test(smem_u32(&dfull[part * C::ACCS + then.stage]), dphase >> then.stage & 1);
+            if (!(ok = w4_wait_warp(&dfull[part * C::ACCS + pr.stage], pr.phase, p.status, ready))) break;
+            pr.next(C::ACCS);
+            ready = mbar_test(smem_u32(&dfull[part * C::ACCS + pr.stage]), pr.phase);
           }
           tc_fence_after();
           const float s = w4_scale(my_scales[slot * (slot_bytes / 2) + gr * 64], p.scale_half);
@@ -587,13 +584,8 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
             }
           }
           held = dr.stage;
-          if (a.split > 1 || kt + 1 < span.end || gr + 1 < groups) give_back(held);
-          // (the other half's groups lie between two tiles of this one)
-          dr.next(C::ACCS);
-          if (C::H == 2 && gr + 1 == groups) {
-#pragma unroll
-            for (int i = 0; i < groups; ++i) dr.next(C::ACCS);
-          }
+          if (a.split > 1 || kt + 1 < span.end || gr + 1 < groups) give_back();
+          dr.next(C::ACCS, C::H);
         }
         if (++slot == C::SLOTS) slot = 0;
       }
@@ -661,7 +653,7 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
           }
         }
       }
-      give_back(held);
+      give_back();
     }
     if (a.split > 1) {
       __syncwarp();
