@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(256) k_w4_unpack(const PackDev p) {
 }
 
 bool sizes_ok(int32_t n, int32_t k, int32_t group) {
-  return n > 0 && k > 0 && (group == 32 || group == 64 || group == 128) && k % group == 0 && n <= (1 << 30);
+  return n > 0 && k > 0 && (group == 32 || group == 64 || group == 128) && k % group == 0 && n <= (1 << 30) && k <= (1 << 24);
 }
 
 // The parts of pack and unpack that are alike; a status.
@@ -198,6 +198,8 @@ extern "C" int t2w_w4_linear(const t2w_w4_linear_args* a, void* stream) {
   p.residual = a->residual;
   p.res_ld = a->res_ld;
   p.out = a->out;
+  // A pass over the weights for every 8 rows against one for all: 12 x 4096 x 11008, gated, 27 us for 33 on tcgen05, 16 x 4096 x
+  // 6144 12.2 for 12.0, 32 x 4096 x 6144 22 for 12.
   const auto launch = a->rows <= 16 ? launch_w4_few : launch_w4_many;
   return done(launch(p, w.group, w.has_zeros, w.gated, a->dtype == T2W_DT_FP16, static_cast<cudaStream_t>(stream)));
 }

@@ -55,6 +55,37 @@ struct W4Dev {
   int64_t res_ld;
   void* out;  // [rows][n] contiguous
 };
+// How many clusters of `split` blocks of a kernel are resident at once: clusters lie within a GPC each, so that it is fewer than the
+// blocks without clusters are (of 148 one an SM, 132 in clusters of 4, 120 in clusters of 8).  `cache` keeps the answer for
+// each device and split (1, 2, 4, 8); 0 is none yet.
+struct ClusterRoom {
+  std::atomic<int> at[16][4] = {};
+};
+template <class K>
+int cluster_room(K* kernel, int split, int threads, int smem, ClusterRoom& cache) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  std::atomic<int>* kept = dev >= 0 && dev < 16 ? &cache.at[dev][split == 1 ? 0 : split == 2 ? 1 : split == 4 ? 2 : 3] : nullptr;
+  if (kept && kept->load(std::memory_order_relaxed) > 0) return kept->load(std::memory_order_relaxed);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(split);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();  // (a shape that does not fit is not an error of the call)
+    return 0;
+  }
+  if (kept) kept->store(n, std::memory_order_relaxed);
+  return n;
+}
+
 // Launchers: one for few rows of x, one for many (each takes any number).
 cudaError_t launch_w4_few(const W4Dev& p, int group, bool zeros, bool gated, bool half, cudaStream_t st);
 cudaError_t launch_w4_many(const W4Dev& p, int group, bool zeros, bool gated, bool half, cudaStream_t st);

@@ -671,6 +671,23 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
 }
 
 template <bool HALF, int NX, int G>
+int many_smem(bool zeros) {
+  const int tile = w4_tile_bytes(G, zeros), fixed = (Cfg<NX>::fixed(G) + 127) / 128 * 128;
+  // as many packed tiles under way as there is room for, in whole turns: so each has its warpgroup, which sees all its phases
+  const int room = (kMaxSmem - fixed) / (2 * tile), stages = (room < kMaxCodes ? room : kMaxCodes) / Cfg<NX>::TURNS * Cfg<NX>::TURNS;
+  return fixed + stages * 2 * tile;
+}
+
+// Clusters of `split` blocks that are resident at once.
+template <bool HALF, int NX, int G>
+int room_for(int split, bool zeros) {
+  static std::atomic<uint64_t> done{0};
+  if (smem_attr_once(k_w4_many<HALF, NX, G>, kMaxSmem, done) != cudaSuccess) return 0;
+  static ClusterRoom room;
+  return cluster_room(k_w4_many<HALF, NX, G>, split, Cfg<NX>::THREADS, many_smem<HALF, NX, G>(zeros), room);
+}
+
+template <bool HALF, int NX, int G>
 cudaError_t launch(const W4Dev& p, bool zeros, bool gated, int split, cudaStream_t st) {
   using C = Cfg<NX>;
   ManyArgs a = {};
@@ -685,11 +702,9 @@ cudaError_t launch(const W4Dev& p, bool zeros, bool gated, int split, cudaStream
   a.split = split;
   CUtensorMap map;
   if (!make_tmap_2d(&map, p.x, 2, p.rows, p.k, (uint64_t)p.x_ld * 2, C::U, 64)) return cudaErrorInvalidValue;
-  // as many packed tiles under way as there is room for, in whole turns: so each has its warpgroup, which sees all its phases
-  const int fixed = (C::fixed(G) + 127) / 128 * 128, room = (kMaxSmem - fixed) / (2 * a.tile_bytes);
-  a.code_stages = (room < kMaxCodes ? room : kMaxCodes) / C::TURNS * C::TURNS;
+  const int smem = many_smem<HALF, NX, G>(zeros);
+  a.code_stages = (smem - (C::fixed(G) + 127) / 128 * 128) / (2 * a.tile_bytes);
   if (a.code_stages < 2 * C::TURNS) return cudaErrorInvalidValue;
-  const int smem = fixed + a.code_stages * 2 * a.tile_bytes;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = smem_attr_once(k_w4_many<HALF, NX, G>, kMaxSmem, done);
   if (e != cudaSuccess) return e;
@@ -716,28 +731,53 @@ cudaError_t launch(const W4Dev& p, bool zeros, bool gated, int split, cudaStream
   return cudaLaunchKernelEx(&cfg, k_w4_many<HALF, NX, G>, map, a);
 }
 
-template <bool HALF, int NX>
-cudaError_t pick_group(const W4Dev& p, int group, bool zeros, bool gated, int split, cudaStream_t st) {
-  if (group == 32) return launch<HALF, NX, 32>(p, zeros, gated, split, st);
-  if (group == 64) return launch<HALF, NX, 64>(p, zeros, gated, split, st);
-  return launch<HALF, NX, 128>(p, zeros, gated, split, st);
+// The tile's width and the split of k with the least time by what was measured (us, groups of 128): a tile of 128 k takes
+// 0.45 for NX = 32, 0.47 for 64, 0.73 for 128 and 0.87 for 256 (with groups of 64 about 1.2 and of 32 about 1.7 times that), the
+// end of a block's tile 1.5 to 5, and the cluster's joining 1.5 more.  Blocks of a cluster have one tile, so all clusters have to be
+// resident at once.
+struct Choice {
+  int nx = 0, split = 1;
+  int64_t cost = INT64_MAX;
+};
+template <bool HALF, int NX, int G>
+void consider(const W4Dev& p, bool zeros, Choice& best) {
+  constexpr int kTile = (NX == 32 ? 45 : NX == 64 ? 47 : NX == 128 ? 73 : 87) * (G == 32 ? 17 : G == 64 ? 12 : 10) / 10, kEnd = NX == 32 ? 150 : NX == 64 ? 200 : NX == 128 ? 300 : 500;
+  const int64_t tiles = (int64_t)((p.blocks + 1) / 2) * ((p.rows + NX - 1) / NX);
+  for (int s = 1; s <= 8 && p.tiles_k >= 2 * s; s *= 2) {
+    if (s > 1 && tiles > room_for<HALF, NX, G>(s, zeros)) break;
+    const int64_t rounds = s > 1 ? 1 : (tiles + num_sms() - 1) / num_sms();
+    const int64_t cost = rounds * ((int64_t)((p.tiles_k + s - 1) / s) * kTile + kEnd) + (s > 1 ? 150 : 0);
+    if (cost < best.cost) best = {NX, s, cost};
+  }
+  if (p.tiles_k == 1) {  // (nothing to split)
+    const int64_t cost = (tiles + num_sms() - 1) / num_sms() * (kTile + kEnd);
+    if (cost < best.cost) best = {NX, 1, cost};
+  }
+}
+
+template <bool HALF, int G>
+cudaError_t pick(const W4Dev& p, bool zeros, bool gated, cudaStream_t st) {
+  Choice best;
+  consider<HALF, 32, G>(p, zeros, best);
+  if (p.rows > 32) consider<HALF, 64, G>(p, zeros, best);
+  if (p.rows > 64) consider<HALF, 128, G>(p, zeros, best);
+  if (p.rows > 128) consider<HALF, 256, G>(p, zeros, best);
+  if (best.nx == 32) return launch<HALF, 32, G>(p, zeros, gated, best.split, st);
+  if (best.nx == 64) return launch<HALF, 64, G>(p, zeros, gated, best.split, st);
+  if (best.nx == 128) return launch<HALF, 128, G>(p, zeros, gated, best.split, st);
+  return launch<HALF, 256, G>(p, zeros, gated, best.split, st);
 }
 template <bool HALF>
-cudaError_t pick(const W4Dev& p, int group, bool zeros, bool gated, cudaStream_t st) {
-  const int nx = p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : p.rows <= 128 ? 128 : 256;
-  const int64_t tiles = (int64_t)((p.blocks + 1) / 2) * ((p.rows + nx - 1) / nx);
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= num_sms() && p.tiles_k >= 2 * split) split *= 2;
-  if (nx == 32) return pick_group<HALF, 32>(p, group, zeros, gated, split, st);
-  if (nx == 64) return pick_group<HALF, 64>(p, group, zeros, gated, split, st);
-  if (nx == 128) return pick_group<HALF, 128>(p, group, zeros, gated, split, st);
-  return pick_group<HALF, 256>(p, group, zeros, gated, split, st);
+cudaError_t pick_group(const W4Dev& p, int group, bool zeros, bool gated, cudaStream_t st) {
+  if (group == 32) return pick<HALF, 32>(p, zeros, gated, st);
+  if (group == 64) return pick<HALF, 64>(p, zeros, gated, st);
+  return pick<HALF, 128>(p, zeros, gated, st);
 }
 
 }  // namespace
 
 cudaError_t launch_w4_many(const W4Dev& p, int group, bool zeros, bool gated, bool half, cudaStream_t st) {
-  return half ? pick<true>(p, group, zeros, gated, st) : pick<false>(p, group, zeros, gated, st);
+  return half ? pick_group<true>(p, group, zeros, gated, st) : pick_group<false>(p, group, zeros, gated, st);
 }
 
 }  // namespace t2w
