@@ -11,10 +11,12 @@
 #include "kernels.h"
 #include "w4.h"
 
+#include <algorithm>
+
 namespace t2w {
 namespace {
 
-constexpr int kMaxThreads = 384;
+constexpr int kMaxThreads = 256, kPieces = 1024;  // of a block
 
 struct RotDev {
   const uint16_t* in[2];
@@ -72,7 +74,7 @@ T2W_DEV Piece piece_of(const RotDev& p, int item, int64_t row0) {
 }
 
 template <bool HALF, bool ADJACENT>
-__global__ void __launch_bounds__(kMaxThreads) k_rotary(const RotDev p) {
+__global__ void __launch_bounds__(kMaxThreads, 6) k_rotary(const RotDev p) {
   extern __shared__ float2 turn[];  // [rows of the block][pairs] cosine, sine
   pdl_wait();
   pdl_launch();
@@ -199,10 +201,10 @@ extern "C" int t2w_rotary(const t2w_rotary_args* a, void* stream) {
   p.items = (int)heads * p.pieces;
   p.inv_items = inverse_of(p.items);
   p.inv_pieces = inverse_of(p.pieces);
-  // A row's pieces in equal rounds of at most kMaxThreads; short rows share a block of about 256 threads.
-  p.per_block = p.items < 128 ? 256 / p.items : 1;
-  if (p.per_block > a->rows) p.per_block = a->rows;
-  const int total = p.per_block * p.items, rounds = (total + kMaxThreads - 1) / kMaxThreads;
+  // Rows of a block: as many as bring it about 1024 pieces (its threads then take about as many sines as it has threads, and
+  // each has its next piece under way while it turns one), but no more than leave four blocks for each SM.
+  p.per_block = std::max(1, std::min({kPieces / p.items, a->rows / (4 * num_sms()), 4096 / p.pairs}));
+  const int total = std::min(p.per_block, a->rows) * p.items, rounds = (total + kMaxThreads - 1) / kMaxThreads;
   const int threads = ((total + rounds - 1) / rounds + 31) / 32 * 32;
   const dim3 grid((unsigned)((a->rows + p.per_block - 1) / p.per_block));
   const size_t smem = (size_t)p.per_block * p.pairs * sizeof(float2);
