@@ -116,6 +116,41 @@ def test_rows_that_are_not_finite_stay_to_themselves(rows):
             x[bad] = keep
 
 
+@pytest.mark.parametrize("rows,k,n", [
+    (1, 32, 40000), (8, 512, 20000),    # few rows: more row blocks than the clusters take in one pass, one and four tiles of k
+    (3, 4096, 700), (16, 1056, 9000),   # a warp's tiles of two row blocks; two columns of blocks
+    (20, 128, 39000), (33, 384, 20000),  # more rows: more tiles than blocks, with an odd number of row blocks
+    (700, 192, 7000), (1025, 64, 5000)])
+@pytest.mark.parametrize("group", [32, 64])
+def test_many_row_blocks(rows, k, n, group):
+    """Row blocks by the hundred, against the statement on the GPU."""
+    group = group if k % group == 0 else 32
+    gen = torch.Generator().manual_seed(rows + n)
+    w = cuda(ref.weights(n, k, group, True, BF16, gen))
+    x, bias = normal(gen, rows, k).cuda(), normal(gen, n).cuda()
+    y, lim = ref.linear(x, w, bias)
+    held(w4.linear(x, w4.pack(*w), bias), (y.cpu(), lim.cpu()))
+    half = tuple(None if t is None else t[:n // 2] for t in w), tuple(None if t is None else t[n // 2:n // 2 * 2] for t in w)
+    y, lim = ref.gated(x, *half, "silu")
+    held(w4.gated(x, w4.pack_gated(*half)), (y.cpu(), lim.cpu()))
+
+
+@pytest.mark.parametrize("rows", [2, 40, 130])
+def test_offsets_past_32_bits(rows):
+    """A weight of 4.6 GB: its last rows."""
+    k, n = 65536, 131136
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    codes = torch.randint(0, 16, (n, k), generator=gen, device="cuda", dtype=torch.uint8)
+    scales = (torch.rand(n, k // 128, generator=gen, device="cuda") * 0.01).to(BF16)
+    p = w4.pack(codes, scales)
+    assert p.buffer.numel() > 2 ** 32
+    x = torch.randn(rows, k, generator=gen, device="cuda").to(BF16)
+    out = w4.linear(x, p)
+    for part in (slice(0, 40), slice(n - 100, n)):
+        y, lim = ref.linear(x.cpu(), (codes[part].cpu(), scales[part].cpu(), None))
+        held(out[:, part], (y, lim))
+
+
 def test_strides_and_rows():
     gen = torch.Generator().manual_seed(3)
     k, n = 256, 72

@@ -25,7 +25,8 @@ def test_bytes():
     assert size(32, 128, 64, 0, 1) == size(64, 128, 64, 0, 0)  # a pair of 32 rows each
     assert size(33, 128, 64, 0, 1) == size(80, 128, 64, 0, 0)
     assert size(1 << 20, 1 << 16, 128, 0, 0) > 1 << 35
-    for n, k, g in ((0, 128, 128), (-1, 128, 128), (1, 0, 32), (1, 128, 48), (1, 96, 64), (1, 128, 256), (1, 120, 32), (1, -128, 128)):
+    for n, k, g in ((0, 128, 128), (-1, 128, 128), (1, 0, 32), (1, 128, 48), (1, 96, 64), (1, 128, 256), (1, 120, 32), (1, -128, 128),
+                    (1, (1 << 24) + 128, 128), ((1 << 30) + 1, 32, 32)):
         assert size(n, k, g, 0, 0) == INVALID
 
 
