@@ -29,30 +29,35 @@ constexpr int kBars = kWarps * kStages * 8;
 
 constexpr int few_smem(int tile) { return kBars + kWarps * kStages * tile + (kWarps * 2 + kSlots) * kSeg; }
 
+// c = a b + d
 template <bool HALF>
-T2W_DEV void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+T2W_DEV void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float d0, float d1, float d2, float d3) {
   if constexpr (HALF)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(d0), "f"(d1), "f"(d2), "f"(d3));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(d0), "f"(d1), "f"(d2), "f"(d3));
 }
 
 struct XFrag {
   uint2 v[8];  // [16 k]: 4 consecutive k each
 };
 
-// A lane's pieces of x for a k tile: row m, k = 128 tile + 16 j + 4 t; zeros past either end (k is a multiple of 32, so a
-// piece lies inside or outside).
-T2W_DEV void load_x(XFrag& f, const W4Dev& p, int m, int tile, int t) {
-  const int k0 = tile * kW4K + 4 * t;
-  const uint16_t* row = static_cast<const uint16_t*>(p.x) + (int64_t)m * p.x_ld + k0;
+// A lane's pieces of x for a k tile, from the row's place: k = 128 tile + 16 j + 4 t; zeros past the end (k is a multiple of 32,
+// so a piece lies inside or outside), where the weights are 0 but x may be anything.
+T2W_DEV void load_x(XFrag& f, const uint16_t* row, int k, int tile, int t) {
+  const int left = k - tile * kW4K - 4 * t;
+  const uint2* from = reinterpret_cast<const uint2*>(row + tile * kW4K);
+  if (left > 112) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    f.v[j] = (m < p.rows && k0 + 16 * j < p.k) ? *reinterpret_cast<const uint2*>(row + 16 * j) : make_uint2(0, 0);
+    for (int j = 0; j < 8; ++j) f.v[j] = from[4 * j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f.v[j] = 16 * j < left ? from[4 * j] : make_uint2(0, 0);
+  }
 }
 
 T2W_DEV void st_cluster4(uint32_t addr, float4 v) {
@@ -104,8 +109,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int log_s
   if (split > 1) cluster_arrive();  // (waited for before another block's memory is written: it has to run by then)
   int count = min(most, rb_end - rb_begin), tiles = count * T, at = first_of(tiles, me), end = first_of(tiles, me + 1), kt = at % T;
   pdl_wait();
+  // (lanes of columns that there are not read the last row: their sums are not used)
+  const uint16_t* row = static_cast<const uint16_t*>(p.x) + (int64_t)min(m0 + g, p.rows - 1) * p.x_ld + 4 * t;
   XFrag x;
-  if (at < end) load_x(x, p, m0 + g, kt, t);
+  if (at < end) load_x(x, row, p.k, kt, t);
   pdl_launch();
 
   int stage = 0;
@@ -138,18 +145,24 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int log_s
         break;
       }
       const uint8_t* buf = ring + stage * kTile;
-      alignas(16) uint16_t scale[kGroups][8];
+      alignas(16) uint16_t raw[kGroups][8];
+      float scale[kGroups][8];
       alignas(8) uint8_t zero[kGroups][8];
 #pragma unroll
       for (int j = 0; j < kGroups; ++j) {
-        *reinterpret_cast<uint4*>(scale[j]) = *reinterpret_cast<const uint4*>(buf + kW4Codes + j * 128 + g * 16);
+        *reinterpret_cast<uint4*>(raw[j]) = *reinterpret_cast<const uint4*>(buf + kW4Codes + j * 128 + g * 16);
         if constexpr (ZEROS)
           *reinterpret_cast<uint2*>(zero[j]) = *reinterpret_cast<const uint2*>(buf + kW4Codes + kGroups * 128 + j * 64 + g * 8);
       }
-      const XFrag cur = x;
+      if (p.scale_half) {
+#pragma unroll
+        for (int j = 0; j < kGroups * 8; ++j) scale[j / 8][j % 8] = W4Num<true>::to_float(raw[j / 8][j % 8]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kGroups * 8; ++j) scale[j / 8][j % 8] = W4Num<false>::to_float(raw[j / 8][j % 8]);
+      }
       const bool last = kt + 1 == T;  // of its row block
       kt = last ? 0 : kt + 1;
-      if (i + 1 < end) load_x(x, p, m0 + g, kt, t);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         uint4 code[2];
@@ -157,23 +170,26 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int log_s
         for (int kb = 0; kb < 2; ++kb) code[kb] = reinterpret_cast<const uint4*>(buf)[(r * 2 + kb) * 32 + lane];
 #pragma unroll
         for (int j = 0; j < kGroups; ++j) {
-          float sum[4] = {};
-          const uint32_t zlo = w4_zero<HALF>(ZEROS ? zero[j][2 * r] : 8u), zhi = w4_zero<HALF>(ZEROS ? zero[j][2 * r + 1] : 8u);
+          float sum[4];
+          const uint32_t zlo = w4_zero<HALF>(ZEROS ? zero[j][2 * r] : 8u), zhi = w4_zero_hi<HALF>(ZEROS ? zero[j][2 * r + 1] : 8u);
 #pragma unroll
           for (int s = 0; s < G / 16; ++s) {  // products of 16 k
             const int k = j * (G / 16) + s;
             const uint32_t w = (&code[k >> 2].x)[k & 3];
             uint32_t a[4];
             w4_widen<HALF>(w, zlo, zhi, a);
-            mma16816<HALF>(sum, a, cur.v[k].x, cur.v[k].y);
+            if (s == 0) mma16816<HALF>(sum, a, x.v[k].x, x.v[k].y, 0.f, 0.f, 0.f, 0.f);
+            else mma16816<HALF>(sum, a, x.v[k].x, x.v[k].y, sum[0], sum[1], sum[2], sum[3]);
           }
-          const float slo = w4_scale(scale[j][2 * r], p.scale_half), shi = w4_scale(scale[j][2 * r + 1], p.scale_half);
+          const float slo = scale[j][2 * r], shi = scale[j][2 * r + 1];
           acc[r][0] = fmaf(slo, sum[0], acc[r][0]);
           acc[r][1] = fmaf(slo, sum[1], acc[r][1]);
           acc[r][2] = fmaf(shi, sum[2], acc[r][2]);
           acc[r][3] = fmaf(shi, sum[3], acc[r][3]);
         }
       }
+      // (x for the next tile: other warps' products hide its way; a second set of registers for it cost more than it gave)
+      if (i + 1 < end) load_x(x, row, p.k, kt, t);
       __syncwarp();  // the tile has been read: its place may be filled again
       if (lane == 0) copy(stage);
       if (++stage == kStages) {
@@ -226,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int log_s
       at = first_of(tiles, me);
       end = first_of(tiles, me + 1);
       kt = at % T;
-      if (at < end) load_x(x, p, m0 + g, kt, t);
+      if (at < end) load_x(x, row, p.k, kt, t);
     }
     if (split > 1) {
       cluster_arrive();

@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
             for (int j = 0; j < 4; ++j) {
               const uint32_t zz = z[s][(b * 64 + j * 16) / G];
               uint32_t x[4];
-              w4_widen<HALF>((&c[s][b].x)[j], w4_zero<HALF>(zz & 255), w4_zero<HALF>(zz >> 8), x);
+              w4_widen<HALF>((&c[s][b].x)[j], w4_zero<HALF>(zz & 255), w4_zero_hi<HALF>(zz >> 8), x);
               v[4 * j] = x[0];  // row g, k and k + 2; row g + 8
               v[4 * j + 1] = x[2];
               v[4 * j + 2] = x[1];
