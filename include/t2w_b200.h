@@ -706,7 +706,7 @@ T2W_API int t2w_paged_attn(const t2w_paged_attn_args* a, void* stream);
 
 /* ---- Products with 4-bit weights (no reference counterpart: the reference's weights are 16-bit).  W[n][k] = (code - zero)
  * * scale: codes 0 .. 15, one scale (bf16 or fp16) and one zero (0 .. 15; 8 for a weight without zeros) for each row and
- * `group` consecutive k.  group is 32, 64 or 128 and divides k.
+ * `group` consecutive k.  group is 32, 64 or 128 and divides k; n is at most 2^30, k 2^24.
  * A weight is laid out once by t2w_w4_pack into `buffer` (t2w_w4_bytes, 128-byte aligned, on the current device); a gated
  * weight holds two matrices [n][k], the gate's and the up projection's.  Products read the buffer before the kernel ahead of them in the stream
  * has ended, so whatever writes it (packing, a copy) has to be complete, by an event or a synchronisation that the host has
@@ -759,7 +759,8 @@ T2W_API int t2w_w4_linear(const t2w_w4_linear_args* a, void* stream);
  * table: device uint64 [rotary_dim / 2] with f_i / (2 pi) * 2^64 rounded, then as many axis numbers (0 .. axes - 1).
  * positions: int32, or int64 with wide_positions, [axes][rows] at a pitch of pos_ld, of either sign.
  * Rows [rows][heads][head_dim] of `dtype`, head_dim contiguous, on 16-byte boundaries (pitches multiples of 8); out may be
- * `in` itself, with its pitches, and may not overlap otherwise.  head_dim is a multiple of 8, rotary_dim of 16. */
+ * `in` itself, with its pitches, and may not overlap otherwise, nor q's rows k's (refused where rows at one pitch show it).
+ * head_dim is a multiple of 8, rotary_dim of 16 and at most 4096, heads times rotary_dim / 16 + kept / 8 pieces at most 32767. */
 typedef struct t2w_rotary_rows {
   const void* in;
   void* out;

@@ -147,6 +147,18 @@ bool apart(int64_t rows, int64_t heads, int64_t hd, int64_t row_ld, int64_t head
   return rows == 1 || heads == 1 || row_ld >= (heads - 1) * head_ld + hd || head_ld >= (rows - 1) * row_ld + hd;
 }
 
+// Whether the outputs of q and k share memory, as far as that shows: the same place, or columns of rows at one pitch.
+bool share(const t2w_rotary_rows& q, int64_t q_heads, const t2w_rotary_rows& k, int64_t k_heads, int64_t rows, int64_t hd) {
+  if (q.out == k.out) return true;
+  const int64_t pitch = q.out_row_ld, q_span = (q_heads - 1) * q.out_head_ld + hd, k_span = (k_heads - 1) * k.out_head_ld + hd;
+  const int64_t apart = static_cast<const uint16_t*>(k.out) - static_cast<const uint16_t*>(q.out);
+  if (rows == 1) return apart < q_span && -apart < k_span;
+  if (pitch != k.out_row_ld || q_span > pitch || k_span > pitch) return false;
+  if (apart >= rows * pitch || -apart >= rows * pitch) return false;
+  const int64_t column = (apart % pitch + pitch) % pitch;  // of k's rows in q's
+  return column < q_span || column + k_span > pitch;
+}
+
 }  // namespace
 }  // namespace t2w
 
@@ -185,7 +197,7 @@ extern "C" int t2w_rotary(const t2w_rotary_args* a, void* stream) {
     p.out_row[w] = s[w]->out_row_ld;
     p.out_head[w] = s[w]->out_head_ld;
   }
-  if (p.in[0] && p.in[1] && p.out[0] == p.out[1]) return T2W_ERR_INVALID;
+  if (p.in[0] && p.in[1] && share(a->q, a->q_heads, a->k, a->k_heads, a->rows, a->head_dim)) return T2W_ERR_INVALID;
   p.pieces = p.turned + (kept ? (a->head_dim - a->rotary_dim) / 8 : 0);
   if (heads * p.pieces > 32767 || a->rotary_dim > 4096) return T2W_ERR_UNSUPPORTED;
   p.positions = a->positions;

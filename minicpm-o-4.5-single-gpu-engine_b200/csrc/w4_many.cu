@@ -14,8 +14,9 @@
 // widened weights would take 256 clocks to write and 256 to read, where the products take 4 NX clocks.
 // What a hand-over costs decides the rest: passing an mbarrier that is ready takes about 100 clocks, a commit 80, the
 // issue of 4 products 65, a round of waiting, expecting and two copies 650 (one thread brings 23 GB/s in pieces of 4 KB).  So
-// copies and products are issued by several warps in turn, and with groups of 128 one barrier tells the products' warp what a half waits for (x and a free
-// accumulator; the weights too where there is one half), and one commit tells that its stage is free and its accumulator full.
+// copies and products are issued by several warps in turn, and with groups of 128 one barrier tells the products' warp what a
+// half waits for (x and a free accumulator; the weights too where there is one half), and one commit tells that its stage is
+// free and its accumulator full.
 // With few tiles k is split over a cluster, whose blocks add their sums through distributed shared memory in a fixed order.
 // The first tiles of W come before the kernel waits for the one ahead of it in the stream.  No TMA multicast.
 #include "common.cuh"
@@ -114,17 +115,26 @@ T2W_DEV void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t 
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-T2W_DEV void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
+// 64 columns by two loads (one of 64 would need more registers than the kernel begins with); the wait is inside the block, so
+// that no use of a register can come before it.
+T2W_DEV void tmem_ld32x2(uint32_t taddr, float (&v)[64]) {
+  uint32_t r[64];
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr), "r"(taddr + 32)
       : "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
 T2W_DEV void tmem_ld8(uint32_t taddr, float (&v)[8]) {
   uint32_t r[8];
@@ -567,12 +577,7 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
           for (int c = 0; c < C::U; c += kLoad) {
             float v[kLoad];
             if constexpr (kLoad == 64) {
-              uint32_t raw[2][32];  // (one instruction for 64 would need more registers than the kernel begins with)
-              tmem_ld32_nowait(taddr + dr.stage * C::U, raw[0]);
-              tmem_ld32_nowait(taddr + dr.stage * C::U + 32, raw[1]);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(raw[i / 32][i % 32]);
+              tmem_ld32x2(taddr + dr.stage * C::U, v);
             } else {
               tmem_ld32(taddr + dr.stage * C::U + c, v);
             }

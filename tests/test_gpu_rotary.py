@@ -191,6 +191,12 @@ def test_refusals():
               lambda: turn.apply_(q, q, pos), lambda: turn(q.clone().requires_grad_(), k, pos)):
         with pytest.raises(RuntimeError):
             f()
+    rows = torch.zeros(4, 12, 64, dtype=BF16, device="cuda")  # columns of the same rows: apart, and one head in both
+    turn.apply_(rows[:, :8], rows[:, 8:10], pos)
+    turn.apply_(rows[:, 4:], rows[:, :4], pos)
+    for a, b in ((rows[:, :8], rows[:, 7:9]), (rows[:, 4:], rows[:, 3:5]), (rows[1:, :8], rows[:3, 7:])):
+        with pytest.raises(L.T2WError):
+            turn.apply_(a, b, pos[:, :a.shape[0]])
     with pytest.raises(ValueError):
         turn(q[..., :32], None, pos)
     turn(q, k, pos)

@@ -88,7 +88,8 @@ def rotary_args(**kw):
     (dict(positions=None), INVALID), (dict(table=None), INVALID), (dict(pos_ld=3), INVALID), (dict(q_in=None), INVALID),
     (dict(q_in=(1 << 20) + 8), INVALID), (dict(q_in_row_ld=516), INVALID), (dict(q_out=(1 << 21) + 2), INVALID),
     (dict(q_out_row_ld=64), INVALID), (dict(q_out_head_ld=0), INVALID), (dict(q_out=1 << 20, q_out_row_ld=1024), INVALID),
-    (dict(q_out=1 << 22), INVALID), (dict(q_heads=20000, q_in_head_ld=64, q_out_row_ld=64 * 20000), UNSUPPORTED)])
+    (dict(q_out=1 << 22), INVALID), (dict(q_out=(1 << 22) - 64), INVALID), (dict(q_out=(1 << 22) + 2 * 512 + 128), INVALID),
+    (dict(rows=1, pos_ld=1, axes=1, q_out=(1 << 22) + 128), INVALID), (dict(q_heads=20000, q_in_head_ld=64, q_out_row_ld=64 * 20000), UNSUPPORTED)])
 def test_turns_that_there_are_not(kw, status):
     assert L.load().t2w_rotary(ctypes.byref(rotary_args(**kw)), None) == status
 
