@@ -108,6 +108,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int log_s
   __syncwarp();
   if (split > 1) cluster_arrive();  // (waited for before another block's memory is written: it has to run by then)
   int count = min(most, rb_end - rb_begin), tiles = count * T, at = first_of(tiles, me), end = first_of(tiles, me + 1), kt = at % T;
+  auto write_bounds = [&]() {
+    if (threadIdx.x <= kWarps) warp_at[threadIdx.x] = first_of(tiles, rank * kWarps + threadIdx.x);
+    if (threadIdx.x >= 32 && threadIdx.x <= 32 + split) {
+      const int s = threadIdx.x - 32, first = first_of(tiles, s * kWarps);
+      block_at[s] = first;
+      if (s < split) block_row[s] = first / T;
+    }
+  };
+  write_bounds();
   pdl_wait();
   // (lanes of columns that there are not read the last row: their sums are not used)
   const uint16_t* row = static_cast<const uint16_t*>(p.x) + (int64_t)min(m0 + g, p.rows - 1) * p.x_ld + 4 * t;
@@ -119,12 +128,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int log_s
   uint32_t phase = 0;
   bool ok = true;
   for (int rb0 = rb_begin; rb0 < rb_end;) {
-    if (threadIdx.x <= kWarps) warp_at[threadIdx.x] = first_of(tiles, rank * kWarps + threadIdx.x);
-    if (threadIdx.x >= 32 && threadIdx.x <= 32 + split) {
-      const int s = threadIdx.x - 32, first = first_of(tiles, s * kWarps);
-      block_at[s] = first;
-      if (s < split) block_row[s] = first / T;
-    }
     float acc[4][4];
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -217,21 +220,21 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int log_s
 #pragma unroll
     for (int w = 0; w <= kWarps; ++w) bound[w] = warp_at[w];
     const uint32_t base = smem_u32(parts);
-    const int wide = cols > 4, e = threadIdx.x, in = wide ? e * 4 : e * 8;  // fours of columns: 64 or 128
-    for (int b = block_row[rank], from = b * T; from < block_at[rank + 1]; ++b, from += T) {
-      if (e < 64 << wide) {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    // 64 threads (128 for more than 4 columns) to a row block, four columns to a thread
+    const int wide = cols > 4, e = threadIdx.x & ((64 << wide) - 1), in = wide ? e * 4 : e * 8;
+    for (int b = block_row[rank] + (threadIdx.x >> (6 + wide)); b * T < block_at[rank + 1]; b += kThreads >> (6 + wide)) {
+      const int from = b * T;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w)
-          if (bound[w] < bound[w + 1] && bound[w] < from + T && bound[w + 1] > from) {
-            const float4 q = *reinterpret_cast<const float4*>(segs + (w * 2 + (bound[w] < from)) * (kSeg / 4) + in);
-            v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
-          }
-        int first = 0;  // of the blocks that have tiles of b
-        while (block_at[first + 1] <= from) ++first;
-        const int at_slot = ((b >> log_split) << log_per) + rank - first;
-        st_cluster4(cluster_addr(base + at_slot * kSeg + in * 4, b & (split - 1)), v);
-      }
+      for (int w = 0; w < kWarps; ++w)
+        if (bound[w] < bound[w + 1] && bound[w] < from + T && bound[w + 1] > from) {
+          const float4 q = *reinterpret_cast<const float4*>(segs + (w * 2 + (bound[w] < from)) * (kSeg / 4) + in);
+          v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
+        }
+      int first = 0;  // of the blocks that have tiles of b
+      while (block_at[first + 1] <= from) ++first;
+      const int at_slot = ((b >> log_split) << log_per) + rank - first;
+      st_cluster4(cluster_addr(base + at_slot * kSeg + in * 4, b & (split - 1)), v);
     }
     // (what the next pass begins with is under way meanwhile)
     const int this_rb = rb0, this_count = count;
@@ -253,30 +256,30 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int log_s
     // The outputs of this block's row blocks, along n in a warp.
     constexpr int kOut = GATED ? 32 : 64;
     const int o = threadIdx.x % kOut;
-    for (int j = 0, b = rank; b < this_count; ++j, b += split) {
+    const int owned = (this_count - rank + split - 1) >> log_split;
+    for (int q = threadIdx.x / kOut; q < owned * cols; q += kThreads / kOut) {
+      const int j = q / cols, m = q - j * cols, b = (j << log_split) + rank;
       const int64_t n = (int64_t)(this_rb + b) * kOut + o;
+      if (n >= p.n) continue;
       int from = 0, sources = 0;  // the blocks that have tiles of b
       for (int s = 0; s < split; ++s) {
         from += block_at[s + 1] <= b * T;
         sources += block_at[s] < (b + 1) * T;
       }
       sources -= from;
-      for (int m = threadIdx.x / kOut; m < cols; m += kThreads / kOut) {
-        if (n >= p.n) continue;
-        const float* in = parts + (j << log_per) * (kSeg / 4) + (GATED ? (o >> 3) * 16 + (o & 7) : o) * kCols + m;
-        float v = 0.f, u = 0.f;
-        for (int s = 0; s < sources; ++s, in += kSeg / 4) {
-          v += in[0];
-          if constexpr (GATED) u += in[8 * kCols];
-        }
-        if constexpr (GATED) {
-          v = w4_act(v, p.act) * u;
-        } else {
-          if (p.bias) v += W4Num<HALF>::to_float(static_cast<const uint16_t*>(p.bias)[n]);
-          if (p.residual) v += W4Num<HALF>::to_float(static_cast<const uint16_t*>(p.residual)[(m0 + m) * p.res_ld + n]);
-        }
-        static_cast<uint16_t*>(p.out)[(int64_t)(m0 + m) * p.n + n] = W4Num<HALF>::from_float(v);
+      const float* in = parts + (j << log_per) * (kSeg / 4) + (GATED ? (o >> 3) * 16 + (o & 7) : o) * kCols + m;
+      float v = 0.f, u = 0.f;
+      for (int s = 0; s < sources; ++s, in += kSeg / 4) {
+        v += in[0];
+        if constexpr (GATED) u += in[8 * kCols];
       }
+      if constexpr (GATED) {
+        v = w4_act(v, p.act) * u;
+      } else {
+        if (p.bias) v += W4Num<HALF>::to_float(static_cast<const uint16_t*>(p.bias)[n]);
+        if (p.residual) v += W4Num<HALF>::to_float(static_cast<const uint16_t*>(p.residual)[(m0 + m) * p.res_ld + n]);
+      }
+      static_cast<uint16_t*>(p.out)[(int64_t)(m0 + m) * p.n + n] = W4Num<HALF>::from_float(v);
     }
     if (rb0 < rb_end) {  // no block is sent new sums before these are read
       if (split > 1) {
@@ -285,6 +288,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int log_s
       } else {
         __syncthreads();
       }
+      write_bounds();
     }
   }
 }
