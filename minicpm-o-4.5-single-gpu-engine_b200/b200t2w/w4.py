@@ -8,7 +8,8 @@ start at ``pack``.
 
 The products run on the current stream of the tensors' GPU, need no workspace, keep nothing between calls and may be captured
 in a CUDA graph.  No weight is rounded: sums are fp32 over ``(code - zero) * x``, multiplied by a group's scale after it, and
-the output is rounded once.  They have no gradient.
+the output is rounded once; so a group's sum has to fit fp32 before its scale (|x| up to 1e35 always does).  They have no
+gradient.
 
 Arguments that cannot be right raise at the call: ``T2WError`` for sizes that the kernels do not have, ``RuntimeError`` for
 tensors of the wrong type, shape, device or alignment, ``ValueError`` for weights that cannot be packed.
