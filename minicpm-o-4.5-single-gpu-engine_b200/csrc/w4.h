@@ -222,13 +222,16 @@ T2W_DEV void w4_store4(uint16_t* out, const uint16_t (&v)[4], int count) {
 }
 T2W_DEV float w4_scale(uint16_t v, int half) { return half ? W4Num<true>::to_float(v) : W4Num<false>::to_float(v); }
 
-// ---------------------------------------------------------------- activations (fp32, relative error of a few 2^-22)
-// y sigmoid(s) = y / (1 + e^-s) by the reciprocal (rcp.approx, which has subnormal results where __fdividef gives 0: for
-// divisors above 2^126); e^-s = inf gives y * 0, +-inf and NaN go as in the formula.
+// ---------------------------------------------------------------- activations
+// y sigmoid(s), from e = e^-|s|, which is at most 1 and so never too large: y / (1 + e), times e where s < 0.  (y / (1 + e^-s)
+// is 0 below s = -88.7, where e^-s passes fp32, and y e^s is not yet under bf16's least numbers.)  Relative error (8 + 1.2 |s|)
+// 2^-23 (__expf is off by 2 + 1.2 |s| steps); from s = -87.3 down e is subnormal, which adds steps of 2^-149 |y|.  Infinities
+// and NaN go as in the formula.
 T2W_DEV float w4_sigmoid_mul(float y, float s) {
+  const float e = __expf(-fabsf(s));
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-s)));
-  return y * r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return y * (s < 0.f ? e * r : r);
 }
 T2W_DEV float w4_act(float g, int act) {
   if (act == T2W_ACT_SILU) return w4_sigmoid_mul(g, g);

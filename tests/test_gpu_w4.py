@@ -1,6 +1,8 @@
 """GPU: products with 4-bit weights (``b200t2w.w4``) against a plain statement in 64 bits.  Codes, scales and zeros are read
 back exactly; what products may be off by is derived in ``w4_ref``."""
 
+import math
+
 import pytest
 import torch
 
@@ -69,6 +71,34 @@ def test_gated(rows, k, f, act):
         out = w4.gated(x.cuda(), p, act)
         held(out, ref.gated(x, gate, up, act))
         p.check()
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+@pytest.mark.parametrize("act,gates", [("silu", (-80.0, -110.0, -0.5)), ("gelu_tanh", (-10.0, -11.5, -0.0625))])
+def test_gated_far_below_zero(rows, act, gates):
+    """Gate sums whose sigmoid is near the least fp32 numbers, where the activation is still more than bf16's.
+
+    One product of each sum is not 0, so sums are exact.  Beside the relative error of ``w4_ref.gated``: GELU's argument s has
+    four roundings, so that e^s is off by |s| 2^-22 of itself; a subnormal e^s and its product with g are off by a step,
+    2^-149, each (twice that is allowed)."""
+    g = torch.arange(*gates, dtype=torch.float64)
+    n = g.numel()
+    gate, up = (torch.full((8, 32), 8, dtype=torch.uint8) for _ in range(2))
+    gate[:, 0] = up[:, 1] = 9
+    one = torch.ones(8, 1, dtype=BF16)
+    p = w4.pack_gated((gate.cuda(), one.cuda()), (up.cuda(), one.cuda()))
+    for u in (1.0, -2.0 ** 20, 2.0 ** 60):
+        for first in range(0, n, rows):
+            part = g[first:first + rows]
+            x = torch.zeros(rows, 32, dtype=BF16)
+            x[:part.numel(), 0], x[:, 1] = part.to(BF16), u
+            assert torch.equal(x[:part.numel(), 0].double(), part)
+            v = x[:, :1].double()
+            s = v if act == "silu" else 2 * math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)
+            a = v * torch.sigmoid(s)
+            e = (8 + 3.2 * s.abs()) * 2.0 ** -23 * a.abs() + 2.0 ** -148 * (v.abs() + 1)
+            y = (a * u).expand(rows, 8)
+            held(w4.gated(x.cuda(), p, act), (y, ref.rounded(y, (e * abs(u) + 2.0 ** -24 * y.abs()).expand(rows, 8), BF16)))
 
 
 @pytest.mark.parametrize("n,k,group,zeros,dtype", [(1, 32, 32, False, BF16), (65, 160, 32, True, FP16), (200, 384, 128, True, BF16),
