@@ -597,7 +597,8 @@ at::Tensor w4_product(const char* op, const at::Tensor& x, const at::Tensor& buf
   a.act = (int32_t)act;
   TORCH_CHECK(x.dim() == 2 && x.size(1) == w.k && x.stride(1) == 1 && x.device() == buffer.device(), op, ": x is [rows, ", w.k,
               "] with contiguous rows on ", buffer.device().str());
-  TORCH_CHECK(!x.requires_grad() || !at::GradMode::is_enabled(), op, ": has no gradient");
+  for (const at::Tensor* t : {&x, bias ? &*bias : nullptr, residual ? &*residual : nullptr})
+    TORCH_CHECK(!t || !t->requires_grad() || !at::GradMode::is_enabled(), op, ": has no gradient");
   a.rows = to_i32(op, "rows", x.size(0));
   a.x_ld = a.rows > 1 ? x.stride(0) : w.k;
   TORCH_CHECK(a.x_ld >= w.k && a.x_ld % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0, op,

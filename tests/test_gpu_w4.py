@@ -317,6 +317,24 @@ def test_refusals():
     assert bool(torch.isfinite(w4.linear(x, p)).all())  # and the library goes on
 
 
+def test_bias_and_residual_that_want_a_gradient():
+    """The products have no gradient: what would have to get one is refused where gradients are recorded."""
+    gen = torch.Generator().manual_seed(4)
+    w = ref.weights(64, 128, 64, True, BF16, gen)
+    p = w4.pack(*cuda(w))
+    x, r, b = normal(gen, 4, 128), normal(gen, 4, 64), normal(gen, 64)
+    xs, rs, bs = x.cuda(), r.cuda().requires_grad_(), torch.nn.Parameter(b.cuda())
+    for kw in (dict(bias=bs), dict(residual=rs), dict(bias=bs.detach(), residual=rs), dict(bias=bs, residual=rs.detach())):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            w4.linear(xs, p, **kw)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        w4.feed_forward(xs, w4.pack_gated(cuda(w), cuda(w)), w4.pack(*cuda(ref.weights(64, 64, 64, True, BF16, gen))), residual=rs)
+    with torch.no_grad():
+        out = w4.linear(xs, p, bs, rs)
+    assert not out.requires_grad
+    held(out, ref.linear(x, w, b, r))
+
+
 def test_weights_that_cannot_be_packed():
     gen = torch.Generator().manual_seed(1)
     codes, scales, zeros = cuda(ref.weights(64, 128, 64, True, BF16, gen))
