@@ -12,6 +12,7 @@
 #include "w4.h"
 
 #include <algorithm>
+#include <cstdlib>
 
 namespace t2w {
 namespace {
@@ -147,16 +148,29 @@ bool apart(int64_t rows, int64_t heads, int64_t hd, int64_t row_ld, int64_t head
   return rows == 1 || heads == 1 || row_ld >= (heads - 1) * head_ld + hd || head_ld >= (rows - 1) * row_ld + hd;
 }
 
-// Whether the outputs of q and k share memory, as far as that shows: the same place, or columns of rows at one pitch.
+// Whether a stretch of hd values every q_ld from 0 on (q_heads of them) meets one of hd every k_ld from `at` on.
+bool meet(int64_t q_heads, int64_t q_ld, int64_t k_heads, int64_t k_ld, int64_t at, int64_t hd) {
+  for (int64_t h = 0; h < k_heads; ++h) {
+    const int64_t from = at + h * k_ld;
+    // the last of q's that begins at or before it, and the next
+    const int64_t i = q_heads > 1 && from > 0 ? std::min(from / q_ld, q_heads - 1) : 0;
+    for (int64_t j = i; j <= i + 1 && j < q_heads; ++j)
+      if (j * q_ld < from + hd && from < j * q_ld + hd) return true;
+  }
+  return false;
+}
+
+// Whether the outputs of q and k share memory, as far as that shows: the same place, or rows at one pitch, head by head (heads of
+// the two may alternate).  A row of k lies `column` behind one of q's and pitch - column before the next.
 bool share(const t2w_rotary_rows& q, int64_t q_heads, const t2w_rotary_rows& k, int64_t k_heads, int64_t rows, int64_t hd) {
   if (q.out == k.out) return true;
   const int64_t pitch = q.out_row_ld, q_span = (q_heads - 1) * q.out_head_ld + hd, k_span = (k_heads - 1) * k.out_head_ld + hd;
   const int64_t apart = static_cast<const uint16_t*>(k.out) - static_cast<const uint16_t*>(q.out);
-  if (rows == 1) return apart < q_span && -apart < k_span;
+  auto at = [&](int64_t offset) { return meet(q_heads, q.out_head_ld, k_heads, k.out_head_ld, offset, hd); };
+  if (rows == 1) return at(apart);
   if (pitch != k.out_row_ld || q_span > pitch || k_span > pitch) return false;
-  if (apart >= rows * pitch || -apart >= rows * pitch) return false;
-  const int64_t column = (apart % pitch + pitch) % pitch;  // of k's rows in q's
-  return column < q_span || column + k_span > pitch;
+  const int64_t column = (apart % pitch + pitch) % pitch, behind = (apart - column) / pitch;  // k's row 0 in q's row `behind`
+  return (std::abs(behind) < rows && at(column)) || (std::abs(behind + 1) < rows && at(column - pitch));
 }
 
 }  // namespace

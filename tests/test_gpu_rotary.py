@@ -161,6 +161,27 @@ def test_rows_heads_and_strides():
     assert torch.equal(torch.isnan(got).cpu(), hit) and torch.equal(got.cpu()[~hit], want.cpu()[~hit])
 
 
+@pytest.mark.parametrize("rows", [1, 5])
+def test_heads_of_q_and_k_in_turn(rows):
+    """In place in rows [heads, 3, head_dim], where q's and k's heads alternate and share nothing; and strided heads that do."""
+    gen = torch.Generator().manual_seed(rows)
+    turn = Rotary(64, [16, 16])
+    pos = torch.randint(0, 900, (2, rows), generator=gen).cuda()
+    x = torch.randn(rows, 8, 3, 64, generator=gen).to(BF16).cuda()
+    a, b = turn(x[:, :, 0], x[:, :, 1], pos)
+    y = x.clone()
+    turn.apply_(y[:, :, 0], y[:, :, 1], pos)
+    assert torch.equal(y[:, :, 0], a) and torch.equal(y[:, :, 1], b) and torch.equal(y[:, :, 2], x[:, :, 2])
+    y = x.clone()
+    turn.apply_(y[:, :, 2], y[:, 1:5, 0], pos)
+    assert torch.equal(y[:, :, 2], turn(x[:, :, 2], None, pos)[0]) and torch.equal(y[:, 1:5, 0], a[:, 1:5])
+    assert torch.equal(y[:, :, 1], x[:, :, 1]) and torch.equal(y[:, 5:, 0], x[:, 5:, 0])
+    for off in (8, 56, 3 * 64 + 8, 2 * 64 + 8):  # a part of a head in common
+        k = y.view(-1).as_strided((rows, 5, 64), (8 * 3 * 64, 3 * 64, 1), off)
+        with pytest.raises(L.T2WError):
+            turn.apply_(y[:, :, 0], k, pos)
+
+
 def test_captured():
     gen = torch.Generator().manual_seed(8)
     turn = Rotary(128, [16, 24, 24])

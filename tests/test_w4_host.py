@@ -94,6 +94,36 @@ def test_turns_that_there_are_not(kw, status):
     assert L.load().t2w_rotary(ctypes.byref(rotary_args(**kw)), None) == status
 
 
+def test_rows_that_meet():
+    """q and k in place at one row pitch are refused exactly where they have a value in common, heads that alternate among
+    them.  Heads of 4112 values are more than the kernel has, so that a call that is not refused for this is refused next."""
+    gen = torch.Generator().manual_seed(3)
+
+    def pick(*of):
+        return of[int(torch.randint(0, len(of), (1,), generator=gen))]
+
+    hd, seen = 4112, {True: 0, False: 0}
+    for _ in range(3000):
+        rows = pick(1, 1, 2, 3)
+        heads = [pick(1, 2, 3) for _ in range(2)]
+        ld = [hd + 8 * pick(0, 0, 1, hd // 8, hd // 4, hd // 8 + 3) for _ in range(2)]
+        if pick(True, False):
+            ld[1] = ld[0]
+        span = [(h - 1) * d + hd for h, d in zip(heads, ld)]
+        pitch = max(span) + 8 * pick(0, 0, 1, hd // 8, 100)
+        apart = pick(-1, 1) * (pitch * pick(0, 0, 0, 1, 2, 3) + 8 * pick(0, 1, hd // 8 - 1, hd // 8, hd // 8 + 1, hd // 4, 3 * hd // 8))
+        places = [[base + r * pitch + h * d for r in range(rows) for h in range(n)]
+                  for base, n, d in zip((0, apart), heads, ld)]
+        common = any(abs(a - b) < hd for a in places[0] for b in places[1])
+        q, k = ({"in": base, "out": base, "in_row_ld": pitch, "out_row_ld": pitch, "in_head_ld": d, "out_head_ld": d}
+                for base, d in zip((1 << 40, (1 << 40) + 2 * apart), ld))
+        a = L.RotaryArgs(rows=rows, q_heads=heads[0], k_heads=heads[1], head_dim=hd, rotary_dim=hd, axes=1, q=L.RotaryRows(**q),
+                         k=L.RotaryRows(**k), positions=1 << 20, pos_ld=rows, table=1 << 20)
+        assert L.load().t2w_rotary(ctypes.byref(a), None) == (INVALID if common else UNSUPPORTED), (rows, heads, ld, pitch, apart)
+        seen[common] += 1
+    assert min(seen.values()) > 500
+
+
 def test_no_turns_are_no_work():
     for kw in (dict(rows=0), dict(q_heads=0, k_heads=0)):
         assert L.load().t2w_rotary(ctypes.byref(rotary_args(**kw)), None) == 0
