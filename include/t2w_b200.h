@@ -757,7 +757,7 @@ T2W_API int t2w_w4_linear(const t2w_w4_linear_args* a, void* stream);
  * cos - y sin, y cos + x sin).  A pair is values i and i + rotary_dim / 2 of the head, or with `adjacent` 2 i and 2 i + 1; values
  * past rotary_dim stay.
  * table: device uint64 [rotary_dim / 2] with f_i / (2 pi) * 2^64 rounded, then as many axis numbers (0 .. axes - 1).
- * positions: int32, or int64 with wide_positions, [axes][rows] at a pitch of pos_ld, of either sign.
+ * positions: int32, or int64 with wide_positions, [axes][rows] at a pitch of pos_ld (0: all axes have the same), of either sign.
  * Rows [rows][heads][head_dim] of `dtype`, head_dim contiguous, on 16-byte boundaries (pitches multiples of 8); out may be
  * `in` itself, with its pitches, and may not overlap otherwise, nor q's rows k's (refused where rows at one pitch show it).
  * head_dim is a multiple of 8, rotary_dim of 16 and at most 4096, heads times rotary_dim / 16 + kept / 8 pieces at most 32767. */

@@ -68,8 +68,9 @@ class Rotary:
 
     def __call__(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inverse: bool = False):
         """The turned ``q [rows, heads, head_dim]`` and ``k [rows, kv_heads, head_dim]`` (bf16 or fp16; k may be None), new
-        and contiguous, for ``positions`` (int32 or int64 ``[axes, rows]``, or ``[rows]`` for one axis).  ``inverse`` turns
-        back: by the negative angles, which is also the gradient of the forward call."""
+        and contiguous, for ``positions`` (int32 or int64 ``[axes, rows]``, or ``[rows]`` for one axis; rows of text may be
+        one line for all axes, ``expand``-ed).  ``inverse`` turns back: by the negative angles, which is also the gradient of
+        the forward call."""
         r = O.call("rotary", self._fits(q), k, positions, self.table, self.rotary_dim, self.axes, self.adjacent, inverse)
         return r[0], (r[1] if k is not None else None)
 

@@ -187,7 +187,7 @@ extern "C" int t2w_rotary(const t2w_rotary_args* a, void* stream) {
   const int64_t heads = (int64_t)a->q_heads + a->k_heads;
   if (a->rows == 0 || heads == 0) return T2W_OK;
   if (!a->positions || !a->table || (reinterpret_cast<uintptr_t>(a->table) & 7) || a->pos_ld < 0 ||
-      (a->axes > 1 && a->pos_ld < a->rows))
+      (a->axes > 1 && a->pos_ld != 0 && a->pos_ld < a->rows))
     return T2W_ERR_INVALID;
   RotDev p = {};
   p.turned = a->rotary_dim / 16;

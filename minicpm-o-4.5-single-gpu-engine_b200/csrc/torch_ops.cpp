@@ -667,7 +667,7 @@ std::vector<at::Tensor> rotate(const char* op, const at::Tensor& q, const std::o
               op, ": positions are [", axes, ", ", a.rows, "] with contiguous rows on ", q.device().str());
   a.wide_positions = wide;
   a.pos_ld = flat || axes == 1 ? a.rows : positions.stride(0);
-  TORCH_CHECK(a.pos_ld >= a.rows, op, ": the axes of positions do not overlap");
+  TORCH_CHECK(a.pos_ld == 0 || a.pos_ld >= a.rows, op, ": the axes of positions are apart, or one for all");
   a.positions = positions.data_ptr();
   std::vector<at::Tensor> r;
   auto fill = [&](const char* name, const at::Tensor& x, int32_t& heads, t2w_rotary_rows& rows) {

@@ -161,6 +161,22 @@ def test_rows_heads_and_strides():
     assert torch.equal(torch.isnan(got).cpu(), hit) and torch.equal(got.cpu()[~hit], want.cpu()[~hit])
 
 
+@pytest.mark.parametrize("rows", [1, 2, 70])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_one_line_of_positions_for_all_axes(rows, dtype):
+    gen = torch.Generator().manual_seed(rows)
+    turn = Rotary(64, [12, 10, 10])
+    x = torch.randn(rows, 4, 64, generator=gen).to(BF16)
+    line = torch.randint(0, 90000, (rows,), generator=gen, dtype=dtype)
+    q, pos = x.cuda(), line.cuda().expand(3, rows)
+    assert pos.stride(0) == 0
+    want = turn(q, None, pos.contiguous())[0]
+    assert torch.equal(turn(q, None, pos)[0], want)
+    held(want, x, line.expand(3, rows), axis_of([12, 10, 10]), inv_freq(64, 10000.0), 64, False, False)
+    turn.apply_(q, None, pos)
+    assert torch.equal(q, want)
+
+
 @pytest.mark.parametrize("rows", [1, 5])
 def test_heads_of_q_and_k_in_turn(rows):
     """In place in rows [heads, 3, head_dim], where q's and k's heads alternate and share nothing; and strided heads that do."""

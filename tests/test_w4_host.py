@@ -94,6 +94,14 @@ def test_turns_that_there_are_not(kw, status):
     assert L.load().t2w_rotary(ctypes.byref(rotary_args(**kw)), None) == status
 
 
+@pytest.mark.parametrize("rows,pos_ld,status", [(4, 0, UNSUPPORTED), (1, 0, UNSUPPORTED), (4, 4, UNSUPPORTED), (4, 1, INVALID),
+                                                (4, -4, INVALID)])
+def test_pitches_of_positions(rows, pos_ld, status):
+    """0 is one line for all axes.  (20000 heads are more than the kernel has: what is not refused for its pitch is refused next.)"""
+    kw = dict(rows=rows, pos_ld=pos_ld, q_heads=20000, q_in_head_ld=64, q_out_row_ld=64 * 20000, q_out=1 << 23)
+    assert L.load().t2w_rotary(ctypes.byref(rotary_args(**kw)), None) == status
+
+
 def test_rows_that_meet():
     """q and k in place at one row pitch are refused exactly where they have a value in common, heads that alternate among
     them.  Heads of 4112 values are more than the kernel has, so that a call that is not refused for this is refused next."""
