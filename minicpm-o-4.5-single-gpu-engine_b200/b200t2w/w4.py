@@ -55,7 +55,8 @@ class Weight4:
         return tuple(r) if self.is_gated else r[0]
 
     def check(self) -> None:
-        """Wait for the GPU and raise ``T2WError`` if a product with this weight gave up on a wait (its outputs are void)."""
+        """Wait for the GPU and raise ``T2WError`` if a product with this weight has given up on a wait since the last look
+        (its outputs are void)."""
         L.check("t2w_w4_linear", O.call("w4_status", self.buffer, self.n, self.k, self.group, self.kind))
 
 

@@ -582,7 +582,7 @@ std::vector<at::Tensor> w4_unpack(const at::Tensor& buffer, int64_t n, int64_t k
   return r;
 }
 
-int64_t w4_status(const at::Tensor& buffer, int64_t n, int64_t k, int64_t group, int64_t kind) {
+int64_t w4_status(at::Tensor& buffer, int64_t n, int64_t k, int64_t group, int64_t kind) {
   const t2w_w4_weight w = weight_of("w4_status", buffer, n, k, group, kind);
   const c10::DeviceGuard guard(buffer.device());
   return t2w_w4_status(&w, stream_of(buffer));
@@ -758,7 +758,7 @@ TORCH_LIBRARY(b200t2w, m) {
         "Tensor? up_codes, Tensor? up_scales, Tensor? up_zeros) -> ()",
         &w4_pack);
   m.def("w4_unpack(Tensor buffer, int n, int k, int group, int kind) -> Tensor[]", &w4_unpack);
-  m.def("w4_status(Tensor buffer, int n, int k, int group, int kind) -> int", &w4_status);
+  m.def("w4_status(Tensor(a!) buffer, int n, int k, int group, int kind) -> int", &w4_status);
   m.def("w4_linear(Tensor x, Tensor buffer, int n, int k, int group, int kind, Tensor? bias, Tensor? residual) -> Tensor",
         &w4_linear);
   m.def("w4_gated(Tensor x, Tensor buffer, int n, int k, int group, int kind, int act) -> Tensor", &w4_gated);

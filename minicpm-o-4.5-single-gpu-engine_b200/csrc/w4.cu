@@ -165,6 +165,10 @@ extern "C" int t2w_w4_status(const t2w_w4_weight* w, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaMemcpyAsync(&s, w->buffer, sizeof(s), cudaMemcpyDeviceToHost, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && s != T2W_OK) {  // told once: products after it are judged by themselves
+    e = cudaMemsetAsync(w->buffer, 0, sizeof(s), st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  }
   if (e == cudaSuccess) return s;
   return done(e);
 }

@@ -281,6 +281,25 @@ def test_captured_and_on_other_streams(rows):
     down.check()
 
 
+@pytest.mark.parametrize("rows", [2, 40])
+def test_a_status_is_told_once(rows):
+    """A status as a wait that gave up records it is raised by one ``check``, and products after it are judged by themselves."""
+    gen = torch.Generator().manual_seed(7)
+    w, x = ref.weights(80, 160, 32, True, BF16, gen), normal(gen, rows, 160)
+    p = w4.pack(*cuda(w))
+    laid_out = p.buffer.clone()
+    p.buffer[:4].view(torch.int32).fill_(-4)
+    torch.cuda.synchronize()
+    with pytest.raises(L.T2WError) as e:
+        p.check()
+    assert e.value.status == -4
+    p.check()
+    out = w4.linear(x.cuda(), p)
+    p.check()
+    held(out, ref.linear(x, w))
+    assert torch.equal(p.buffer, laid_out)
+
+
 def test_refusals():
     gen = torch.Generator().manual_seed(1)
     w = ref.weights(64, 128, 64, True, BF16, gen)
