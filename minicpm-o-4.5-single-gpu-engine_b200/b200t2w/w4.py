@@ -63,9 +63,10 @@ class Weight4:
 def quantize(weight: torch.Tensor, group: int = 128, zeros: bool = False):
     """Codes (uint8 ``[n, k]``), scales (``weight``'s type, ``[n, k / group]``) and zeros (uint8, or None) of a bf16 or fp16
     matrix: each group's largest magnitude / 7 is its scale, or with ``zeros`` its range (0 in it) / 15, rounded to the
-    type; codes are the nearest to weight / scale (ties to even)."""
+    type; codes are the nearest to weight / scale (ties to even).  They are values of their own, without a gradient."""
     if weight.dtype not in (torch.bfloat16, torch.float16) or weight.dim() != 2:
         raise ValueError("a bf16 or fp16 matrix is quantised")
+    weight = weight.detach()  # (a parameter's scales would keep the fp32 copies made here for a gradient)
     n, k = weight.shape
     if group not in (32, 64, 128) or k == 0 or k % group:
         raise ValueError(f"groups of 32, 64 or 128 that divide the {k} inputs")

@@ -174,6 +174,14 @@ def test_quantize(dtype, zeros, group):
             assert codes[r, g * group:(g + 1) * group].tolist() == want
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+def test_a_parameter_is_quantised_without_a_gradient(zeros):
+    w = torch.randn(6, 128, generator=torch.Generator().manual_seed(1)).to(BF16)
+    got, want = w4.quantize(torch.nn.Parameter(w), 64, zeros), w4.quantize(w, 64, zeros)
+    for a, b in zip(got, want):
+        assert (a is None and b is None) or (torch.equal(a, b) and not a.requires_grad and a.grad_fn is None)
+
+
 def test_matrices_that_cannot_be_quantised():
     w = torch.randn(4, 128).to(BF16)
     for bad, kw in ((w.float(), {}), (w[0], {}), (w, dict(group=16)), (w[:, :96], dict(group=64)), (w[:, :0], {})):
