@@ -730,7 +730,7 @@ typedef struct t2w_w4_source {
 T2W_API int64_t t2w_w4_bytes(int32_t n, int32_t k, int32_t group, int32_t zeros, int32_t gated);
 /* Lay `a` (gated: the gate `a` and the up projection `b`) out into w->buffer.  Codes and zeros are taken modulo 16. */
 T2W_API int t2w_w4_pack(const t2w_w4_weight* w, const t2w_w4_source* a, const t2w_w4_source* b, void* stream);
-/* The values (code - zero) * scale, exact, into fp32 [n][k] matrices at these pitches (b: the up projection's). */
+/* The values (code - zero) * scale, exact, into fp32 [n][k] matrices at these pitches, at least k (b: the up projection's). */
 T2W_API int t2w_w4_unpack(const t2w_w4_weight* w, float* a, int64_t a_ld, float* b, int64_t b_ld, void* stream);
 /* What products with this weight have recorded since the last such call: T2W_OK, or T2W_ERR_TIMEOUT if one gave up on a wait
  * (its outputs are void; then cleared).  By a copy on `stream` that this call waits for. */

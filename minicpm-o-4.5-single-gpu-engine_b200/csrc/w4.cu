@@ -111,6 +111,9 @@ int fill(PackDev& p, const t2w_w4_weight* w) {
 }
 dim3 tile_grid(int64_t tiles) { return dim3(65535 < tiles ? 65535 : (unsigned)tiles, (unsigned)((tiles + 65534) / 65535)); }
 
+// Whether a pointer lies on `bytes` (a power of two).
+bool lies_on(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
 int done(cudaError_t e) {
   if (e == cudaSuccess) return T2W_OK;
   set_cuda_error(e);
@@ -134,7 +137,8 @@ extern "C" int t2w_w4_pack(const t2w_w4_weight* w, const t2w_w4_source* a, const
   const t2w_w4_source* src[2] = {a, b};
   if (!a || (p.gated && !b)) return T2W_ERR_INVALID;
   for (int i = 0; i < (p.gated ? 2 : 1); ++i) {
-    if (!src[i]->codes || !src[i]->scales || (p.has_zeros && !src[i]->zeros)) return T2W_ERR_INVALID;
+    if (!src[i]->codes || !src[i]->scales || !lies_on(src[i]->scales, 2) || (p.has_zeros && !src[i]->zeros))
+      return T2W_ERR_INVALID;
     p.codes[i] = static_cast<const uint8_t*>(src[i]->codes);
     p.scales[i] = static_cast<const uint16_t*>(src[i]->scales);
     p.zeros[i] = static_cast<const uint8_t*>(src[i]->zeros);
@@ -150,7 +154,9 @@ extern "C" int t2w_w4_pack(const t2w_w4_weight* w, const t2w_w4_source* a, const
 extern "C" int t2w_w4_unpack(const t2w_w4_weight* w, float* a, int64_t a_ld, float* b, int64_t b_ld, void* stream) {
   PackDev p = {};
   if (const int e = fill(p, w)) return e;
-  if (!a || (p.gated && !b)) return T2W_ERR_INVALID;
+  if (!a || (p.gated && !b) || !lies_on(a, 4) || (p.gated && !lies_on(b, 4)) ||
+      (p.n > 1 && (a_ld < p.k || (p.gated && b_ld < p.k))))
+    return T2W_ERR_INVALID;
   p.out[0] = a;
   p.out[1] = b;
   p.out_ld[0] = a_ld;
@@ -182,8 +188,8 @@ extern "C" int t2w_w4_linear(const t2w_w4_linear_args* a, void* stream) {
   if (w.gated && (a->bias || a->residual)) return T2W_ERR_INVALID;
   if (a->rows == 0) return T2W_OK;
   // x is read in 16-byte pieces
-  if (!a->x || !a->out || (reinterpret_cast<uintptr_t>(a->x) & 15) || a->x_ld % 8 || a->x_ld < 0 ||
-      (reinterpret_cast<uintptr_t>(a->out) & 1) || (a->rows > 1 && a->x_ld < a->w.k) ||
+  if (!a->x || !a->out || !lies_on(a->x, 16) || a->x_ld % 8 || a->x_ld < 0 || !lies_on(a->out, 2) || !lies_on(a->bias, 2) ||
+      !lies_on(a->residual, 2) || (a->rows > 1 && a->x_ld < a->w.k) ||
       (a->residual && a->rows > 1 && a->res_ld < a->w.n))
     return T2W_ERR_INVALID;
   W4Dev p = {};

@@ -59,6 +59,28 @@ def test_products_that_there_are_not(kw, status):
     assert L.load().t2w_w4_linear(ctypes.byref(linear_args(**kw)), None) == status
 
 
+@pytest.mark.parametrize("kw", [dict(bias=(1 << 20) + 1), dict(residual=(1 << 20) + 1, res_ld=64)])
+def test_values_that_lie_between_two_addresses(kw):
+    assert L.load().t2w_w4_linear(ctypes.byref(linear_args(**kw)), None) == INVALID
+    assert L.load().t2w_w4_linear(ctypes.byref(linear_args(rows=40, **kw)), None) == INVALID
+
+
+@pytest.mark.parametrize("gated", [0, 1])
+def test_layouts_that_there_are_not(gated):
+    lib, at = L.load(), 1 << 20
+    w = L.W4Weight(n=64, k=128, group=64, scale_dtype=0, zeros=1, gated=gated, buffer=at)
+    good = dict(codes=at, scales=at, zeros=at, code_ld=128, scale_ld=2, zero_ld=2)
+    for kw in (dict(codes=None), dict(scales=None), dict(scales=at + 1), dict(zeros=None)):
+        bad = ctypes.byref(L.W4Source(**(good | kw)))
+        assert lib.t2w_w4_pack(ctypes.byref(w), bad, ctypes.byref(L.W4Source(**good)), None) == INVALID
+        if gated:
+            assert lib.t2w_w4_pack(ctypes.byref(w), ctypes.byref(L.W4Source(**good)), bad, None) == INVALID
+    for out, ld in ((None, 128), (at + 2, 128), (at, 127), (at, 0), (at, -128)):
+        assert lib.t2w_w4_unpack(ctypes.byref(w), out, ld, at, 128, None) == INVALID
+        if gated:
+            assert lib.t2w_w4_unpack(ctypes.byref(w), at, 128, out, ld, None) == INVALID
+
+
 def test_no_rows_are_no_work():
     assert L.load().t2w_w4_linear(ctypes.byref(linear_args(rows=0, x=None, out=None)), None) == 0
 
