@@ -186,7 +186,8 @@ extern "C" int t2w_rotary(const t2w_rotary_args* a, void* stream) {
     return T2W_ERR_INVALID;
   const int64_t heads = (int64_t)a->q_heads + a->k_heads;
   if (a->rows == 0 || heads == 0) return T2W_OK;
-  if (!a->positions || !a->table || (reinterpret_cast<uintptr_t>(a->table) & 7) || a->pos_ld < 0 ||
+  if (!a->positions || !a->table || (reinterpret_cast<uintptr_t>(a->table) & 7) ||
+      (reinterpret_cast<uintptr_t>(a->positions) & (a->wide_positions ? 7 : 3)) || a->pos_ld < 0 ||
       (a->axes > 1 && a->pos_ld != 0 && a->pos_ld < a->rows))
     return T2W_ERR_INVALID;
   RotDev p = {};

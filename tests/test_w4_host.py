@@ -124,6 +124,12 @@ def test_pitches_of_positions(rows, pos_ld, status):
     assert L.load().t2w_rotary(ctypes.byref(rotary_args(**kw)), None) == status
 
 
+@pytest.mark.parametrize("off,wide,status", [(2, 0, INVALID), (4, 0, UNSUPPORTED), (4, 1, INVALID), (8, 1, UNSUPPORTED)])
+def test_positions_that_lie_between_two_addresses(off, wide, status):
+    kw = dict(positions=(1 << 20) + off, wide_positions=wide, q_heads=20000, q_in_head_ld=64, q_out_row_ld=64 * 20000)
+    assert L.load().t2w_rotary(ctypes.byref(rotary_args(**kw)), None) == status
+
+
 def test_rows_that_meet():
     """q and k in place at one row pitch are refused exactly where they have a value in common, heads that alternate among
     them.  Heads of 4112 values are more than the kernel has, so that a call that is not refused for this is refused next."""
