@@ -233,7 +233,7 @@ extern "C" int t2w_rotary(const t2w_rotary_args* a, void* stream) {
   p.per_block = std::max(1, std::min({kPieces / p.items, a->rows / (4 * num_sms()), 4096 / p.pairs}));
   const int total = std::min(p.per_block, a->rows) * p.items, rounds = (total + kMaxThreads - 1) / kMaxThreads;
   const int threads = ((total + rounds - 1) / rounds + 31) / 32 * 32;
-  const dim3 grid((unsigned)((a->rows + p.per_block - 1) / p.per_block));
+  const dim3 grid((unsigned)(((int64_t)a->rows + p.per_block - 1) / p.per_block));
   const size_t smem = (size_t)p.per_block * p.pairs * sizeof(float2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;

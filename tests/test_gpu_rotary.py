@@ -198,6 +198,25 @@ def test_heads_of_q_and_k_in_turn(rows):
             turn.apply_(y[:, :, 0], k, pos)
 
 
+def test_as_many_rows_as_there_may_be():
+    """2^31 - 1 rows of one head: the first and the last ones, in place."""
+    rows, hd = 2 ** 31 - 1, 16
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 90 << 30:
+        pytest.skip("needs 77 GB of GPU memory")
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randn(600, 1, hd, generator=gen).to(BF16)
+    pos = torch.randint(0, 5000, (600,), generator=gen, dtype=torch.int32)
+    q = torch.zeros(rows, 1, hd, dtype=BF16, device="cuda")
+    p = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    q[:300], q[-300:], p[:300], p[-300:] = x[:300].cuda(), x[300:].cuda(), pos[:300].cuda(), pos[300:].cuda()
+    Rotary(hd).apply_(q, None, p)
+    held(torch.cat([q[:300], q[-300:]]), x, pos[None], axis_of([hd // 2]), inv_freq(hd, 10000.0), hd, False, False)
+    assert not bool(q[300:1000].any()) and not bool(q[-1000:-300].any())
+    del q, p
+    torch.cuda.empty_cache()
+
+
 def test_captured():
     gen = torch.Generator().manual_seed(8)
     turn = Rotary(128, [16, 24, 24])
