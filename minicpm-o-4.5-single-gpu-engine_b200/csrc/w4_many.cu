@@ -675,6 +675,10 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
   }
 }
 
+// Tiles of 128 rows of W x nx rows of x.
+constexpr int64_t tiles_of(int blocks, int rows, int nx) { return ((int64_t)blocks + 1) / 2 * (((int64_t)rows + nx - 1) / nx); }
+static_assert(tiles_of(1, 0x7fffffff, 256) == 1 << 23 && tiles_of(3, 257, 256) == 4, "as many rows as a call may have");
+
 template <bool HALF, int NX, int G>
 int many_smem(bool zeros) {
   const int tile = w4_tile_bytes(G, zeros), fixed = (Cfg<NX>::fixed(G) + 127) / 128 * 128;
@@ -701,7 +705,7 @@ cudaError_t launch(const W4Dev& p, bool zeros, bool gated, int split, cudaStream
   a.gated = gated;
   a.tile_bytes = w4_tile_bytes(G, zeros);
   a.tiles_n = (p.blocks + 1) / 2;
-  const int64_t tiles = (int64_t)a.tiles_n * ((p.rows + NX - 1) / NX);
+  const int64_t tiles = tiles_of(p.blocks, p.rows, NX);
   if (tiles > (1 << 27)) return cudaErrorInvalidValue;
   a.tiles = (int)tiles;
   a.split = split;
@@ -747,7 +751,7 @@ struct Choice {
 template <bool HALF, int NX, int G>
 void consider(const W4Dev& p, bool zeros, Choice& best) {
   constexpr int kTile = (NX == 32 ? 45 : NX == 64 ? 47 : NX == 128 ? 73 : 87) * (G == 32 ? 17 : G == 64 ? 12 : 10) / 10, kEnd = NX == 32 ? 150 : NX == 64 ? 200 : NX == 128 ? 300 : 500;
-  const int64_t tiles = (int64_t)((p.blocks + 1) / 2) * ((p.rows + NX - 1) / NX);
+  const int64_t tiles = tiles_of(p.blocks, p.rows, NX);
   for (int s = 1; s <= 8 && p.tiles_k >= 2 * s; s *= 2) {
     if (s > 1 && tiles > room_for<HALF, NX, G>(s, zeros)) break;
     const int64_t rounds = s > 1 ? 1 : (tiles + num_sms() - 1) / num_sms();
