@@ -248,6 +248,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int log_s
       if (at < end) load_x(x, row, p.k, kt, t);
     }
     if (split > 1) {
+      __syncwarp();  // (the cluster's barrier takes whole warps, here and below)
       cluster_arrive();
       cluster_wait();
     } else {
@@ -283,6 +284,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_w4_few(const W4Dev p, int log_s
     }
     if (rb0 < rb_end) {  // no block is sent new sums before these are read
       if (split > 1) {
+        __syncwarp();
         cluster_arrive();
         cluster_wait();
       } else {

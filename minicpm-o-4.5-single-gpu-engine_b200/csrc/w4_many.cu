@@ -626,6 +626,7 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
 #pragma unroll 1
         for (int c0 = 0; c0 < C::U; c0 += kChunk) {
           float v[kChunk];
+          __syncwarp();  // (lanes without outputs have gone other ways)
           tmem_ld8(own + c0, v);
           if (res) {
             res += kChunk * p.res_ld;
@@ -649,6 +650,7 @@ __global__ void __launch_bounds__(Cfg<NX>::THREADS, 1)
 #pragma unroll 1
         for (int c0 = 0; c0 < C::U; c0 += kChunk) {
           float v[kChunk];
+          __syncwarp();
           tmem_ld8(own + c0, v);
 #pragma unroll
           for (int c = 0; c < kChunk; c += 2) {
