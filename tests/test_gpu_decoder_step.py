@@ -14,6 +14,7 @@ from b200t2w import lib as L
 from b200t2w import w4
 from b200t2w.paged import B200PagedCache
 from b200t2w.rotary import Rotary
+from test_gpu_paged import attention as plain_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -89,6 +90,48 @@ def test_parts(fresh):
         held(z, ref.linear(h.cpu(), step.down, None, y.cpu()))
     for p in (step.p_qkv, step.p_out, step.p_gate_up, step.p_down):
         p.check()
+
+
+@pytest.mark.parametrize("fresh", [[1], [9, 1, 30, 0, 7], [100, 60]])
+def test_attention_of_the_step(fresh):
+    """The step's attention against the plain one over what its cache holds, and what it holds against the turned keys and the
+    values of the fused rows.
+
+    The attention's bound is that of ``test_gpu_paged``.  A cached value is rounded to e4m3 once, and once more where a later row
+    raises its page's scale: twice half a step, 2^-4 of the value or 2^-10 of the scale, the second of what the first left."""
+    step, gen = Step(len(fresh) + 20), torch.Generator().manual_seed(sum(fresh) + 1)
+    rows, cache = sum(fresh), cache_of(len(fresh), 300)
+    f = torch.tensor(fresh, dtype=torch.int32, device="cuda")
+    told = [[[] for _ in fresh] for _ in range(2)]  # keys and values of each request
+    for _ in range(2):
+        x = torch.randn(rows, WIDTH, generator=gen).bfloat16()
+        positions = torch.randint(0, 4000, (3, rows), generator=gen)
+        plan = cache.plan(f, rows=rows, max_fresh=max(fresh))
+        _, after, a, *_ = step(x.cuda(), positions.cuda(), cache, plan)
+        plan.check()
+        after = after.double().cpu().view(rows, ALL, HD)
+        out = a.double().cpu().view(rows, HEADS, HD)
+        table, start = cache.table.cpu(), 0
+        codes = [t[0].float().double().cpu() * s[0].double().cpu()[..., None, None] for t, s in
+                 ((cache.k, cache.k_scale), (cache.v, cache.v_scale))]
+        scale = [s[0].double().cpu() for s in (cache.k_scale, cache.v_scale)]
+        for r, n in enumerate(fresh):
+            part = after[start:start + n]
+            held_rows = []
+            for w in range(2):
+                told[w][r].append(part[:, HEADS + w * KV:HEADS + (w + 1) * KV])
+                want = torch.cat(told[w][r])
+                pages = table[r, :-(-want.shape[0] // PAGE)].long()
+                got = codes[w][pages].transpose(1, 2).reshape(-1, KV, HD)[:want.shape[0]]
+                each = scale[w][pages].repeat_interleave(PAGE, 0)[:want.shape[0], :, None]
+                once = 2.0 ** -4 * want.abs() + 2.0 ** -10 * each
+                assert bool(((got - want).abs() <= once + 2.0 ** -4 * (want.abs() + once) + 2.0 ** -10 * each).all())
+                held_rows.append(got)
+            for h in range(HEADS):
+                k, v = (t[:, h // (HEADS // KV)] for t in held_rows)
+                o, _, size, b = plain_attention(part[:, h], k, v, True, HD ** -0.5)
+                held(out[start:start + n, h], (o, 2.0 ** -8 * o.abs() + (2.0 ** -10 + 2.0 ** -15 * b[:, None]) * size + 1e-30))
+            start += n
 
 
 @pytest.mark.parametrize("requests", [3, 40])
