@@ -1,10 +1,12 @@
-"""Rotary positions with one or several axes (text; height and width of an image; time, height and width of a video) for
-the queries and keys of an attention, both in one kernel.
+"""Rotary positions with one or several axes (a language model's text; time, height and width of the images and videos among
+it) for the queries and keys of an attention, both in one kernel.
 
 Runs on the current stream of the tensors' GPU, keeps nothing between calls and may be captured in a CUDA graph.  Rows are
 views with strides of whole 16-byte pieces, such as columns of fused projection rows.  Arguments that cannot be right raise at
-the call: ``T2WError`` for sizes that the kernel does not have (head_dim a multiple of 8, rotary_dim of 16), ``RuntimeError``
-for tensors of the wrong type, shape, device or alignment, ``ValueError`` for a table that cannot be made.
+the call: ``ValueError`` for a table that cannot be made (head_dim a multiple of 8, rotary_dim of 16, sections that add up) and
+for heads of another size, ``T2WError`` for sizes that the kernel does not have (rotary_dim above 4096, tens of thousands of heads)
+and for q and k that share memory in place, ``RuntimeError`` for tensors of the wrong type, shape, device or alignment, or that
+require a gradient where gradients are recorded.
 """
 
 from __future__ import annotations
@@ -26,6 +28,10 @@ class Rotary:
     axis has any left.
     ``pairs``: "half" pairs values i and i + rotary_dim / 2 of a head, "adjacent" 2 i and 2 i + 1.  Values past
     ``rotary_dim`` (``head_dim`` unless given) stay as they are.
+
+    There is one ladder of frequencies over all pairs, whatever their axes.  Models that start it again for each axis, as image
+    towers with height and width do, give it as ``inv_freq``: ``2 * [base ** (-4 * i / rotary_dim) for i in range(rotary_dim // 4)]``
+    for two axes with half of the pairs each.
 
     Angles are whole positions times frequencies in 64-bit fixed point, modulo a turn: as exact at a million as at one."""
 

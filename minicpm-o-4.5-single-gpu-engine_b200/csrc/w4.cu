@@ -208,8 +208,9 @@ extern "C" int t2w_w4_linear(const t2w_w4_linear_args* a, void* stream) {
   p.residual = a->residual;
   p.res_ld = a->res_ld;
   p.out = a->out;
-  // A pass over the weights for every 8 rows against one for all: 12 x 4096 x 11008, gated, 27 us for 33 on tcgen05, 16 x 4096 x
-  // 6144 12.2 for 12.0, 32 x 4096 x 6144 22 for 12.
+  // A pass over the weights for every 8 rows against one for all, 16 rows in this form and 17 on tcgen05 (us): k x n 4096 x 6144 10.8
+  // and 12.0, 11008 x 4096 15.4 and 15.5, 1024 x 1024 4.3 and 4.9, gated 4096 x 11008 25.6 and 33, 2048 x 5632 10.3 and 11.6; a
+  // third pass is slower (32 x 4096 x 6144: 22 for 12).
   const auto launch = a->rows <= 16 ? launch_w4_few : launch_w4_many;
   return done(launch(p, w.group, w.has_zeros, w.gated, a->dtype == T2W_DT_FP16, static_cast<cudaStream_t>(stream)));
 }

@@ -1,5 +1,8 @@
 // Products with 4-bit weights for few rows of x: y[m][n] = sum_k x[m][k] W[n][k] (+ bias, + residual, or a gated pair's
-// activation and product), bound by the weights' bytes.
+// activation and product).  The floor is the weights' bytes.  What bounds it is that 16 warps an SM fill no unit (1 x 4096 x 131072:
+// 58 us, 4.7 TB/s, 59% of the issue slots in use; a warp's time is 16% issuing, 22% fixed latencies, 16% waiting for the half-rate
+// integer pipe, 17% for its turn, 8% at barriers), and in small calls the ends: the fence before a cluster's barrier takes 22% of
+// the warps' time in 1 x 4096 x 11008, gated.
 //
 // A cluster of 1, 2 or 4 blocks of 8 warps has a number of row blocks (64 rows of W), whose tiles (64 x 128) it shares out evenly,
 // in order, to its warps.  A warp streams its tiles (one bulk copy each, into a ring of its own) through m16n8k16 products,
@@ -10,7 +13,7 @@
 // Warps meet once, at the end: each leaves the sums of the one or two row blocks that its tiles were of, a block adds its warps'
 // and sends them to the block of the cluster that finishes the row block (distributed shared memory), which adds those after
 // the cluster's one barrier: no workspace, no atomics, the same order in every call.  (A meeting for each row block instead, k
-// shared out to the warps: 20 us for 1 x 4096 x 11008, gated, of which 14 without any product; 13.9 now.  Sums read from the other
+// shared out to the warps: 20 us for 1 x 4096 x 11008, gated, of which 14 without any product; 14.1 now.  Sums read from the other
 // blocks, which takes a second barrier before they may end: 4 us of 21.)
 #include "common.cuh"
 #include "kernels.h"

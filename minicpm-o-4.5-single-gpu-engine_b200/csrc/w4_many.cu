@@ -13,7 +13,8 @@
 // The weights go through TMEM because shared memory is what such a kernel runs out of: 128 bytes a clock, of which 128 k of
 // widened weights would take 256 clocks to write and 256 to read, where the products take 4 NX clocks.
 // What a hand-over costs decides the rest: passing an mbarrier that is ready takes about 100 clocks, a commit 80, the
-// issue of 4 products 65, a round of waiting, expecting and two copies 650 (one thread brings 23 GB/s in pieces of 4 KB).  So
+// issue of 4 products 65, a round of waiting, expecting and one copy 600 (one thread brings 12.9 GB/s in pieces of 4 KB, 26.5 in
+// pieces of 8 KB).  So
 // copies and products are issued by several warps in turn, and with groups of 128 one barrier tells the products' warp what a
 // half waits for (x and a free accumulator; the weights too where there is one half), and one commit tells that its stage is
 // free and its accumulator full.
@@ -742,9 +743,10 @@ cudaError_t launch(const W4Dev& p, bool zeros, bool gated, int split, cudaStream
   return cudaLaunchKernelEx(&cfg, k_w4_many<HALF, NX, G>, map, a);
 }
 
-// The tile's width and the split of k with the least time by what was measured (us, groups of 128): a tile of 128 k takes
-// 0.45 for NX = 32, 0.47 for 64, 0.73 for 128 and 0.87 for 256 (with groups of 64 about 1.2 and of 32 about 1.7 times that), the
-// end of a block's tile 1.5 to 5, and the cluster's joining 1.5 more.  Blocks of a cluster have one tile, so all clusters have to be
+// The tile's width and the split of k with the least time by a rule of thumb (us, groups of 128): a tile of 128 k is taken to
+// cost 0.45 for NX = 32, 0.47 for 64, 0.73 for 128 and 0.87 for 256 (with groups of 64 1.2 and of 32 1.7 times that), the
+// end of a block's tile 1.5 to 5, and the cluster's joining 1.5 more.  Measured, in one round of 148 tiles: 0.43, 0.48, 0.61 and
+// 0.77; with groups of 64 1.3 to 1.5 times that and of 32 1.9 to 2.4 times, so the rule is kind to narrow groups, all widths alike.  Blocks of a cluster have one tile, so all clusters have to be
 // resident at once.
 struct Choice {
   int nx = 0, split = 1;

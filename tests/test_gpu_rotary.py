@@ -106,6 +106,17 @@ def test_interleaved_sections_and_own_frequencies():
     held(turn(x.cuda(), None, pos.cuda())[0], x, pos, axis_of([14, 9, 9]), own, 64, False, False)
 
 
+@pytest.mark.parametrize("adjacent", [False, True])
+def test_frequencies_that_start_again(adjacent):
+    """Height and width with a ladder of their own each, as image towers have them, given as own frequencies."""
+    gen = torch.Generator().manual_seed(5)
+    rot, x = 80, torch.randn(30, 2, 80, generator=gen).to(BF16)
+    pos = torch.randint(0, 70, (2, 30), generator=gen)
+    turn = Rotary(rot, [20, 20], pairs="adjacent" if adjacent else "half",
+                  inv_freq=2 * [10000.0 ** (-4 * i / rot) for i in range(rot // 4)])
+    held(turn(x.cuda(), None, pos.cuda())[0], x, pos, axis_of([20, 20]), torch.cat([inv_freq(rot // 2, 10000.0)] * 2), rot, adjacent, False)
+
+
 def test_inverse_is_the_gradient():
     """With L = sum w . turned(x): the gradient is the inverse turn of w, against the formula's (autograd in 64 bits) and
     against differences of L."""
