@@ -185,9 +185,9 @@ T2W_DEV uint32_t w4_zero_hi(uint32_t z) {
   return HALF ? 0xd400d400u + z * 0x00100010u /* -(64 + zero) */ : w4_zero<HALF>(z);
 }
 // The four registers of a word: code - zero, with zlo for rows g and zhi (of w4_zero_hi) for rows g + 8.  A code's bits are
-// put under an exponent that makes its steps whole (a long-known way to turn few bits into a float without a conversion).  fp16 has room for two codes side by side: one 16 times too large is
-// brought back by the multiplication-addition that takes its zero off (exact: 6 bits and a sign), which saves two of three
-// shifts; bf16 has not.
+// put under an exponent that makes its steps whole (a long-known way to turn few bits into a float without a conversion).
+// fp16 has room for two codes side by side: one 16 times too large is brought back by the multiplication-addition that takes
+// its zero off (exact: 6 bits and a sign), which saves two of three shifts; bf16 has not.
 template <bool HALF>
 T2W_DEV void w4_widen(uint32_t w, uint32_t zlo, uint32_t zhi, uint32_t (&a)[4]) {
   if constexpr (HALF) {

@@ -746,8 +746,8 @@ cudaError_t launch(const W4Dev& p, bool zeros, bool gated, int split, cudaStream
 // The tile's width and the split of k with the least time by a rule of thumb (us, groups of 128): a tile of 128 k is taken to
 // cost 0.45 for NX = 32, 0.47 for 64, 0.73 for 128 and 0.87 for 256 (with groups of 64 1.2 and of 32 1.7 times that), the
 // end of a block's tile 1.5 to 5, and the cluster's joining 1.5 more.  Measured, in one round of 148 tiles: 0.43, 0.48, 0.61 and
-// 0.77; with groups of 64 1.3 to 1.5 times that and of 32 1.9 to 2.4 times, so the rule is kind to narrow groups, all widths alike.  Blocks of a cluster have one tile, so all clusters have to be
-// resident at once.
+// 0.77; with groups of 64 1.3 to 1.5 times that and of 32 1.9 to 2.4 times, so the rule is kind to narrow groups, all widths
+// alike.  Blocks of a cluster have one tile, so all clusters have to be resident at once.
 struct Choice {
   int nx = 0, split = 1;
   int64_t cost = INT64_MAX;
